@@ -277,8 +277,43 @@ class GemmParams(ctypes.Structure):
     ]
 
 
+class TreeParams(ctypes.Structure):
+    """``asrlayer_tree_params`` (csrc/layers.hpp)."""
+
+    _fields_ = [
+        *[(name, _ptr) for name in ("q", "k", "v", "k_draft", "v_draft", "out")],
+        *[(f"{t}_{axis}_stride", _i64) for t in ("q", "k", "v", "kd", "vd", "o") for axis in ("batch", "token", "head")],
+        ("masks", _ptr),
+        ("masks_batch_stride", _i64),
+        ("lengths", _ptr),
+        ("block_table", _ptr),
+        *[(name, _i64) for name in ("bt_stride", "k_page_stride", "v_page_stride")],
+        *[(name, _i32) for name in ("page_size", "num_pages", "lengths64", "batch", "tokens", "heads_q", "heads_kv",
+                                    "head_dim", "max_len_k", "dtype")],
+        ("scale", ctypes.c_float),
+    ]
+
+
+class CommitParams(ctypes.Structure):
+    """``asrlayer_commit_params`` (csrc/layers.hpp)."""
+
+    _fields_ = [
+        *[(name, _ptr) for name in ("k_draft", "v_draft", "k", "v")],
+        *[(f"{t}_{axis}_stride", _i64) for t in ("kd", "vd", "k", "v") for axis in ("layer", "batch", "token", "head")],
+        *[(name, _ptr) for name in ("path", "count", "lengths", "block_table")],
+        ("bt_stride", _i64),
+        *[(name, _i32) for name in ("page_size", "num_pages", "lengths64", "layers", "batch", "tokens", "heads_kv",
+                                    "head_dim", "max_len_k", "dtype")],
+    ]
+
+
 # The layers' own entry points (csrc/layers.hpp).
 LAYER_SIGNATURES = {
+    "asrlayer_tree": (ctypes.c_int, [ctypes.POINTER(TreeParams), _ptr, ctypes.c_size_t, _ptr]),
+    "asrlayer_tree_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(TreeParams)]),
+    "asrlayer_tree_masks": (ctypes.c_int, [_ptr, _i64, _i64, _i32, _ptr, _ptr]),
+    "asrlayer_accept": (ctypes.c_int, [_ptr, _ptr, _i64, _ptr, _ptr, _i64, _i32, _ptr, _ptr, _ptr, _ptr]),
+    "asrlayer_commit": (ctypes.c_int, [ctypes.POINTER(CommitParams), _ptr]),
     "asrlayer_embed_rows": (ctypes.c_int, [ctypes.POINTER(EmbedParams), _ptr]),
     "asrlayer_gemm": (ctypes.c_int, [ctypes.POINTER(GemmParams), _ptr]),
     "asrlayer_rows_linear": (ctypes.c_int, [ctypes.POINTER(LinearParams), _ptr]),

@@ -569,3 +569,161 @@ int asrlayer_gemm(const asrlayer_gemm_params* params, void* stream) {
 }
 
 }  // extern "C"
+
+namespace {
+
+// Sizes of asrlayer_tree.
+int check_tree(const asrlayer_tree_params* params) {
+  if (params == nullptr) return fail(ASRATTN_ERR_INVALID, "params is NULL");
+  const asrlayer_tree_params& p = *params;
+  const int rc = check_common(p.dtype, p.heads_q, p.heads_kv, p.head_dim, p.scale);
+  if (rc != ASRATTN_OK) return rc;
+  if (p.head_dim != 64 && p.head_dim != 128 && p.head_dim != 256)
+    return fail(ASRATTN_ERR_UNSUPPORTED, "no tree kernel for head_dim %d (supported: 64, 128, 256)", p.head_dim);
+  if (p.batch < 0 || p.max_len_k < 0)
+    return fail(ASRATTN_ERR_INVALID, "batch (%d) and max_len_k (%d) must be >= 0", p.batch, p.max_len_k);
+  if (p.tokens < 1 || p.tokens > 64)
+    return fail(ASRATTN_ERR_UNSUPPORTED, "a tree has 1 to 64 drafted tokens, got %d", p.tokens);
+  if (p.batch > 65535 || p.heads_q > 4096) return fail(ASRATTN_ERR_UNSUPPORTED, "more than 65535 rows or 4096 heads");
+  return ASRATTN_OK;
+}
+
+struct TreeWorkspace {
+  size_t stats, arrive, total;
+};
+
+// units: workgroups times splits over all rows; words: units of work.
+TreeWorkspace tree_workspace(const asrlayer_tree_params& p, int row_tiles, size_t units, size_t words) {
+  TreeWorkspace w;
+  const size_t rows = units * row_tiles * 16;
+  w.stats = align256(rows * (size_t)p.head_dim * sizeof(float));
+  w.arrive = w.stats + align256(rows * 2 * sizeof(float));
+  w.total = w.arrive + align256(words * sizeof(unsigned long long));
+  return w;
+}
+
+// Whether every key and value a part of 16 positions holds has a 32-bit offset.
+bool part_addressable(int64_t stride, int dtype) {
+  return stride >= 0 && stride * 16 * elem_bytes(dtype) < (1LL << 30);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t asrlayer_tree_workspace_size(const asrlayer_tree_params* params) {
+  if (check_tree(params) != ASRATTN_OK) return (size_t)-1;
+  const asrattn::TreePlan plan = asrattn::tree_plan(*params);
+  if (plan.splits == 1) return 0;
+  // A plan that splits has at most 256 workgroups, whatever its batch and tokens.
+  return tree_workspace(*params, plan.row_tiles, 256, 256).total;
+}
+
+int asrlayer_tree(const asrlayer_tree_params* params, void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = check_tree(params);
+  if (rc != ASRATTN_OK) return rc;
+  const asrlayer_tree_params& p = *params;
+  if (p.batch == 0) return ok();
+  if (p.q == nullptr || p.k_draft == nullptr || p.v_draft == nullptr || p.out == nullptr || p.masks == nullptr ||
+      (p.max_len_k > 0 && (p.k == nullptr || p.v == nullptr)))
+    return fail(ASRATTN_ERR_INVALID, "q, k, v, the drafts, out and masks must be non-NULL");
+  if (!vec_aligned(p.q, p.dtype, {p.q_batch_stride, p.q_token_stride, p.q_head_stride}) ||
+      !vec_aligned(p.k, p.dtype, {p.k_batch_stride, p.k_token_stride, p.k_head_stride}) ||
+      !vec_aligned(p.v, p.dtype, {p.v_batch_stride, p.v_token_stride, p.v_head_stride}) ||
+      !vec_aligned(p.k_draft, p.dtype, {p.kd_batch_stride, p.kd_token_stride, p.kd_head_stride}) ||
+      !vec_aligned(p.v_draft, p.dtype, {p.vd_batch_stride, p.vd_token_stride, p.vd_head_stride}))
+    return fail(ASRATTN_ERR_INVALID,
+                "q, k, v and the drafts need 16-byte aligned pointers and strides that are multiples of 16 bytes");
+  if (!part_addressable(p.k_token_stride, p.dtype) || !part_addressable(p.v_token_stride, p.dtype) ||
+      !part_addressable(p.kd_token_stride, p.dtype) || !part_addressable(p.vd_token_stride, p.dtype))
+    return fail(ASRATTN_ERR_UNSUPPORTED, "positions lie 64 MiB or more apart");
+  if (p.block_table != nullptr) {
+    if (p.page_size < 16 || (p.page_size & (p.page_size - 1)) != 0)
+      return fail(ASRATTN_ERR_UNSUPPORTED, "page_size must be a power of two >= 16, got %d", p.page_size);
+    if (p.num_pages < 0 || p.bt_stride < 1)
+      return fail(ASRATTN_ERR_INVALID, "num_pages must be >= 0 and bt_stride >= 1");
+    if ((long long)p.max_len_k > p.bt_stride * (long long)p.page_size)
+      return fail(ASRATTN_ERR_INVALID, "max_len_k (%d) exceeds the block table's reach (%lld pages of %d)", p.max_len_k,
+                  (long long)p.bt_stride, p.page_size);
+    if (!vec_aligned(p.k, p.dtype, {p.k_page_stride}) || !vec_aligned(p.v, p.dtype, {p.v_page_stride}))
+      return fail(ASRATTN_ERR_INVALID, "page strides must be multiples of 16 bytes");
+  }
+  const asrattn::TreePlan plan = asrattn::tree_plan(p);
+  if ((long long)p.heads_kv * plan.row_blocks > 65535)
+    return fail(ASRATTN_ERR_UNSUPPORTED, "more than 65535 blocks of query rows");
+  float* ws_o = nullptr;
+  float* ws_ml = nullptr;
+  unsigned long long* ws_arrive = nullptr;
+  if (plan.splits > 1) {
+    const size_t words = (size_t)p.batch * p.heads_kv * plan.row_blocks;
+    const TreeWorkspace w = tree_workspace(p, plan.row_tiles, words * plan.splits, words);
+    if (workspace == nullptr || workspace_bytes < w.total)
+      return fail(ASRATTN_ERR_WORKSPACE, "the tree needs %zu workspace bytes, got %zu", w.total,
+                  workspace == nullptr ? (size_t)0 : workspace_bytes);
+    if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+      return fail(ASRATTN_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+    char* base = static_cast<char*>(workspace);
+    ws_o = reinterpret_cast<float*>(base);
+    ws_ml = reinterpret_cast<float*>(base + w.stats);
+    ws_arrive = reinterpret_cast<unsigned long long*>(base + w.arrive);
+  }
+  return from_hip(asrattn::launch_tree(p, plan, ws_o, ws_ml, ws_arrive, static_cast<hipStream_t>(stream)),
+                  "asrlayer_tree");
+}
+
+int asrlayer_tree_masks(const int64_t* parents, int64_t parents_batch_stride, int64_t batch, int32_t tokens,
+                        int64_t* masks, void* stream) {
+  if (tokens < 1 || tokens > 64)
+    return fail(ASRATTN_ERR_UNSUPPORTED, "a tree has 1 to 64 drafted tokens, got %d", tokens);
+  if (batch < 0 || batch > 0x7fffffffLL) return fail(ASRATTN_ERR_INVALID, "batch (%lld) out of range", (long long)batch);
+  if (batch == 0) return ok();
+  if (parents == nullptr || masks == nullptr) return fail(ASRATTN_ERR_INVALID, "parents and masks must be non-NULL");
+  return from_hip(asrattn::launch_tree_masks(parents, parents_batch_stride, batch, tokens, masks,
+                                             static_cast<hipStream_t>(stream)),
+                  "asrlayer_tree_masks");
+}
+
+int asrlayer_accept(const int64_t* tokens, const int64_t* parents, int64_t parents_batch_stride,
+                    const int64_t* choices, const int64_t* limit, int64_t batch, int32_t width, int64_t* path,
+                    int64_t* emitted, int64_t* count, void* stream) {
+  if (width < 1 || width > 64)
+    return fail(ASRATTN_ERR_UNSUPPORTED, "a tree has 1 to 64 drafted tokens, got %d", width);
+  if (batch < 0 || batch > 0x7fffffffLL) return fail(ASRATTN_ERR_INVALID, "batch (%lld) out of range", (long long)batch);
+  if (batch == 0) return ok();
+  if (tokens == nullptr || parents == nullptr || choices == nullptr || path == nullptr || emitted == nullptr ||
+      count == nullptr)
+    return fail(ASRATTN_ERR_INVALID, "tokens, parents, choices, path, emitted and count must be non-NULL");
+  return from_hip(asrattn::launch_accept(tokens, parents, parents_batch_stride, choices, limit, batch, width, path,
+                                         emitted, count, static_cast<hipStream_t>(stream)),
+                  "asrlayer_accept");
+}
+
+int asrlayer_commit(const asrlayer_commit_params* params, void* stream) {
+  if (params == nullptr) return fail(ASRATTN_ERR_INVALID, "params is NULL");
+  const asrlayer_commit_params& p = *params;
+  if (p.dtype != ASRATTN_F32 && p.dtype != ASRATTN_BF16) return fail(ASRATTN_ERR_INVALID, "dtype %d", p.dtype);
+  if (p.layers < 0 || p.batch < 0 || p.max_len_k < 0 || p.heads_kv < 1 || p.head_dim < 1)
+    return fail(ASRATTN_ERR_INVALID, "layers, batch and max_len_k must be >= 0, heads_kv and head_dim positive");
+  if (p.tokens < 1 || p.tokens > 64)
+    return fail(ASRATTN_ERR_UNSUPPORTED, "a tree has 1 to 64 drafted tokens, got %d", p.tokens);
+  const int per_vec = 16 / elem_bytes(p.dtype);
+  if (p.head_dim % per_vec != 0)
+    return fail(ASRATTN_ERR_UNSUPPORTED, "head_dim %d is not a multiple of 16 bytes", p.head_dim);
+  if (p.batch > 65535 || p.layers > 65535 || (long long)p.heads_kv * p.head_dim > (1 << 24))
+    return fail(ASRATTN_ERR_UNSUPPORTED, "more than 65535 rows or layers, or 2^24 values a position");
+  if (p.layers == 0 || p.batch == 0) return ok();
+  if (p.k_draft == nullptr || p.v_draft == nullptr || (p.max_len_k > 0 && (p.k == nullptr || p.v == nullptr)) ||
+      p.path == nullptr || p.count == nullptr || p.lengths == nullptr)
+    return fail(ASRATTN_ERR_INVALID, "the drafts, k, v, path, count and lengths must be non-NULL");
+  if (!vec_aligned(p.k_draft, p.dtype, {p.kd_layer_stride, p.kd_batch_stride, p.kd_token_stride, p.kd_head_stride}) ||
+      !vec_aligned(p.v_draft, p.dtype, {p.vd_layer_stride, p.vd_batch_stride, p.vd_token_stride, p.vd_head_stride}) ||
+      !vec_aligned(p.k, p.dtype, {p.k_layer_stride, p.k_batch_stride, p.k_token_stride, p.k_head_stride}) ||
+      !vec_aligned(p.v, p.dtype, {p.v_layer_stride, p.v_batch_stride, p.v_token_stride, p.v_head_stride}))
+    return fail(ASRATTN_ERR_INVALID, "tensors need 16-byte aligned pointers and strides that are multiples of 16 bytes");
+  if (p.block_table != nullptr &&
+      (p.page_size < 1 || p.num_pages < 0 || p.bt_stride < 1 || (long long)p.max_len_k > p.bt_stride * (long long)p.page_size))
+    return fail(ASRATTN_ERR_INVALID, "a block table takes a page size, a pool and max_len_k within its reach");
+  return from_hip(asrattn::launch_commit(p, static_cast<hipStream_t>(stream)), "asrlayer_commit");
+}
+
+}  // extern "C"

@@ -156,4 +156,30 @@ __device__ __forceinline__ int decode_key_count(const int32_t* seqused, const in
   return (int)n;
 }
 
+// s_waitcnt vmcnt(0) (gfx9 encoding; expcnt and lgkmcnt at their maxima).
+constexpr int kWaitVmem = (0x7 << 4) | (0xF << 8);
+
+// Partials pass between workgroups on different XCDs, whose L2 caches are
+// not coherent: agent-scope accesses go through to memory.
+__device__ __forceinline__ void store_shared(float* p, float x) {
+  __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float load_shared(const float* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// p[0] and p[1], 8-byte aligned.
+__device__ __forceinline__ void load_shared2(const float* p, float& first, float& second) {
+  const float2 v = __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p),
+                                                                __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  first = v.x;
+  second = v.y;
+}
+
+// p[0] = first and p[1] = second, 8-byte aligned.
+__device__ __forceinline__ void store_shared2(float* p, float first, float second) {
+  __hip_atomic_store(reinterpret_cast<unsigned long long*>(p),
+                     __builtin_bit_cast(unsigned long long, make_float2(first, second)), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+
 }  // namespace asrattn

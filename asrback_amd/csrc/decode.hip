@@ -9,8 +9,6 @@
 
 namespace asrattn {
 
-namespace {
-
 // A tag no other launch of this process has had for 2^48 launches, and that
 // neither a count nor a partial left in a reused workspace resembles: a
 // counter from a start set by the clock, its bits mixed by an odd multiplier
@@ -23,8 +21,6 @@ unsigned long long launch_tag() {
   while (tag == 0) tag = (next.fetch_add(1, std::memory_order_relaxed) * 0x9e3779b97f4a7c15ull) & kMask;
   return tag;
 }
-
-}  // namespace
 
 bool decode_supported(int dtype, int head_dim, int group) {
   const bool dt = dtype == ASRATTN_F32 || dtype == ASRATTN_BF16;

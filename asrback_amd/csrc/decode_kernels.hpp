@@ -45,9 +45,6 @@ namespace asrattn {
 namespace {
 
 
-// s_waitcnt vmcnt(0) (gfx9 encoding; expcnt and lgkmcnt at their maxima).
-constexpr int kWaitVmem = (0x7 << 4) | (0xF << 8);
-
 template <typename T, int HD, int G, int W>
 struct DecodeShape {
   static constexpr int kEPL = Elem<T>::kPerVec;   // elements per lane per load
@@ -97,22 +94,6 @@ __device__ __forceinline__ float dot16<bf16_raw>(const uint4& q, const uint4& k)
   acc = __builtin_amdgcn_fdot2_f32_bf16(pair(q.y), pair(k.y), acc, false);
   acc = __builtin_amdgcn_fdot2_f32_bf16(pair(q.z), pair(k.z), acc, false);
   return __builtin_amdgcn_fdot2_f32_bf16(pair(q.w), pair(k.w), acc, false);
-}
-
-// Partials pass between workgroups on different XCDs, whose L2 caches are
-// not coherent: agent-scope accesses go through to memory.
-__device__ __forceinline__ void store_shared(float* p, float x) {
-  __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float load_shared(const float* p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-// p[0] and p[1], 8-byte aligned.
-__device__ __forceinline__ void load_shared2(const float* p, float& first, float& second) {
-  const float2 v = __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p),
-                                                                __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-  first = v.x;
-  second = v.y;
 }
 
 // Online-softmax state of one stream for the G query heads of a kv head.

@@ -77,6 +77,34 @@ hipError_t launch_rows_linear(const asrlayer_linear_params& p, hipStream_t strea
 // Token and position embeddings of a decoder step (asrlayer_embed_rows).
 hipError_t launch_embed_rows(const asrlayer_embed_params& p, hipStream_t stream);
 
+// Attention of drafted trees (asrlayer_tree) over `splits` workgroups per
+// (sequence, kv head, block of query rows); for splits > 1 the workspace holds
+// the partials and an arrival word per such unit, and the split that arrives
+// last folds them.
+struct TreePlan {
+  int row_tiles;   // 16-row tiles a workgroup holds
+  int row_blocks;  // workgroups over a kv head's query rows
+  int splits;
+};
+TreePlan tree_plan(const asrlayer_tree_params& p);
+// The most row tiles a workgroup of this head size takes.
+int tree_most_row_tiles(int head_dim);
+hipError_t launch_tree(const asrlayer_tree_params& p, const TreePlan& plan, float* ws_o, float* ws_ml,
+                       unsigned long long* ws_arrive, hipStream_t stream);
+
+// Drafted trees' masks, walk and commit (asrlayer_tree_masks, asrlayer_accept,
+// asrlayer_commit).
+hipError_t launch_tree_masks(const int64_t* parents, int64_t parents_batch_stride, int64_t batch, int tokens,
+                             int64_t* masks, hipStream_t stream);
+hipError_t launch_accept(const int64_t* tokens, const int64_t* parents, int64_t parents_batch_stride,
+                         const int64_t* choices, const int64_t* limit, int64_t batch, int width, int64_t* path,
+                         int64_t* emitted, int64_t* count, hipStream_t stream);
+hipError_t launch_commit(const asrlayer_commit_params& p, hipStream_t stream);
+
+// A tag for a split launch's arrival words that no other launch of the process
+// has (decode.hip).
+unsigned long long launch_tag();
+
 // A linear layer over bf16 rows (asrlayer_gemm).
 hipError_t launch_gemm(const asrlayer_gemm_params& p, hipStream_t stream);
 

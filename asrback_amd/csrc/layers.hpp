@@ -5,6 +5,7 @@
 // allocation, no synchronization, asrattn_last_error for messages).
 #pragma once
 
+#include <stddef.h>
 #include <stdint.h>
 
 #include "asrattn.h"
@@ -113,5 +114,95 @@ typedef struct asrlayer_gemm_params {
 } asrlayer_gemm_params;
 
 int asrlayer_gemm(const asrlayer_gemm_params* params, void* stream);
+
+// Attention of drafted tokens over a cache and the drafted tokens before them:
+// per sequence b, token t, query head h of kv head h / (heads_q / heads_kv),
+//
+//   s_j  = scale q[b, t, h] . k[b, j]          j < n_b
+//   s'_i = scale q[b, t, h] . k_draft[b, i]    bit i of masks[b, t] set
+//   out[b, t, h] = softmax over both, times v and v_draft
+//
+// n_b = lengths[b] (int32, or int64 with lengths64) clamped to [0, max_len_k].
+// A token with mask 0 is none: its rows are zeros.  Mask bits at tokens and
+// past them count for nothing.  tokens at most 64; q, out (batch, tokens,
+// heads_q, head_dim); k_draft, v_draft (batch, tokens, heads_kv, head_dim);
+// k, v (batch, max_len_k, heads_kv, head_dim), or with a block table pools as
+// asrattn_decode_paged takes them (keys of entries outside the pool are
+// skipped).  head_dim 64, 128 or 256.  The workspace holds the partials of
+// split keys (asrlayer_tree_workspace_size, 256-byte aligned); its contents
+// before the call do not matter, and calls that share it run in stream order.
+typedef struct asrlayer_tree_params {
+  const void *q, *k, *v, *k_draft, *v_draft;
+  void* out;
+  int64_t q_batch_stride, q_token_stride, q_head_stride;
+  int64_t k_batch_stride, k_token_stride, k_head_stride;
+  int64_t v_batch_stride, v_token_stride, v_head_stride;
+  int64_t kd_batch_stride, kd_token_stride, kd_head_stride;
+  int64_t vd_batch_stride, vd_token_stride, vd_head_stride;
+  int64_t o_batch_stride, o_token_stride, o_head_stride;
+  const int64_t* masks;  // (batch, tokens): rows masks_batch_stride apart
+  int64_t masks_batch_stride;
+  const void* lengths;
+  const int32_t* block_table;
+  int64_t bt_stride, k_page_stride, v_page_stride;
+  int32_t page_size, num_pages;
+  int32_t lengths64, batch, tokens, heads_q, heads_kv, head_dim, max_len_k, dtype;
+  float scale;
+} asrlayer_tree_params;
+
+int asrlayer_tree(const asrlayer_tree_params* params, void* workspace, size_t workspace_bytes, void* stream);
+
+// Workspace bytes of these sizes (tensors and strides may be unset): 0 when the
+// call runs unsplit, (size_t)-1 for sizes it does not take; otherwise enough for
+// any smaller batch and fewer tokens as well.
+size_t asrlayer_tree_workspace_size(const asrlayer_tree_params* params);
+
+// Ancestor masks of drafted trees: masks[b, t] has bit t and the bits of t's
+// ancestors.  parents (batch, tokens), rows parents_batch_stride apart: a
+// token before t, or -1 (as is any value from t on) for none; below -1 the
+// token is padding and its mask 0.  tokens at most 64; masks contiguous.
+int asrlayer_tree_masks(const int64_t* parents, int64_t parents_batch_stride, int64_t batch, int32_t tokens,
+                        int64_t* masks, void* stream);
+
+// The walk of a greedy choice down drafted trees, from token 0: the next token
+// is the first one after it whose parent it is and that equals its choice.
+//
+//   path[b, i]    the i-th token of the walk, -1 past its end
+//   emitted[b, i] choices[b, path[b, i]], -1 past its end
+//   count[b]      its length: 0 where limit[b] <= 0 or token 0 is padding
+//                 (parent below -1), else at least 1 and at most limit[b]
+//
+// tokens, choices, path, emitted (batch, width) contiguous; parents rows
+// parents_batch_stride apart; limit (batch) or NULL; width at most 64.
+int asrlayer_accept(const int64_t* tokens, const int64_t* parents, int64_t parents_batch_stride,
+                    const int64_t* choices, const int64_t* limit, int64_t batch, int32_t width, int64_t* path,
+                    int64_t* emitted, int64_t* count, void* stream);
+
+// Accepted tokens' keys and values from the draft buffers into the cache, for
+// every layer l, sequence b and i < count[b]:
+//
+//   k[l, b, lengths[b] + i] = k_draft[l, b, path[b, i]]     and v likewise
+//
+// k, v (layers, batch, max_len_k, heads_kv, head_dim), or with a block table
+// pools (layers, num_pages, page_size, heads_kv, head_dim); drafts (layers,
+// batch, tokens, heads_kv, head_dim).  Positions outside [0, max_len_k) or on
+// no page, and path entries outside [0, tokens), are not written.
+typedef struct asrlayer_commit_params {
+  const void *k_draft, *v_draft;
+  void *k, *v;
+  int64_t kd_layer_stride, kd_batch_stride, kd_token_stride, kd_head_stride;
+  int64_t vd_layer_stride, vd_batch_stride, vd_token_stride, vd_head_stride;
+  // Batch strides are page strides with a block table.
+  int64_t k_layer_stride, k_batch_stride, k_token_stride, k_head_stride;
+  int64_t v_layer_stride, v_batch_stride, v_token_stride, v_head_stride;
+  const int64_t *path, *count;  // (batch, tokens) and (batch), contiguous
+  const void* lengths;
+  const int32_t* block_table;
+  int64_t bt_stride;
+  int32_t page_size, num_pages;
+  int32_t lengths64, layers, batch, tokens, heads_kv, head_dim, max_len_k, dtype;
+} asrlayer_commit_params;
+
+int asrlayer_commit(const asrlayer_commit_params* params, void* stream);
 
 }  // extern "C"

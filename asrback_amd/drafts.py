@@ -1,0 +1,325 @@
+"""Drafted tokens on the HIP kernels of ``libasrattn.so``: verifying a tree of
+them in one pass of a decoder and keeping what the model agrees with.
+
+A drafted tree holds up to :data:`MAX_TOKENS` tokens a row.  Token 0 is the
+row's newest token, the one a plain step would decode next (its key and value
+are not in the cache yet); every other token names its parent, an earlier
+token of the tree.  A pass over all of them costs little more than a plain
+step, which is bound by reading the weights and the cache, and yields as many
+tokens as the longest branch the model's own choices follow:
+
+* :func:`tree_masks` turns parents into ancestor bit masks (once per tree);
+* :func:`tree_attention` attends every drafted token over the cache, which all
+  of them see, and its own ancestors, whose keys and values lie in draft
+  buffers beside the cache;
+* :func:`accept_drafts` walks each tree along the greedy choices;
+* :func:`commit_drafts` writes the accepted tokens' keys and values of every
+  layer from the draft buffers into the cache.
+
+As in :mod:`asrback_amd.attention`, calls launch on the current HIP stream,
+never synchronize, and can be captured into a graph; nothing here has a
+gradient, and calls that would need one are refused.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from .attention import (
+    _DTYPES, PageTable, _aligned, _check_device, _dtype_code, _paged, _ptr, _split_workspace, _stream,
+)
+
+# Tokens of a drafted tree, one bit each of an ancestor mask.
+MAX_TOKENS = 64
+
+_increment_version = torch.autograd.graph.increment_version
+
+
+def _no_gradient(what: str, *tensors: Tensor) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no gradient; call it under torch.no_grad() or on detached tensors")
+
+
+def _int64(t: Tensor, name: str, shape: tuple[int, ...]) -> Tensor:
+    if t.dtype != torch.int64:
+        raise TypeError(f"{name} must be int64, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def _per_tree(t: Tensor, name: str, batch: int, tokens: int) -> tuple[Tensor, int]:
+    """``(tokens,)`` or ``(batch, tokens)`` int64 rows and their batch stride."""
+    if t.dtype != torch.int64:
+        raise TypeError(f"{name} must be int64, got {t.dtype}")
+    if t.shape not in ((tokens,), (batch, tokens)):
+        raise ValueError(f"{name} must be ({tokens},) or ({batch}, {tokens}), got {tuple(t.shape)}")
+    if tokens > 1 and t.stride(-1) != 1:
+        t = t.contiguous()
+    return t, 0 if t.dim() == 1 else t.stride(0)
+
+
+def _tokens(tokens: int) -> None:
+    if not 1 <= tokens <= MAX_TOKENS:
+        raise ValueError(f"a tree has 1 to {MAX_TOKENS} drafted tokens, got {tokens}")
+
+
+def _cuda(device: torch.device, what: str) -> None:
+    if device.type != "cuda":
+        raise RuntimeError(f"{what} runs on the GPU only; got tensors on {device}")
+
+
+def _lengths(lengths: Tensor | None, batch: int) -> Tensor | None:
+    if lengths is None:
+        return None
+    if lengths.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"lengths must be int32 or int64, got {lengths.dtype}")
+    if lengths.shape != (batch,):
+        raise ValueError(f"lengths must be ({batch},), got {tuple(lengths.shape)}")
+    return lengths.contiguous()
+
+
+def tree_masks(parents: Tensor) -> Tensor:
+    """Ancestor masks of drafted trees (``asrlayer_tree_masks``): int64, bit
+    ``i`` of a token's mask set where ``i`` is the token or one of its ancestors.
+
+    ``parents`` int64 ``(tokens,)`` or ``(batch, tokens)``: each token's parent,
+    an earlier token, or -1 where only the cache precedes it (so does a value
+    from the token on); below -1 the token is padding, and its mask 0."""
+    if parents.dtype != torch.int64:
+        raise TypeError(f"parents must be int64, got {parents.dtype}")
+    if parents.dim() not in (1, 2):
+        raise ValueError(f"parents must be (tokens,) or (batch, tokens), got {tuple(parents.shape)}")
+    tokens = parents.shape[-1]
+    _tokens(tokens)
+    batch = parents.shape[0] if parents.dim() == 2 else 1
+    parents, stride = _per_tree(parents, "parents", batch, tokens)
+    device = _check_device(parents)
+    _cuda(device, "tree_masks")
+    masks = torch.empty(parents.shape, dtype=torch.int64, device=device)
+    lib = _lib.load()
+    _lib.check(lib.asrlayer_tree_masks(parents.data_ptr(), stride, batch, tokens, masks.data_ptr(), _stream(device)),
+               "asrlayer_tree_masks")
+    return masks
+
+
+def _tree_sizes(batch: int, tokens: int, heads_q: int, heads_kv: int, head_dim: int, max_len: int, dtype: int,
+                scale: float) -> _lib.TreeParams:
+    params = _lib.TreeParams()
+    params.batch, params.tokens, params.heads_q, params.heads_kv = batch, tokens, heads_q, heads_kv
+    params.head_dim, params.max_len_k, params.dtype, params.scale = head_dim, max_len, dtype, scale
+    return params
+
+
+def tree_attention(
+    q: Tensor,
+    k: Tensor,
+    v: Tensor,
+    k_draft: Tensor,
+    v_draft: Tensor,
+    masks: Tensor,
+    *,
+    lengths: Tensor | None = None,
+    scale: float | None = None,
+    out: Tensor | None = None,
+    workspace: Tensor | None = None,
+    pages: PageTable | None = None,
+) -> Tensor:
+    """Attention of drafted trees over a cache (``asrlayer_tree``).
+
+    ``q`` ``(batch, tokens, heads_q, head_dim)``; ``k``/``v`` ``(batch, length,
+    heads_kv, head_dim)``, any strides with a unit last one (pass
+    ``cache.transpose(1, 2)`` for a ``(batch, heads, length, head_dim)``
+    cache), or with ``pages`` the pools ``(num_pages, page_size, heads_kv,
+    head_dim)``; ``k_draft``/``v_draft`` ``(batch, tokens, heads_kv,
+    head_dim)``, the drafted tokens' own.  Token ``t`` of row ``b`` attends the
+    cache's keys ``0 .. lengths[b] - 1`` (int32 or int64, default: all of
+    them; outside the cache they are clamped to it) and the drafted keys whose
+    bits are set in ``masks[b, t]`` (int64 ``(batch, tokens)``, or ``(tokens,)``
+    for one tree in every row; :func:`tree_masks`).  A token with mask 0 is
+    padding: it attends nothing and gets zeros.
+
+    float32 or bfloat16, head_dim 64, 128 or 256, any number of query heads
+    per kv head, up to :data:`MAX_TOKENS` tokens.  ``workspace``: the split
+    partials' memory (:func:`tree_workspace_size`,
+    :func:`asrback_amd.attention.workspace`).  Returns ``(batch, tokens,
+    heads_q, head_dim)``."""
+    for name, t in (("q", q), ("k", k), ("v", v), ("k_draft", k_draft), ("v_draft", v_draft)):
+        if t.dim() != 4:
+            raise ValueError(f"{name} must have 4 dimensions, got shape {tuple(t.shape)}")
+    batch, tokens, heads_q, head_dim = q.shape
+    heads_kv = k.shape[2]
+    if v.shape != k.shape or k.shape[3] != head_dim:
+        raise ValueError(f"k and v must share one shape with q's head_dim {head_dim}; got {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}")
+    if pages is None and k.shape[0] != batch:
+        raise ValueError(f"q has {batch} rows, the cache {k.shape[0]}")
+    if heads_kv == 0 or heads_q % heads_kv or heads_q == 0:
+        raise ValueError(f"{heads_q} query heads are not a positive multiple of {heads_kv} kv heads")
+    for name, t in (("k_draft", k_draft), ("v_draft", v_draft)):
+        if t.shape != (batch, tokens, heads_kv, head_dim):
+            raise ValueError(f"{name} must be ({batch}, {tokens}, {heads_kv}, {head_dim}), got {tuple(t.shape)}")
+    _tokens(tokens)
+    masks, masks_stride = _per_tree(masks, "masks", batch, tokens)
+    lengths = _lengths(lengths, batch)
+    dtype = _dtype_code(q, k, v, k_draft, v_draft)
+    _no_gradient("tree_attention", q, k, v, k_draft, v_draft)
+    q, k_draft, v_draft = _aligned(q), _aligned(k_draft), _aligned(v_draft)
+    k, v = _aligned(k), _aligned(v)
+    if out is None:
+        out = torch.empty((batch, tokens, heads_q, head_dim), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(-1) != 1:
+        raise ValueError("out must match q's shape and dtype, with a unit last stride")
+    device = _check_device(q, k, v, k_draft, v_draft, masks, lengths, out, None if pages is None else pages.block_table)
+    params = _tree_sizes(batch, tokens, heads_q, heads_kv, head_dim, k.shape[1], dtype,
+                         1.0 / math.sqrt(head_dim) if scale is None else scale)
+    params.q, params.k, params.v, params.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    params.k_draft, params.v_draft = k_draft.data_ptr(), v_draft.data_ptr()
+    params.q_batch_stride, params.q_token_stride, params.q_head_stride, _ = q.stride()
+    params.k_batch_stride, params.k_token_stride, params.k_head_stride, _ = k.stride()
+    params.v_batch_stride, params.v_token_stride, params.v_head_stride, _ = v.stride()
+    params.kd_batch_stride, params.kd_token_stride, params.kd_head_stride, _ = k_draft.stride()
+    params.vd_batch_stride, params.vd_token_stride, params.vd_head_stride, _ = v_draft.stride()
+    params.o_batch_stride, params.o_token_stride, params.o_head_stride, _ = out.stride()
+    params.masks, params.masks_batch_stride = masks.data_ptr(), masks_stride
+    if lengths is not None:
+        params.lengths, params.lengths64 = lengths.data_ptr(), int(lengths.dtype == torch.int64)
+    if pages is not None:
+        pk, params.max_len_k = _paged(pages, k, v, batch)
+        params.block_table, params.bt_stride = pk.block_table, pk.bt_stride
+        params.page_size, params.num_pages = pk.page_size, pk.num_pages
+        params.k_page_stride, params.v_page_stride = pk.k_page_stride, pk.v_page_stride
+        params.k_batch_stride = params.v_batch_stride = 0
+    lib = _lib.load()
+    workspace = _split_workspace(lib.asrlayer_tree_workspace_size(ctypes.byref(params)), workspace, device)
+    size = 0 if workspace is None else workspace.numel()
+    _lib.check(lib.asrlayer_tree(ctypes.byref(params), _ptr(workspace), size, _stream(device)), "asrlayer_tree")
+    return out
+
+
+def tree_workspace_size(batch: int, tokens: int, heads_q: int, heads_kv: int, head_dim: int, max_len: int,
+                        dtype: torch.dtype = torch.bfloat16) -> int:
+    """Bytes of split partials a :func:`tree_attention` call of these sizes
+    needs (``asrlayer_tree_workspace_size``; 0 when it runs unsplit): where it
+    is not 0, enough for every smaller batch and fewer tokens over the same
+    cache.  Raises for sizes the library does not take."""
+    if dtype not in _DTYPES:
+        raise TypeError(f"attention supports float32 and bfloat16, got {dtype}")
+    params = _tree_sizes(batch, tokens, heads_q, heads_kv, head_dim, max_len, _DTYPES[dtype], 1.0)
+    lib = _lib.load()
+    need = lib.asrlayer_tree_workspace_size(ctypes.byref(params))
+    if need == ctypes.c_size_t(-1).value:
+        raise ValueError(lib.asrattn_last_error().decode("utf-8", "replace"))
+    return int(need)
+
+
+def accept_drafts(tokens: Tensor, parents: Tensor, choices: Tensor,
+                  limit: Tensor | None = None) -> tuple[Tensor, Tensor, Tensor]:
+    """The walk of the model's choices down drafted trees
+    (``asrlayer_accept``).
+
+    ``tokens`` int64 ``(batch, width)`` are the drafted tokens, ``choices``
+    int64 ``(batch, width)`` the token the model puts after each of them
+    (:func:`~asrback_amd.attention.greedy_choice` of its logits), ``parents``
+    as for :func:`tree_masks`.  Token 0 is accepted; after each accepted token
+    comes the first one behind it whose parent it is and that equals its
+    choice.  Returns int64 ``path`` ``(batch, width)``, the accepted tokens'
+    indices, ``emitted`` ``(batch, width)``, the choice after each of them (the
+    tokens this pass generated), both -1 past the walk's end, and ``count``
+    ``(batch,)``, its length.  ``limit`` int64 ``(batch,)`` caps it; rows with
+    a limit below 1, or whose token 0 is padding, accept nothing."""
+    if tokens.dim() != 2:
+        raise ValueError(f"tokens must be (batch, width), got {tuple(tokens.shape)}")
+    batch, width = tokens.shape
+    _tokens(width)
+    tokens = _int64(tokens, "tokens", (batch, width))
+    choices = _int64(choices, "choices", (batch, width))
+    parents, stride = _per_tree(parents, "parents", batch, width)
+    if limit is not None:
+        limit = _int64(limit, "limit", (batch,))
+    device = _check_device(tokens, parents, choices, limit)
+    _cuda(device, "accept_drafts")
+    path, emitted = torch.empty_like(tokens), torch.empty_like(tokens)
+    count = torch.empty(batch, dtype=torch.int64, device=device)
+    lib = _lib.load()
+    _lib.check(
+        lib.asrlayer_accept(tokens.data_ptr(), parents.data_ptr(), stride, choices.data_ptr(), _ptr(limit), batch, width,
+                            path.data_ptr(), emitted.data_ptr(), count.data_ptr(), _stream(device)),
+        "asrlayer_accept",
+    )
+    return path, emitted, count
+
+
+def commit_drafts(
+    keys: Tensor,
+    values: Tensor,
+    k_draft: Tensor,
+    v_draft: Tensor,
+    path: Tensor,
+    count: Tensor,
+    lengths: Tensor,
+    *,
+    pages: PageTable | None = None,
+) -> None:
+    """Write accepted drafts into the cache, every layer in one launch
+    (``asrlayer_commit``): position ``lengths[b] + i`` of row ``b`` gets the key
+    and value of drafted token ``path[b, i]``, for ``i < count[b]``.
+
+    ``keys``/``values`` ``(layers, batch, length, heads_kv, head_dim)``, or with
+    ``pages`` pools ``(layers, num_pages, page_size, heads_kv, head_dim)``, are
+    written in place (any strides of whole 16-byte vectors, the last one unit);
+    ``k_draft``/``v_draft`` ``(layers, batch, tokens, heads_kv, head_dim)`` must
+    not share memory with them.  ``path`` int64 ``(batch, tokens)`` and
+    ``count`` int64 ``(batch,)`` come from :func:`accept_drafts`; ``lengths``
+    int32 or int64 ``(batch,)`` are the rows' keys before the call.  Positions
+    outside the cache or on no page are left alone, as are path entries outside
+    the tree."""
+    for name, t in (("keys", keys), ("values", values), ("k_draft", k_draft), ("v_draft", v_draft)):
+        if t.dim() != 5:
+            raise ValueError(f"{name} must have 5 dimensions, got shape {tuple(t.shape)}")
+    layers, batch, tokens, heads_kv, head_dim = k_draft.shape
+    if v_draft.shape != k_draft.shape:
+        raise ValueError(f"k_draft and v_draft shapes differ: {tuple(k_draft.shape)}, {tuple(v_draft.shape)}")
+    if values.shape != keys.shape or keys.shape[0] != layers or keys.shape[3:] != (heads_kv, head_dim):
+        raise ValueError(f"keys and values must share one shape with {layers} layers of ({heads_kv}, {head_dim}); got "
+                         f"{tuple(keys.shape)}, {tuple(values.shape)}")
+    if pages is None and keys.shape[1] != batch:
+        raise ValueError(f"the drafts have {batch} rows, the cache {keys.shape[1]}")
+    _tokens(tokens)
+    path = _int64(path, "path", (batch, tokens))
+    count = _int64(count, "count", (batch,))
+    if lengths is None:
+        raise TypeError("lengths must be a tensor")
+    lengths = _lengths(lengths, batch)
+    dtype = _dtype_code(keys, values, k_draft, v_draft)
+    _no_gradient("commit_drafts", keys, values, k_draft, v_draft)
+    if not torch.is_inference_mode_enabled() and (keys.is_inference() or values.is_inference()):
+        raise RuntimeError("inplace update to inference tensors outside InferenceMode is not allowed")
+    for name, t in (("keys", keys), ("values", values)):
+        if t.numel() and _aligned(t) is not t:
+            raise ValueError(f"{name} needs a unit last stride and 16-byte aligned rows (it is written in place)")
+    k_draft, v_draft = _aligned(k_draft), _aligned(v_draft)
+    device = _check_device(keys, values, k_draft, v_draft, path, count, lengths,
+                           None if pages is None else pages.block_table)
+    params = _lib.CommitParams()
+    params.k_draft, params.v_draft = k_draft.data_ptr(), v_draft.data_ptr()
+    params.k, params.v = keys.data_ptr(), values.data_ptr()
+    for prefix, t in (("kd", k_draft), ("vd", v_draft), ("k", keys), ("v", values)):
+        for axis, stride in zip(("layer", "batch", "token", "head"), t.stride()):
+            setattr(params, f"{prefix}_{axis}_stride", stride)
+    params.path, params.count = path.data_ptr(), count.data_ptr()
+    params.lengths, params.lengths64 = lengths.data_ptr(), int(lengths.dtype == torch.int64)
+    params.layers, params.batch, params.tokens, params.heads_kv = layers, batch, tokens, heads_kv
+    params.head_dim, params.max_len_k, params.dtype = head_dim, keys.shape[2], dtype
+    if pages is not None:
+        pk, params.max_len_k = _paged(pages, keys[0], values[0], batch) if layers else (_lib.PagedKV(), 0)
+        params.block_table, params.bt_stride = pk.block_table, pk.bt_stride
+        params.page_size, params.num_pages = pk.page_size, pk.num_pages
+    lib = _lib.load()
+    _lib.check(lib.asrlayer_commit(ctypes.byref(params), _stream(device)), "asrlayer_commit")
+    _increment_version((keys, values))
