@@ -307,8 +307,22 @@ class CommitParams(ctypes.Structure):
     ]
 
 
+class Linear4Params(ctypes.Structure):
+    """``asrlayer_linear4_params`` (csrc/layers.hpp)."""
+
+    _fields_ = [
+        ("x", _ptr),
+        ("x_row_stride", _i64),
+        *[(name, _ptr) for name in ("packed", "scales", "zeros", "bias", "out")],
+        ("out_row_stride", _i64),
+        ("rows", _i64),
+        *[(name, _i32) for name in ("n", "k", "group", "dtype")],
+    ]
+
+
 # The layers' own entry points (csrc/layers.hpp).
 LAYER_SIGNATURES = {
+    "asrlayer_linear4": (ctypes.c_int, [ctypes.POINTER(Linear4Params), _ptr]),
     "asrlayer_tree": (ctypes.c_int, [ctypes.POINTER(TreeParams), _ptr, ctypes.c_size_t, _ptr]),
     "asrlayer_tree_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(TreeParams)]),
     "asrlayer_tree_masks": (ctypes.c_int, [_ptr, _i64, _i64, _i32, _ptr, _ptr]),

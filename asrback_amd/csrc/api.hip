@@ -726,4 +726,24 @@ int asrlayer_commit(const asrlayer_commit_params* params, void* stream) {
   return from_hip(asrattn::launch_commit(p, static_cast<hipStream_t>(stream)), "asrlayer_commit");
 }
 
+int asrlayer_linear4(const asrlayer_linear4_params* params, void* stream) {
+  if (params == nullptr) return fail(ASRATTN_ERR_INVALID, "params is NULL");
+  const asrlayer_linear4_params& p = *params;
+  if (p.dtype != ASRATTN_F32 && p.dtype != ASRATTN_BF16) return fail(ASRATTN_ERR_INVALID, "dtype %d", p.dtype);
+  if (p.rows < 0 || p.n < 1 || p.k < 1)
+    return fail(ASRATTN_ERR_INVALID, "rows must be >= 0, n and k positive");
+  if (p.group != 32 && p.group != 64 && p.group != 128)
+    return fail(ASRATTN_ERR_UNSUPPORTED, "group %d (supported: 32, 64, 128)", p.group);
+  if (p.k % p.group != 0) return fail(ASRATTN_ERR_INVALID, "k (%d) is not a multiple of group (%d)", p.k, p.group);
+  if (p.n > (1 << 28) || p.k > (1 << 24) || p.rows > (1LL << 20))
+    return fail(ASRATTN_ERR_UNSUPPORTED, "more than 2^20 rows, 2^28 outputs or 2^24 inputs");
+  if (p.rows == 0) return ok();
+  if (p.x == nullptr || p.packed == nullptr || p.scales == nullptr || p.out == nullptr)
+    return fail(ASRATTN_ERR_INVALID, "x, packed, scales and out must be non-NULL");
+  if (!vec_aligned(p.x, p.dtype, {p.x_row_stride}) || !vec_aligned(p.packed, p.dtype, {}) ||
+      !vec_aligned(p.scales, p.dtype, {}) || !vec_aligned(p.zeros, p.dtype, {}))
+    return fail(ASRATTN_ERR_INVALID, "x, packed, scales and zeros need 16-byte aligned pointers and rows");
+  return from_hip(asrattn::launch_linear4(p, static_cast<hipStream_t>(stream)), "asrlayer_linear4");
+}
+
 }  // extern "C"

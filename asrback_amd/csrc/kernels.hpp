@@ -101,6 +101,9 @@ hipError_t launch_accept(const int64_t* tokens, const int64_t* parents, int64_t 
                          int64_t* emitted, int64_t* count, hipStream_t stream);
 hipError_t launch_commit(const asrlayer_commit_params& p, hipStream_t stream);
 
+// Rows through a matrix of 4-bit weights (asrlayer_linear4).
+hipError_t launch_linear4(const asrlayer_linear4_params& p, hipStream_t stream);
+
 // A tag for a split launch's arrival words that no other launch of the process
 // has (decode.hip).
 unsigned long long launch_tag();

@@ -205,4 +205,29 @@ typedef struct asrlayer_commit_params {
 
 int asrlayer_commit(const asrlayer_commit_params* params, void* stream);
 
+// Rows through a matrix of 4-bit weights with group scales:
+//
+//   out[r, n] = sum_k x[r, k] scale[n, k / group] (q[n, k] - zero[n, k / group]) (+ bias[n])
+//
+// q and zero in 0 .. 15 (zeros NULL: 8), sums in float32, rounded once.  x
+// rows x_row_stride apart; out rows out_row_stride apart; scales and bias in
+// x's type; group 32, 64 or 128, k a multiple of it.  The matrix lies in blocks
+// of 16 outputs by 128 inputs, padded to whole blocks (scales of padding 0):
+//
+//   packed (n / 16, k / 128, 64, 4) dwords: dword s of lane 16 g + i holds
+//     output i's inputs 32 s + 8 g + j, j = 0 2 4 6 1 3 5 7 from the low nibble up
+//   scales (n / 16, k / group, 16)
+//   zeros  (n / 16, k / group, 8) bytes: output i in nibble i
+typedef struct asrlayer_linear4_params {
+  const void* x;
+  int64_t x_row_stride;
+  const void *packed, *scales, *zeros, *bias;
+  void* out;
+  int64_t out_row_stride;
+  int64_t rows;
+  int32_t n, k, group, dtype;
+} asrlayer_linear4_params;
+
+int asrlayer_linear4(const asrlayer_linear4_params* params, void* stream);
+
 }  // extern "C"

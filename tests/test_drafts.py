@@ -157,7 +157,8 @@ def test_library_refuses(lib):
     assert lib.asrlayer_commit(ctypes.byref(c), None) == _lib.ERR_UNSUPPORTED
 
 
-@pytest.mark.parametrize("name,struct", [("TreeParams", "asrlayer_tree_params"), ("CommitParams", "asrlayer_commit_params")])
+@pytest.mark.parametrize("name,struct", [("TreeParams", "asrlayer_tree_params"), ("CommitParams", "asrlayer_commit_params"),
+                                         ("Linear4Params", "asrlayer_linear4_params")])
 def test_structs_match_the_header(name, struct, tmp_path):
     from asrback_amd import _lib
 

@@ -1,0 +1,170 @@
+"""GPU: linear layers with 4-bit weights.
+
+Integers and powers of two make every sum exact in float32, so those cases ask
+for the exact result, rounded once.  Real values are held to what the kernel
+rounds: the result once (2^-8 of it in bf16, 2^-24 in float32), and its float32
+sums: per output at most 2^-24 c sum |x| |scale| times the values an operand and
+its offset reach (bf16: 2 x 143, float32: 2 x 15), c the additions on a value's way
+(twice the group's, one a group, the waves').
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def say(*args):
+    print(*args, flush=True)
+
+
+def quantized(outputs, inputs, group, zeros, dtype, g, powers=False):
+    values = torch.randint(0, 16, (outputs, inputs), generator=g, dtype=torch.uint8)
+    shape = (outputs, inputs // group)
+    if powers:
+        scales = 2.0 ** -torch.randint(0, 4, shape, generator=g).float()
+    else:
+        scales = torch.rand(shape, generator=g) * 0.02 + 0.01
+    points = torch.randint(0, 16, shape, generator=g, dtype=torch.uint8) if zeros else None
+    return values, scales.to(dtype), points
+
+
+def matrix(values, scales, points, group):
+    spread = lambda t: t.double().repeat_interleave(group, 1)  # noqa: E731
+    return (values.double() - (8.0 if points is None else spread(points))) * spread(scales)
+
+
+SHAPES = [
+    # rows, inputs, outputs, group
+    (1, 32, 1, 32), (1, 2048, 2048, 128), (2, 64, 15, 64), (3, 384, 1536, 32), (5, 96, 17, 32), (7, 192, 33, 64),
+    (16, 2048, 300, 128), (17, 1024, 40, 64), (31, 1280, 100, 32), (33, 640, 24, 128), (48, 6144, 64, 64),
+    (64, 2048, 10000, 128), (65, 256, 31, 128), (130, 1152, 50, 32), (4, 16896, 40, 128), (1, 5120, 9, 32),
+    (20, 4224, 21, 128), (300, 2048, 96, 64),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,inputs,outputs,group", SHAPES)
+def test_exact_on_integers(dtype, rows, inputs, outputs, group):
+    from asrback_amd.linear4 import linear4, pack4, unpack4
+
+    g = torch.Generator().manual_seed(rows * 7 + inputs)
+    for zeros, bias in ((False, False), (True, True)):
+        say("linear4", dtype, rows, inputs, outputs, group, zeros, bias)
+        values, scales, points = quantized(outputs, inputs, group, zeros, dtype, g, powers=True)
+        weight = pack4(values.cuda(), scales.cuda(), None if points is None else points.cuda())
+        w = matrix(values, scales, points, group)
+        assert torch.equal(unpack4(weight).cpu().double(), w)
+        x = torch.randint(-4, 5, (rows, inputs), generator=g).to(dtype)
+        b = torch.randint(-9, 10, (outputs,), generator=g).to(dtype) if bias else None
+        out = linear4(x.cuda(), weight, None if b is None else b.cuda())
+        ref = x.double() @ w.T
+        if bias:
+            ref = ref + b.double()
+        assert torch.equal(out.cpu(), ref.to(dtype))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,inputs,outputs,group", SHAPES[1::3] + [(3, 2048, 151936, 128)])
+def test_real_values(dtype, rows, inputs, outputs, group):
+    from asrback_amd.linear4 import linear4, pack4
+
+    g = torch.Generator().manual_seed(rows * 11 + inputs)
+    zeros = rows % 2 == 1
+    say("linear4 real", dtype, rows, inputs, outputs, group)
+    values, scales, points = quantized(outputs, inputs, group, zeros, dtype, g)
+    weight = pack4(values.cuda(), scales.cuda(), None if points is None else points.cuda())
+    x = torch.randn(rows, inputs, generator=g).to(dtype)
+    out = linear4(x.cuda(), weight).cpu().double()
+    at = torch.arange(outputs)[:: max(1, outputs // 500)]
+    points = None if points is None else points[at]
+    ref = x.double() @ matrix(values[at], scales[at], points, group).T
+    sums = x.double().abs() @ scales[at].double().repeat_interleave(group, 1).T
+    reach, step = (286, 2.0**-8) if dtype == BF16 else (30, 2.0**-24)
+    bound = step * ref.abs() + 2.0**-24 * (2 * group + inputs // group + 32) * reach * sums
+    assert ((out[:, at] - ref).abs() <= bound).all()
+    # Far closer in the mean: the sums' errors do not add up.
+    norm = float((out[:, at] - ref).norm() / ref.norm())
+    assert norm < (2.0**-8 if dtype == BF16 else 2.0**-18), norm
+
+
+def test_layouts_of_x_out_and_other_rows():
+    """Leading dimensions, strided and misaligned rows, a given out, no rows; rows
+    do not touch each other, NaN and infinities included."""
+    from asrback_amd.linear4 import linear4, pack4
+
+    g = torch.Generator().manual_seed(3)
+    values, scales, points = quantized(70, 256, 64, True, BF16, g, powers=True)
+    weight = pack4(values.cuda(), scales.cuda(), points.cuda())
+    w = matrix(values, scales, points, 64)
+    say("layouts")
+    wide = torch.randint(-4, 5, (3, 5, 600), generator=g).to(BF16).cuda()
+    for x in (wide[..., :256], wide[..., 8:264], wide[..., 3:259], wide[:, ::2, 256:512], wide[1, 1, :256],
+              wide[:, :, :256].transpose(0, 1)):
+        ref = (x.double().cpu() @ w.T).to(BF16)
+        assert torch.equal(linear4(x, weight).cpu(), ref)
+        out = torch.full(ref.shape, 7.0, dtype=BF16, device="cuda")
+        assert linear4(x, weight, out=out) is out and torch.equal(out.cpu(), ref)
+    assert linear4(wide[:0, :, :256], weight).shape == (0, 5, 70)
+    say("rows apart")
+    x = wide[0, :, :256].clone()
+    x[1] = float("nan")
+    x[3, 5] = float("inf")
+    out = linear4(x, weight).cpu()
+    keep = [0, 2, 4]
+    assert torch.equal(out[keep], (x[keep].double().cpu() @ w.T).to(BF16))
+    assert out[1].isnan().all() and not out[3].isfinite().any()
+
+
+def test_graph_replays_and_module():
+    from asrback_amd.linear4 import Linear4, linear4, quantize4, quantize_linears, unpack4
+
+    g = torch.Generator().manual_seed(4)
+    model = torch.nn.Sequential(torch.nn.Linear(256, 130), torch.nn.Sequential(torch.nn.Linear(130, 8),
+                                torch.nn.Linear(8, 128, bias=False)), torch.nn.Linear(128, 64, bias=False))
+    model = model.to("cuda", BF16)
+    first, last = model[0], model[2]
+    with torch.no_grad():
+        for symmetric in (True, False):
+            for layer in (first, last):
+                weight = quantize4(layer.weight, 64, symmetric)
+                step = weight.scales.float().max()
+                # Half a step of the group's scale, another half where the zero point is
+                # rounded as well, and the scale's own rounding (2^-8) at the ends, 7 or
+                # 15 steps out.
+                assert float((unpack4(weight) - layer.weight.float()).abs().max()) <= float(step) * (0.5 + 7 * 2**-8 if symmetric else 1 + 15 * 2**-8)
+    say("module")
+    assert quantize_linears(model, 64) == 2
+    assert type(model[0]) is Linear4 and type(model[2]) is Linear4 and type(model[1][0]) is torch.nn.Linear
+    assert torch.equal(model[0].bias, first.bias)
+    x = torch.randn(6, 256, generator=g).to("cuda", BF16)
+    with torch.no_grad():
+        got = model[0](x)
+        want = (x.double().cpu() @ unpack4(model[0].weight4).double().cpu().T) + first.bias.double().cpu()
+        assert float((got.double().cpu() - want).norm() / want.norm()) < 2.0**-8
+    # State dicts and devices.
+    other = Linear4(quantize4(torch.zeros(130, 256, dtype=BF16), 64), torch.zeros(130, dtype=BF16)).cuda()
+    other.load_state_dict(model[0].state_dict())
+    with torch.no_grad():
+        assert torch.equal(other(x), got)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        model[0](x.requires_grad_())
+    say("graph")
+    static = torch.empty(6, 256, dtype=BF16, device="cuda")
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            model[0](static)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = model[0](static)
+        for _ in range(4):
+            static.copy_(torch.randn(6, 256, generator=g))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, linear4(static, model[0].weight4, model[0].bias))
