@@ -325,7 +325,7 @@ LAYER_SIGNATURES = {
     "asrlayer_linear4": (ctypes.c_int, [ctypes.POINTER(Linear4Params), _ptr]),
     "asrlayer_tree": (ctypes.c_int, [ctypes.POINTER(TreeParams), _ptr, ctypes.c_size_t, _ptr]),
     "asrlayer_tree_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(TreeParams)]),
-    "asrlayer_tree_masks": (ctypes.c_int, [_ptr, _i64, _i64, _i32, _ptr, _ptr]),
+    "asrlayer_tree_masks": (ctypes.c_int, [_ptr, _i64, _i64, _i32, _ptr, _ptr, _ptr]),
     "asrlayer_accept": (ctypes.c_int, [_ptr, _ptr, _i64, _ptr, _ptr, _i64, _i32, _ptr, _ptr, _ptr, _ptr]),
     "asrlayer_commit": (ctypes.c_int, [ctypes.POINTER(CommitParams), _ptr]),
     "asrlayer_embed_rows": (ctypes.c_int, [ctypes.POINTER(EmbedParams), _ptr]),

@@ -672,13 +672,14 @@ int asrlayer_tree(const asrlayer_tree_params* params, void* workspace, size_t wo
 }
 
 int asrlayer_tree_masks(const int64_t* parents, int64_t parents_batch_stride, int64_t batch, int32_t tokens,
-                        int64_t* masks, void* stream) {
+                        int64_t* masks, int64_t* depths, void* stream) {
   if (tokens < 1 || tokens > 64)
     return fail(ASRATTN_ERR_UNSUPPORTED, "a tree has 1 to 64 drafted tokens, got %d", tokens);
   if (batch < 0 || batch > 0x7fffffffLL) return fail(ASRATTN_ERR_INVALID, "batch (%lld) out of range", (long long)batch);
   if (batch == 0) return ok();
-  if (parents == nullptr || masks == nullptr) return fail(ASRATTN_ERR_INVALID, "parents and masks must be non-NULL");
-  return from_hip(asrattn::launch_tree_masks(parents, parents_batch_stride, batch, tokens, masks,
+  if (parents == nullptr || masks == nullptr || depths == nullptr)
+    return fail(ASRATTN_ERR_INVALID, "parents, masks and depths must be non-NULL");
+  return from_hip(asrattn::launch_tree_masks(parents, parents_batch_stride, batch, tokens, masks, depths,
                                              static_cast<hipStream_t>(stream)),
                   "asrlayer_tree_masks");
 }

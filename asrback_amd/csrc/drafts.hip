@@ -12,7 +12,7 @@ namespace {
 // mask is final once lane t - 1's is: a scan over the lanes, each step one lane
 // read.
 __global__ __launch_bounds__(64) void tree_masks_kernel(const int64_t* parents, int64_t parents_batch_stride, int tokens,
-                                                        int64_t* masks) {
+                                                        int64_t* masks, int64_t* depths) {
   const int64_t b = blockIdx.x;
   const int lane = threadIdx.x;
   const int64_t parent = parents[b * parents_batch_stride + min(lane, tokens - 1)];
@@ -25,7 +25,10 @@ __global__ __launch_bounds__(64) void tree_masks_kernel(const int64_t* parents, 
     const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(mask >> 32), from);
     if (lane == t) mask |= (uint64_t)hi << 32 | lo;
   }
-  if (lane < tokens) masks[b * tokens + lane] = (int64_t)mask;
+  if (lane < tokens) {
+    masks[b * tokens + lane] = (int64_t)mask;
+    depths[b * tokens + lane] = max((int)__popcll(mask) - 1, 0);
+  }
 }
 
 // A wave per tree: lane j holds token j.  Each step is one comparison on all
@@ -99,9 +102,9 @@ __global__ __launch_bounds__(256) void commit_kernel(const asrlayer_commit_param
 }  // namespace
 
 hipError_t launch_tree_masks(const int64_t* parents, int64_t parents_batch_stride, int64_t batch, int tokens,
-                             int64_t* masks, hipStream_t stream) {
+                             int64_t* masks, int64_t* depths, hipStream_t stream) {
   hipLaunchKernelGGL(tree_masks_kernel, dim3((unsigned)batch), dim3(64), 0, stream, parents, parents_batch_stride, tokens,
-                     masks);
+                     masks, depths);
   return hipGetLastError();
 }
 

@@ -95,7 +95,7 @@ hipError_t launch_tree(const asrlayer_tree_params& p, const TreePlan& plan, floa
 // Drafted trees' masks, walk and commit (asrlayer_tree_masks, asrlayer_accept,
 // asrlayer_commit).
 hipError_t launch_tree_masks(const int64_t* parents, int64_t parents_batch_stride, int64_t batch, int tokens,
-                             int64_t* masks, hipStream_t stream);
+                             int64_t* masks, int64_t* depths, hipStream_t stream);
 hipError_t launch_accept(const int64_t* tokens, const int64_t* parents, int64_t parents_batch_stride,
                          const int64_t* choices, const int64_t* limit, int64_t batch, int width, int64_t* path,
                          int64_t* emitted, int64_t* count, hipStream_t stream);

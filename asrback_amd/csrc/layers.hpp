@@ -160,9 +160,10 @@ size_t asrlayer_tree_workspace_size(const asrlayer_tree_params* params);
 // Ancestor masks of drafted trees: masks[b, t] has bit t and the bits of t's
 // ancestors.  parents (batch, tokens), rows parents_batch_stride apart: a
 // token before t, or -1 (as is any value from t on) for none; below -1 the
-// token is padding and its mask 0.  tokens at most 64; masks contiguous.
+// token is padding and its mask 0.  depths[b, t] counts t's ancestors (0 for
+// padding).  tokens at most 64; masks and depths contiguous.
 int asrlayer_tree_masks(const int64_t* parents, int64_t parents_batch_stride, int64_t batch, int32_t tokens,
-                        int64_t* masks, void* stream);
+                        int64_t* masks, int64_t* depths, void* stream);
 
 // The walk of a greedy choice down drafted trees, from token 0: the next token
 // is the first one after it whose parent it is and that equals its choice.

@@ -84,13 +84,15 @@ def _lengths(lengths: Tensor | None, batch: int) -> Tensor | None:
     return lengths.contiguous()
 
 
-def tree_masks(parents: Tensor) -> Tensor:
-    """Ancestor masks of drafted trees (``asrlayer_tree_masks``): int64, bit
-    ``i`` of a token's mask set where ``i`` is the token or one of its ancestors.
+def tree_masks(parents: Tensor) -> tuple[Tensor, Tensor]:
+    """Ancestor masks of drafted trees and their tokens' depths
+    (``asrlayer_tree_masks``), int64 of the shape of ``parents``: bit ``i`` of a
+    token's mask is set where ``i`` is the token or one of its ancestors, its
+    depth is how many ancestors it has (its position behind the cache).
 
     ``parents`` int64 ``(tokens,)`` or ``(batch, tokens)``: each token's parent,
     an earlier token, or -1 where only the cache precedes it (so does a value
-    from the token on); below -1 the token is padding, and its mask 0."""
+    from the token on); below -1 the token is padding, and its mask and depth 0."""
     if parents.dtype != torch.int64:
         raise TypeError(f"parents must be int64, got {parents.dtype}")
     if parents.dim() not in (1, 2):
@@ -102,10 +104,11 @@ def tree_masks(parents: Tensor) -> Tensor:
     device = _check_device(parents)
     _cuda(device, "tree_masks")
     masks = torch.empty(parents.shape, dtype=torch.int64, device=device)
+    depths = torch.empty_like(masks)
     lib = _lib.load()
-    _lib.check(lib.asrlayer_tree_masks(parents.data_ptr(), stride, batch, tokens, masks.data_ptr(), _stream(device)),
-               "asrlayer_tree_masks")
-    return masks
+    _lib.check(lib.asrlayer_tree_masks(parents.data_ptr(), stride, batch, tokens, masks.data_ptr(), depths.data_ptr(),
+                                       _stream(device)), "asrlayer_tree_masks")
+    return masks, depths
 
 
 def _tree_sizes(batch: int, tokens: int, heads_q: int, heads_kv: int, head_dim: int, max_len: int, dtype: int,

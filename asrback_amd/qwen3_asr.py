@@ -24,10 +24,15 @@ decode loop around them (``DecodeState``, ``choose``, ``TextGreedyDecoder``:
   rows hold the pages their prompt and generation limit need.  Its layers
   index like the slab (``keys[rows, positions] = k``), so the attention
   modules take either cache.
+* Drafted tokens, which the reference has not: ``verify`` of ``TextAttention``,
+  ``TextModel`` and ``TextGreedyDecoder`` runs a tree of them through the model
+  in one pass (:mod:`asrback_amd.drafts`) and keeps those that greedy steps
+  would have produced.
 """
 
 from __future__ import annotations
 
+import contextlib
 from dataclasses import dataclass
 from typing import Callable
 
@@ -38,7 +43,9 @@ from torch import Tensor, nn
 
 from . import attention
 from .attention import KeyPrefix, PageTable, decode, decode_append, greedy_choice, varlen_attn
+from .drafts import MAX_TOKENS, accept_drafts, commit_drafts, tree_attention, tree_masks, tree_workspace_size
 from .layers import computes, prompt_rows, prompt_rows_takes
+from .linear4 import Linear4
 from .transcription import CapturedGraph, to_device
 
 # Positions per row of the KV cache (qwen3_asr.py:57-59).
@@ -236,6 +243,32 @@ class PagedKVCache:
         self.free_pages.extend(reversed(pages))
 
 
+@dataclass
+class DraftCache:
+    """Keys and values of drafted tokens, ``(layers, batch, tokens, kv_heads,
+    head_dim)`` each, beside the cache that takes the accepted ones."""
+
+    keys: Tensor
+    values: Tensor
+
+    @classmethod
+    def allocate(cls, config: dict, batch: int, tokens: int, device, dtype) -> DraftCache:
+        shape = (config["num_hidden_layers"], batch, tokens, config["num_key_value_heads"], config["head_dim"])
+        return cls(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
+
+    def narrow(self, batch_size: int, tokens: int) -> DraftCache:
+        return DraftCache(self.keys[:, :batch_size, :tokens], self.values[:, :batch_size, :tokens])
+
+    def commit(self, cache: KVCache | PagedKVCache, path: Tensor, count: Tensor, lengths: Tensor) -> None:
+        """Write the accepted tokens into ``cache``
+        (:func:`~asrback_amd.drafts.commit_drafts`)."""
+        if isinstance(cache, PagedKVCache):
+            pages = PageTable(cache.block_table, CACHE_LENGTH)
+            commit_drafts(cache.pool_keys, cache.pool_values, self.keys, self.values, path, count, lengths, pages=pages)
+        else:
+            commit_drafts(cache.keys, cache.values, self.keys, self.values, path, count, lengths)
+
+
 def _cache_layer(layer) -> tuple[Tensor, PageTable | None]:
     """The tensor the kernels read for one layer's keys or values, and its
     page table (None for the slab)."""
@@ -349,6 +382,30 @@ class TextAttention(nn.Module):
         return self.o_proj(output.flatten(1))
 
 
+    def verify(self, x, keys, values, k_draft, v_draft, rows, lengths, masks, cos, sin) -> Tensor:
+        """Drafted trees ``x`` ``(batch, tokens, width)``: each token attends the
+        ``lengths`` keys its row holds in the cache (``keys``/``values`` as for
+        :meth:`step`) and its ancestors (``masks``,
+        :func:`~asrback_amd.drafts.tree_masks`), whose keys and values go to
+        ``k_draft``/``v_draft`` ``(batch, tokens, kv_heads, head_dim)``; the cache
+        stays as it is.  ``cos``/``sin`` ``(batch, tokens, head_dim)`` at each
+        token's position, ``rows`` 0 .. batch - 1 (int64)."""
+        key_cache, pages = _cache_layer(keys)
+        value_cache, _ = _cache_layer(values)
+        batch, tokens, _ = x.shape
+        qkv = self.qkv_proj(x)
+        q, k, v = (t.view(batch, tokens, -1, self.head_dim) for t in qkv.split(self.sizes, dim=-1))
+        if (type(self.q_norm) is RMSNorm and type(self.k_norm) is RMSNorm
+                and prompt_rows_takes(q, k, v, k_draft, v_draft, rows, None, self.q_norm, self.k_norm, cos, sin)):
+            q, _, _ = prompt_rows(q, k, v, k_draft, v_draft, rows, None, self.q_norm, self.k_norm, cos, sin)
+        else:
+            q = rotate(self.q_norm(q), cos, sin)
+            k_draft.copy_(rotate(self.k_norm(k), cos, sin))
+            v_draft.copy_(v)
+        output = tree_attention(q, key_cache, value_cache, k_draft, v_draft, masks, lengths=lengths, pages=pages)
+        return self.o_proj(output.flatten(2))
+
+
 class TextMLP(nn.Module):
     def __init__(self, config: dict) -> None:
         super().__init__()
@@ -401,6 +458,26 @@ class TextModel(nn.Module):
         for index, layer in enumerate(self.layers):
             keys, values = cache.keys[index], cache.values[index]
             x = layer(x, lambda attention, h: attention.step(h, keys, values, positions, mask, cos, sin))
+        return self.norm(x)
+
+
+    def verify(self, tokens, lengths, cache: KVCache | PagedKVCache, drafts: DraftCache, masks, depths, cos,
+               sin) -> Tensor:
+        """Hidden states ``(batch, tokens, width)`` of drafted trees
+        ``tokens`` ``(batch, tokens)`` behind the ``lengths`` (int64) keys each row
+        holds in ``cache``: token ``t`` is at position ``lengths + depths[t]``
+        (``masks``, ``depths``: :func:`~asrback_amd.drafts.tree_masks`) and sees its
+        ancestors.  Their keys and values go to ``drafts``; ``cos``/``sin`` are
+        the full tables."""
+        x = self.embed_tokens(tokens)
+        positions = (lengths[:, None] + depths).clamp(max=len(cos) - 1)
+        cos, sin = cos[positions], sin[positions]
+        rows = torch.arange(len(tokens), device=tokens.device)
+        for index, layer in enumerate(self.layers):
+            keys, values = cache.keys[index], cache.values[index]
+            k_draft, v_draft = drafts.keys[index], drafts.values[index]
+            x = layer(x, lambda attention, h: attention.verify(h, keys, values, k_draft, v_draft, rows, lengths, masks,
+                                                               cos, sin))
         return self.norm(x)
 
 
@@ -476,12 +553,14 @@ class TextGreedyDecoder:
     reference's varlen path.  With ``page_size`` the cache is a
     :class:`PagedKVCache` of ``num_pages`` pages (default: as many
     positions as the slab): a row holds the pages for its prompt and its
-    generation limit from admission until it finishes.
+    generation limit from admission until it finishes.  :meth:`verify` takes
+    drafted trees instead of single steps; ``draft_tokens`` is the tree size
+    whose passes are captured in graphs as well.
     """
 
     def __init__(self, text: TextModel, lm_head: nn.Module, config: dict, max_batch_size: int,
                  eos_ids: list[int], graphs: bool = True, page_size: int | None = None,
-                 num_pages: int | None = None) -> None:
+                 num_pages: int | None = None, draft_tokens: int = 0) -> None:
         self.text = text
         self.lm_head = lm_head
         self.config = config
@@ -500,9 +579,14 @@ class TextGreedyDecoder:
             self.cache = PagedKVCache.allocate(config, max_batch_size, pages, page_size, self.device, self.dtype)
         self.state = DecodeState.allocate(max_batch_size, self.device)
         self.eos_ids = torch.tensor(eos_ids, dtype=torch.long, device=self.device)
+        self.draft_tokens = draft_tokens
+        self.drafts = DraftCache.allocate(config, max_batch_size, draft_tokens, self.device, self.dtype)
+        # The drafted tokens and parents of the captured passes.
+        self._drafted = torch.zeros((2, max_batch_size, draft_tokens), dtype=torch.long, device=self.device)
         self.workspace = torch.empty(self._workspace_bytes(), dtype=torch.uint8, device=self.device)
         self.rows: dict[int, dict] = {}
         self.graphs: dict[tuple[int, int], CapturedGraph] = {}
+        self.verify_graphs: dict[int, CapturedGraph] = {}
         if graphs:
             self._capture_graphs()
 
@@ -510,7 +594,7 @@ class TextGreedyDecoder:
         """Split partials of the largest step over the buckets: the decode
         launch per layer and the greedy choice over the logits."""
         config = self.config
-        vocab = self.lm_head.weight.shape[0]
+        vocab = self.lm_head.out_features if isinstance(self.lm_head, Linear4) else self.lm_head.weight.shape[0]
         need = 256
         for batch in self.buckets:
             for length in self.kv_buckets:
@@ -518,12 +602,17 @@ class TextGreedyDecoder:
                     batch, config["num_attention_heads"], config["num_key_value_heads"], config["head_dim"],
                     length, self.dtype))
             need = max(need, attention.choice_workspace_size(batch, vocab))
+            if self.draft_tokens:
+                need = max(need, attention.choice_workspace_size(batch * self.draft_tokens, vocab), tree_workspace_size(
+                    batch, self.draft_tokens, config["num_attention_heads"], config["num_key_value_heads"],
+                    config["head_dim"], CACHE_LENGTH, self.dtype))
         return need
 
     @torch.inference_mode()
     def _capture_graphs(self) -> None:
-        """One greedy step per (batch bucket, KV bucket); warm-up steps advance
-        the rows, so they start inside the cache."""
+        """One greedy step per (batch bucket, KV bucket) and one pass over drafted
+        trees per batch bucket; warm-up steps advance the rows, so they start
+        inside the cache."""
         pool = torch.cuda.graph_pool_handle()
         for batch_size in self.buckets:
             state = self.state.narrow(batch_size)
@@ -534,6 +623,15 @@ class TextGreedyDecoder:
                 state.end.fill_(CACHE_LENGTH - 1)
                 self.graphs[batch_size, length] = CapturedGraph(
                     lambda state=state, cache=cache: self.step(state, cache), pool
+                )
+            if self.draft_tokens:
+                state.finished.zero_()
+                state.position.zero_()
+                cache = self.cache.narrow(batch_size, CACHE_LENGTH)
+                drafted, parents = self._drafted[:, :batch_size]
+                self.verify_graphs[batch_size] = CapturedGraph(
+                    lambda state=state, cache=cache, drafted=drafted, parents=parents: self._verify(
+                        state, cache, drafted, parents), pool
                 )
         self.state.free(torch.arange(self.max_batch_size, device=self.device))
 
@@ -632,6 +730,75 @@ class TextGreedyDecoder:
         for r in rows:
             r["bound"] = min(r["bound"] + count, r["end"])
         return count
+
+    def _verify(self, state: DecodeState, cache: KVCache | PagedKVCache, drafted: Tensor, parents: Tensor) -> Tensor:
+        """:meth:`step` over drafted trees: every row advances by the tokens the
+        model's own greedy choices accept; returns how many per row."""
+        batch, width = drafted.shape
+        drafts = (self.drafts if width == self.draft_tokens else
+                  DraftCache.allocate(self.config, batch, width, self.device, self.dtype)).narrow(batch, width)
+        masks, depths = tree_masks(parents)
+        tokens = torch.cat((state.tokens[:, None], drafted[:, 1:]), 1)
+        # Trees of another size than the workspace is made for take temporaries.
+        with attention.workspace(self.workspace) if width == self.draft_tokens else contextlib.nullcontext():
+            # Padding may hold any number.
+            known = tokens.clamp(0, self.text.embed_tokens.num_embeddings - 1)
+            hidden = self.text.verify(known, state.position, cache, drafts, masks, depths, self.cos, self.sin)
+            choices, logprobs = choose(self.logits(hidden.flatten(0, 1)))
+        limit = (state.end - state.position).masked_fill(state.finished, 0)
+        path, emitted, count = accept_drafts(tokens, parents, choices.view(batch, width), limit)
+        # Nothing follows an end of sequence.
+        held = path >= 0
+        ended = torch.isin(emitted, self.eos_ids) & held
+        held &= ended.cumsum(1) - ended.long() == 0
+        count = held.sum(1)
+        drafts.commit(cache, path, count, state.position)
+        kept = logprobs.view(batch, width).gather(1, path.clamp(min=0)).masked_fill(~held, 0.0)
+        state.sum_logprobs.add_(kept.sum(1))
+        step = torch.arange(CACHE_LENGTH, device=self.device) - state.position[:, None] - 1
+        new = emitted.gather(1, step.clamp(0, width - 1))
+        state.generated.copy_(torch.where((step >= 0) & (step < count[:, None]), new, state.generated))
+        position = state.position + count
+        last = emitted.gather(1, (count - 1).clamp(min=0)[:, None])[:, 0]
+        state.tokens.copy_(torch.where(count > 0, last, state.tokens))
+        state.finished.logical_or_((ended & held).any(1) | (position >= state.end))
+        state.position.copy_(position)
+        return count
+
+    @torch.inference_mode()
+    def verify(self, drafted: Tensor, parents: Tensor) -> None:
+        """One pass over drafted trees in place of single greedy steps:
+        ``drafted`` int64 ``(rows, tokens)`` holds, for every slot from 0 past the
+        last occupied one, tokens that may come next; column 0 stands for the
+        row's newest token (its entry is not read), the others follow their
+        ``parents`` (int64 ``(tokens,)`` or ``(rows, tokens)``; token 0's is -1,
+        values below -1 are padding).  Rows advance by at least one token and by
+        as many drafted ones as greedy steps would have produced, with the same
+        results; finished and free rows stay as they are.  Trees of
+        ``draft_tokens`` tokens replay captured graphs."""
+        if not self.rows:
+            raise RuntimeError("no occupied rows")
+        rows = max(self.rows) + 1
+        if drafted.dim() != 2 or drafted.shape[0] < rows or drafted.dtype != torch.int64:
+            raise ValueError(f"drafted must be int64 (at least {rows} rows, tokens), got {drafted.dtype} "
+                             f"{tuple(drafted.shape)}")
+        width = drafted.shape[1]
+        if not 1 <= width <= MAX_TOKENS:
+            raise ValueError(f"a tree has 1 to {MAX_TOKENS} drafted tokens, got {width}")
+        if parents.dtype != torch.int64 or parents.shape not in ((width,), drafted.shape):
+            raise ValueError(f"parents must be int64 ({width},) or {tuple(drafted.shape)}, got {parents.dtype} "
+                             f"{tuple(parents.shape)}")
+        parents = parents.expand(drafted.shape)[:rows]
+        if self.verify_graphs and width == self.draft_tokens:
+            bucket = next(size for size in self.buckets if size >= rows)
+            self._drafted[0, :rows] = drafted[:rows]
+            self._drafted[1, :rows] = parents
+            self._drafted[1, rows:bucket] = -2  # free rows: no token
+            self.verify_graphs[bucket].replay()
+        else:
+            self._verify(self.state.narrow(rows), self.cache.narrow(rows, CACHE_LENGTH), drafted[:rows], parents)
+        for r in self.rows.values():
+            r["bound"] = min(r["bound"] + width, r["end"])
 
     @torch.inference_mode()
     def finished_rows(self) -> dict[int, tuple[list[int], float]]:

@@ -146,8 +146,8 @@ def test_library_refuses(lib):
     assert tree(**paged | {"page_size": 8}) == tree(**paged | {"page_size": 48}) == _lib.ERR_UNSUPPORTED
     assert tree(**paged | {"bt_stride": 63}) == tree(**paged | {"k_page_stride": 4}) == _lib.ERR_INVALID
     assert lib.asrlayer_tree(None, None, 0, None) == lib.asrlayer_commit(None, None) == _lib.ERR_INVALID
-    assert lib.asrlayer_tree_masks(None, 0, 1, 8, None, None) == _lib.ERR_INVALID
-    assert lib.asrlayer_tree_masks(4096, 0, 1, 65, 4096, None) == _lib.ERR_UNSUPPORTED
+    assert lib.asrlayer_tree_masks(None, 0, 1, 8, None, None, None) == _lib.ERR_INVALID
+    assert lib.asrlayer_tree_masks(4096, 0, 1, 65, 4096, 4096, None) == _lib.ERR_UNSUPPORTED
     assert lib.asrlayer_accept(4096, 4096, 0, 4096, None, -1, 8, 4096, 4096, 4096, None) == _lib.ERR_INVALID
     assert lib.asrlayer_accept(4096, 4096, 0, 4096, None, 0, 8, 4096, 4096, 4096, None) == _lib.OK
     c = _lib.CommitParams()

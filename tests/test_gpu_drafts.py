@@ -152,8 +152,9 @@ def test_tree_attention_matches_float64(case):
     q, k, v, kd, vd, pages, k_rows, v_rows = make(dtype, batch, tokens, heads, kv_heads, d, length, page, g, layout)
     parents = [random_parents(tokens, g, padding=(b % 2) * min(2, tokens - 1)) for b in range(batch)]
     masks = [reference_masks(p) for p in parents]
-    device_masks = drafts.tree_masks(torch.tensor(parents, device="cuda"))
+    device_masks, depths = drafts.tree_masks(torch.tensor(parents, device="cuda"))
     assert device_masks.tolist() == [signed(m) for m in masks]
+    assert depths.tolist() == [[max(bin(m).count("1") - 1, 0) for m in row] for row in masks]
     out = drafts.tree_attention(q, k, v, kd, vd, device_masks, lengths=torch.tensor(lengths, device="cuda"), pages=pages)
     torch.cuda.synchronize()
     ref, absolute, slack = reference(q, [k_rows[b, :n] for b, n in enumerate(lengths)],
@@ -292,7 +293,7 @@ def test_graphs_sharing_a_workspace_and_other_streams():
     need = 0
     for dtype, batch, tokens, heads, kv, d, length, page in shapes:
         q, k, v, kd, vd, pages, _, _ = make(dtype, batch, tokens, heads, kv, d, length, page, g)
-        masks = drafts.tree_masks(torch.tensor(random_parents(tokens, g), device="cuda"))
+        masks, _ = drafts.tree_masks(torch.tensor(random_parents(tokens, g), device="cuda"))
         lengths = torch.tensor([length - 7], device="cuda")
         size = drafts.tree_workspace_size(batch, tokens, heads, kv, d, length, dtype)
         assert size > 0
@@ -353,15 +354,18 @@ def test_tree_masks_edges():
     from asrback_amd import drafts
 
     say("masks")
+    masks = lambda parents: drafts.tree_masks(parents.cuda())[0].tolist()  # noqa: E731
     chain = torch.arange(-1, 63)
-    assert drafts.tree_masks(chain.cuda()).tolist() == signed([(1 << (i + 1)) - 1 for i in range(64)])
-    assert drafts.tree_masks(torch.tensor([-1], device="cuda")).tolist() == [1]
+    assert masks(chain) == signed([(1 << (i + 1)) - 1 for i in range(64)])
+    assert drafts.tree_masks(chain.cuda())[1].tolist() == list(range(64))
+    assert masks(torch.tensor([-1])) == [1]
     # Parents that are no earlier token count as the context; children of padding
     # see themselves alone.
-    odd = torch.tensor([[0, 0, 5, -2, 3, -9], [1 << 40, -1, 2, 1, 4, -1 << 40]], device="cuda")
-    assert drafts.tree_masks(odd).tolist() == [[1, 3, 4, 0, 16, 0], [1, 2, 4, 10, 16, 0]]
-    assert drafts.tree_masks(odd.t().contiguous().t()).tolist() == drafts.tree_masks(odd).tolist()
-    assert drafts.tree_masks(odd[:0]).shape == (0, 6)
+    odd = torch.tensor([[0, 0, 5, -2, 3, -9], [1 << 40, -1, 2, 1, 4, -1 << 40]])
+    assert masks(odd) == [[1, 3, 4, 0, 16, 0], [1, 2, 4, 10, 16, 0]]
+    assert drafts.tree_masks(odd.cuda())[1].tolist() == [[0, 1, 0, 0, 0, 0], [0, 0, 0, 1, 0, 0]]
+    assert masks(odd.t().contiguous().t()) == masks(odd)
+    assert drafts.tree_masks(odd[:0].cuda())[0].shape == (0, 6)
 
 
 @pytest.mark.parametrize("batch,width,shared", [(1, 1, False), (3, 2, True), (40, 17, False), (25, 64, False), (7, 64, True)])
