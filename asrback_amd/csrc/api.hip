@@ -584,7 +584,8 @@ int check_tree(const asrlayer_tree_params* params) {
     return fail(ASRATTN_ERR_INVALID, "batch (%d) and max_len_k (%d) must be >= 0", p.batch, p.max_len_k);
   if (p.tokens < 1 || p.tokens > 64)
     return fail(ASRATTN_ERR_UNSUPPORTED, "a tree has 1 to 64 drafted tokens, got %d", p.tokens);
-  if (p.batch > 65535 || p.heads_q > 4096) return fail(ASRATTN_ERR_UNSUPPORTED, "more than 65535 rows or 4096 heads");
+  if (p.batch > 65535 || p.heads_q > 4096 || p.max_len_k > (1 << 30))
+    return fail(ASRATTN_ERR_UNSUPPORTED, "more than 65535 rows, 4096 heads or 2^30 positions");
   return ASRATTN_OK;
 }
 

@@ -85,10 +85,10 @@ struct TreePlan {
   int row_tiles;   // 16-row tiles a workgroup holds
   int row_blocks;  // workgroups over a kv head's query rows
   int splits;
+  int waves;        // of a workgroup
+  bool fold_apart;  // fold the partials in a launch of its own
 };
 TreePlan tree_plan(const asrlayer_tree_params& p);
-// The most row tiles a workgroup of this head size takes.
-int tree_most_row_tiles(int head_dim);
 hipError_t launch_tree(const asrlayer_tree_params& p, const TreePlan& plan, float* ws_o, float* ws_ml,
                        unsigned long long* ws_arrive, hipStream_t stream);
 

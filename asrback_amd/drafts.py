@@ -24,6 +24,7 @@ gradient, and calls that would need one are refused.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -41,7 +42,7 @@ _increment_version = torch.autograd.graph.increment_version
 
 
 def _no_gradient(what: str, *tensors: Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if any(t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no gradient; call it under torch.no_grad() or on detached tensors")
 
 
@@ -111,12 +112,16 @@ def tree_masks(parents: Tensor) -> tuple[Tensor, Tensor]:
     return masks, depths
 
 
-def _tree_sizes(batch: int, tokens: int, heads_q: int, heads_kv: int, head_dim: int, max_len: int, dtype: int,
-                scale: float) -> _lib.TreeParams:
+@functools.lru_cache(maxsize=256)
+def _tree_workspace(batch: int, tokens: int, heads_q: int, heads_kv: int, head_dim: int, max_len: int,
+                    dtype: int) -> int:
+    """``asrlayer_tree_workspace_size`` of these sizes (-1 for ones it does not
+    take)."""
     params = _lib.TreeParams()
     params.batch, params.tokens, params.heads_q, params.heads_kv = batch, tokens, heads_q, heads_kv
-    params.head_dim, params.max_len_k, params.dtype, params.scale = head_dim, max_len, dtype, scale
-    return params
+    params.head_dim, params.max_len_k, params.dtype, params.scale = head_dim, max_len, dtype, 1.0
+    need = _lib.load().asrlayer_tree_workspace_size(ctypes.byref(params))
+    return -1 if need == ctypes.c_size_t(-1).value else need
 
 
 def tree_attention(
@@ -152,56 +157,55 @@ def tree_attention(
     partials' memory (:func:`tree_workspace_size`,
     :func:`asrback_amd.attention.workspace`).  Returns ``(batch, tokens,
     heads_q, head_dim)``."""
-    for name, t in (("q", q), ("k", k), ("v", v), ("k_draft", k_draft), ("v_draft", v_draft)):
-        if t.dim() != 4:
-            raise ValueError(f"{name} must have 4 dimensions, got shape {tuple(t.shape)}")
-    batch, tokens, heads_q, head_dim = q.shape
-    heads_kv = k.shape[2]
-    if v.shape != k.shape or k.shape[3] != head_dim:
-        raise ValueError(f"k and v must share one shape with q's head_dim {head_dim}; got {tuple(k.shape)}, "
+    q_shape, k_shape, draft_shape = q.shape, k.shape, k_draft.shape
+    if not len(q_shape) == len(k_shape) == len(draft_shape) == 4:
+        raise ValueError(f"q, k and k_draft must have 4 dimensions, got shapes {tuple(q_shape)}, {tuple(k_shape)}, "
+                         f"{tuple(draft_shape)}")
+    batch, tokens, heads_q, head_dim = q_shape
+    length, heads_kv = k_shape[1:3]
+    if v.shape != k_shape or k_shape[3] != head_dim:
+        raise ValueError(f"k and v must share one shape with q's head_dim {head_dim}; got {tuple(k_shape)}, "
                          f"{tuple(v.shape)}")
-    if pages is None and k.shape[0] != batch:
-        raise ValueError(f"q has {batch} rows, the cache {k.shape[0]}")
+    if pages is None and k_shape[0] != batch:
+        raise ValueError(f"q has {batch} rows, the cache {k_shape[0]}")
     if heads_kv == 0 or heads_q % heads_kv or heads_q == 0:
         raise ValueError(f"{heads_q} query heads are not a positive multiple of {heads_kv} kv heads")
-    for name, t in (("k_draft", k_draft), ("v_draft", v_draft)):
-        if t.shape != (batch, tokens, heads_kv, head_dim):
-            raise ValueError(f"{name} must be ({batch}, {tokens}, {heads_kv}, {head_dim}), got {tuple(t.shape)}")
+    if draft_shape != (batch, tokens, heads_kv, head_dim) or v_draft.shape != draft_shape:
+        raise ValueError(f"k_draft and v_draft must be ({batch}, {tokens}, {heads_kv}, {head_dim}), got "
+                         f"{tuple(draft_shape)}, {tuple(v_draft.shape)}")
     _tokens(tokens)
     masks, masks_stride = _per_tree(masks, "masks", batch, tokens)
     lengths = _lengths(lengths, batch)
     dtype = _dtype_code(q, k, v, k_draft, v_draft)
-    _no_gradient("tree_attention", q, k, v, k_draft, v_draft)
-    q, k_draft, v_draft = _aligned(q), _aligned(k_draft), _aligned(v_draft)
-    k, v = _aligned(k), _aligned(v)
+    if torch.is_grad_enabled():
+        _no_gradient("tree_attention", q, k, v, k_draft, v_draft)
+    q, k, v, k_draft, v_draft = _aligned(q), _aligned(k), _aligned(v), _aligned(k_draft), _aligned(v_draft)
     if out is None:
-        out = torch.empty((batch, tokens, heads_q, head_dim), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(-1) != 1:
+        out = torch.empty(q_shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q_shape or out.dtype != q.dtype or out.stride(-1) != 1:
         raise ValueError("out must match q's shape and dtype, with a unit last stride")
-    device = _check_device(q, k, v, k_draft, v_draft, masks, lengths, out, None if pages is None else pages.block_table)
-    params = _tree_sizes(batch, tokens, heads_q, heads_kv, head_dim, k.shape[1], dtype,
-                         1.0 / math.sqrt(head_dim) if scale is None else scale)
-    params.q, params.k, params.v, params.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-    params.k_draft, params.v_draft = k_draft.data_ptr(), v_draft.data_ptr()
-    params.q_batch_stride, params.q_token_stride, params.q_head_stride, _ = q.stride()
-    params.k_batch_stride, params.k_token_stride, params.k_head_stride, _ = k.stride()
-    params.v_batch_stride, params.v_token_stride, params.v_head_stride, _ = v.stride()
-    params.kd_batch_stride, params.kd_token_stride, params.kd_head_stride, _ = k_draft.stride()
-    params.vd_batch_stride, params.vd_token_stride, params.vd_head_stride, _ = v_draft.stride()
-    params.o_batch_stride, params.o_token_stride, params.o_head_stride, _ = out.stride()
-    params.masks, params.masks_batch_stride = masks.data_ptr(), masks_stride
-    if lengths is not None:
-        params.lengths, params.lengths64 = lengths.data_ptr(), int(lengths.dtype == torch.int64)
-    if pages is not None:
-        pk, params.max_len_k = _paged(pages, k, v, batch)
-        params.block_table, params.bt_stride = pk.block_table, pk.bt_stride
-        params.page_size, params.num_pages = pk.page_size, pk.num_pages
-        params.k_page_stride, params.v_page_stride = pk.k_page_stride, pk.v_page_stride
-        params.k_batch_stride = params.v_batch_stride = 0
-    lib = _lib.load()
-    workspace = _split_workspace(lib.asrlayer_tree_workspace_size(ctypes.byref(params)), workspace, device)
+    k_strides, v_strides = k.stride()[:3], v.stride()[:3]
+    if pages is None:
+        device = _check_device(q, k, v, k_draft, v_draft, masks, lengths, out)
+        paged = (None, 0, 0, 0, 0, 0)
+    else:
+        device = _check_device(q, k, v, k_draft, v_draft, masks, lengths, out, pages.block_table)
+        pk, length = _paged(pages, k, v, batch)
+        paged = (pk.block_table, pk.bt_stride, pk.k_page_stride, pk.v_page_stride, pk.page_size, pk.num_pages)
+        k_strides, v_strides = (0, *k_strides[1:]), (0, *v_strides[1:])
+    params = _lib.TreeParams(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), k_draft.data_ptr(), v_draft.data_ptr(), out.data_ptr(),
+        *q.stride()[:3], *k_strides, *v_strides, *k_draft.stride()[:3], *v_draft.stride()[:3], *out.stride()[:3],
+        masks.data_ptr(), masks_stride, None if lengths is None else lengths.data_ptr(), *paged,
+        lengths is not None and lengths.dtype == torch.int64, batch, tokens, heads_q, heads_kv, head_dim, length, dtype,
+        1.0 / math.sqrt(head_dim) if scale is None else scale)
+    need = _tree_workspace(batch, tokens, heads_q, heads_kv, head_dim, length, dtype)
+    # Sizes that the library does not take: the call says why.
+    workspace = _split_workspace(max(need, 0), workspace, device)
     size = 0 if workspace is None else workspace.numel()
-    _lib.check(lib.asrlayer_tree(ctypes.byref(params), _ptr(workspace), size, _stream(device)), "asrlayer_tree")
+    status = _lib.load().asrlayer_tree(ctypes.byref(params), _ptr(workspace), size, _stream(device))
+    if status:
+        _lib.check(status, "asrlayer_tree")
     return out
 
 
@@ -213,12 +217,12 @@ def tree_workspace_size(batch: int, tokens: int, heads_q: int, heads_kv: int, he
     cache.  Raises for sizes the library does not take."""
     if dtype not in _DTYPES:
         raise TypeError(f"attention supports float32 and bfloat16, got {dtype}")
-    params = _tree_sizes(batch, tokens, heads_q, heads_kv, head_dim, max_len, _DTYPES[dtype], 1.0)
-    lib = _lib.load()
-    need = lib.asrlayer_tree_workspace_size(ctypes.byref(params))
-    if need == ctypes.c_size_t(-1).value:
-        raise ValueError(lib.asrattn_last_error().decode("utf-8", "replace"))
-    return int(need)
+    sizes = (batch, tokens, heads_q, heads_kv, head_dim, max_len, _DTYPES[dtype])
+    need = _tree_workspace(*sizes)
+    if need < 0:
+        _tree_workspace.__wrapped__(*sizes)  # leaves its message
+        raise ValueError(_lib.load().asrattn_last_error().decode("utf-8", "replace"))
+    return need
 
 
 def accept_drafts(tokens: Tensor, parents: Tensor, choices: Tensor,
@@ -238,23 +242,22 @@ def accept_drafts(tokens: Tensor, parents: Tensor, choices: Tensor,
     a limit below 1, or whose token 0 is padding, accept nothing."""
     if tokens.dim() != 2:
         raise ValueError(f"tokens must be (batch, width), got {tuple(tokens.shape)}")
-    batch, width = tokens.shape
+    shape = tokens.shape
+    batch, width = shape
     _tokens(width)
-    tokens = _int64(tokens, "tokens", (batch, width))
-    choices = _int64(choices, "choices", (batch, width))
+    tokens, choices = _int64(tokens, "tokens", shape), _int64(choices, "choices", shape)
     parents, stride = _per_tree(parents, "parents", batch, width)
     if limit is not None:
         limit = _int64(limit, "limit", (batch,))
     device = _check_device(tokens, parents, choices, limit)
     _cuda(device, "accept_drafts")
-    path, emitted = torch.empty_like(tokens), torch.empty_like(tokens)
+    path, emitted = torch.empty((2, batch, width), dtype=torch.int64, device=device).unbind()
     count = torch.empty(batch, dtype=torch.int64, device=device)
-    lib = _lib.load()
-    _lib.check(
-        lib.asrlayer_accept(tokens.data_ptr(), parents.data_ptr(), stride, choices.data_ptr(), _ptr(limit), batch, width,
-                            path.data_ptr(), emitted.data_ptr(), count.data_ptr(), _stream(device)),
-        "asrlayer_accept",
-    )
+    status = _lib.load().asrlayer_accept(
+        tokens.data_ptr(), parents.data_ptr(), stride, choices.data_ptr(), _ptr(limit), batch, width, path.data_ptr(),
+        emitted.data_ptr(), count.data_ptr(), _stream(device))
+    if status:
+        _lib.check(status, "asrlayer_accept")
     return path, emitted, count
 
 
@@ -282,17 +285,17 @@ def commit_drafts(
     int32 or int64 ``(batch,)`` are the rows' keys before the call.  Positions
     outside the cache or on no page are left alone, as are path entries outside
     the tree."""
-    for name, t in (("keys", keys), ("values", values), ("k_draft", k_draft), ("v_draft", v_draft)):
-        if t.dim() != 5:
-            raise ValueError(f"{name} must have 5 dimensions, got shape {tuple(t.shape)}")
-    layers, batch, tokens, heads_kv, head_dim = k_draft.shape
-    if v_draft.shape != k_draft.shape:
-        raise ValueError(f"k_draft and v_draft shapes differ: {tuple(k_draft.shape)}, {tuple(v_draft.shape)}")
-    if values.shape != keys.shape or keys.shape[0] != layers or keys.shape[3:] != (heads_kv, head_dim):
+    cache_shape, draft_shape = keys.shape, k_draft.shape
+    if len(cache_shape) != 5 or len(draft_shape) != 5:
+        raise ValueError(f"keys and k_draft must have 5 dimensions, got shapes {tuple(cache_shape)}, {tuple(draft_shape)}")
+    layers, batch, tokens, heads_kv, head_dim = draft_shape
+    if v_draft.shape != draft_shape:
+        raise ValueError(f"k_draft and v_draft shapes differ: {tuple(draft_shape)}, {tuple(v_draft.shape)}")
+    if values.shape != cache_shape or cache_shape[0] != layers or cache_shape[3:] != (heads_kv, head_dim):
         raise ValueError(f"keys and values must share one shape with {layers} layers of ({heads_kv}, {head_dim}); got "
-                         f"{tuple(keys.shape)}, {tuple(values.shape)}")
-    if pages is None and keys.shape[1] != batch:
-        raise ValueError(f"the drafts have {batch} rows, the cache {keys.shape[1]}")
+                         f"{tuple(cache_shape)}, {tuple(values.shape)}")
+    if pages is None and cache_shape[1] != batch:
+        raise ValueError(f"the drafts have {batch} rows, the cache {cache_shape[1]}")
     _tokens(tokens)
     path = _int64(path, "path", (batch, tokens))
     count = _int64(count, "count", (batch,))
@@ -300,29 +303,28 @@ def commit_drafts(
         raise TypeError("lengths must be a tensor")
     lengths = _lengths(lengths, batch)
     dtype = _dtype_code(keys, values, k_draft, v_draft)
-    _no_gradient("commit_drafts", keys, values, k_draft, v_draft)
+    if torch.is_grad_enabled():
+        _no_gradient("commit_drafts", keys, values, k_draft, v_draft)
     if not torch.is_inference_mode_enabled() and (keys.is_inference() or values.is_inference()):
         raise RuntimeError("inplace update to inference tensors outside InferenceMode is not allowed")
-    for name, t in (("keys", keys), ("values", values)):
-        if t.numel() and _aligned(t) is not t:
-            raise ValueError(f"{name} needs a unit last stride and 16-byte aligned rows (it is written in place)")
+    if (_aligned(keys) is not keys or _aligned(values) is not values) and keys.numel():
+        raise ValueError("keys and values need a unit last stride and 16-byte aligned rows (they are written in place)")
     k_draft, v_draft = _aligned(k_draft), _aligned(v_draft)
-    device = _check_device(keys, values, k_draft, v_draft, path, count, lengths,
-                           None if pages is None else pages.block_table)
-    params = _lib.CommitParams()
-    params.k_draft, params.v_draft = k_draft.data_ptr(), v_draft.data_ptr()
-    params.k, params.v = keys.data_ptr(), values.data_ptr()
-    for prefix, t in (("kd", k_draft), ("vd", v_draft), ("k", keys), ("v", values)):
-        for axis, stride in zip(("layer", "batch", "token", "head"), t.stride()):
-            setattr(params, f"{prefix}_{axis}_stride", stride)
-    params.path, params.count = path.data_ptr(), count.data_ptr()
-    params.lengths, params.lengths64 = lengths.data_ptr(), int(lengths.dtype == torch.int64)
-    params.layers, params.batch, params.tokens, params.heads_kv = layers, batch, tokens, heads_kv
-    params.head_dim, params.max_len_k, params.dtype = head_dim, keys.shape[2], dtype
-    if pages is not None:
-        pk, params.max_len_k = _paged(pages, keys[0], values[0], batch) if layers else (_lib.PagedKV(), 0)
-        params.block_table, params.bt_stride = pk.block_table, pk.bt_stride
-        params.page_size, params.num_pages = pk.page_size, pk.num_pages
-    lib = _lib.load()
-    _lib.check(lib.asrlayer_commit(ctypes.byref(params), _stream(device)), "asrlayer_commit")
+    length = cache_shape[2]
+    if pages is None:
+        device = _check_device(keys, values, k_draft, v_draft, path, count, lengths)
+        paged = (None, 0, 0, 0)
+    else:
+        device = _check_device(keys, values, k_draft, v_draft, path, count, lengths, pages.block_table)
+        if not layers:
+            return
+        pk, length = _paged(pages, keys[0], values[0], batch)
+        paged = (pk.block_table, pk.bt_stride, pk.page_size, pk.num_pages)
+    params = _lib.CommitParams(
+        k_draft.data_ptr(), v_draft.data_ptr(), keys.data_ptr(), values.data_ptr(), *k_draft.stride()[:4],
+        *v_draft.stride()[:4], *keys.stride()[:4], *values.stride()[:4], path.data_ptr(), count.data_ptr(),
+        lengths.data_ptr(), *paged, lengths.dtype == torch.int64, layers, batch, tokens, heads_kv, head_dim, length, dtype)
+    status = _lib.load().asrlayer_commit(ctypes.byref(params), _stream(device))
+    if status:
+        _lib.check(status, "asrlayer_commit")
     _increment_version((keys, values))

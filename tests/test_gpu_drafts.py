@@ -85,7 +85,7 @@ def check(got, ref, absolute, slack, dtype, label):
     got = got.double().cpu()
     bound = 2.0**-24 * absolute * slack
     bound += 2.0**-8 * (absolute + ref.abs()) if dtype == BF16 else 2.0**-24 * ref.abs()
-    bad = (got - ref).abs() > 1.01 * bound + 1e-38
+    bad = ~((got - ref).abs() <= 1.01 * bound + 1e-38)  # NaN is bad
     assert not bad.any(), f"{label}: {int(bad.sum())} of {bad.numel()} elements, worst {float(((got - ref).abs() / bound.clamp(min=1e-38)).max()):.3g} of the bound"
 
 
@@ -133,6 +133,14 @@ CASES = [
     (BF16, 2, 12, 8, 2, 64, 3000, [2999, 2], 0, "heads_first"),
     (F32, 1, 6, 3, 3, 64, 2100, [2100], 0, "slab"),
     (BF16, 1, 24, 2, 1, 256, 2000, [1999], 0, "slab"),
+    # many rows over long caches: two row tiles a workgroup, several workgroups a kv head
+    (BF16, 1, 61, 8, 1, 128, 20000, [17000], 0, "slab"),
+    (BF16, 1, 64, 8, 1, 64, 20000, [19999], 64, "slab"),
+    (F32, 1, 64, 8, 1, 64, 20000, [1234], 0, "heads_first"),
+    # more workgroups than CUs: four waves each
+    (BF16, 33, 2, 16, 8, 128, 96, [33, 96, 0, 1] * 8 + [17], 32, "slab"),
+    (F32, 40, 1, 8, 8, 128, 64, [33, 64, 0, 1] * 10, 0, "slab"),
+    (BF16, 70, 3, 8, 4, 256, 48, [33, 48, 0, 1, 20] * 14, 0, "slab"),
     # pages: shorter than a tile, of one tile, longer; a last page in part
     (BF16, 3, 8, 4, 2, 128, 112, [111, 16, 0], 16, "slab"),
     (BF16, 2, 8, 4, 2, 128, 448, [447, 130], 64, "slab"),
