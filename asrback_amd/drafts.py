@@ -25,44 +25,88 @@ from __future__ import annotations
 
 import ctypes
 import functools
-import math
 
 import torch
 from torch import Tensor
 
 from . import _lib
 from .attention import (
-    _DTYPES, PageTable, _aligned, _check_device, _dtype_code, _paged, _ptr, _split_workspace, _stream,
+    _DTYPES, PageTable, _aligned, _check_device, _dtype_code, _paged, _ptr, _split_workspace,
 )
 
 # Tokens of a drafted tree, one bit each of an ancestor mask.
 MAX_TOKENS = 64
 
 _increment_version = torch.autograd.graph.increment_version
+# The current stream's handle on a device.
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _no_gradient(what: str, *tensors: Tensor) -> None:
-    if any(t.requires_grad for t in tensors):
+def _operands(what: str, tensors: tuple[Tensor, ...], written: tuple[Tensor, ...] = ()) -> tuple:
+    """What a call passes of tensors of four or five axes that must share one
+    supported type and the current GPU: their pointers, their strides (but the last) in a row, the
+    dtype's code, the device's index, and the tensors themselves, those whose rows
+    cannot be read with 16-byte vectors copied (of ``written`` ones refused)."""
+    first = tensors[0]
+    dtype, index = first.dtype, first.get_device()
+    same, gradient, bits, ends, pointers, strides = True, False, 0, 0, [], []
+    for t in tensors:
+        if t.dtype is not dtype or t.get_device() != index:
+            same = False
+        if t.requires_grad:
+            gradient = True
+        pointer = t.data_ptr()
+        pointers.append(pointer)
+        ends |= pointer
+        stride = t.stride()
+        # A vector is a power of two of elements: one test for all strides.
+        if len(stride) == 4:
+            a, b, c, last = stride
+            strides += (a, b, c)
+            bits |= a | b | c
+        else:
+            a, b, c, d, last = stride
+            strides += (a, b, c, d)
+            bits |= a | b | c | d
+        if last != 1:
+            ends |= 1
+    if not same or index < 0 or dtype not in _DTYPES or index != torch.cuda.current_device():
+        _dtype_code(*tensors)  # these say what is wrong
+        _check_device(*tensors)
+    if gradient and torch.is_grad_enabled():
         raise RuntimeError(f"{what} has no gradient; call it under torch.no_grad() or on detached tensors")
+    if ends & 15 or bits & (7 if dtype is torch.bfloat16 else 3):
+        aligned = tuple(_aligned(t) for t in tensors)
+        for t, held in zip(tensors, aligned):
+            if t is not held and t.numel() and any(t is w for w in written):
+                raise ValueError("keys and values need a unit last stride and 16-byte aligned rows (they are written in "
+                                 "place)")
+        tensors = aligned
+        pointers = [t.data_ptr() for t in tensors]
+        strides = [stride for t in tensors for stride in t.stride()[:-1]]
+    return pointers, strides, _DTYPES[dtype], index, tensors
 
 
 def _int64(t: Tensor, name: str, shape: tuple[int, ...]) -> Tensor:
-    if t.dtype != torch.int64:
+    if t.dtype is not torch.int64:
         raise TypeError(f"{name} must be int64, got {t.dtype}")
     if t.shape != shape:
-        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
-    return t.contiguous()
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _per_tree(t: Tensor, name: str, batch: int, tokens: int) -> tuple[Tensor, int]:
     """``(tokens,)`` or ``(batch, tokens)`` int64 rows and their batch stride."""
-    if t.dtype != torch.int64:
+    if t.dtype is not torch.int64:
         raise TypeError(f"{name} must be int64, got {t.dtype}")
-    if t.shape not in ((tokens,), (batch, tokens)):
+    strides = t.stride()
+    if t.shape == (batch, tokens):
+        if strides[1] == 1 or tokens == 1:
+            return t, strides[0]
+        return t.contiguous(), tokens
+    if t.shape != (tokens,):
         raise ValueError(f"{name} must be ({tokens},) or ({batch}, {tokens}), got {tuple(t.shape)}")
-    if tokens > 1 and t.stride(-1) != 1:
-        t = t.contiguous()
-    return t, 0 if t.dim() == 1 else t.stride(0)
+    return t if strides[0] == 1 or tokens == 1 else t.contiguous(), 0
 
 
 def _tokens(tokens: int) -> None:
@@ -70,19 +114,33 @@ def _tokens(tokens: int) -> None:
         raise ValueError(f"a tree has 1 to {MAX_TOKENS} drafted tokens, got {tokens}")
 
 
-def _cuda(device: torch.device, what: str) -> None:
-    if device.type != "cuda":
-        raise RuntimeError(f"{what} runs on the GPU only; got tensors on {device}")
+def _cuda(what: str, *tensors: Tensor | None) -> int:
+    """The index of the current GPU, which must hold the tensors."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            _check_device(*tensors)
+    if index < 0:
+        raise RuntimeError(f"{what} runs on the GPU only; got tensors on {tensors[0].device}")
+    if index != torch.cuda.current_device():
+        _check_device(*tensors)
+    return index
+
+
+def _on(index: int, *tensors: Tensor | None) -> None:
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise RuntimeError(f"tensors on different devices: cuda:{index} and {t.device}")
 
 
 def _lengths(lengths: Tensor | None, batch: int) -> Tensor | None:
     if lengths is None:
         return None
-    if lengths.dtype not in (torch.int32, torch.int64):
+    if lengths.dtype is not torch.int64 and lengths.dtype is not torch.int32:
         raise TypeError(f"lengths must be int32 or int64, got {lengths.dtype}")
     if lengths.shape != (batch,):
         raise ValueError(f"lengths must be ({batch},), got {tuple(lengths.shape)}")
-    return lengths.contiguous()
+    return lengths if lengths.stride() == (1,) else lengths.contiguous()
 
 
 def tree_masks(parents: Tensor) -> tuple[Tensor, Tensor]:
@@ -102,13 +160,12 @@ def tree_masks(parents: Tensor) -> tuple[Tensor, Tensor]:
     _tokens(tokens)
     batch = parents.shape[0] if parents.dim() == 2 else 1
     parents, stride = _per_tree(parents, "parents", batch, tokens)
-    device = _check_device(parents)
-    _cuda(device, "tree_masks")
-    masks = torch.empty(parents.shape, dtype=torch.int64, device=device)
+    index = _cuda("tree_masks", parents)
+    masks = torch.empty_like(parents, memory_format=torch.contiguous_format)
     depths = torch.empty_like(masks)
     lib = _lib.load()
     _lib.check(lib.asrlayer_tree_masks(parents.data_ptr(), stride, batch, tokens, masks.data_ptr(), depths.data_ptr(),
-                                       _stream(device)), "asrlayer_tree_masks")
+                                       _raw_stream(index)), "asrlayer_tree_masks")
     return masks, depths
 
 
@@ -176,34 +233,31 @@ def tree_attention(
     _tokens(tokens)
     masks, masks_stride = _per_tree(masks, "masks", batch, tokens)
     lengths = _lengths(lengths, batch)
-    dtype = _dtype_code(q, k, v, k_draft, v_draft)
-    if torch.is_grad_enabled():
-        _no_gradient("tree_attention", q, k, v, k_draft, v_draft)
-    q, k, v, k_draft, v_draft = _aligned(q), _aligned(k), _aligned(v), _aligned(k_draft), _aligned(v_draft)
+    pointers, strides, dtype, index, held = _operands("tree_attention", (q, k, v, k_draft, v_draft))
     if out is None:
-        out = torch.empty(q_shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q_shape or out.dtype != q.dtype or out.stride(-1) != 1:
         raise ValueError("out must match q's shape and dtype, with a unit last stride")
-    k_strides, v_strides = k.stride()[:3], v.stride()[:3]
     if pages is None:
-        device = _check_device(q, k, v, k_draft, v_draft, masks, lengths, out)
-        paged = (None, 0, 0, 0, 0, 0)
+        _on(index, masks, lengths, out)
+        paged = (0, 0, 0, 0, 0, 0)
     else:
-        device = _check_device(q, k, v, k_draft, v_draft, masks, lengths, out, pages.block_table)
-        pk, length = _paged(pages, k, v, batch)
+        _on(index, masks, lengths, out, pages.block_table)
+        pk, length = _paged(pages, held[1], held[2], batch)
         paged = (pk.block_table, pk.bt_stride, pk.k_page_stride, pk.v_page_stride, pk.page_size, pk.num_pages)
-        k_strides, v_strides = (0, *k_strides[1:]), (0, *v_strides[1:])
-    params = _lib.TreeParams(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), k_draft.data_ptr(), v_draft.data_ptr(), out.data_ptr(),
-        *q.stride()[:3], *k_strides, *v_strides, *k_draft.stride()[:3], *v_draft.stride()[:3], *out.stride()[:3],
-        masks.data_ptr(), masks_stride, None if lengths is None else lengths.data_ptr(), *paged,
-        lengths is not None and lengths.dtype == torch.int64, batch, tokens, heads_q, heads_kv, head_dim, length, dtype,
-        1.0 / math.sqrt(head_dim) if scale is None else scale)
+        strides[3] = strides[6] = 0  # the pools' first axis is no row
+    params = _lib.pack_tree(
+        *pointers, out.data_ptr(), *strides, *out.stride()[:3], masks.data_ptr(), masks_stride,
+        0 if lengths is None else lengths.data_ptr(), *paged, lengths is not None and lengths.dtype is torch.int64, batch,
+        tokens, heads_q, heads_kv, head_dim, length, dtype, head_dim**-0.5 if scale is None else scale)
     need = _tree_workspace(batch, tokens, heads_q, heads_kv, head_dim, length, dtype)
-    # Sizes that the library does not take: the call says why.
-    workspace = _split_workspace(max(need, 0), workspace, device)
-    size = 0 if workspace is None else workspace.numel()
-    status = _lib.load().asrlayer_tree(ctypes.byref(params), _ptr(workspace), size, _stream(device))
+    size = 0
+    if need > 0:
+        workspace = _split_workspace(need, workspace, out.device)
+    if workspace is not None:
+        size, workspace = workspace.numel(), workspace.data_ptr()
+    # Sizes that the library does not take (need -1): the call says why.
+    status = _lib.load().asrlayer_tree(params, workspace, size, _raw_stream(index))
     if status:
         _lib.check(status, "asrlayer_tree")
     return out
@@ -249,13 +303,12 @@ def accept_drafts(tokens: Tensor, parents: Tensor, choices: Tensor,
     parents, stride = _per_tree(parents, "parents", batch, width)
     if limit is not None:
         limit = _int64(limit, "limit", (batch,))
-    device = _check_device(tokens, parents, choices, limit)
-    _cuda(device, "accept_drafts")
-    path, emitted = torch.empty((2, batch, width), dtype=torch.int64, device=device).unbind()
-    count = torch.empty(batch, dtype=torch.int64, device=device)
+    index = _cuda("accept_drafts", tokens, parents, choices, limit)
+    path, emitted = torch.empty_like(tokens), torch.empty_like(tokens)
+    count = tokens.new_empty(batch) if limit is None else torch.empty_like(limit)
     status = _lib.load().asrlayer_accept(
         tokens.data_ptr(), parents.data_ptr(), stride, choices.data_ptr(), _ptr(limit), batch, width, path.data_ptr(),
-        emitted.data_ptr(), count.data_ptr(), _stream(device))
+        emitted.data_ptr(), count.data_ptr(), _raw_stream(index))
     if status:
         _lib.check(status, "asrlayer_accept")
     return path, emitted, count
@@ -302,29 +355,24 @@ def commit_drafts(
     if lengths is None:
         raise TypeError("lengths must be a tensor")
     lengths = _lengths(lengths, batch)
-    dtype = _dtype_code(keys, values, k_draft, v_draft)
-    if torch.is_grad_enabled():
-        _no_gradient("commit_drafts", keys, values, k_draft, v_draft)
+    pointers, strides, dtype, index, held = _operands("commit_drafts", (k_draft, v_draft, keys, values), (keys, values))
     if not torch.is_inference_mode_enabled() and (keys.is_inference() or values.is_inference()):
         raise RuntimeError("inplace update to inference tensors outside InferenceMode is not allowed")
-    if (_aligned(keys) is not keys or _aligned(values) is not values) and keys.numel():
-        raise ValueError("keys and values need a unit last stride and 16-byte aligned rows (they are written in place)")
-    k_draft, v_draft = _aligned(k_draft), _aligned(v_draft)
     length = cache_shape[2]
     if pages is None:
-        device = _check_device(keys, values, k_draft, v_draft, path, count, lengths)
-        paged = (None, 0, 0, 0)
+        _on(index, path, count, lengths)
+        paged = (0, 0, 0, 0)
     else:
-        device = _check_device(keys, values, k_draft, v_draft, path, count, lengths, pages.block_table)
+        _on(index, path, count, lengths, pages.block_table)
         if not layers:
             return
         pk, length = _paged(pages, keys[0], values[0], batch)
         paged = (pk.block_table, pk.bt_stride, pk.page_size, pk.num_pages)
-    params = _lib.CommitParams(
-        k_draft.data_ptr(), v_draft.data_ptr(), keys.data_ptr(), values.data_ptr(), *k_draft.stride()[:4],
-        *v_draft.stride()[:4], *keys.stride()[:4], *values.stride()[:4], path.data_ptr(), count.data_ptr(),
-        lengths.data_ptr(), *paged, lengths.dtype == torch.int64, layers, batch, tokens, heads_kv, head_dim, length, dtype)
-    status = _lib.load().asrlayer_commit(ctypes.byref(params), _stream(device))
+    params = _lib.pack_commit(
+        *pointers, *strides, path.data_ptr(), count.data_ptr(), lengths.data_ptr(), *paged,
+        lengths.dtype is torch.int64, layers, batch, tokens, heads_kv, head_dim, length, dtype)
+    status = _lib.load().asrlayer_commit(params, _raw_stream(index))
     if status:
         _lib.check(status, "asrlayer_commit")
+    del held  # copies live until the launch
     _increment_version((keys, values))

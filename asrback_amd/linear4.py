@@ -14,19 +14,20 @@ gradient, and calls that would need one are refused.
 
 from __future__ import annotations
 
-import ctypes
 from dataclasses import dataclass
 
 import torch
 from torch import Tensor, nn
 
 from . import _lib
-from .attention import _aligned, _check_device, _dtype_code, _ptr, _stream
+from .attention import _DTYPES, _aligned, _check_device
 
 GROUPS = (32, 64, 128)
 _BLOCK_N, _BLOCK_K = 16, 128
 # Inputs of a dword's nibbles, from the low one up (csrc/layers.hpp).
 _ORDER = (0, 2, 4, 6, 1, 3, 5, 7)
+# The current stream's handle on a device.
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 @dataclass(frozen=True)
@@ -153,30 +154,36 @@ def linear4(x: Tensor, weight: Weight4, bias: Tensor | None = None, *, out: Tens
     step or a drafted tree (up to 64 are read against the weights in one
     pass); more rows are right, the weights being read once for each 64.
     Returns ``(..., outputs)``."""
-    if x.dim() < 1 or x.shape[-1] != weight.inputs:
-        raise ValueError(f"x must be (..., {weight.inputs}), got {tuple(x.shape)}")
-    shape = (*x.shape[:-1], weight.outputs)
-    if bias is not None and bias.shape != (weight.outputs,):
-        raise ValueError(f"bias must be ({weight.outputs},), got {tuple(bias.shape)}")
-    if x.dtype != weight.scales.dtype:
-        raise TypeError(f"x is {x.dtype}, the weight's scales {weight.scales.dtype}")
-    dtype = _dtype_code(x, weight.scales, *(() if bias is None else (bias,)))
+    shape = x.shape
+    packed, scales, zeros, outputs, inputs = weight.packed, weight.scales, weight.zeros, weight.outputs, weight.inputs
+    if not shape or shape[-1] != inputs:
+        raise ValueError(f"x must be (..., {inputs}), got {tuple(shape)}")
+    dtype, index = x.dtype, x.get_device()
+    if dtype is not scales.dtype:
+        raise TypeError(f"x is {dtype}, the weight's scales {scales.dtype}")
+    if bias is not None and (bias.shape != (outputs,) or bias.dtype is not dtype):
+        raise ValueError(f"bias must be {dtype} ({outputs},), got {bias.dtype} {tuple(bias.shape)}")
+    if index < 0:
+        raise RuntimeError(f"linear4 runs on the GPU only; got a tensor on {x.device}")
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         raise RuntimeError("linear4 has no gradient; call it under torch.no_grad() or on detached tensors")
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
-    elif out.shape != shape or out.dtype != x.dtype or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous {shape} tensor of x's dtype")
-    rows = x if x.dim() == 2 else x.reshape(-1, weight.inputs)
-    rows = _aligned(rows)
-    device = _check_device(rows, weight.packed, weight.scales, weight.zeros, bias, out)
+        out = x.new_empty((*shape[:-1], outputs))
+    elif out.shape != (*shape[:-1], outputs) or out.dtype is not dtype or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {(*shape[:-1], outputs)} tensor of x's dtype")
+    rows = _aligned(x if len(shape) == 2 else x.reshape(-1, inputs))
+    others = (packed, scales, zeros, bias, out)
+    if index != torch.cuda.current_device() or any(t is not None and t.get_device() != index for t in others):
+        _check_device(x, *others)  # says what is wrong
     if bias is not None:
         bias = bias.contiguous()
-    params = _lib.Linear4Params(
-        rows.data_ptr(), rows.stride(0), weight.packed.data_ptr(), weight.scales.data_ptr(), _ptr(weight.zeros),
-        _ptr(bias), out.data_ptr(), weight.outputs, rows.shape[0], weight.outputs, weight.inputs, weight.group, dtype)
-    lib = _lib.load()
-    _lib.check(lib.asrlayer_linear4(ctypes.byref(params), _stream(device)), "asrlayer_linear4")
+    params = _lib.pack_linear4(
+        rows.data_ptr(), rows.stride(0), packed.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(),
+        0 if bias is None else bias.data_ptr(), out.data_ptr(), outputs, rows.shape[0], outputs, inputs, weight.group,
+        _DTYPES[dtype])
+    status = _lib.load().asrlayer_linear4(params, _raw_stream(index))
+    if status:
+        _lib.check(status, "asrlayer_linear4")
     return out
 
 
