@@ -217,8 +217,9 @@ int asrlayer_commit(const asrlayer_commit_params* params, void* stream);
 //
 //   packed (n / 16, k / 128, 64, 4) dwords: dword s of lane 16 g + i holds
 //     output i's inputs 32 s + 8 g + j, j = 0 2 4 6 1 3 5 7 from the low nibble up
-//   scales (n / 16, k / group, 16)
-//   zeros  (n / 16, k / group, 8) bytes: output i in nibble i
+//   scales (n / 16, k / 128, 4, 128 / group, 4): of outputs 4 g .. 4 g + 3, g the
+//     third index, over the block's groups
+//   zeros  the same, four to two bytes, from the low nibble up
 typedef struct asrlayer_linear4_params {
   const void* x;
   int64_t x_row_stride;

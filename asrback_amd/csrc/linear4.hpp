@@ -21,8 +21,22 @@
 //     for four outputs, the group's sum of x one value per lane.
 //   * A workgroup's waves split the inputs, each keeping its part of x in
 //     registers, and go through the workgroup's blocks of outputs with it; the
-//     next block's weights load while this one's are multiplied.  The waves' sums
-//     meet in LDS once a block (two buffers, one barrier).
+//     next block's weights load while this one's are multiplied (two blocks ahead
+//     cost registers and gave 36.1 us for 34.3 at 4 x 2048 x 151936; loads past
+//     the caches 33.8, but 8.0 for 7.4 at 64 x 2048 x 4096 and 13.0 for 12.2 at 64
+//     x 2048 x 12288).  The waves' sums meet in LDS once a block (two buffers, one
+//     barrier that leaves the loads in flight).
+//   * Every wave of every turn issues the same loads and stores, absent ones with an
+//     empty range: the waits count them, and a branch would set them for its shorter
+//     path.  That took 41.9 us to 34.3 there.
+//   * x is loaded by whole rows (neighbouring lanes in one row; a load whose lanes lie
+//     in 16 rows takes four times as long in the vector cache) and changes lanes
+//     through the wave's own LDS.
+//
+// Measured (bf16, group 128): 4 x 2048 x 151936 in 35 us, 4.7 TB/s of the 6.0 that
+// a reading kernel reaches; 16 x 2048 x 12288 in 6.7 us and 1 x 2048 x 2048 in 3.9,
+// where launching (1.8 us) and one round trip each for x and the first weights are
+// most; 64 x 6144 x 2048 in 12 us, six turns of x through LDS after each other.
 #pragma once
 
 #include "common.hpp"
@@ -34,8 +48,6 @@ namespace {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
-
-constexpr int kL4Waves = 8;  // at most, of a workgroup
 
 template <typename T>
 struct L4 {
@@ -74,45 +86,120 @@ __device__ __forceinline__ void l4_step(uint32_t w, const uint4 (*x)[L4<T>::kXV]
   }
 }
 
-// RT: 16-row tiles of x; NB: blocks of 128 inputs a wave keeps; GROUP: inputs of
-// a scale.  Waves: kL4Waves or fewer.
-template <typename T, int RT, int NB, int GROUP>
-__global__ __launch_bounds__(64 * kL4Waves) void linear4_kernel(const asrlayer_linear4_params p, int blocks_n, int blocks_k) {
-  constexpr int kXV = L4<T>::kXV, kGroups = 128 / GROUP, kSteps = GROUP / 32;
+// Where 16-byte piece c of row r lies in a block of LPR-piece rows in LDS, so that a
+// piece of 16 rows lies in 16 different groups of banks.
+template <int LPR>
+__device__ __forceinline__ int l4_piece(int r, int c) {
+  return r * LPR + (c ^ (r & 15));
+}
+
+// The weights a wave multiplies at a time: NB blocks, their scales and zero points.
+template <typename T, int NB, int GROUP>
+struct L4Weights {
+  static constexpr int kGroups = 128 / GROUP;
+  static constexpr int kSV = kGroups * 4 * (int)sizeof(T) / 8;  // scales of a block, in 8 bytes
+  uint4 w[NB];
+  uint2 s[NB][kSV];
+  uint32_t z[NB][(kGroups + 1) / 2];
+  float bias;  // of output i
+};
+
+// Workgroups whose registers fit a CU.
+template <typename T, int W, int RT, int NB, int GROUP, bool CHUNKED>
+constexpr int l4_per_cu() {
+  return sizeof(T) == 2 && W == 8 && GROUP >= 64 && NB <= 2 && !(CHUNKED && RT == 2) ? 2 : 1;
+}
+
+// RT: 16-row tiles of x; NB: blocks of 128 inputs a wave holds at a time; GROUP:
+// inputs of a scale; CHUNKED: more inputs than the waves hold, x following the
+// weights chunk by chunk.
+template <typename T, int W, int RT, int NB, int GROUP, bool CHUNKED>
+__global__ __launch_bounds__(64 * W, (W / 4 * l4_per_cu<T, W, RT, NB, GROUP, CHUNKED>())) void linear4_kernel(
+    const asrlayer_linear4_params p, int blocks_n, int blocks_k) {
+  using W4 = L4Weights<T, NB, GROUP>;
+  constexpr int kXV = L4<T>::kXV, kGroups = 128 / GROUP, kSteps = GROUP / 32, kSV = W4::kSV;
   constexpr float kOffset = L4<T>::kOffset;
+  constexpr int kLPR = 128 * (int)sizeof(T) / 16;  // 16-byte pieces of a row in a block
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int waves = blockDim.x >> 6;
   const int64_t row0 = (int64_t)blockIdx.y * (RT * 16);
   const int chunk = waves * NB;  // blocks of inputs the workgroup holds at a time
   const uint4* const packed = static_cast<const uint4*>(p.packed);
-  const T* const scales = static_cast<const T*>(p.scales);
-  const uint16_t* const zeros = static_cast<const uint16_t*>(p.zeros);
+  const char* const scales = static_cast<const char*>(p.scales);
+  const char* const zeros = static_cast<const char*>(p.zeros);
 
-  __shared__ __attribute__((aligned(16))) float sm[2][kL4Waves][RT][16][20];
+  __shared__ __attribute__((aligned(16))) float sm[2][W][RT][16][20];
+  __shared__ uint4 sm_x[W][16 * kLPR];
+
+  // Absent zero points and bias are loads of nothing, that give 0, and not branches:
+  // each path's loads have to be the same for the waits to be exact.
+  const uint32_t unset = zeros == nullptr ? 0x88888888u : 0u;
+  auto load_w = [&](int cn, int first, W4& a) {
+    const int row = min(cn, blocks_n - 1);
+    const auto br = buffer_rsrc(static_cast<const T*>(p.bias) + row * 16,
+                                p.bias == nullptr ? 0 : min(16, p.n - row * 16) * (int)sizeof(T));
+    if constexpr (sizeof(T) == 2)
+      a.bias = __uint_as_float((uint32_t)__builtin_amdgcn_raw_buffer_load_b16(br, i * 2, 0, 0) << 16);
+    else
+      a.bias = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(br, i * 4, 0, 0));
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int kb = min(first + nb * waves + wave, blocks_k - 1);  // past the last: x is zero there
+      const int64_t block = (int64_t)row * blocks_k + kb;
+      a.w[nb] = packed[block * 64 + lane];
+      const uint2* sp = reinterpret_cast<const uint2*>(scales + (block * 4 + g) * (kSV * 8));
+#pragma unroll
+      for (int q = 0; q < kSV; ++q) a.s[nb][q] = sp[q];
+      const auto zr = buffer_rsrc(zeros + block * (kGroups * 8), zeros == nullptr ? 0 : kGroups * 8);
+      if constexpr (kGroups == 1) {
+        a.z[nb][0] = __builtin_amdgcn_raw_buffer_load_b16(zr, g * 2, 0, 0) ^ unset;
+      } else if constexpr (kGroups == 2) {
+        a.z[nb][0] = __builtin_amdgcn_raw_buffer_load_b32(zr, g * 4, 0, 0) ^ unset;
+      } else {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b64(zr, g * 8, 0, 0);
+        a.z[nb][0] = v[0] ^ unset, a.z[nb][1] = v[1] ^ unset;
+      }
+    }
+  };
 
   uint4 x[NB][4][RT][kXV];
   float sums[NB][kGroups][RT];  // of x over each group
-  // This wave's blocks of inputs from first on, and x in them.
+  // This wave's blocks of inputs from `first` on: x by rows, then as the product takes
+  // it, and its sums.
+  constexpr int kRows = 64 / kLPR, kTurns = 16 / kRows;  // rows a load, loads a block
+  uint4 raw[NB][RT][kTurns];
   auto load_x = [&](int first) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const int kb = first + nb * waves + wave;
+      const int k = (first + nb * waves + wave) * 128 + lane % kLPR * (16 / (int)sizeof(T));
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int k = kb * 128 + s * 32 + g * 8;
+      for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          const int64_t row = min(row0 + rt * 16 + i, p.rows - 1);
-          const T* at = static_cast<const T*>(p.x) + row * p.x_row_stride + min(k, p.k - 8);
-#pragma unroll
-          for (int v = 0; v < kXV; ++v) {
-            x[nb][s][rt][v] = *reinterpret_cast<const uint4*>(at + v * (8 / kXV));
-            if (k >= p.k) x[nb][s][rt][v] = make_uint4(0u, 0u, 0u, 0u);
-          }
+        for (int u = 0; u < kTurns; ++u) {
+          const int64_t row = min(row0 + rt * 16 + u * kRows + lane / kLPR, p.rows - 1);
+          raw[nb][rt][u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + row * p.x_row_stride +
+                                                           min(k, p.k - 16 / (int)sizeof(T)));
+          if (k >= p.k) raw[nb][rt][u] = make_uint4(0u, 0u, 0u, 0u);
         }
-      }
     }
+  };
+  auto settle_x = [&] {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+        for (int u = 0; u < kTurns; ++u) sm_x[wave][l4_piece<kLPR>(u * kRows + lane / kLPR, lane % kLPR)] = raw[nb][rt][u];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int v = 0; v < kXV; ++v) x[nb][s][rt][v] = sm_x[wave][l4_piece<kLPR>(i, (s * 4 + g) * kXV + v)];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+        __builtin_amdgcn_wave_barrier();
+      }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -137,132 +224,161 @@ __global__ __launch_bounds__(64 * kL4Waves) void linear4_kernel(const asrlayer_l
         }
   };
 
-  uint4 w[NB], wn[NB];
-  T sc[NB][kGroups][4], scn[NB][kGroups][4];
-  uint32_t zr[NB][kGroups], zrn[NB][kGroups];
-  auto load_w = [&](int cn, int first, uint4* wv, T (*s)[kGroups][4], uint32_t (*z)[kGroups]) {
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const int kb = min(first + nb * waves + wave, blocks_k - 1);  // past the last: x is zero there
-      const int64_t block = (int64_t)cn * blocks_k + kb;
-      wv[nb] = packed[block * 64 + lane];
-#pragma unroll
-      for (int q = 0; q < kGroups; ++q) {
-        const int64_t at = block * kGroups + q;
-        if constexpr (sizeof(T) == 2) {
-          const uint2 v = *reinterpret_cast<const uint2*>(scales + at * 16 + g * 4);
-          s[nb][q][0] = (T)v.x, s[nb][q][1] = (T)(v.x >> 16), s[nb][q][2] = (T)v.y, s[nb][q][3] = (T)(v.y >> 16);
-        } else {
-          const float4 v = *reinterpret_cast<const float4*>(scales + at * 16 + g * 4);
-          s[nb][q][0] = v.x, s[nb][q][1] = v.y, s[nb][q][2] = v.z, s[nb][q][3] = v.w;
-        }
-        z[nb][q] = zeros != nullptr ? (uint32_t)zeros[at * 4 + g] : 0x8888u;
-      }
+  // The turn (a block of outputs, a chunk of inputs) after one.
+  auto after = [&](int& cn, int& first) {
+    if (CHUNKED) first += chunk;
+    if (!CHUNKED || first >= blocks_k) {
+      first = 0;
+      cn += gridDim.x;
     }
   };
 
-  if (blocks_k <= chunk) load_x(0);
+  W4 a, b;  // this turn's weights and the next's
+  int cn = blockIdx.x, first = 0, cn_next = cn, first_next = 0;
+  load_w(cn, 0, a);
+  load_x(0);
+  if (!CHUNKED) settle_x();
   int buffer = 0;
-  int cn = blockIdx.x;
-  load_w(min(cn, blocks_n - 1), 0, w, sc, zr);
-  for (; cn < blocks_n; cn += gridDim.x) {
-    f32x4_t total[RT];
+  f32x4_t total[RT];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) total[rt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    for (int first = 0; first < blocks_k; first += chunk) {
-      if (blocks_k > chunk) load_x(first);
-      // The next weights this wave multiplies (the last again at the end).
-      const bool last = first + chunk >= blocks_k;
-      load_w(last ? min(cn + (int)gridDim.x, blocks_n - 1) : cn, last ? 0 : first + chunk, wn, scn, zrn);
+  for (int rt = 0; rt < RT; ++rt) total[rt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  while (cn < blocks_n) {
+    if (CHUNKED) {
+      settle_x();
+      load_x(first + chunk < blocks_k ? first + chunk : 0);
+    }
+    after(cn_next, first_next);
+    load_w(cn_next, first_next, b);  // past the last block: the last again
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const uint32_t words[4] = {w[nb].x, w[nb].y, w[nb].z, w[nb].w};
+    for (int nb = 0; nb < NB; ++nb) {
+      const uint32_t words[4] = {a.w[nb].x, a.w[nb].y, a.w[nb].z, a.w[nb].w};
 #pragma unroll
-        for (int q = 0; q < kGroups; ++q) {
-          f32x4_t acc[RT];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float zero = kOffset + (float)((zr[nb][q] >> (4 * r)) & 0xfu);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) acc[rt][r] = -zero * sums[nb][q][rt];
-          }
-#pragma unroll
-          for (int s = 0; s < kSteps; ++s) l4_step<T, RT>(words[q * kSteps + s], x[nb][q * kSteps + s], acc);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) total[rt][r] = fmaf(acc[rt][r], Elem<T>::load1(&sc[nb][q][r]), total[rt][r]);
+      for (int q = 0; q < kGroups; ++q) {
+        const uint32_t zr = a.z[nb][q / 2] >> (q % 2 * 16);
+        float sc[4];
+        if constexpr (sizeof(T) == 2) {
+          sc[0] = bf16_lo(a.s[nb][q].x), sc[1] = bf16_hi(a.s[nb][q].x);
+          sc[2] = bf16_lo(a.s[nb][q].y), sc[3] = bf16_hi(a.s[nb][q].y);
+        } else {
+          sc[0] = __uint_as_float(a.s[nb][2 * q].x), sc[1] = __uint_as_float(a.s[nb][2 * q].y);
+          sc[2] = __uint_as_float(a.s[nb][2 * q + 1].x), sc[3] = __uint_as_float(a.s[nb][2 * q + 1].y);
         }
-      }
+        f32x4_t acc[RT];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        w[nb] = wn[nb];
+        for (int r = 0; r < 4; ++r) {
+          const float zero = kOffset + (float)((zr >> (4 * r)) & 0xfu);
 #pragma unroll
-        for (int q = 0; q < kGroups; ++q) {
-          zr[nb][q] = zrn[nb][q];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) sc[nb][q][r] = scn[nb][q][r];
+          for (int rt = 0; rt < RT; ++rt) acc[rt][r] = -zero * sums[nb][q][rt];
         }
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) l4_step<T, RT>(words[q * kSteps + s], x[nb][q * kSteps + s], acc);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) total[rt][r] = fmaf(acc[rt][r], sc[r], total[rt][r]);
       }
     }
+    const float bias = a.bias;
+    a = b;
+    const int block = cn;
+    after(cn, first);
+    if (CHUNKED && cn == block) continue;  // more inputs of this block; uniform
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+    for (int rt = 0; rt < RT; ++rt) {
       *reinterpret_cast<float4*>(&sm[buffer][wave][rt][i][g * 4]) =
           make_float4(total[rt][0], total[rt][1], total[rt][2], total[rt][3]);
-    __syncthreads();
-    // Four outputs of a row a thread.
-    for (int t = threadIdx.x; t < RT * 64; t += blockDim.x) {
-      const int rt = t >> 6, r = (t >> 2) & 15, c = (t & 3) * 4;
-      const int64_t row = row0 + rt * 16 + r;
-      if (row >= p.rows) continue;
-      float y[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int u = 0; u < waves; ++u) {
-        const float4 v = *reinterpret_cast<const float4*>(&sm[buffer][u][rt][r][c]);
-        y[0] += v.x, y[1] += v.y, y[2] += v.z, y[3] += v.w;
-      }
-      T* out = static_cast<T*>(p.out) + row * p.out_row_stride;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int n = cn * 16 + c + e;
-        if (n >= p.n) continue;
-        if (p.bias != nullptr) y[e] += Elem<T>::load1(static_cast<const T*>(p.bias) + n);
-        Elem<T>::store1(out + n, y[e]);
-      }
+      total[rt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
+    // An LDS-only barrier: the weights stay in flight across it.
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    // A wave finishes 2 RT rows, 16 lanes a row.  Every wave issues the same stores
+    // (nothing leaves past a row's range): were they in a branch, the wait for the
+    // next weights would be set for the path without them and cover later loads too.
+    constexpr int kFinish = RT * 16 / W;
+    auto finish = [&](int row_w) {
+      const int mine = row_w + min(g, kFinish - 1);
+      float y = 0.f;
+      for (int u = 0; u < waves; ++u) y += sm[buffer][u][mine >> 4][mine & 15][i];
+      y += bias;
+#pragma unroll
+      for (int r = 0; r < kFinish; ++r) {
+        const int64_t row = row0 + row_w + r;
+        const auto rsrc = buffer_rsrc(static_cast<T*>(p.out) + row * p.out_row_stride + block * 16,
+                                      row < p.rows ? min(16, p.n - block * 16) * (int)sizeof(T) : 0);
+        const uint32_t off = g == r ? i * sizeof(T) : 0xffff0000u;
+        if constexpr (sizeof(T) == 2)
+          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (__bf16)y), rsrc, off, 0, 0);
+        else
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(y), rsrc, off, 0, 0);
+      }
+    };
+    finish(wave * kFinish);
+    for (int row_w = (waves + wave) * kFinish; row_w < 16 * RT; row_w += waves * kFinish) finish(row_w);
     buffer ^= 1;
   }
 }
 
-template <typename T, int RT, int NB>
-hipError_t launch_l4_group(const asrlayer_linear4_params& p, int waves, hipStream_t stream) {
+template <typename T, int W, int RT, int NB, bool CHUNKED>
+hipError_t launch_l4_group(const asrlayer_linear4_params& p, hipStream_t stream) {
   const int blocks_n = (p.n + 15) / 16, blocks_k = (p.k + 127) / 128;
-  const int row_blocks = (int)((p.rows + RT * 16 - 1) / (RT * 16));
-  const int most = 512 / row_blocks < 1 ? 1 : 512 / row_blocks;
-  const dim3 grid(blocks_n < most ? blocks_n : most, row_blocks), block(64 * waves);
-  if (p.group == 32)
-    hipLaunchKernelGGL((linear4_kernel<T, RT, NB, 32>), grid, block, 0, stream, p, blocks_n, blocks_k);
-  else if (p.group == 64)
-    hipLaunchKernelGGL((linear4_kernel<T, RT, NB, 64>), grid, block, 0, stream, p, blocks_n, blocks_k);
+  const int64_t row_blocks = (p.rows + RT * 16 - 1) / (RT * 16);
+  // One workgroup a CU, or two where they fit and the blocks are many: a second one
+  // loads x again, so at fewer blocks it costs (16 rows of 2048 to 16384 outputs, 1024
+  // blocks: 7.7 us with 512 workgroups, 7.3 with 256; 24576: 9.1 and 9.2; 32768: 11.0
+  // and 11.8; 4 rows to 151936: 34.9 and 42.9).  Workgroups of the same outputs, one
+  // a block of rows, lie a multiple of 8 apart, on one XCD, whose L2 then reads the
+  // weights once (96 rows to 12288: 14.7 us for 15.1).
+  const bool two = (p.group == 32 ? l4_per_cu<T, W, RT, NB, 32, CHUNKED>()
+                                  : l4_per_cu<T, W, RT, NB, 128, CHUNKED>()) > 1 && blocks_n * row_blocks >= 2048;
+  int64_t across = (two ? 512 : 256) / row_blocks;
+  if (across > 8) across -= across % 8;
+  if (across < 1) across = 1;
+  const dim3 grid(blocks_n < across ? blocks_n : across, row_blocks), block(64 * (blocks_k < W ? blocks_k : W));
+  if constexpr (W == 8 || RT == 1) {
+    if (p.group == 32) {
+      hipLaunchKernelGGL((linear4_kernel<T, W, RT, NB, 32, CHUNKED>), grid, block, 0, stream, p, blocks_n, blocks_k);
+      return hipGetLastError();
+    }
+  }
+  if (p.group == 64)
+    hipLaunchKernelGGL((linear4_kernel<T, W, RT, NB, 64, CHUNKED>), grid, block, 0, stream, p, blocks_n, blocks_k);
   else
-    hipLaunchKernelGGL((linear4_kernel<T, RT, NB, 128>), grid, block, 0, stream, p, blocks_n, blocks_k);
+    hipLaunchKernelGGL((linear4_kernel<T, W, RT, NB, 128, CHUNKED>), grid, block, 0, stream, p, blocks_n, blocks_k);
   return hipGetLastError();
 }
 
+// Two row tiles where 256 workgroups are left: half the reads of the weights (64 x
+// 2048 x 12288: 11.2 us for 13.1; 64 x 1024 x 4096: 4.8 for 5.2); with fewer, one
+// (24 x 5120 x 1280: 6.9 us for 9.4).  All of x in registers where it fits, so that
+// x is read once a workgroup; else in chunks, again for each block of outputs:
+// 64 x 4096 x 12288 in 17.6 us with 16 waves holding x, 35.5 in chunks; 16 x 4096 x
+// 6144 with four blocks a wave in 8.1 us, 9.2 in chunks.  At 256 blocks of outputs
+// or fewer a workgroup has one and nothing to keep x for.  Chunks take 16 waves where that
+// halves their number: 8 x 6144 x 2048 (6 chunks or 3) in 6.7 us for 7.7; at 24 x
+// 5120 x 1280 (5 or 3) 7.2 for 6.9.  Groups
+// of 32 need more registers than 16 waves have: 32 x 4096 x 6144 in 12.8 us with four
+// blocks a wave, 19.0 with 16 waves.  float32's x is twice as large: 8 waves always.
 template <typename T>
 hipError_t launch_l4(const asrlayer_linear4_params& p, hipStream_t stream) {
-  const int blocks_k = (p.k + 127) / 128;
-  const int waves = blocks_k < kL4Waves ? blocks_k : kL4Waves;
-  const int per_wave = (blocks_k + waves - 1) / waves;
-  if (p.rows <= 16) {
-    if (per_wave <= 1) return launch_l4_group<T, 1, 1>(p, waves, stream);
-    if (per_wave <= 2) return launch_l4_group<T, 1, 2>(p, waves, stream);
-    return launch_l4_group<T, 1, 4>(p, waves, stream);
+  const int blocks_n = (p.n + 15) / 16, blocks_k = (p.k + 127) / 128;
+  const bool four = sizeof(T) == 2 && blocks_k > 16 && blocks_k <= 32 && blocks_n > 256;  // blocks a wave
+  if (p.rows > 16 && (int64_t)blocks_n * ((p.rows + 31) / 32) >= 256 && !(four && p.group == 32)) {
+    if (blocks_k <= 8) return launch_l4_group<T, 8, 2, 1, false>(p, stream);
+    if constexpr (sizeof(T) == 2) {
+      if (blocks_k <= 16) return launch_l4_group<T, 8, 2, 2, false>(p, stream);
+      if (blocks_k <= 32 && p.group > 32) return launch_l4_group<T, 16, 2, 2, false>(p, stream);
+    }
+    return launch_l4_group<T, 8, 2, 1, true>(p, stream);
   }
-  if (p.rows <= 32) {
-    if (per_wave <= 1) return launch_l4_group<T, 2, 1>(p, waves, stream);
-    return launch_l4_group<T, 2, 2>(p, waves, stream);
+  if (blocks_k <= 8) return launch_l4_group<T, 8, 1, 1, false>(p, stream);
+  if (blocks_k <= 16) return launch_l4_group<T, 8, 1, 2, false>(p, stream);
+  if constexpr (sizeof(T) == 2) {
+    if (four) return launch_l4_group<T, 8, 1, 4, false>(p, stream);
+    if ((blocks_k + 15) / 16 * 2 <= (blocks_k + 7) / 8) return launch_l4_group<T, 16, 1, 1, true>(p, stream);
   }
-  return launch_l4_group<T, 4, 1>(p, waves, stream);
+  return launch_l4_group<T, 8, 1, 1, true>(p, stream);
 }
 
 }  // namespace

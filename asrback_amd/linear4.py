@@ -45,6 +45,17 @@ class Weight4:
     group: int
 
 
+def _check_layout(packed: Tensor, scales: Tensor, zeros: Tensor | None, outputs: int, inputs: int, group: int) -> None:
+    """The tensors are as large as the kernel reads them, and in its order (a module's
+    buffers can be replaced, and take the strides of another memory format)."""
+    blocks = -(-outputs // _BLOCK_N) * -(-inputs // _BLOCK_K)
+    groups = blocks * (_BLOCK_K // group)
+    if not (packed.numel() == blocks * 256 and packed.dtype is torch.int32 and packed.is_contiguous()
+            and scales.numel() == groups * 16 and scales.is_contiguous()
+            and (zeros is None or (zeros.numel() == groups * 8 and zeros.dtype is torch.uint8 and zeros.is_contiguous()))):
+        raise ValueError(f"packed, scales and zeros are not a packed ({outputs}, {inputs}) matrix with groups of {group}")
+
+
 def _check_group(group: int, inputs: int) -> None:
     if group not in GROUPS:
         raise ValueError(f"group {group} (supported: {', '.join(map(str, GROUPS))})")
@@ -90,10 +101,10 @@ def pack4(values: Tensor, scales: Tensor, zeros: Tensor | None = None) -> Weight
         packed[first:last] = torch.stack(pairs, -1).contiguous().view(torch.int32).view(-1, blocks_k, 64, 4)
 
     def spread(t: Tensor) -> Tensor:
-        """``(outputs, groups)`` as ``(block_n, groups, 16)``, zeros around it."""
+        """``(outputs, groups)`` as ``(block_n, block_k, 4, groups of a block, 4)``."""
         whole = t.new_zeros((blocks_n * _BLOCK_N, groups))
         whole[:outputs, : t.shape[1]] = t
-        return whole.view(blocks_n, _BLOCK_N, groups).transpose(1, 2).contiguous()
+        return whole.view(blocks_n, 4, 4, blocks_k, -1).permute(0, 3, 1, 4, 2).contiguous()
 
     if zeros is not None:
         nibbles = spread(zeros)
@@ -111,7 +122,7 @@ def unpack4(weight: Weight4) -> Tensor:
     values = values.reshape(blocks_n * _BLOCK_N, -1, weight.group).float()
 
     def gather(t: Tensor) -> Tensor:
-        return t.transpose(1, 2).reshape(blocks_n * _BLOCK_N, -1, 1).float()
+        return t.permute(0, 2, 4, 1, 3).reshape(blocks_n * _BLOCK_N, -1, 1).float()
 
     zeros = 8.0
     if weight.zeros is not None:
@@ -150,19 +161,27 @@ def linear4(x: Tensor, weight: Weight4, bias: Tensor | None = None, *, out: Tens
     """``x @ w.T + bias`` for the matrix ``w`` that ``weight`` stands for
     (``asrlayer_linear4``): ``x`` ``(..., inputs)`` float32 or bfloat16, the
     type of the weight's scales, ``bias`` ``(outputs,)`` of the same type.
-    Sums are float32 and rounded once.  Built for the few rows of a decoder
-    step or a drafted tree (up to 64 are read against the weights in one
-    pass); more rows are right, the weights being read once for each 64.
-    Returns ``(..., outputs)``."""
+    Sums are float32 and rounded once; a row with an infinity or a NaN comes out
+    without a finite value.  Built for the few rows of a decoder step or a
+    drafted tree (up to 32 are read against the weights in one pass); more rows
+    are right, the weights being read again for each 32.  ``out`` must not share
+    memory with ``x``.  Returns ``(..., outputs)``."""
+    return _product(x, weight.packed, weight.scales, weight.zeros, weight.outputs, weight.inputs, weight.group, bias, out)
+
+
+def _product(x: Tensor, packed: Tensor, scales: Tensor, zeros: Tensor | None, outputs: int, inputs: int, group: int,
+             bias: Tensor | None, out: Tensor | None) -> Tensor:
     shape = x.shape
-    packed, scales, zeros, outputs, inputs = weight.packed, weight.scales, weight.zeros, weight.outputs, weight.inputs
     if not shape or shape[-1] != inputs:
         raise ValueError(f"x must be (..., {inputs}), got {tuple(shape)}")
     dtype, index = x.dtype, x.get_device()
     if dtype is not scales.dtype:
         raise TypeError(f"x is {dtype}, the weight's scales {scales.dtype}")
+    if dtype not in _DTYPES:
+        raise TypeError(f"linear4 supports float32 and bfloat16, got {dtype}")
     if bias is not None and (bias.shape != (outputs,) or bias.dtype is not dtype):
         raise ValueError(f"bias must be {dtype} ({outputs},), got {bias.dtype} {tuple(bias.shape)}")
+    _check_layout(packed, scales, zeros, outputs, inputs, group)
     if index < 0:
         raise RuntimeError(f"linear4 runs on the GPU only; got a tensor on {x.device}")
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
@@ -179,7 +198,7 @@ def linear4(x: Tensor, weight: Weight4, bias: Tensor | None = None, *, out: Tens
         bias = bias.contiguous()
     params = _lib.pack_linear4(
         rows.data_ptr(), rows.stride(0), packed.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(),
-        0 if bias is None else bias.data_ptr(), out.data_ptr(), outputs, rows.shape[0], outputs, inputs, weight.group,
+        0 if bias is None else bias.data_ptr(), out.data_ptr(), outputs, rows.shape[0], outputs, inputs, group,
         _DTYPES[dtype])
     status = _lib.load().asrlayer_linear4(params, _raw_stream(index))
     if status:
@@ -190,8 +209,8 @@ def linear4(x: Tensor, weight: Weight4, bias: Tensor | None = None, *, out: Tens
 class Linear4(nn.Module):
     """``nn.Linear`` with 4-bit weights (:func:`linear4`); made by
     :meth:`from_linear` or from a :class:`Weight4`.  The matrix lies in
-    buffers, so ``.to(device)`` and state dicts carry it; its type is fixed
-    (``.to(dtype)`` is refused by the next call)."""
+    buffers, so ``.to(device)`` and state dicts carry it, and ``.to(dtype)``
+    rounds its scales and bias."""
 
     def __init__(self, weight: Weight4, bias: Tensor | None = None) -> None:
         super().__init__()
@@ -210,7 +229,8 @@ class Linear4(nn.Module):
         return Weight4(self.packed, self.scales, self.zeros, self.out_features, self.in_features, self.group)
 
     def forward(self, x: Tensor) -> Tensor:
-        return linear4(x, self.weight4, self.bias)
+        return _product(x, self.packed, self.scales, self.zeros, self.out_features, self.in_features, self.group, self.bias,
+                        None)
 
     def extra_repr(self) -> str:
         return (f"in_features={self.in_features}, out_features={self.out_features}, group={self.group}, "

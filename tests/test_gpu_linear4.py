@@ -43,7 +43,9 @@ SHAPES = [
     (1, 32, 1, 32), (1, 2048, 2048, 128), (2, 64, 15, 64), (3, 384, 1536, 32), (5, 96, 17, 32), (7, 192, 33, 64),
     (16, 2048, 300, 128), (17, 1024, 40, 64), (31, 1280, 100, 32), (33, 640, 24, 128), (48, 6144, 64, 64),
     (64, 2048, 10000, 128), (65, 256, 31, 128), (130, 1152, 50, 32), (4, 16896, 40, 128), (1, 5120, 9, 32),
-    (20, 4224, 21, 128), (300, 2048, 96, 64),
+    (20, 4224, 21, 128), (300, 2048, 96, 64), (64, 6144, 2048, 64), (33, 2048, 4100, 32), (40, 1024, 9000, 32),
+    (64, 4096, 2100, 128), (50, 3200, 2100, 32), (3, 4096, 4200, 64), (9, 2592, 4200, 32), (7, 2304, 4130, 128),
+    (70, 1024, 11000, 64), (40, 2048, 16400, 64), (5, 10240, 70, 64),
 ]
 
 

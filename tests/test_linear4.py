@@ -20,16 +20,17 @@ def test_layout_of_a_packed_matrix():
         weight = pack4(values, scales, zeros)
         blocks_n, blocks_k = -(-outputs // 16), -(-inputs // 128)
         assert weight.packed.shape == (blocks_n, blocks_k, 64, 4) and weight.packed.dtype == torch.int32
-        assert weight.scales.shape == (blocks_n, blocks_k * 128 // group, 16)
-        assert weight.zeros.shape == (blocks_n, blocks_k * 128 // group, 8)
+        assert weight.scales.shape == (blocks_n, blocks_k, 4, 128 // group, 4)
+        assert weight.zeros.shape == (blocks_n, blocks_k, 4, 128 // group, 2)
         order = (0, 2, 4, 6, 1, 3, 5, 7)
         for n, k in torch.stack((torch.randint(0, outputs, (60,), generator=g),
                                  torch.randint(0, inputs, (60,), generator=g)), 1).tolist():
             block, s, lane_group, j = k // 128, k % 128 // 32, k % 32 // 8, k % 8
             word = int(weight.packed[n // 16, block, 16 * lane_group + n % 16, s])
             assert word >> 4 * order.index(j) & 15 == int(values[n, k])
-            assert weight.scales[n // 16, k // group, n % 16] == scales[n, k // group]
-            assert int(weight.zeros[n // 16, k // group, n % 16 // 2]) >> 4 * (n % 2) & 15 == int(zeros[n, k // group])
+            at = n // 16, block, n % 16 // 4, k % 128 // group
+            assert weight.scales[at][n % 4] == scales[n, k // group]
+            assert int(weight.zeros[at][n % 4 // 2]) >> 4 * (n % 2) & 15 == int(zeros[n, k // group])
         whole = (values.float().view(outputs, -1, group) - zeros.float()[..., None]) * scales[..., None]
         assert torch.equal(unpack4(weight), whole.flatten(1))
         plain = pack4(values, scales)
@@ -50,7 +51,7 @@ def test_rounding():
             weight = quantize4(matrix, 64, symmetric)
             assert weight.scales.dtype == dtype
             back = unpack4(weight).view(20, 4, 64)
-            steps = weight.scales.transpose(1, 2).reshape(32, 4)[:20].float()
+            steps = weight.scales.permute(0, 2, 4, 1, 3).reshape(32, 4)[:20].float()
             # Half a step; with a zero point, which is rounded to a step as well, one.
             # The scale, rounded to bf16 (2^-8), moves the ends by 7 or 15 of its own.
             slack = (0.5 if symmetric else 1.0) + (15 * 2**-8 if dtype == torch.bfloat16 else 1e-4)
@@ -93,7 +94,24 @@ def test_refusals():
         linear4(torch.zeros(3, 64, dtype=torch.bfloat16), weight)
     with pytest.raises(ValueError, match="bias"):
         linear4(torch.zeros(3, 64), weight, torch.zeros(9))
-    assert Linear4(weight).weight4 == weight
+    with pytest.raises(TypeError, match="float32 and bfloat16"):
+        Linear4(weight).half()(torch.zeros(3, 64, dtype=torch.float16))
+    layer = Linear4(weight)
+    assert layer.weight4 == weight
+    # Buffers that are not what the kernel would read.
+    matrix = pack4(torch.zeros(40, 300 * 32, dtype=torch.uint8), torch.ones(40, 300))
+    assert matrix.packed.shape[:2] == (3, 75)
+    for name, bad in (("packed", layer.packed[:, :, :32].contiguous()), ("packed", layer.packed.float()),
+                      ("scales", layer.scales[..., :2].contiguous()), ("zeros", torch.zeros(3, dtype=torch.uint8))):
+        layer = Linear4(weight)
+        setattr(layer, name, bad)
+        with pytest.raises(ValueError, match="packed"):
+            layer(torch.zeros(3, 64))
+    wide = Linear4(matrix)
+    wide.packed = wide.packed.to(memory_format=torch.channels_last)
+    assert not wide.packed.is_contiguous()
+    with pytest.raises(ValueError, match="packed"):
+        wide(torch.zeros(3, 9600))
 
     lib = _lib.load()
     p = _lib.Linear4Params()
