@@ -49,6 +49,8 @@ namespace {
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+typedef short i16x2_t __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
 
@@ -77,6 +79,9 @@ struct TreeShape {
   // The most waves of a workgroup (of a kilobyte a position, four: 512 registers
   // each).
   static constexpr int kWaves = HD * kES > 512 ? 4 : 8;
+  // Waves the registers leave room for on a SIMD, said to the compiler: for one of
+  // four waves it would take twice the registers, and half the workgroups fit.
+  static constexpr int kWavesPerSimd = HD * kES > 512 ? 1 : 2;
   static constexpr int kKeys = 16 * kSub;           // keys of a tile
   static constexpr int kKV = HD * kES / 64;         // a lane's 16-byte pieces of a key part
   static constexpr int kLPR = HD * kES / 16;        // 16-byte pieces of a position
@@ -146,12 +151,13 @@ __device__ __forceinline__ float row_sum(float x) {
   return a + b;
 }
 
-// A dword of T with its infinities and NaN replaced by zeros.
+// Ones over the infinities and NaN of a dword of T: one more in the exponent carries
+// into the sign.
 template <typename T>
-__device__ __forceinline__ uint32_t finite_part(uint32_t x) {
-  if constexpr (sizeof(T) == 4) return (x & 0x7f800000u) == 0x7f800000u ? 0u : x;
-  const uint32_t lo = (x & 0x7f80u) == 0x7f80u ? 0u : x & 0xffffu;
-  return (x & 0x7f800000u) == 0x7f800000u ? lo : (x & 0xffff0000u) | lo;
+__device__ __forceinline__ uint32_t not_finite(uint32_t x) {
+  if constexpr (sizeof(T) == 4) return (uint32_t)((int32_t)((x & 0x7fffffffu) + 0x00800000u) >> 31);
+  const u16x2_t t = __builtin_bit_cast(u16x2_t, x & 0x7fff7fffu) + (unsigned short)0x80;
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2_t, t) >> (short)15);
 }
 
 // Offset of a load that is to return zeros.
@@ -264,7 +270,7 @@ __device__ __forceinline__ int lds_piece(int r, int c) {
 
 // A workgroup: RT x 16 query rows, its W waves the shares of the keys.
 template <typename T, int HD, int RT, int W, bool PAGED>
-__global__ __launch_bounds__(64 * W) void tree_kernel(const TreeArgs a) {
+__global__ __launch_bounds__(64 * W, (TreeShape<T, HD>::kWavesPerSimd)) void tree_kernel(const TreeArgs a) {
   using S = TreeShape<T, HD>;
   constexpr int kSub = S::kSub, kKeys = S::kKeys, kKV = S::kKV, kVD = S::kVD, kEV = S::kEV, kNC = S::kNC;
   constexpr int kES = S::kES, kDC = S::kDC;
@@ -307,14 +313,16 @@ __global__ __launch_bounds__(64 * W) void tree_kernel(const TreeArgs a) {
   uint4* const sm_q = sm_pool + W * kKeyPieces;
   float(*const sm_o)[16][kDC + 4] = reinterpret_cast<float(*)[16][kDC + 4]>(sm_pool);
 
-  // The workgroup's query rows (rows past the last repeat it).
+  // The workgroup's query rows (rows past the last repeat it).  Vectors of the
+  // compiler's own: an array of structs it moves to LDS, addressed by sizes that it
+  // reads from the launch's packet in host memory (6 us).
   constexpr int kTurns = (kQueryPieces + 64 * W - 1) / (64 * W);
-  uint4 staged[kTurns];
+  u32x4_t staged[kTurns];
 #pragma unroll
   for (int u = 0; u < kTurns; ++u) {
     const int at = min((int)threadIdx.x + u * 64 * W, kQueryPieces - 1);
     const Row r = row_of(a, group, min(rb * kRows + at / kLPR, a.rows - 1));
-    staged[u] = reinterpret_cast<const uint4*>(
+    staged[u] = reinterpret_cast<const u32x4_t*>(
         static_cast<const T*>(p.q) + (int64_t)b * p.q_batch_stride + (int64_t)r.token * p.q_token_stride +
         (int64_t)(hkv * group + r.head) * p.q_head_stride)[at % kLPR];
   }
@@ -437,7 +445,7 @@ __global__ __launch_bounds__(64 * W) void tree_kernel(const TreeArgs a) {
 #pragma unroll
   for (int u = 0; u < kTurns; ++u) {
     const int at = min((int)threadIdx.x + u * 64 * W, kQueryPieces - 1);
-    sm_q[lds_piece<kLPR>(at / kLPR, at % kLPR)] = staged[u];
+    sm_q[lds_piece<kLPR>(at / kLPR, at % kLPR)] = __builtin_bit_cast(uint4, staged[u]);
   }
   // An LDS-only barrier: the keys and values stay in flight across it.
   auto lds_barrier = [] {
@@ -558,7 +566,7 @@ __global__ __launch_bounds__(64 * W) void tree_kernel(const TreeArgs a) {
     }
 
     // O^T += V^T P^T
-    bool bad = false;
+    uint32_t bad = 0;
 #pragma unroll
     for (int c = 0; c < kNC; ++c) {
       uint32_t x[kSub][4][kVD];  // the lane's piece of its four keys' values
@@ -574,8 +582,9 @@ __global__ __launch_bounds__(64 * W) void tree_kernel(const TreeArgs a) {
             // weight of zero times it is not zero: such elements leave the product,
             // and the rows that do see them take them as they are, below.
             if constexpr (drafted) {
-              x[h][r][d] = finite_part<T>(at[d]);
-              bad = bad || x[h][r][d] != at[d];
+              const uint32_t left_out = not_finite<T>(at[d]);
+              x[h][r][d] = at[d] & ~left_out;
+              bad |= left_out;
             }
           }
         }
@@ -610,7 +619,7 @@ __global__ __launch_bounds__(64 * W) void tree_kernel(const TreeArgs a) {
       }
     }
     if constexpr (drafted) {
-      if (__any(bad)) infinite |= 1u << (t - cache_tiles);
+      if (__any(bad != 0)) infinite |= 1u << (t - cache_tiles);
     }
     load_values(t + W, next_pages);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
@@ -670,7 +679,7 @@ __global__ __launch_bounds__(64 * W) void tree_kernel(const TreeArgs a) {
             const int at = (dc * kParts + c) * kEV + e;
             x.x = o[rt][at][r], x.y = o[rt][at + 1][r], x.z = o[rt][at + 2][r], x.w = o[rt][at + 3][r];
             if (mask[rt] == 0) x = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (rt * 16 + i < held) *reinterpret_cast<float4*>(&sm_o[wave][i][(c * 16 + g * 4 + r) * kEV + e]) = x;
+            *reinterpret_cast<float4*>(&sm_o[wave][i][(c * 16 + g * 4 + r) * kEV + e]) = x;
           }
       __syncthreads();
       const int items = min(max(held - rt * 16, 0), 16) * kVecs;
@@ -792,7 +801,8 @@ hipError_t launch_head(const TreeArgs& a, const TreePlan& plan, hipStream_t stre
     if (plan.row_tiles == 1 && plan.waves == 8) return launch_waves<T, HD, 1, 8>(a, stream);
   }
   if constexpr (HD * sizeof(T) <= 256) {
-    if (plan.row_tiles == 2) return launch_waves<T, HD, 2, 8>(a, stream);
+    if (plan.row_tiles == 2)
+      return plan.waves == 8 ? launch_waves<T, HD, 2, 8>(a, stream) : launch_waves<T, HD, 2, 4>(a, stream);
   }
   return launch_waves<T, HD, 1, 4>(a, stream);
 }
@@ -824,10 +834,13 @@ TreePlan tree_plan(const asrlayer_tree_params& p) {
   plan.row_tiles = tiles >= 2 && bytes <= 256 && units2 * p.max_len_k >= 256 * 1024 ? 2 : 1;
   plan.row_blocks = (tiles + plan.row_tiles - 1) / plan.row_tiles;
   const long long units = pairs * plan.row_blocks;
-  // More workgroups than CUs: of four waves, of which two fit a CU, so that one's
-  // beginning and end hide behind the other (16 rows, 512 workgroups over 480
-  // keys: 30.0 us, 33.9 of eight; 64 workgroups, 14.4 and 11.5).
-  plan.waves = bytes > 512 || (plan.row_tiles == 1 && units > 256) ? 4 : 8;
+  // More workgroups than CUs: of four waves, of which two or three fit a CU, so that
+  // one's beginning and end hide behind the others (16 rows, 512 workgroups over 480
+  // keys: 27.7 us, 33.2 of eight; 128 rows, 1536 over 900: 76.9 and 100.7; 248 rows of
+  // 64 dimensions, 1056 over 54: 15.0 and 29.4; 64 workgroups over 480: 14.4 and 11.5).
+  // Two waves gain where keys are few (11.4 there) and lose elsewhere (86.1 at 900
+  // keys, 108.4 for 86.2 at 3500).
+  plan.waves = bytes > 512 || units > 256 ? 4 : 8;
   // Splits up to a workgroup a CU, of half a turn's keys at least, where they save two
   // and a half turns: partials, arrival and fold cost about as much (two splits of
   // 480 keys 12.9 us, unsplit 11.5; 1216 keys of 512 bytes: four 15.0, unsplit 20.1).

@@ -141,6 +141,12 @@ CASES = [
     (BF16, 33, 2, 16, 8, 128, 96, [33, 96, 0, 1] * 8 + [17], 32, "slab"),
     (F32, 40, 1, 8, 8, 128, 64, [33, 64, 0, 1] * 10, 0, "slab"),
     (BF16, 70, 3, 8, 4, 256, 48, [33, 48, 0, 1, 20] * 14, 0, "slab"),
+    (F32, 22, 17, 12, 4, 128, 64, [33, 64, 0, 1] * 5 + [5, 50], 0, "slab"),
+    (F32, 17, 18, 16, 4, 256, 64, [33, 64, 0, 1] * 4 + [50], 0, "slab"),
+    (BF16, 16, 40, 8, 4, 128, 1536, [33, 500, 0, 1] * 4, 0, "slab"),
+    (BF16, 22, 40, 8, 4, 64, 1024, [33, 300, 0, 1] * 5 + [1024, 17], 64, "slab"),
+    (BF16, 16, 40, 8, 4, 128, 1536, [33, 500, 0, 130] * 4, 128, "slab"),
+    (F32, 22, 40, 8, 4, 64, 1024, [33, 300, 0, 1] * 5 + [200, 17], 0, "slab"),
     # pages: shorter than a tile, of one tile, longer; a last page in part
     (BF16, 3, 8, 4, 2, 128, 112, [111, 16, 0], 16, "slab"),
     (BF16, 2, 8, 4, 2, 128, 448, [447, 130], 64, "slab"),
