@@ -843,13 +843,27 @@ TreePlan tree_plan(const asrlayer_tree_params& p) {
   plan.waves = bytes > 512 || units > 256 ? 4 : 8;
   // Splits up to a workgroup a CU, of half a turn's keys at least, where they save two
   // and a half turns: partials, arrival and fold cost about as much (two splits of
-  // 480 keys 12.9 us, unsplit 11.5; 1216 keys of 512 bytes: four 15.0, unsplit 20.1).
+  // 480 keys 12.9 us, unsplit 11.5; 1216 keys of 512 bytes: four 14.6, unsplit 19.4).
   const int turn = plan.waves * (bytes > 256 || p.dtype == ASRATTN_F32 ? 16 : 32);  // keys a workgroup takes at once
   plan.splits = 1;
   if (units < 256) {
+    // A turn takes about 1.2 us and a split costs the fold 0.13: the sum of both is least
+    // at about the root of eight times the turns (6 rows over 3000 float32 keys of
+    // 64: 14.4 us with 42 splits, 10.4 with 14, 14.9 with 4; 2 rows over 4000: 13.5
+    // with 32, 10.8 with 11; 16000: 21.8 with 32, 21.1 with 22).
+    int most = 1;
+    while (most < 64 && (long long)(most + 1) * (most + 1) * turn <= 8LL * p.max_len_k) ++most;
+    // The workgroups of a range of keys share an XCD of 32 CUs: no more ranges than
+    // whole ones fit (168 rows in 6 blocks, 6 pairs over 10000 keys: 43.8 us with 7
+    // splits, 36 workgroups on two XCDs, 29.1 with 6).
+    if (plan.row_blocks > 1) {
+      const long long whole = 32 / plan.row_blocks * 8 / (pairs < 1 ? 1 : pairs);
+      most = most < whole ? most : (int)whole;
+    }
     const int by_units = (int)(256 / (units < 1 ? 1 : units)), by_keys = p.max_len_k / (turn / 2);
-    const int s = by_units < by_keys ? by_units : by_keys;
-    if (s > 1 && (long long)p.max_len_k * (s - 1) * 2 >= 5LL * turn * s) plan.splits = s > 64 ? 64 : s;
+    most = most < by_units ? most : by_units;
+    most = most < by_keys ? most : by_keys;
+    if (most > 1 && (long long)p.max_len_k * (most - 1) * 2 >= 5LL * turn * most) plan.splits = most;
   }
   // One workgroup folds 128 KB of partials in about the time of a launch (65511
   // keys, 262 KB: 67.3 us with a launch, 69.0 without; 64 KB: 16.4 and 15.0).

@@ -110,6 +110,7 @@ def test_workspace_size(lib):
     from asrback_amd.drafts import tree_workspace_size
 
     assert tree_workspace_size(64, 8, 16, 8, 128, 1024) == 0  # 512 units fill the GPU unsplit
+    assert tree_workspace_size(0, 48, 16, 8, 128, 4096) >= 0
     one = tree_workspace_size(1, 8, 16, 8, 128, 4096)
     assert one >= 256 * 16 * 128 * 4 and one % 256 == 0
     for bad in (dict(head_dim=96), dict(tokens=65), dict(tokens=0), dict(heads_q=15)):
