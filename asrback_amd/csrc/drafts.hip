@@ -46,7 +46,7 @@ __global__ __launch_bounds__(64) void accept_kernel(const int64_t* tokens, const
   const int64_t most = limit != nullptr ? load_uniform(limit + b) : width;
   int now = 0, steps = 0;
   int64_t mine = -1, said = -1;
-  bool going = most > 0 && parents[b * parents_batch_stride] >= -1;
+  bool going = most > 0 && __builtin_amdgcn_readfirstlane((int)(parent >= -1)) != 0;
   while (going) {
     const uint64_t chosen = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(choice >> 32), now) << 32 |
                             (uint32_t)__builtin_amdgcn_readlane((int)choice, now);
@@ -70,15 +70,15 @@ __global__ __launch_bounds__(64) void accept_kernel(const int64_t* tokens, const
 // values, 16 bytes a thread; the others end at once.
 __global__ __launch_bounds__(256) void commit_kernel(const asrlayer_commit_params p, int es) {
   const int step = blockIdx.x, b = blockIdx.y, layer = blockIdx.z;
-  if (step >= load_uniform(p.count + b)) return;
-  const int64_t from = load_uniform(p.path + (int64_t)b * p.tokens + step);
+  // Loaded together: each would be a round trip of its own.
+  const int64_t count = load_uniform(p.count + b), from = load_uniform(p.path + (int64_t)b * p.tokens + step);
   const int64_t n = p.lengths64 ? load_uniform(static_cast<const int64_t*>(p.lengths) + b)
                                 : (int64_t)load_uniform(static_cast<const int32_t*>(p.lengths) + b);
-  const int64_t to = n + step;
-  if (from < 0 || from >= p.tokens || n < 0 || n >= p.max_len_k || to >= p.max_len_k) return;
-  int64_t row = b, slot = to;
+  if (step >= count || from < 0 || from >= p.tokens || n < 0 || n >= p.max_len_k - step) return;
+  const int to = (int)n + step;
+  int row = b, slot = to;
   if (p.block_table != nullptr) {
-    const int64_t page = to / p.page_size;
+    const int page = to / p.page_size;
     row = load_uniform(p.block_table + (int64_t)b * p.bt_stride + page);
     slot = to - page * p.page_size;
     if (row < 0 || row >= p.num_pages) return;
