@@ -5,7 +5,8 @@ for the exact result, rounded once.  Real values are held to what the kernel
 rounds: the result once (2^-8 of it in bf16, 2^-24 in float32), and its float32
 sums: per output at most 2^-24 c sum |x| |scale| times the values an operand and
 its offset reach (bf16: 2 x 143, float32: 2 x 15), c the additions on a value's way
-(twice the group's, one a group, the waves').
+(twice the group's, in float32, whose x goes in three parts, four times; one a group,
+the waves').
 """
 
 from __future__ import annotations
@@ -46,6 +47,7 @@ SHAPES = [
     (20, 4224, 21, 128), (300, 2048, 96, 64), (64, 6144, 2048, 64), (33, 2048, 4100, 32), (40, 1024, 9000, 32),
     (64, 4096, 2100, 128), (50, 3200, 2100, 32), (3, 4096, 4200, 64), (9, 2592, 4200, 32), (7, 2304, 4130, 128),
     (70, 1024, 11000, 64), (40, 2048, 16400, 64), (5, 10240, 70, 64),
+    (3, 2304, 4300, 32), (20, 2688, 4200, 128), (36, 4352, 4300, 64), (5, 4224, 8400, 64), (35, 4352, 9000, 32),
 ]
 
 
@@ -86,8 +88,8 @@ def test_real_values(dtype, rows, inputs, outputs, group):
     points = None if points is None else points[at]
     ref = x.double() @ matrix(values[at], scales[at], points, group).T
     sums = x.double().abs() @ scales[at].double().repeat_interleave(group, 1).T
-    reach, step = (286, 2.0**-8) if dtype == BF16 else (30, 2.0**-24)
-    bound = step * ref.abs() + 2.0**-24 * (2 * group + inputs // group + 32) * reach * sums
+    reach, step, ways = (286, 2.0**-8, 2) if dtype == BF16 else (30, 2.0**-24, 4)
+    bound = step * ref.abs() + 2.0**-24 * (ways * group + inputs // group + 32) * reach * sums
     assert ((out[:, at] - ref).abs() <= bound).all()
     # Far closer in the mean: the sums' errors do not add up.
     norm = float((out[:, at] - ref).norm() / ref.norm())
