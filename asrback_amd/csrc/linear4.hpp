@@ -29,6 +29,9 @@
 //     the caches 33.8, but 8.0 for 7.4 at 64 x 2048 x 4096 and 13.0 for 12.2 at 64
 //     x 2048 x 12288).  The waves' sums meet in LDS once a block (two buffers, one
 //     barrier that leaves the loads in flight).
+//   * The groups' sums of x are products with ones, on the matrix cores that idle
+//     meanwhile (64 x 6144 x 2048: 9.8 us for 12.2 with additions; the zero points'
+//     products there as well, as one of depth one, gave 10.1).
 //   * Every wave of every turn issues the same loads and stores, absent ones with an
 //     empty range: the waits count them, and a branch would set them for its shorter
 //     path.  That took 41.9 us to 34.3 there.
@@ -36,10 +39,10 @@
 //     in 16 rows takes four times as long in the vector cache) and changes lanes
 //     through the wave's own LDS.
 //
-// Measured (bf16, group 128): 4 x 2048 x 151936 in 35 us, 4.7 TB/s of the 6.0 that
-// a reading kernel reaches; 16 x 2048 x 12288 in 6.7 us and 1 x 2048 x 2048 in 3.9,
+// Measured (bf16, group 128): 4 x 2048 x 151936 in 34.5 us, 4.7 TB/s of the 6.0 that
+// a reading kernel reaches; 16 x 2048 x 12288 in 6.3 us and 1 x 2048 x 2048 in 3.8,
 // where launching (1.8 us) and one round trip each for x and the first weights are
-// most; 64 x 6144 x 2048 in 12 us, six turns of x through LDS after each other.
+// most; 64 x 6144 x 2048 in 9.8 us, six turns of x through LDS after each other.
 #pragma once
 
 #include "common.hpp"
@@ -229,24 +232,37 @@ __global__ __launch_bounds__(64 * W, (W / 4 * l4_per_cu<T, W, RT, NB, MB, GROUP,
 #pragma unroll
         for (int q = 0; q < kGroups; ++q) {
           float sum = 0.f;
+          f32x4_t sums4 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int s = q * kSteps; s < (q + 1) * kSteps; ++s) {
             uint4 in[kXV];
 #pragma unroll
-            for (int v = 0; v < kXV; ++v) {
-              in[v] = sm_x[wave][l4_piece<kLPR>(i, (s * 4 + g) * kXV + v)];
-              float f[8 / kXV];
-              unpack<T>(in[v], f);
-#pragma unroll
-              for (int e = 0; e < 8 / kXV; ++e) sum += f[e];
-            }
+            for (int v = 0; v < kXV; ++v) in[v] = sm_x[wave][l4_piece<kLPR>(i, (s * 4 + g) * kXV + v)];
             l4_parts<T>(in, x[nb][s][rt]);
+            if constexpr (sizeof(T) == 2) {
+              // A product with ones: every output's row holds the sums.
+              const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+              sums4 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, ones),
+                                                              __builtin_bit_cast(bf16x8_t, in[0]), sums4, 0, 0, 0);
+            } else {
+#pragma unroll
+              for (int v = 0; v < kXV; ++v) {
+                float f[8 / kXV];
+                unpack<T>(in[v], f);
+#pragma unroll
+                for (int e = 0; e < 8 / kXV; ++e) sum += f[e];
+              }
+            }
           }
-          float a, b;
-          lane_pair<16>(sum, a, b);
-          sum = a + b;
-          lane_pair<32>(sum, a, b);
-          sums[nb][q][rt] = a + b;
+          if constexpr (sizeof(T) == 2) {
+            sums[nb][q][rt] = sums4[0];
+          } else {
+            float a, b;
+            lane_pair<16>(sum, a, b);
+            sum = a + b;
+            lane_pair<32>(sum, a, b);
+            sums[nb][q][rt] = a + b;
+          }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
         __builtin_amdgcn_wave_barrier();
@@ -364,13 +380,14 @@ hipError_t launch_l4_group(const asrlayer_linear4_params& p, hipStream_t stream)
   const int blocks_n = (p.n + 15) / 16, blocks_k = (p.k + 127) / 128;
   const int64_t row_blocks = (p.rows + RT * 16 - 1) / (RT * 16);
   // One workgroup a CU, or two where they fit and the blocks are many: a second one
-  // loads x again, so at fewer blocks it costs (16 rows of 2048 to 16384 outputs, 1024
-  // blocks: 7.7 us with 512 workgroups, 7.3 with 256; 24576: 9.1 and 9.2; 32768: 11.0
-  // and 11.8; 4 rows to 151936: 34.9 and 42.9).  Workgroups of the same outputs, one
+  // loads x again, so at fewer blocks it costs (16 rows of 2048 to 12288 outputs, 768
+  // blocks: 6.9 us with 512 workgroups, 6.6 with 256; 16384: 7.3 and 7.3; 24576: 8.7 and
+  // 9.0; 4 rows to 151936: 34.7 and 43.6; two row tiles, 64 rows to 12288: 12.5 and
+  // 12.2, 33 rows of 1024 to 16384: 9.4 and 10.2).  Workgroups of the same outputs, one
   // a block of rows, lie a multiple of 8 apart, on one XCD, whose L2 then reads the
-  // weights once (96 rows to 12288: 14.7 us for 15.1).
+  // weights once (80 rows to 151936: 122.1 us for 124.1).
   const bool two = (p.group == 32 ? l4_per_cu<T, W, RT, NB, MB, 32, CHUNKED>()
-                                  : l4_per_cu<T, W, RT, NB, MB, 128, CHUNKED>()) > 1 && blocks_n * row_blocks >= 2048;
+                                  : l4_per_cu<T, W, RT, NB, MB, 128, CHUNKED>()) > 1 && blocks_n * row_blocks >= (RT == 1 ? 1536 : 2048);
   int64_t across = (two ? 512 : 256) / row_blocks;
   if (across > 8) across -= across % 8;
   if (across < 1) across = 1;
@@ -404,22 +421,23 @@ hipError_t launch_l4_chunked(const asrlayer_linear4_params& p, hipStream_t strea
 }
 
 // Two row tiles where 256 workgroups are left: half the reads of the weights (64 x
-// 2048 x 12288: 11.2 us for 13.1; 64 x 1024 x 4096: 4.8 for 5.2); with fewer, one
-// (24 x 5120 x 1280: 6.9 us for 9.4).  All of x in registers where it fits, so that
-// x is read once a workgroup; else in chunks, again for each block of outputs:
-// 64 x 4096 x 12288 in 17.6 us with 16 waves holding x, 35.5 in chunks; 16 x 4096 x
-// 6144 with four blocks a wave in 8.1 us, 9.2 in chunks.  At 256 blocks of outputs
-// or fewer a workgroup has one and nothing to keep x for.  Chunks take 16 waves there
-// if that halves their number: 8 x 6144 x 2048 (6 chunks or 3) in 6.7 us for 7.7; at 24
-// x 5120 x 1280 (5 or 3) 7.2 for 6.9.  Groups of 32 need more registers than 16 waves
-// leave: 32 x 4096 x 6144 in 12.8 us with four blocks a wave, 19.0 with 16 waves.  So
+// 2048 x 12288: 11.1 us for 12.8; 64 x 1024 x 4096: 4.8 for 5.3); with fewer, one
+// (24 x 5120 x 1280: 6.2 us for 8.2).  All of x in registers where it fits, so that
+// x is read once a workgroup; else in chunks, again for each turn over the outputs:
+// 64 x 4096 x 12288 in 17.0 us with 16 waves holding x, 23.1 in chunks; 16 x 4096 x
+// 12288 with four blocks a wave in 9.3 us, 10.9 in chunks; 4 x 2560 x 151936 with three
+// 54.5, with four, of which some are none, 60.7.  Up to 512 blocks of outputs chunks,
+// which two share, are as good (16 x 4096 x 6144: 7.6 us, 7.8 holding x).  Chunks take 16
+// waves at 256 blocks or fewer if that halves their number: 8 x 6144 x 2048 (6 chunks
+// or 3) in 6.5 us for 7.0; at 24 x 5120 x 1280 (5 or 3) 6.8 for 6.2.  Groups of 32 need
+// more registers than 16 waves leave: 32 x 4096 x 6144 in 11.7 us, 19.0 with 16 waves.  So
 // does float32, whose x is three times as large: 8 waves, and two row tiles only where
 // each wave holds one block of inputs.
 template <typename T>
 hipError_t launch_l4(const asrlayer_linear4_params& p, hipStream_t stream) {
   const int blocks_n = (p.n + 15) / 16, blocks_k = (p.k + 127) / 128;
-  const bool four = sizeof(T) == 2 && blocks_k > 16 && blocks_k <= 32 && blocks_n > 256;  // blocks a wave
-  if (p.rows > 16 && (int64_t)blocks_n * ((p.rows + 31) / 32) >= 256 && !(four && p.group == 32) &&
+  const bool several = sizeof(T) == 2 && blocks_k > 16 && blocks_k <= 32 && blocks_n > 512;  // blocks a wave
+  if (p.rows > 16 && (int64_t)blocks_n * ((p.rows + 31) / 32) >= 256 && !(several && p.group == 32) &&
       (sizeof(T) == 2 || blocks_k <= 8)) {
     if (blocks_k <= 8) return launch_l4_group<T, 8, 2, 1, 1, false>(p, stream);
     if constexpr (sizeof(T) == 2) {
@@ -431,7 +449,8 @@ hipError_t launch_l4(const asrlayer_linear4_params& p, hipStream_t stream) {
   if (blocks_k <= 8) return launch_l4_group<T, 8, 1, 1, 1, false>(p, stream);
   if (blocks_k <= 16) return launch_l4_group<T, 8, 1, 2, 1, false>(p, stream);
   if constexpr (sizeof(T) == 2) {
-    if (four) return launch_l4_group<T, 8, 1, 4, 1, false>(p, stream);
+    if (several)
+      return blocks_k <= 24 ? launch_l4_group<T, 8, 1, 3, 1, false>(p, stream) : launch_l4_group<T, 8, 1, 4, 1, false>(p, stream);
     if (blocks_n * ((p.rows + 15) / 16) <= 256 && (blocks_k + 15) / 16 * 2 <= (blocks_k + 7) / 8)
       return launch_l4_group<T, 16, 1, 1, 1, true>(p, stream);
   }

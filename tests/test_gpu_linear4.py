@@ -48,6 +48,7 @@ SHAPES = [
     (64, 4096, 2100, 128), (50, 3200, 2100, 32), (3, 4096, 4200, 64), (9, 2592, 4200, 32), (7, 2304, 4130, 128),
     (70, 1024, 11000, 64), (40, 2048, 16400, 64), (5, 10240, 70, 64),
     (3, 2304, 4300, 32), (20, 2688, 4200, 128), (36, 4352, 4300, 64), (5, 4224, 8400, 64), (35, 4352, 9000, 32),
+    (5, 2432, 8300, 64), (3, 4096, 8300, 32), (30, 2688, 8250, 32), (2, 2816, 8400, 128), (2, 2048, 24700, 64),
 ]
 
 
