@@ -652,6 +652,9 @@ int asrlayer_tree(const asrlayer_tree_params* params, void* workspace, size_t wo
   const asrattn::TreePlan plan = asrattn::tree_plan(p);
   if ((long long)p.heads_kv * plan.row_blocks > 65535)
     return fail(ASRATTN_ERR_UNSUPPORTED, "more than 65535 blocks of query rows");
+  // A launch has fewer than 2^32 threads along an axis, up to 512 a workgroup.
+  if (plan.row_blocks > 1 && ((long long)p.batch * p.heads_kv * plan.splits + 8) * plan.row_blocks >= (1 << 23))
+    return fail(ASRATTN_ERR_UNSUPPORTED, "more than 2^23 blocks of query rows over all rows and heads");
   float* ws_o = nullptr;
   float* ws_ml = nullptr;
   unsigned long long* ws_arrive = nullptr;
@@ -676,7 +679,7 @@ int asrlayer_tree_masks(const int64_t* parents, int64_t parents_batch_stride, in
                         int64_t* masks, int64_t* depths, void* stream) {
   if (tokens < 1 || tokens > 64)
     return fail(ASRATTN_ERR_UNSUPPORTED, "a tree has 1 to 64 drafted tokens, got %d", tokens);
-  if (batch < 0 || batch > 0x7fffffffLL) return fail(ASRATTN_ERR_INVALID, "batch (%lld) out of range", (long long)batch);
+  if (batch < 0 || batch > (1 << 25)) return fail(ASRATTN_ERR_INVALID, "batch (%lld) out of range", (long long)batch);
   if (batch == 0) return ok();
   if (parents == nullptr || masks == nullptr || depths == nullptr)
     return fail(ASRATTN_ERR_INVALID, "parents, masks and depths must be non-NULL");
@@ -690,7 +693,7 @@ int asrlayer_accept(const int64_t* tokens, const int64_t* parents, int64_t paren
                     int64_t* emitted, int64_t* count, void* stream) {
   if (width < 1 || width > 64)
     return fail(ASRATTN_ERR_UNSUPPORTED, "a tree has 1 to 64 drafted tokens, got %d", width);
-  if (batch < 0 || batch > 0x7fffffffLL) return fail(ASRATTN_ERR_INVALID, "batch (%lld) out of range", (long long)batch);
+  if (batch < 0 || batch > (1 << 25)) return fail(ASRATTN_ERR_INVALID, "batch (%lld) out of range", (long long)batch);
   if (batch == 0) return ok();
   if (tokens == nullptr || parents == nullptr || choices == nullptr || path == nullptr || emitted == nullptr ||
       count == nullptr)
@@ -737,8 +740,8 @@ int asrlayer_linear4(const asrlayer_linear4_params* params, void* stream) {
   if (p.group != 32 && p.group != 64 && p.group != 128)
     return fail(ASRATTN_ERR_UNSUPPORTED, "group %d (supported: 32, 64, 128)", p.group);
   if (p.k % p.group != 0) return fail(ASRATTN_ERR_INVALID, "k (%d) is not a multiple of group (%d)", p.k, p.group);
-  if (p.n > (1 << 28) || p.k > (1 << 24) || p.rows > (1LL << 20))
-    return fail(ASRATTN_ERR_UNSUPPORTED, "more than 2^20 rows, 2^28 outputs or 2^24 inputs");
+  if (p.n > (1 << 28) || p.k > (1 << 24) || p.rows > 65535 * 16)
+    return fail(ASRATTN_ERR_UNSUPPORTED, "more than 1048560 rows, 2^28 outputs or 2^24 inputs");
   if (p.rows == 0) return ok();
   if (p.x == nullptr || p.packed == nullptr || p.scales == nullptr || p.out == nullptr)
     return fail(ASRATTN_ERR_INVALID, "x, packed, scales and out must be non-NULL");

@@ -45,6 +45,14 @@ class Weight4:
     group: int
 
 
+def _overlap(a: Tensor, b: Tensor) -> bool:
+    """Whether the memory from the first to the last element of both meets."""
+    if not a.numel() or not b.numel():
+        return False
+    ends = [t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) for t in (a, b)]
+    return a.data_ptr() < ends[1] and b.data_ptr() < ends[0]
+
+
 def _check_layout(packed: Tensor, scales: Tensor, zeros: Tensor | None, outputs: int, inputs: int, group: int) -> None:
     """The tensors are as large as the kernel reads them, and in its order (a module's
     buffers can be replaced, and take the strides of another memory format)."""
@@ -152,6 +160,8 @@ def quantize4(weight: Tensor, group: int = 128, symmetric: bool = True) -> Weigh
         step = scales.float()
         offset = torch.where(step > 0, -low / step, 0.0).round_().clamp_(0, 15)
         zeros, offset = offset.to(torch.uint8), offset[..., None]
+    if not torch.isfinite(scales).all():
+        raise ValueError("the matrix holds infinities, NaN or values too large for a scale")
     step = scales.float()[..., None]
     values = torch.where(step > 0, w / step, 0.0).round_().add_(offset).clamp_(0, 15).to(torch.uint8)
     return pack4(values.view(outputs, inputs), scales, zeros)
@@ -190,6 +200,8 @@ def _product(x: Tensor, packed: Tensor, scales: Tensor, zeros: Tensor | None, ou
         out = x.new_empty((*shape[:-1], outputs))
     elif out.shape != (*shape[:-1], outputs) or out.dtype is not dtype or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {(*shape[:-1], outputs)} tensor of x's dtype")
+    elif _overlap(out, x):
+        raise ValueError("out shares memory with x, whose rows every part of the product reads")
     rows = _aligned(x if len(shape) == 2 else x.reshape(-1, inputs))
     others = (packed, scales, zeros, bias, out)
     if index != torch.cuda.current_device() or any(t is not None and t.get_device() != index for t in others):

@@ -142,12 +142,15 @@ def test_library_refuses(lib):
     assert tree(head_dim=512) == tree(tokens=65) == tree(tokens=0) == tree(batch=70000) == _lib.ERR_UNSUPPORTED
     assert tree(masks=None) == tree(q=4100) == tree(k_token_stride=4) == _lib.ERR_INVALID
     assert tree(k_token_stride=1 << 26) == tree(vd_token_stride=-8) == _lib.ERR_UNSUPPORTED
+    assert tree(batch=65535, heads_q=4096, heads_kv=64, tokens=64) == _lib.ERR_UNSUPPORTED  # 2^29 workgroups
     paged = dict(block_table=4096, bt_stride=64, page_size=64, num_pages=3)
     assert tree(**paged) == _lib.ERR_WORKSPACE
     assert tree(**paged | {"page_size": 8}) == tree(**paged | {"page_size": 48}) == _lib.ERR_UNSUPPORTED
     assert tree(**paged | {"bt_stride": 63}) == tree(**paged | {"k_page_stride": 4}) == _lib.ERR_INVALID
     assert lib.asrlayer_tree(None, None, 0, None) == lib.asrlayer_commit(None, None) == _lib.ERR_INVALID
     assert lib.asrlayer_tree_masks(None, 0, 1, 8, None, None, None) == _lib.ERR_INVALID
+    assert lib.asrlayer_tree_masks(4096, 0, (1 << 25) + 1, 8, 4096, 4096, None) == _lib.ERR_INVALID
+    assert lib.asrlayer_accept(4096, 4096, 0, 4096, None, (1 << 25) + 1, 8, 4096, 4096, 4096, None) == _lib.ERR_INVALID
     assert lib.asrlayer_tree_masks(4096, 0, 1, 65, 4096, 4096, None) == _lib.ERR_UNSUPPORTED
     assert lib.asrlayer_accept(4096, 4096, 0, 4096, None, -1, 8, 4096, 4096, 4096, None) == _lib.ERR_INVALID
     assert lib.asrlayer_accept(4096, 4096, 0, 4096, None, 0, 8, 4096, 4096, 4096, None) == _lib.OK

@@ -125,6 +125,20 @@ def test_layouts_of_x_out_and_other_rows():
     assert out[1].isnan().all() and not out[3].isfinite().any()
 
 
+def test_out_apart_from_x():
+    from asrback_amd.linear4 import linear4, quantize4
+
+    g = torch.Generator().manual_seed(6)
+    weight = quantize4(torch.randn(256, 256, generator=g).to("cuda", BF16), 64)
+    arena = torch.randn(12, 256, generator=g).to("cuda", BF16)
+    x = arena[:4]
+    ref = linear4(x, weight)
+    for out in (arena[:4], arena[3:7]):
+        with pytest.raises(ValueError, match="shares memory"):
+            linear4(x, weight, out=out)
+    assert torch.equal(linear4(x, weight, out=arena[4:8]), ref)
+
+
 def test_graph_replays_and_module():
     from asrback_amd.linear4 import Linear4, linear4, quantize4, quantize_linears, unpack4
 

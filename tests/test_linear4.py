@@ -85,6 +85,12 @@ def test_refusals():
         quantize4(torch.zeros(8, 96), 48)
     with pytest.raises(ValueError, match="matrix"):
         quantize4(torch.zeros(8, 64).half(), 64)
+    for bad in (float("inf"), float("nan")):
+        matrix = torch.zeros(8, 64)
+        matrix[3, 5] = bad
+        for symmetric in (True, False):
+            with pytest.raises(ValueError, match="infinities"):
+                quantize4(matrix, 64, symmetric)
     weight = pack4(values, scales)
     with pytest.raises(RuntimeError, match="GPU only"):
         linear4(torch.zeros(3, 64), weight)
@@ -125,5 +131,7 @@ def test_refusals():
     assert lib.asrlayer_linear4(ctypes.byref(p), None) == _lib.ERR_UNSUPPORTED
     p.group, p.k = 64, 96
     assert lib.asrlayer_linear4(ctypes.byref(p), None) == _lib.ERR_INVALID
-    p.k, p.rows = 128, 0
+    p.k, p.x_row_stride, p.rows = 128, 128, 65535 * 16 + 1
+    assert lib.asrlayer_linear4(ctypes.byref(p), None) == _lib.ERR_UNSUPPORTED
+    p.rows = 0
     assert lib.asrlayer_linear4(ctypes.byref(p), None) == _lib.OK
