@@ -228,6 +228,36 @@ def test_masked_places_hold_anything(dtype, d, page):
           torch.where(fine, absolute, zero.double()), torch.where(slack.isfinite(), slack, zero.double()), dtype, "masked")
 
 
+@pytest.mark.parametrize("dtype,batch,d,length", [(BF16, 24, 128, 1536), (BF16, 8, 64, 4096), (F32, 24, 64, 1536),
+                                                  (BF16, 24, 256, 64), (F32, 24, 128, 64)])
+def test_infinite_drafted_values_stay_with_their_rows(dtype, batch, d, length):
+    """Launches of two row tiles and of four waves: infinities and NaN in two
+    dimensions of a drafted value reach those dimensions of the rows that see it
+    and change no other bit."""
+    from asrback_amd import drafts
+
+    say("infinite drafts", dtype, batch, d, length)
+    g = torch.Generator().manual_seed(d + length)
+    tokens, kv_heads = 33, 4
+    q, k, v, kd, vd, _, _, _ = make(dtype, batch, tokens, 2 * kv_heads, kv_heads, d, length, 0, g)
+    parents = torch.tensor([random_parents(tokens, g, padding=2) for _ in range(batch)])
+    masks, _ = drafts.tree_masks(parents.cuda())
+    lengths = torch.randint(0, 60, (batch,), generator=g).cuda()
+    bad = (7, 20)
+    vd[:, bad[0], :, 5] = 0.0
+    vd[:, bad[1], :, d - 1] = 0.0
+    clean = drafts.tree_attention(q, k, v, kd, vd, masks, lengths=lengths)
+    vd[:, bad[0], :, 5] = float("inf")
+    vd[:, bad[1], :, d - 1] = float("nan")
+    out = drafts.tree_attention(q, k, v, kd, vd, masks, lengths=lengths)
+    sees = [(masks >> j & 1).bool() for j in bad]
+    assert sees[0].sum() > batch and sees[1].sum() > batch // 2
+    assert not out[..., 5][sees[0]].isfinite().any() and out[..., d - 1][sees[1]].isnan().all()
+    out[..., 5][sees[0]] = clean[..., 5][sees[0]]
+    out[..., d - 1][sees[1]] = clean[..., d - 1][sees[1]]
+    assert torch.equal(out, clean)
+
+
 def test_missing_pages_and_counts_out_of_range():
     """Keys on no page or on one outside the pool are skipped; counts are clamped
     to the cache."""
