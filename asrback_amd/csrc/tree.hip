@@ -844,9 +844,13 @@ TreePlan tree_plan(const asrlayer_tree_params& p) {
   // Splits up to a workgroup a CU, of half a turn's keys at least, where they save two
   // and a half turns: partials, arrival and fold cost about as much (two splits of
   // 480 keys 12.9 us, unsplit 11.5; 1216 keys of 512 bytes: four 14.6, unsplit 19.4).
-  const int turn = plan.waves * (bytes > 256 || p.dtype == ASRATTN_F32 ? 16 : 32);  // keys a workgroup takes at once
-  plan.splits = 1;
-  if (units < 256) {
+  // The splits of workgroups of so many waves: up to a workgroup a CU, of half a turn's
+  // keys at least, where they save two and a half turns: partials, arrival and fold
+  // cost about as much (two splits of 480 keys 12.9 us, unsplit 11.5; 1216 keys of 512
+  // bytes: four 14.6, unsplit 19.4).
+  const int by_units = (int)(256 / (units < 1 ? 1 : units));
+  auto splits = [&](int waves) {
+    const int turn = waves * (bytes > 256 || p.dtype == ASRATTN_F32 ? 16 : 32);  // keys a workgroup takes at once
     // A turn takes about 1.2 us and a split costs the fold 0.13: the sum of both is least
     // at about the root of eight times the turns (6 rows over 3000 float32 keys of
     // 64: 14.4 us with 42 splits, 10.4 with 14, 14.9 with 4; 2 rows over 4000: 13.5
@@ -860,10 +864,22 @@ TreePlan tree_plan(const asrlayer_tree_params& p) {
       const long long whole = 32 / plan.row_blocks * 8 / (pairs < 1 ? 1 : pairs);
       most = most < whole ? most : (int)whole;
     }
-    const int by_units = (int)(256 / (units < 1 ? 1 : units)), by_keys = p.max_len_k / (turn / 2);
+    const int by_keys = p.max_len_k / (turn / 2);
     most = most < by_units ? most : by_units;
     most = most < by_keys ? most : by_keys;
-    if (most > 1 && (long long)p.max_len_k * (most - 1) * 2 >= 5LL * turn * most) plan.splits = most;
+    return most > 1 && (long long)p.max_len_k * (most - 1) * 2 >= 5LL * turn * most ? most : 1;
+  };
+  plan.splits = splits(plan.waves);
+  // Rows few enough that their fold costs little are split further, over workgroups
+  // of four waves with half the turn, where CUs are left (2 rows over 480 keys: 7.4 us
+  // with 5 splits of eight waves, 6.9 with 8 of four; over 4000, 10.7 and 9.9; 16 rows
+  // over 1800, 10.1 and 12.2; 2 rows over 16000, all CUs either way, 21.1 and 21.5).
+  if (plan.splits > 1 && plan.waves == 8 && rows <= 4) {
+    const int more = splits(4);
+    if (more > plan.splits && more < by_units) {
+      plan.waves = 4;
+      plan.splits = more;
+    }
   }
   // One workgroup folds 128 KB of partials in about the time of a launch (65511
   // keys, 262 KB: 67.3 us with a launch, 69.0 without; 64 KB: 16.4 and 15.0).

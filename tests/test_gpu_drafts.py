@@ -133,6 +133,11 @@ CASES = [
     (BF16, 2, 12, 8, 2, 64, 3000, [2999, 2], 0, "heads_first"),
     (F32, 1, 6, 3, 3, 64, 2100, [2100], 0, "slab"),
     (BF16, 1, 24, 2, 1, 256, 2000, [1999], 0, "slab"),
+    # of up to four rows: of four waves
+    (BF16, 1, 1, 16, 8, 128, 4096, [3001], 0, "slab"),
+    (F32, 1, 2, 6, 6, 64, 2100, [2077], 0, "heads_first"),
+    (BF16, 1, 4, 2, 2, 64, 3000, [2999], 64, "slab"),
+    (BF16, 2, 1, 8, 2, 256, 1500, [1499, 0], 0, "slab"),
     # many rows over long caches: two row tiles a workgroup, several workgroups a kv head
     (BF16, 1, 61, 8, 1, 128, 20000, [17000], 0, "slab"),
     (BF16, 1, 64, 8, 1, 64, 20000, [19999], 64, "slab"),
