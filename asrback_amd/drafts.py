@@ -87,6 +87,30 @@ def _operands(what: str, tensors: tuple[Tensor, ...], written: tuple[Tensor, ...
     return pointers, strides, _DTYPES[dtype], index, tensors
 
 
+def _plain_operands(q: Tensor, k: Tensor, v: Tensor, k_draft: Tensor, v_draft: Tensor) -> tuple | None:
+    """:func:`_operands` of tensors of four axes that the kernel takes as they are, in
+    two thirds of its time; None where one is not."""
+    dtype, index = q.dtype, q.get_device()
+    if not (k.dtype is dtype and v.dtype is dtype and k_draft.dtype is dtype and v_draft.dtype is dtype
+            and k.get_device() == index and v.get_device() == index and k_draft.get_device() == index
+            and v_draft.get_device() == index) or dtype not in _DTYPES or index < 0 or index != torch.cuda.current_device():
+        return None
+    if q.requires_grad or k.requires_grad or v.requires_grad or k_draft.requires_grad or v_draft.requires_grad:
+        return None
+    a0, a1, a2, a = q.stride()
+    b0, b1, b2, b = k.stride()
+    c0, c1, c2, c = v.stride()
+    d0, d1, d2, d = k_draft.stride()
+    e0, e1, e2, e = v_draft.stride()
+    pointers = (q.data_ptr(), k.data_ptr(), v.data_ptr(), k_draft.data_ptr(), v_draft.data_ptr())
+    ends = pointers[0] | pointers[1] | pointers[2] | pointers[3] | pointers[4]
+    bits = a0 | a1 | a2 | b0 | b1 | b2 | c0 | c1 | c2 | d0 | d1 | d2 | e0 | e1 | e2
+    if not a == b == c == d == e == 1 or ends & 15 or bits & (7 if dtype is torch.bfloat16 else 3):
+        return None
+    return (pointers, [a0, a1, a2, b0, b1, b2, c0, c1, c2, d0, d1, d2, e0, e1, e2], _DTYPES[dtype], index,
+            (q, k, v, k_draft, v_draft))
+
+
 def _int64(t: Tensor, name: str, shape: tuple[int, ...]) -> Tensor:
     if t.dtype is not torch.int64:
         raise TypeError(f"{name} must be int64, got {t.dtype}")
@@ -233,7 +257,8 @@ def tree_attention(
     _tokens(tokens)
     masks, masks_stride = _per_tree(masks, "masks", batch, tokens)
     lengths = _lengths(lengths, batch)
-    pointers, strides, dtype, index, held = _operands("tree_attention", (q, k, v, k_draft, v_draft))
+    pointers, strides, dtype, index, held = (_plain_operands(q, k, v, k_draft, v_draft)
+                                             or _operands("tree_attention", (q, k, v, k_draft, v_draft)))
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q_shape or out.dtype != q.dtype or out.stride(-1) != 1:

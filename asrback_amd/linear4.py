@@ -44,6 +44,9 @@ class Weight4:
     inputs: int
     group: int
 
+    def __post_init__(self) -> None:
+        _check_layout(self.packed, self.scales, self.zeros, self.outputs, self.inputs, self.group)
+
 
 def _overlap(a: Tensor, b: Tensor) -> bool:
     """Whether the memory from the first to the last element of both meets."""
@@ -54,8 +57,10 @@ def _overlap(a: Tensor, b: Tensor) -> bool:
 
 
 def _check_layout(packed: Tensor, scales: Tensor, zeros: Tensor | None, outputs: int, inputs: int, group: int) -> None:
-    """The tensors are as large as the kernel reads them, and in its order (a module's
-    buffers can be replaced, and take the strides of another memory format)."""
+    """The tensors are as large as the kernel reads them, and in its order: once for a
+    :class:`Weight4`, at each call of a module, whose buffers can be replaced and
+    take the strides of another memory format."""
+    _check_group(group, inputs)
     blocks = -(-outputs // _BLOCK_N) * -(-inputs // _BLOCK_K)
     groups = blocks * (_BLOCK_K // group)
     if not (packed.numel() == blocks * 256 and packed.dtype is torch.int32 and packed.is_contiguous()
@@ -191,7 +196,6 @@ def _product(x: Tensor, packed: Tensor, scales: Tensor, zeros: Tensor | None, ou
         raise TypeError(f"linear4 supports float32 and bfloat16, got {dtype}")
     if bias is not None and (bias.shape != (outputs,) or bias.dtype is not dtype):
         raise ValueError(f"bias must be {dtype} ({outputs},), got {bias.dtype} {tuple(bias.shape)}")
-    _check_layout(packed, scales, zeros, outputs, inputs, group)
     if index < 0:
         raise RuntimeError(f"linear4 runs on the GPU only; got a tensor on {x.device}")
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
@@ -241,6 +245,7 @@ class Linear4(nn.Module):
         return Weight4(self.packed, self.scales, self.zeros, self.out_features, self.in_features, self.group)
 
     def forward(self, x: Tensor) -> Tensor:
+        _check_layout(self.packed, self.scales, self.zeros, self.out_features, self.in_features, self.group)
         return _product(x, self.packed, self.scales, self.zeros, self.out_features, self.in_features, self.group, self.bias,
                         None)
 
