@@ -111,6 +111,28 @@ def _plain_operands(q: Tensor, k: Tensor, v: Tensor, k_draft: Tensor, v_draft: T
             (q, k, v, k_draft, v_draft))
 
 
+def _plain_caches(k_draft: Tensor, v_draft: Tensor, keys: Tensor, values: Tensor) -> tuple | None:
+    """:func:`_plain_operands` of four tensors of five axes."""
+    dtype, index = k_draft.dtype, k_draft.get_device()
+    if not (v_draft.dtype is dtype and keys.dtype is dtype and values.dtype is dtype and v_draft.get_device() == index
+            and keys.get_device() == index and values.get_device() == index) or dtype not in _DTYPES or index < 0 \
+            or index != torch.cuda.current_device():
+        return None
+    if k_draft.requires_grad or v_draft.requires_grad or keys.requires_grad or values.requires_grad:
+        return None
+    a0, a1, a2, a3, a = k_draft.stride()
+    b0, b1, b2, b3, b = v_draft.stride()
+    c0, c1, c2, c3, c = keys.stride()
+    d0, d1, d2, d3, d = values.stride()
+    pointers = (k_draft.data_ptr(), v_draft.data_ptr(), keys.data_ptr(), values.data_ptr())
+    bits = a0 | a1 | a2 | a3 | b0 | b1 | b2 | b3 | c0 | c1 | c2 | c3 | d0 | d1 | d2 | d3
+    if (not a == b == c == d == 1 or (pointers[0] | pointers[1] | pointers[2] | pointers[3]) & 15
+            or bits & (7 if dtype is torch.bfloat16 else 3)):
+        return None
+    return (pointers, (a0, a1, a2, a3, b0, b1, b2, b3, c0, c1, c2, c3, d0, d1, d2, d3), _DTYPES[dtype], index,
+            (k_draft, v_draft, keys, values))
+
+
 def _int64(t: Tensor, name: str, shape: tuple[int, ...]) -> Tensor:
     if t.dtype is not torch.int64:
         raise TypeError(f"{name} must be int64, got {t.dtype}")
@@ -324,11 +346,20 @@ def accept_drafts(tokens: Tensor, parents: Tensor, choices: Tensor,
     shape = tokens.shape
     batch, width = shape
     _tokens(width)
-    tokens, choices = _int64(tokens, "tokens", shape), _int64(choices, "choices", shape)
-    parents, stride = _per_tree(parents, "parents", batch, width)
-    if limit is not None:
-        limit = _int64(limit, "limit", (batch,))
-    index = _cuda("accept_drafts", tokens, parents, choices, limit)
+    index = tokens.get_device()
+    if (tokens.dtype is choices.dtype is parents.dtype is torch.int64 and choices.shape == parents.shape == shape
+            and tokens.is_contiguous() and choices.is_contiguous() and parents.is_contiguous()
+            and index == choices.get_device() == parents.get_device() >= 0
+            and (limit is None or (limit.dtype is torch.int64 and limit.shape == (batch,) and limit.is_contiguous()
+                                   and limit.get_device() == index))
+            and index == torch.cuda.current_device()):
+        stride = width
+    else:
+        tokens, choices = _int64(tokens, "tokens", shape), _int64(choices, "choices", shape)
+        parents, stride = _per_tree(parents, "parents", batch, width)
+        if limit is not None:
+            limit = _int64(limit, "limit", (batch,))
+        index = _cuda("accept_drafts", tokens, parents, choices, limit)
     path, emitted = torch.empty_like(tokens), torch.empty_like(tokens)
     count = tokens.new_empty(batch) if limit is None else torch.empty_like(limit)
     status = _lib.load().asrlayer_accept(
@@ -380,7 +411,9 @@ def commit_drafts(
     if lengths is None:
         raise TypeError("lengths must be a tensor")
     lengths = _lengths(lengths, batch)
-    pointers, strides, dtype, index, held = _operands("commit_drafts", (k_draft, v_draft, keys, values), (keys, values))
+    pointers, strides, dtype, index, held = (
+        _plain_caches(k_draft, v_draft, keys, values)
+        or _operands("commit_drafts", (k_draft, v_draft, keys, values), (keys, values)))
     if not torch.is_inference_mode_enabled() and (keys.is_inference() or values.is_inference()):
         raise RuntimeError("inplace update to inference tensors outside InferenceMode is not allowed")
     length = cache_shape[2]
