@@ -19,6 +19,13 @@
 //     the accumulator): every product is exact, and three bf16 matrix instructions take
 //     the place of eight float32 ones of twice the time each (16 x 1024 x 40000: 11.5 us
 //     for 20.0).
+//   * A group's sum comes before its scale, and up to 2^15.2 (float32: 2^12) times the
+//     largest |x| passes through the accumulator: 128 inputs, values up to 143 (15) of
+//     weights and of the zero point.  So that no sum overflows that the scale brings
+//     back into range, sums are kept times 2^-16 (2^-12) until the end.  In bf16 that
+//     is in the operand, which is 0x3b00 | q, and costs nothing.  float32 x is multiplied
+//     by it on its way (16 x 1024 x 40000: 12.0 us for 11.7), and what bf16 cannot hold
+//     of it is lost: 2^-121 of an x, so that those below 2^-97 go in with fewer bits.
 //   * Outputs lie in the rows of the product and x's rows in its columns, so a
 //     lane holds four outputs of one x row: a group's scales are one small load
 //     for four outputs, the group's sum of x one value per lane.
@@ -60,32 +67,27 @@ struct L4 {
   static constexpr int kXV = sizeof(T) == 2 ? 1 : 2;  // 16-byte vectors of 8 inputs
   static constexpr int kXP = sizeof(T) == 2 ? 1 : 3;  // bf16 parts of an input
   static constexpr float kOffset = sizeof(T) == 2 ? 128.f : 0.f;  // what a weight operand adds to q
+  static constexpr float kUnit = sizeof(T) == 2 ? 0x1p-16f : 0x1p-12f;  // what sums are kept times
 };
 
-// 8 inputs as the product's operands: float32 as the sum of three bf16, each the
+// 8 float32 inputs, times kUnit, as the product's operands: the sum of three bf16, each the
 // leading 8 bits of what is left (24 bits: nothing is lost).
-template <typename T>
-__device__ __forceinline__ void l4_parts(const uint4* v, uint4* x) {
-  if constexpr (sizeof(T) == 2) {
-    x[0] = v[0];
-  } else {
-    const uint32_t in[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
-    uint32_t part[3][8];
+__device__ __forceinline__ void l4_parts(const float* in, uint4* x) {
+  uint32_t part[3][8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      part[0][j] = in[j];
-      const float left = __uint_as_float(in[j]) - __uint_as_float(in[j] & 0xffff0000u);
-      part[1][j] = __float_as_uint(left);
-      part[2][j] = __float_as_uint(left - __uint_as_float(part[1][j] & 0xffff0000u));
-    }
+  for (int j = 0; j < 8; ++j) {
+    part[0][j] = __float_as_uint(in[j]);
+    const float left = in[j] - __uint_as_float(part[0][j] & 0xffff0000u);
+    part[1][j] = __float_as_uint(left);
+    part[2][j] = __float_as_uint(left - __uint_as_float(part[1][j] & 0xffff0000u));
+  }
 #pragma unroll
-    for (int c = 0; c < 3; ++c) {
-      constexpr uint32_t kHigh = 0x07060302u;  // the high halves of two dwords
-      x[c] = make_uint4(__builtin_amdgcn_perm(part[c][1], part[c][0], kHigh),
-                        __builtin_amdgcn_perm(part[c][3], part[c][2], kHigh),
-                        __builtin_amdgcn_perm(part[c][5], part[c][4], kHigh),
-                        __builtin_amdgcn_perm(part[c][7], part[c][6], kHigh));
-    }
+  for (int c = 0; c < 3; ++c) {
+    constexpr uint32_t kHigh = 0x07060302u;  // the high halves of two dwords
+    x[c] = make_uint4(__builtin_amdgcn_perm(part[c][1], part[c][0], kHigh),
+                      __builtin_amdgcn_perm(part[c][3], part[c][2], kHigh),
+                      __builtin_amdgcn_perm(part[c][5], part[c][4], kHigh),
+                      __builtin_amdgcn_perm(part[c][7], part[c][6], kHigh));
   }
 }
 
@@ -95,10 +97,11 @@ template <typename T, int RT>
 __device__ __forceinline__ void l4_step(uint32_t w, const uint4 (*x)[L4<T>::kXP], f32x4_t* acc) {
   uint4 a;
   if constexpr (sizeof(T) == 2) {
-    a.x = (w & 0x000f000fu) | 0x43004300u;
-    a.y = ((w >> 4) & 0x000f000fu) | 0x43004300u;
-    a.z = ((w >> 8) & 0x000f000fu) | 0x43004300u;
-    a.w = ((w >> 12) & 0x000f000fu) | 0x43004300u;
+    constexpr uint32_t kWeight = 0x3b003b00u;  // 2^-16 (128 + q) in the low bits' place
+    a.x = (w & 0x000f000fu) | kWeight;
+    a.y = ((w >> 4) & 0x000f000fu) | kWeight;
+    a.z = ((w >> 8) & 0x000f000fu) | kWeight;
+    a.w = ((w >> 12) & 0x000f000fu) | kWeight;
   } else {
     const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
     // Nibbles 0 1 2 3 hold inputs 0 2 4 6, nibbles 4 5 6 7 inputs 1 3 5 7.
@@ -200,7 +203,7 @@ __global__ __launch_bounds__(64 * W, (W / 4 * l4_per_cu<T, W, RT, NB, MB, GROUP,
   };
 
   uint4 x[NB][4][RT][L4<T>::kXP];
-  float sums[NB][kGroups][RT];  // of x over each group
+  float sums[NB][kGroups][RT];  // of x over each group, times kUnit
   // This wave's blocks of inputs from `first` on: x by rows, then as the product takes
   // it, and its sums.
   constexpr int kRows = 64 / kLPR, kTurns = 16 / kRows;  // rows a load, loads a block
@@ -238,20 +241,22 @@ __global__ __launch_bounds__(64 * W, (W / 4 * l4_per_cu<T, W, RT, NB, MB, GROUP,
             uint4 in[kXV];
 #pragma unroll
             for (int v = 0; v < kXV; ++v) in[v] = sm_x[wave][l4_piece<kLPR>(i, (s * 4 + g) * kXV + v)];
-            l4_parts<T>(in, x[nb][s][rt]);
             if constexpr (sizeof(T) == 2) {
-              // A product with ones: every output's row holds the sums.
-              const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
-              sums4 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, ones),
+              x[nb][s][rt][0] = in[0];
+              // A product with kUnit: every output's row holds the sums.
+              const uint4 unit = make_uint4(0x37803780u, 0x37803780u, 0x37803780u, 0x37803780u);
+              sums4 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, unit),
                                                               __builtin_bit_cast(bf16x8_t, in[0]), sums4, 0, 0, 0);
             } else {
+              float f[8];
 #pragma unroll
-              for (int v = 0; v < kXV; ++v) {
-                float f[8 / kXV];
-                unpack<T>(in[v], f);
+              for (int v = 0; v < kXV; ++v) unpack<T>(in[v], f + v * 8 / kXV);
 #pragma unroll
-                for (int e = 0; e < 8 / kXV; ++e) sum += f[e];
+              for (int e = 0; e < 8; ++e) {
+                f[e] *= L4<T>::kUnit;
+                sum += f[e];
               }
+              l4_parts(f, x[nb][s][rt]);
             }
           }
           if constexpr (sizeof(T) == 2) {
@@ -355,7 +360,7 @@ __global__ __launch_bounds__(64 * W, (W / 4 * l4_per_cu<T, W, RT, NB, MB, GROUP,
         const int mine = row_w + min(g, kFinish - 1);
         float y = 0.f;
         for (int u = 0; u < waves; ++u) y += sm[buffer][u][mine >> 4][mine & 15][i];
-        y += bias[m];
+        y = fmaf(y, 1.f / L4<T>::kUnit, bias[m]);
 #pragma unroll
         for (int r = 0; r < kFinish; ++r) {
           const int64_t row = row0 + row_w + r;

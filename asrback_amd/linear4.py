@@ -176,8 +176,9 @@ def linear4(x: Tensor, weight: Weight4, bias: Tensor | None = None, *, out: Tens
     """``x @ w.T + bias`` for the matrix ``w`` that ``weight`` stands for
     (``asrlayer_linear4``): ``x`` ``(..., inputs)`` float32 or bfloat16, the
     type of the weight's scales, ``bias`` ``(outputs,)`` of the same type.
-    Sums are float32 and rounded once; a row with an infinity or a NaN comes out
-    without a finite value.  Built for the few rows of a decoder step or a
+    Sums are float32, of any finite row within range where their scale brings them
+    there, and rounded once; a row with an infinity or a NaN comes out without a
+    finite value.  Built for the few rows of a decoder step or a
     drafted tree (up to 32 are read against the weights in one pass); more rows
     are right, the weights being read again for each 32.  ``out`` must not share
     memory with ``x``.  Returns ``(..., outputs)``."""

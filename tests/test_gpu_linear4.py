@@ -187,3 +187,72 @@ def test_graph_replays_and_module():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, linear4(static, model[0].weight4, model[0].bias))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,inputs,outputs,group", SHAPES)
+def test_exact_on_the_largest_values(dtype, rows, inputs, outputs, group):
+    """Rows of integers times 2^124, whose groups' sums pass the type's range before
+    their scale brings them back, beside rows of ordinary and of tiny ones; and a
+    value of 2^125 that a scale of zero takes out of a row.  Results are below 2^(126
+    + 4 + 15 - 20), and sums of integers below 2^24 times a power of two: exact."""
+    from asrback_amd.linear4 import linear4, pack4
+
+    g = torch.Generator().manual_seed(rows * 5 + inputs)
+    say("linear4 large", dtype, rows, inputs, outputs, group)
+    values, scales, points = quantized(outputs, inputs, group, rows % 2 == 0, dtype, g, powers=True)
+    scales *= 2.0**-20
+    weight = pack4(values.cuda(), scales.cuda(), None if points is None else points.cuda())
+    w = matrix(values, scales, points, group)
+    powers = torch.tensor([124.0, 0.0, 112.0, -100.0, 64.0, 60.0])[torch.arange(rows) % 6]
+    x = (torch.randint(-4, 5, (rows, inputs), generator=g) * 2.0**powers[:, None]).to(dtype)
+    assert x.isfinite().all()
+    assert torch.equal(linear4(x.cuda(), weight).cpu(), (x.double() @ w.T).to(dtype))
+    # One large value in a group whose scales are zero.
+    at = inputs // group // 2
+    scales[:, at] = 0
+    weight = pack4(values.cuda(), scales.cuda(), None if points is None else points.cuda())
+    x = torch.randint(-4, 5, (rows, inputs), generator=g).to(dtype)
+    x[::2, at * group + 3] = 2.0**125
+    ref = (x.double() @ matrix(values, scales, points, group).T).to(dtype)
+    assert torch.equal(linear4(x.cuda(), weight).cpu(), ref)
+
+
+def test_results_past_the_range_are_infinite():
+    from asrback_amd.linear4 import linear4, pack4
+
+    say("linear4 overflow")
+    for dtype in (BF16, F32):
+        values = torch.full((2, 256), 8, dtype=torch.uint8)
+        values[0, :64], values[1, 128:192] = 15, 1
+        weight = pack4(values.cuda(), torch.ones(2, 2, dtype=dtype).cuda())
+        x = torch.full((3, 256), 2.0**125, dtype=dtype)
+        x[1] = 3.0
+        out = linear4(x.cuda(), weight).cpu()
+        inf = float("inf")
+        assert out.tolist() == [[inf, -inf], [64 * 7 * 3.0, -64 * 7 * 3.0], [inf, -inf]]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,inputs,outputs,group", SHAPES[::5])
+def test_smallest_values(dtype, rows, inputs, outputs, group):
+    """Integers times powers of two down to 2^-118 are exact in bf16.  A float32 input
+    goes in to 2^-121, which its weight's product and the sum for the zero point
+    carry to at most 15 and 15 scales."""
+    from asrback_amd.linear4 import linear4, pack4
+
+    g = torch.Generator().manual_seed(rows * 3 + inputs)
+    say("linear4 small", dtype, rows, inputs, outputs, group)
+    values, scales, points = quantized(outputs, inputs, group, True, dtype, g, powers=True)
+    weight = pack4(values.cuda(), scales.cuda(), points.cuda())
+    w = matrix(values, scales, points, group)
+    unit = 2.0 ** torch.tensor([-118.0, -100.0, -60.0])[torch.arange(rows) % 3, None]
+    if dtype == BF16:
+        x = (torch.randint(-4, 5, (rows, inputs), generator=g) * unit).to(dtype)
+        assert torch.equal(linear4(x.cuda(), weight).cpu(), (x.double() @ w.T).to(dtype))
+        return
+    x = torch.randn(rows, inputs, generator=g) * unit
+    out, ref = linear4(x.cuda(), weight).cpu().double(), x.double() @ w.T
+    spread = scales.double().repeat_interleave(group, 1)
+    bound = 2.0**-24 * ref.abs() + 2.0**-24 * (4 * group + inputs // group + 32) * 30 * (x.double().abs() @ spread.T)
+    assert ((out - ref).abs() <= bound + 2.0**-121 * 30 * spread.sum(1)).all()
