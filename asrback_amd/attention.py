@@ -154,14 +154,15 @@ def _dtype_code(*tensors: Tensor) -> int:
 
 def _aligned(t: Tensor) -> Tensor:
     """``t`` itself when its rows (its last axis) can be read with 16-byte
-    vectors, else a contiguous copy."""
+    vectors, else a contiguous copy (also of what torch calls contiguous: a
+    view at an odd offset, or axes of size 1 with odd strides)."""
     *strides, last = t.stride()
     bits = 0
     for stride in strides:
         bits |= stride  # a vector is a power of two of elements: one test for all
     if last == 1 and t.data_ptr() % 16 == 0 and bits % (16 // t.element_size()) == 0:
         return t
-    return t.contiguous()
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _ptr(t: Tensor | None) -> int | None:

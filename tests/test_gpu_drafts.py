@@ -495,3 +495,37 @@ def test_commit_writes_the_accepted_positions_alone(dtype, page):
             if 0 <= int(path[b, 0]) < tokens:
                 want[:, b, 7] = kd[:, b, int(path[b, 0])]
         assert torch.equal(k2, want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_contiguous_tensors_at_odd_offsets(dtype):
+    """Queries and drafts that torch calls contiguous and vectors cannot read: at odd
+    offsets, and single rows, tokens and heads of odd strides."""
+    from asrback_amd import drafts
+
+    say("odd offsets", dtype)
+    g = torch.Generator().manual_seed(5)
+    for batch, tokens, heads, kv_heads in ((2, 3, 4, 2), (1, 1, 4, 1), (1, 5, 1, 1)):
+        q, k, v, kd, vd, _, _, _ = make(dtype, batch, tokens, heads, kv_heads, 64, 40, 0, g)
+        masks, _ = drafts.tree_masks(torch.tensor([random_parents(tokens, g)] * batch).cuda())
+        lengths = torch.tensor([33, 7][:batch]).cuda()
+        ref = drafts.tree_attention(q, k, v, kd, vd, masks, lengths=lengths)
+
+        def odd(t):
+            moved = torch.empty(t.numel() + 3, dtype=dtype, device="cuda")[3:].view(t.shape).copy_(t)
+            assert moved.is_contiguous() and moved.data_ptr() % 16
+            return moved
+
+        def wide(t):
+            return torch.empty((*t.shape[:-1], 65), dtype=dtype, device="cuda")[..., :64].copy_(t)
+
+        for change in (odd, wide):
+            assert torch.equal(drafts.tree_attention(change(q), k, v, change(kd), change(vd), masks, lengths=lengths), ref)
+            layers = torch.zeros(2, batch, 40, kv_heads, 64, dtype=dtype, device="cuda")
+            caches = [layers.clone() for _ in range(4)]
+            path = torch.zeros(batch, tokens, dtype=torch.int64, device="cuda")
+            count = torch.ones(batch, dtype=torch.int64, device="cuda")
+            both = [t.expand(2, *t.shape).contiguous() for t in (kd, vd)]
+            drafts.commit_drafts(*caches[:2], *both, path, count, lengths)
+            drafts.commit_drafts(*caches[2:], *(change(t) for t in both), path, count, lengths)
+            assert caches[0].any() and torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])

@@ -256,3 +256,19 @@ def test_smallest_values(dtype, rows, inputs, outputs, group):
     spread = scales.double().repeat_interleave(group, 1)
     bound = 2.0**-24 * ref.abs() + 2.0**-24 * (4 * group + inputs // group + 32) * 30 * (x.double().abs() @ spread.T)
     assert ((out - ref).abs() <= bound + 2.0**-121 * 30 * spread.sum(1)).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_one_row_of_any_layout(dtype):
+    """A single row of an odd row stride and rows at an odd offset, which torch calls
+    contiguous."""
+    from asrback_amd.linear4 import linear4, pack4
+
+    g = torch.Generator().manual_seed(9)
+    say("linear4 one row", dtype)
+    values, scales, points = quantized(70, 256, 64, True, dtype, g, powers=True)
+    weight = pack4(values.cuda(), scales.cuda(), points.cuda())
+    buffer = torch.randint(-4, 5, (2000,), generator=g).to(dtype).cuda()
+    for x in (buffer[:257].view(1, 257)[:, :256], buffer[3:259].view(1, 256), buffer[3:259], buffer[1:1025].view(2, 2, 256),
+              buffer[:514].view(1, 2, 257)[:, :1, :256]):
+        assert torch.equal(linear4(x, weight).cpu(), (x.double().cpu() @ matrix(values, scales, points, 64).T).to(dtype))
