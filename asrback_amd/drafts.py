@@ -18,7 +18,8 @@ tokens as the longest branch the model's own choices follow:
 
 As in :mod:`asrback_amd.attention`, calls launch on the current HIP stream,
 never synchronize, and can be captured into a graph; nothing here has a
-gradient, and calls that would need one are refused.
+gradient, and calls that would need one, in forward mode too, or that a tracer
+records are refused.
 """
 
 from __future__ import annotations
@@ -33,6 +34,7 @@ from . import _lib
 from .attention import (
     _DTYPES, PageTable, _aligned, _check_device, _dtype_code, _paged, _ptr, _split_workspace,
 )
+from .layers import refuse_unseen
 
 # Tokens of a drafted tree, one bit each of an ancestor mask.
 MAX_TOKENS = 64
@@ -206,6 +208,7 @@ def tree_masks(parents: Tensor) -> tuple[Tensor, Tensor]:
     _tokens(tokens)
     batch = parents.shape[0] if parents.dim() == 2 else 1
     parents, stride = _per_tree(parents, "parents", batch, tokens)
+    refuse_unseen("tree_masks", parents)
     index = _cuda("tree_masks", parents)
     masks = torch.empty_like(parents, memory_format=torch.contiguous_format)
     depths = torch.empty_like(masks)
@@ -279,6 +282,7 @@ def tree_attention(
     _tokens(tokens)
     masks, masks_stride = _per_tree(masks, "masks", batch, tokens)
     lengths = _lengths(lengths, batch)
+    refuse_unseen("tree_attention", q, k, v, k_draft, v_draft)
     pointers, strides, dtype, index, held = (_plain_operands(q, k, v, k_draft, v_draft)
                                              or _operands("tree_attention", (q, k, v, k_draft, v_draft)))
     if out is None:
@@ -346,6 +350,7 @@ def accept_drafts(tokens: Tensor, parents: Tensor, choices: Tensor,
     shape = tokens.shape
     batch, width = shape
     _tokens(width)
+    refuse_unseen("accept_drafts", tokens, parents, choices, limit)
     index = tokens.get_device()
     if (tokens.dtype is choices.dtype is parents.dtype is torch.int64 and choices.shape == parents.shape == shape
             and tokens.is_contiguous() and choices.is_contiguous() and parents.is_contiguous()
@@ -411,6 +416,7 @@ def commit_drafts(
     if lengths is None:
         raise TypeError("lengths must be a tensor")
     lengths = _lengths(lengths, batch)
+    refuse_unseen("commit_drafts", keys, values, k_draft, v_draft)
     pointers, strides, dtype, index, held = (
         _plain_caches(k_draft, v_draft, keys, values)
         or _operands("commit_drafts", (k_draft, v_draft, keys, values), (keys, values)))

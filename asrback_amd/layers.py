@@ -15,6 +15,7 @@ import math
 
 import torch
 from torch import Tensor, nn
+from torch.autograd import forward_ad
 from torch.nn.modules import module as _module
 
 from . import _lib
@@ -42,6 +43,34 @@ def _plain(*tensors: Tensor) -> bool:
     return not (torch.is_autocast_enabled("cuda") or torch.compiler.is_compiling() or torch.jit.is_tracing()
                 or torch.autograd.forward_ad._current_level >= 0 or torch._C._len_torch_dispatch_stack()
                 or torch._C._len_torch_function_stack() or torch._C._functorch.maybe_current_level() is not None)
+
+
+_tracing_state, _functorch_level = torch._C._get_tracing_state, torch._C._functorch.maybe_current_level
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+
+
+def refuse_unseen(what: str, *tensors: Tensor | None) -> None:
+    """Raise where something has to see the ops that ``what``, which has none to
+    run instead, computes in a kernel: forward-mode tangents and functorch's
+    wrappers, which would be dropped, and tracers, whose graph would hold the
+    results' memory and not what fills it."""
+    if not (forward_ad._current_level >= 0 or _tracing_state() is not None or _functorch_level() is not None
+            or _dispatch_modes()):
+        return
+    tracing = _tracing_state() is not None
+    if not tracing and _dispatch_modes():
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode  # (loads much)
+
+        tracing = get_proxy_mode() is not None
+    if tracing:
+        raise RuntimeError(f"{what} cannot be traced: its kernel is no operation of a traced graph")
+    for t in tensors:
+        if t is None:
+            continue
+        if torch._C._functorch.is_functorch_wrapped_tensor(t):
+            raise RuntimeError(f"{what} takes no part in function transforms; call it on plain tensors")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no gradient, in forward mode neither; call it on primal tensors")
 
 
 def _vectors(t: Tensor) -> bool:

@@ -9,7 +9,8 @@ in place of ``nn.Linear``, and :func:`quantize_linears` puts it under a model.
 
 Calls launch on the current HIP stream, never synchronize (the matrix is
 checked when it is packed) and can be captured into a graph; there is no
-gradient, and calls that would need one are refused.
+gradient, and calls that would need one, in forward mode too, or that a tracer
+records are refused.
 """
 
 from __future__ import annotations
@@ -21,6 +22,7 @@ from torch import Tensor, nn
 
 from . import _lib
 from .attention import _DTYPES, _aligned, _check_device
+from .layers import refuse_unseen
 
 GROUPS = (32, 64, 128)
 _BLOCK_N, _BLOCK_K = 16, 128
@@ -197,6 +199,7 @@ def _product(x: Tensor, packed: Tensor, scales: Tensor, zeros: Tensor | None, ou
         raise TypeError(f"linear4 supports float32 and bfloat16, got {dtype}")
     if bias is not None and (bias.shape != (outputs,) or bias.dtype is not dtype):
         raise ValueError(f"bias must be {dtype} ({outputs},), got {bias.dtype} {tuple(bias.shape)}")
+    refuse_unseen("linear4", x, scales, bias)
     if index < 0:
         raise RuntimeError(f"linear4 runs on the GPU only; got a tensor on {x.device}")
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
