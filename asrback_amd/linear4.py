@@ -265,7 +265,8 @@ def quantize_linears(module: nn.Module, group: int = 128, symmetric: bool = True
     once and stays shared."""
     made: dict[nn.Module, Linear4] = {}
     for parent in list(module.modules()):
-        for name, child in list(parent.named_children()):
+        # (named_children leaves out a child's second name)
+        for name, child in list(parent._modules.items()):
             if type(child) is nn.Linear and child.in_features % group == 0:
                 if child not in made:
                     made[child] = Linear4.from_linear(child, group, symmetric)

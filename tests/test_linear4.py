@@ -135,3 +135,19 @@ def test_refusals():
     assert lib.asrlayer_linear4(ctypes.byref(p), None) == _lib.ERR_UNSUPPORTED
     p.rows = 0
     assert lib.asrlayer_linear4(ctypes.byref(p), None) == _lib.OK
+
+
+def test_quantize_linears_replaces_every_name():
+    """A layer under two names of one parent, and under another parent, is rounded once
+    and stays shared."""
+    from asrback_amd.linear4 import Linear4, quantize_linears
+
+    model, inner = torch.nn.Module(), torch.nn.Module()
+    model.a = model.b = inner.c = torch.nn.Linear(64, 8)
+    model.inner, model.none = inner, None
+    model.register_module("absent", None)
+    inner.other = torch.nn.Linear(64, 8, bias=False)
+    inner.narrow = torch.nn.Linear(8, 4)
+    assert quantize_linears(model, 32) == 2
+    assert type(model.a) is Linear4 and model.a is model.b is inner.c
+    assert type(inner.other) is Linear4 and type(inner.narrow) is torch.nn.Linear and model.absent is None
