@@ -22,7 +22,7 @@ from torch import Tensor, nn
 
 from . import _lib
 from .attention import _DTYPES, _aligned, _check_device
-from .layers import refuse_unseen
+from .layers import _FORWARDS, refuse_unseen
 
 GROUPS = (32, 64, 128)
 _BLOCK_N, _BLOCK_K = 16, 128
@@ -258,16 +258,25 @@ class Linear4(nn.Module):
                 f"zeros={self.zeros is not None}, bias={self.bias is not None}")
 
 
+def _as_built(layer: nn.Module) -> bool:
+    """Whether ``layer`` is an ``nn.Linear`` and nothing else: no hooks, no forward of its
+    own."""
+    own = layer.__dict__
+    return (type(layer) is nn.Linear and "forward" not in own and nn.Linear.forward is _FORWARDS[nn.Linear]
+            and not any(hooks for name, hooks in own.items() if name.endswith("_hooks")))
+
+
 def quantize_linears(module: nn.Module, group: int = 128, symmetric: bool = True) -> int:
     """Replace every ``nn.Linear`` under ``module`` (not ``module`` itself) whose
     inputs are whole groups by a :class:`Linear4` of its rounded weights, in
     place; returns how many.  A layer that appears in several places is rounded
-    once and stays shared."""
+    once and stays shared; one that carries hooks or a forward of its own stays as
+    it is."""
     made: dict[nn.Module, Linear4] = {}
     for parent in list(module.modules()):
         # (named_children leaves out a child's second name)
         for name, child in list(parent._modules.items()):
-            if type(child) is nn.Linear and child.in_features % group == 0:
+            if child is not None and _as_built(child) and child.in_features % group == 0:
                 if child not in made:
                     made[child] = Linear4.from_linear(child, group, symmetric)
                 setattr(parent, name, made[child])

@@ -151,3 +151,23 @@ def test_quantize_linears_replaces_every_name():
     assert quantize_linears(model, 32) == 2
     assert type(model.a) is Linear4 and model.a is model.b is inner.c
     assert type(inner.other) is Linear4 and type(inner.narrow) is torch.nn.Linear and model.absent is None
+
+
+def test_quantize_linears_leaves_what_is_hooked():
+    """Layers with hooks of any kind or a forward of their own go on running them."""
+    from asrback_amd.linear4 import Linear4, quantize_linears
+
+    model = torch.nn.Sequential(*(torch.nn.Linear(64, 64) for _ in range(8)))
+    seen = []
+    model[0].register_forward_hook(lambda m, x, y: seen.append("forward"))
+    model[1].register_forward_pre_hook(lambda m, x: seen.append("pre"))
+    model[2].register_full_backward_hook(lambda m, x, y: None)
+    model[3].forward = lambda x: seen.append("own") or x
+    model[4].register_state_dict_post_hook(lambda *a: None)
+    torch.nn.utils.parametrizations.weight_norm(model[5])
+    model[6].register_load_state_dict_post_hook(lambda *a: None)
+    kept = list(model)[:7]
+    assert quantize_linears(model, 64) == 1
+    assert type(model[7]) is Linear4 and all(a is b for a, b in zip(model, kept))
+    torch.nn.Sequential(*kept)(torch.zeros(2, 64))
+    assert seen == ["forward", "pre", "own"]
