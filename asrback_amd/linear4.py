@@ -272,12 +272,13 @@ def quantize_linears(module: nn.Module, group: int = 128, symmetric: bool = True
     place; returns how many.  A layer that appears in several places is rounded
     once and stays shared; one that carries hooks or a forward of its own stays as
     it is."""
-    made: dict[nn.Module, Linear4] = {}
-    for parent in list(module.modules()):
-        # (named_children leaves out a child's second name)
-        for name, child in list(parent._modules.items()):
-            if child is not None and _as_built(child) and child.in_features % group == 0:
-                if child not in made:
-                    made[child] = Linear4.from_linear(child, group, symmetric)
-                setattr(parent, name, made[child])
+    places = [(parent, name, child) for parent in module.modules()
+              # (named_children leaves out a child's second name)
+              for name, child in parent._modules.items()
+              if child is not None and _as_built(child) and child.in_features % group == 0]
+    # All are rounded before the first is replaced: one that cannot be leaves the model
+    # as it is.
+    made = {child: Linear4.from_linear(child, group, symmetric) for child in dict.fromkeys(c for _, _, c in places)}
+    for parent, name, child in places:
+        setattr(parent, name, made[child])
     return len(made)

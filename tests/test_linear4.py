@@ -171,3 +171,17 @@ def test_quantize_linears_leaves_what_is_hooked():
     assert type(model[7]) is Linear4 and all(a is b for a, b in zip(model, kept))
     torch.nn.Sequential(*kept)(torch.zeros(2, 64))
     assert seen == ["forward", "pre", "own"]
+
+
+def test_quantize_linears_replaces_all_or_none():
+    """A matrix that cannot be rounded leaves the whole model as it was."""
+    from asrback_amd.linear4 import quantize_linears
+
+    for bad in (torch.nn.Linear(64, 8).half(), torch.nn.Linear(64, 8)):
+        model = torch.nn.Sequential(torch.nn.Linear(64, 8), torch.nn.Sequential(bad))
+        if bad.weight.dtype == torch.float32:
+            with torch.no_grad():
+                bad.weight[3, 5] = float("inf")
+        with pytest.raises(ValueError):
+            quantize_linears(model, 64)
+        assert all(type(m) in (torch.nn.Linear, torch.nn.Sequential) for m in model.modules())
