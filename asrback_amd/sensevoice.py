@@ -32,6 +32,7 @@ from torch import Tensor, nn
 
 from .attention import flash_fsmn
 from .layers import gemm, gemm_takes, used_takes
+from .linear4 import Linear4
 
 
 class SANMAttention(nn.Module):
@@ -69,17 +70,20 @@ class SANMAttention(nn.Module):
         qkv = gemm(x, linear_in, skip) if project else linear_in(x)
         query, key, value = qkv.split(self.size, dim=-1)
         shape = (batch, length, self.heads, self.size // self.heads)
+        four_bit = isinstance(linear_out, Linear4)  # has no matrix to add its product with
         output, memory = flash_fsmn(
             query.view(shape),
             key.view(shape),
             value.view(shape),
             self.fsmn_block.weight,
             seqused_k=lengths,
-            bias=linear_out.bias,
+            bias=None if four_bit else linear_out.bias,
             zero_padded_rows=self.zero_padded_rows and lengths is not None,
         )
-        # linear_out(output) + memory: the bias is in memory already.
         rows = output.view(batch, length, self.size)
+        if four_bit:
+            return memory.add_(linear_out(rows))
+        # linear_out(output) + memory: the bias is in memory already.
         if project and gemm_takes(rows, linear_out):
             return gemm(rows, linear_out, skip, into=memory)
         memory.view(-1, self.size).addmm_(output.view(-1, self.size), linear_out.weight.t())
