@@ -64,3 +64,43 @@ def test_sensevoice_attention_bf16(device):
     assert_close((out * mask[..., None]).float().cpu(), (expected * mask[..., None]).float().cpu(), "bf16")
     for b, n in enumerate(lengths.tolist()):
         assert torch.equal(out[b, n:], four.linear_out.bias.expand(200 - n, 512))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_whisper(device, dtype):
+    """Encoder, prompt pass and steps; the layers leave the step's row kernels to plain
+    layers."""
+    import json
+
+    from conftest import GOLDEN
+    from oracle import whisper as ow
+    from test_gpu_whisper import gpu_model
+
+    say("4-bit whisper", dtype)
+    fixture = json.loads((GOLDEN / "whisper_tiny_greedy.json").read_text())
+    weights = ow.attention_heavy_weights(ow.WhisperForConditionalGeneration(fixture["config"]), fixture["seeds"]["weights"])
+    four, plain = quantized_pair(gpu_model(fixture, weights, device, dtype), 128)
+    # bf16: some ten roundings a layer (2^-8) in each of eight layers, as their square
+    # root, on either side, and that of the unpacked matrices.
+    bound = 1e-4 if dtype == torch.float32 else 2.0**-8 * (2 * 10 * 8) ** 0.5
+    g = torch.Generator().manual_seed(2)
+    mel = torch.randn(2, 80, 3000, generator=g).to(device, dtype)
+    tokens = torch.randint(0, 50000, (2, 6), generator=g).to(device)
+    positions = torch.arange(448, device=device)
+
+    def close(a, b):
+        assert a.shape == b.shape
+        error = float((a.double() - b.double()).norm() / b.double().norm())
+        assert error < bound, error
+
+    with torch.inference_mode():
+        encoded = [m.model.encoder(mel) for m in (four, plain)]
+        close(*encoded)
+        caches = []
+        for m in (four, plain):
+            caches.append(m.allocate_cache(2))
+            m.set_encoder_output(caches[-1], encoded[1])
+        close(*(m.decode(tokens[:, :4], positions[:4], c, length=4) for m, c in zip((four, plain), caches)))
+        for i in (4, 5):
+            at = torch.full((2,), i, device=device)
+            close(*(m.decode(tokens[:, i:i + 1], at, c) for m, c in zip((four, plain), caches)))
