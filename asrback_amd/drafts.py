@@ -34,7 +34,7 @@ from . import _lib
 from .attention import (
     _DTYPES, PageTable, _aligned, _check_device, _dtype_code, _paged, _ptr, _split_workspace,
 )
-from .layers import refuse_unseen
+from .layers import check_out, refuse_unseen
 
 # Tokens of a drafted tree, one bit each of an ancestor mask.
 MAX_TOKENS = 64
@@ -259,7 +259,8 @@ def tree_attention(
     padding: it attends nothing and gets zeros.
 
     float32 or bfloat16, head_dim 64, 128 or 256, any number of query heads
-    per kv head, up to :data:`MAX_TOKENS` tokens.  ``workspace``: the split
+    per kv head, up to :data:`MAX_TOKENS` tokens.  ``out`` is written in place; it
+    may be ``q`` itself and shares memory with no other input.  ``workspace``: the split
     partials' memory (:func:`tree_workspace_size`,
     :func:`asrback_amd.attention.workspace`).  Returns ``(batch, tokens,
     heads_q, head_dim)``."""
@@ -283,12 +284,17 @@ def tree_attention(
     masks, masks_stride = _per_tree(masks, "masks", batch, tokens)
     lengths = _lengths(lengths, batch)
     refuse_unseen("tree_attention", q, k, v, k_draft, v_draft)
+    given = out is not None
+    if given:
+        if out.shape != q_shape or out.dtype != q.dtype or out.stride(-1) != 1:
+            raise ValueError("out must match q's shape and dtype, with a unit last stride")
+        # A row's queries are read before any of its outputs is written.
+        in_place = out.data_ptr() == q.data_ptr() and out.stride() == q.stride()
+        check_out("tree_attention", out, None if in_place else q, k, v, k_draft, v_draft, masks, lengths)
     pointers, strides, dtype, index, held = (_plain_operands(q, k, v, k_draft, v_draft)
                                              or _operands("tree_attention", (q, k, v, k_draft, v_draft)))
-    if out is None:
+    if not given:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != q_shape or out.dtype != q.dtype or out.stride(-1) != 1:
-        raise ValueError("out must match q's shape and dtype, with a unit last stride")
     if pages is None:
         _on(index, masks, lengths, out)
         paged = (0, 0, 0, 0, 0, 0)
@@ -311,6 +317,8 @@ def tree_attention(
     status = _lib.load().asrlayer_tree(params, workspace, size, _raw_stream(index))
     if status:
         _lib.check(status, "asrlayer_tree")
+    if given:
+        _increment_version(out)
     return out
 
 

@@ -73,6 +73,49 @@ def refuse_unseen(what: str, *tensors: Tensor | None) -> None:
             raise RuntimeError(f"{what} has no gradient, in forward mode neither; call it on primal tensors")
 
 
+def overlap(a: Tensor, b: Tensor) -> bool:
+    """Whether two tensors may share memory: the ranges from their first to their last
+    elements meet, and they are not different parts of the same rows (a stride of ``a``
+    that all their larger strides are multiples of)."""
+    if not a.numel() or not b.numel():
+        return False
+    starts = [t.data_ptr() for t in (a, b)]
+    axes = [[(n, s * t.element_size()) for n, s in zip(t.shape, t.stride()) if n > 1 and s] for t in (a, b)]
+
+    def extent(i: int, below: float) -> int:
+        return (a, b)[i].element_size() + sum((n - 1) * s for n, s in axes[i] if s < below)
+
+    ends = [start + extent(i, math.inf) for i, start in enumerate(starts)]
+    if starts[0] >= ends[1] or starts[1] >= ends[0]:
+        return False
+    for _, row in axes[0]:
+        if all(s < row or s % row == 0 for tensor in axes for _, s in tensor):
+            (first, size), (second, other) = ((starts[i] % row, extent(i, row)) for i in (0, 1))
+            if first + size <= second and second + other <= first + row or \
+                    second + other <= first and first + size <= second + row:
+                return False
+    return True
+
+
+def check_out(what: str, out: Tensor, *inputs: Tensor | None) -> None:
+    """Raise for a given ``out`` that a kernel cannot fill: one that autograd or
+    inference mode guards, one that holds an element twice, or one that shares
+    memory with what the kernel reads."""
+    refuse_unseen(what, out)
+    if out.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{what} has no gradient: out must not require one")
+    if out.is_inference() and not torch.is_inference_mode_enabled():
+        raise RuntimeError("inplace update to inference tensors outside InferenceMode is not allowed")
+    reach = 1
+    for stride, size in sorted((s, n) for n, s in zip(out.shape, out.stride()) if n > 1):
+        if stride < reach and out.numel():
+            raise ValueError(f"out of strides {out.stride()} holds elements more than once")
+        reach += stride * (size - 1)
+    for t in inputs:
+        if t is not None and overlap(out, t):
+            raise ValueError(f"out shares memory with what {what} reads")
+
+
 def _vectors(t: Tensor) -> bool:
     """Whether rows of ``t`` (its last axis) can be read 16 bytes at a time."""
     *strides, last = t.stride()

@@ -22,7 +22,7 @@ from torch import Tensor, nn
 
 from . import _lib
 from .attention import _DTYPES, _aligned, _check_device
-from .layers import _FORWARDS, refuse_unseen
+from .layers import _FORWARDS, _increment_version, check_out, refuse_unseen
 
 GROUPS = (32, 64, 128)
 _BLOCK_N, _BLOCK_K = 16, 128
@@ -48,14 +48,6 @@ class Weight4:
 
     def __post_init__(self) -> None:
         _check_layout(self.packed, self.scales, self.zeros, self.outputs, self.inputs, self.group)
-
-
-def _overlap(a: Tensor, b: Tensor) -> bool:
-    """Whether the memory from the first to the last element of both meets."""
-    if not a.numel() or not b.numel():
-        return False
-    ends = [t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) for t in (a, b)]
-    return a.data_ptr() < ends[1] and b.data_ptr() < ends[0]
 
 
 def _check_layout(packed: Tensor, scales: Tensor, zeros: Tensor | None, outputs: int, inputs: int, group: int) -> None:
@@ -182,8 +174,8 @@ def linear4(x: Tensor, weight: Weight4, bias: Tensor | None = None, *, out: Tens
     there, and rounded once; a row with an infinity or a NaN comes out without a
     finite value.  Built for the few rows of a decoder step or a
     drafted tree (up to 32 are read against the weights in one pass); more rows
-    are right, the weights being read again for each 32.  ``out`` must not share
-    memory with ``x``.  Returns ``(..., outputs)``."""
+    are right, the weights being read again for each 32.  ``out`` is written in
+    place and must not share memory with ``x`` or ``bias``.  Returns ``(..., outputs)``."""
     return _product(x, weight.packed, weight.scales, weight.zeros, weight.outputs, weight.inputs, weight.group, bias, out)
 
 
@@ -200,16 +192,17 @@ def _product(x: Tensor, packed: Tensor, scales: Tensor, zeros: Tensor | None, ou
     if bias is not None and (bias.shape != (outputs,) or bias.dtype is not dtype):
         raise ValueError(f"bias must be {dtype} ({outputs},), got {bias.dtype} {tuple(bias.shape)}")
     refuse_unseen("linear4", x, scales, bias)
+    given = out is not None
+    if given:
+        if out.shape != (*shape[:-1], outputs) or out.dtype is not dtype or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {(*shape[:-1], outputs)} tensor of x's dtype")
+        check_out("linear4", out, x, bias)
     if index < 0:
         raise RuntimeError(f"linear4 runs on the GPU only; got a tensor on {x.device}")
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         raise RuntimeError("linear4 has no gradient; call it under torch.no_grad() or on detached tensors")
-    if out is None:
+    if not given:
         out = x.new_empty((*shape[:-1], outputs))
-    elif out.shape != (*shape[:-1], outputs) or out.dtype is not dtype or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous {(*shape[:-1], outputs)} tensor of x's dtype")
-    elif _overlap(out, x):
-        raise ValueError("out shares memory with x, whose rows every part of the product reads")
     rows = _aligned(x if len(shape) == 2 else x.reshape(-1, inputs))
     others = (packed, scales, zeros, bias, out)
     if index != torch.cuda.current_device() or any(t is not None and t.get_device() != index for t in others):
@@ -223,6 +216,8 @@ def _product(x: Tensor, packed: Tensor, scales: Tensor, zeros: Tensor | None, ou
     status = _lib.load().asrlayer_linear4(params, _raw_stream(index))
     if status:
         _lib.check(status, "asrlayer_linear4")
+    if given:
+        _increment_version(out)
     return out
 
 

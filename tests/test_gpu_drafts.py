@@ -529,3 +529,34 @@ def test_contiguous_tensors_at_odd_offsets(dtype):
             drafts.commit_drafts(*caches[:2], *both, path, count, lengths)
             drafts.commit_drafts(*caches[2:], *(change(t) for t in both), path, count, lengths)
             assert caches[0].any() and torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
+
+
+def test_out_is_written_in_place():
+    """A given out counts as changed, may be the queries themselves and another part of
+    the buffer that holds the inputs."""
+    from asrback_amd import drafts
+    from asrback_amd.linear4 import linear4, pack4
+
+    say("out")
+    g = torch.Generator().manual_seed(6)
+    for dtype, length in ((BF16, 60), (F32, 60), (BF16, 4096)):
+        q, k, v, kd, vd, _, _, _ = make(dtype, 1, 5, 8, 2, 64, length, 0, g)
+        masks, _ = drafts.tree_masks(torch.tensor([-1, 0, 0, 2, 3]).cuda())
+        ref = drafts.tree_attention(q, k, v, kd, vd, masks)
+        arena = torch.cat((q, kd, vd, q), 2)
+        q, kd, vd, out = arena[:, :, :8], arena[:, :, 8:10], arena[:, :, 10:12], arena[:, :, 12:]
+        before = out._version
+        assert drafts.tree_attention(q, k, v, kd, vd, masks, out=out) is out and out._version > before
+        assert torch.equal(out, ref)
+        assert torch.equal(drafts.tree_attention(q, k, v, kd, vd, masks, out=q), ref) and torch.equal(q, ref)
+        with torch.inference_mode():
+            held = torch.empty_like(out)
+            assert torch.equal(drafts.tree_attention(q.copy_(ref), k, v, kd, vd, masks, out=held),
+                               drafts.tree_attention(q, k, v, kd, vd, masks))
+    weight = pack4(torch.randint(0, 16, (64, 64), generator=g, dtype=torch.uint8).cuda(), torch.ones(64, 1).cuda())
+    x, out = torch.randn(3, 64, generator=g).cuda(), torch.empty(3, 64, device="cuda")
+    before = out._version
+    linear4(x, weight, out=out)
+    assert out._version > before and torch.equal(out, linear4(x, weight))
+    with torch.inference_mode():
+        assert torch.equal(linear4(x, weight, out=torch.empty(3, 64, device="cuda")), out)
