@@ -805,7 +805,10 @@ class TextGreedyDecoder:
         """Generated tokens and mean log-probability of the rows that finished,
         which are freed (``qwen3_asr.py:1131-1155``; a trailing EOS is
         dropped)."""
-        finished = self.state.finished[: max(self.rows) + 1].tolist()
+        count = max(self.rows) + 1
+        finished, held = torch.stack((self.state.finished[:count].long(), self.state.position[:count])).tolist()
+        for slot, row in self.rows.items():
+            row["bound"] = held[slot]  # drafted passes leave it above
         done = [slot for slot in self.rows if finished[slot]]
         if not done:
             return {}

@@ -218,3 +218,22 @@ def test_bf16_verify_pass_matches_prefill(device):
         changed = (cache.keys != before).flatten(3).any(-1).any(0)
         assert changed.nonzero().tolist() == [[0, 90], [0, 91], [0, 92], [0, 93], [1, 33], [1, 34]]
         assert torch.equal(cache.values[:, 0, 92], drafts.values[:, 0, 5])
+
+
+def test_steps_after_rejected_drafts(device):
+    """Passes that accept one token of a wide tree leave the next steps their count."""
+    from asrback_amd.qwen3_asr import EOS_CHECK_INTERVAL
+
+    say("steps after rejected drafts")
+    decoder, prompts, expected = _qwen_decoder(device, True, [], draft_tokens=16)
+    slots = decoder.admit(prompts, 12)
+    width = torch.zeros(len(prompts), 16, dtype=torch.int64, device=device)
+    wrong = width + torch.tensor([0] + [QWEN3["vocab_size"]] * 15, device=device)  # no token
+    for taken in (1, 2):
+        decoder.verify(wrong, torch.tensor([-1] + [0] * 15, device=device))
+        assert decoder.finished_rows() == {}
+        assert all(decoder.rows[s]["bound"] == decoder.rows[s]["prompt_length"] + taken for s in slots)
+    assert decoder.advance() == EOS_CHECK_INTERVAL
+    results = {}
+    _drain(decoder, results)
+    assert [results[s] for s in slots] == expected
