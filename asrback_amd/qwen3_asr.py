@@ -591,8 +591,9 @@ class TextGreedyDecoder:
             self._capture_graphs()
 
     def _workspace_bytes(self) -> int:
-        """Split partials of the largest step over the buckets: the decode
-        launch per layer and the greedy choice over the logits."""
+        """Split partials of the largest step over the buckets, the decode
+        launch per layer and the greedy choice over the logits, and of the
+        largest pass over drafted trees."""
         config = self.config
         vocab = self.lm_head.out_features if isinstance(self.lm_head, Linear4) else self.lm_head.weight.shape[0]
         need = 256
@@ -602,10 +603,11 @@ class TextGreedyDecoder:
                     batch, config["num_attention_heads"], config["num_key_value_heads"], config["head_dim"],
                     length, self.dtype))
             need = max(need, attention.choice_workspace_size(batch, vocab))
-            if self.draft_tokens:
-                need = max(need, attention.choice_workspace_size(batch * self.draft_tokens, vocab), tree_workspace_size(
-                    batch, self.draft_tokens, config["num_attention_heads"], config["num_key_value_heads"],
-                    config["head_dim"], CACHE_LENGTH, self.dtype))
+        # Eager passes over trees take any number of rows, and fewer may need more.
+        for batch in range(1, self.max_batch_size + 1) if self.draft_tokens else ():
+            need = max(need, attention.choice_workspace_size(batch * self.draft_tokens, vocab), tree_workspace_size(
+                batch, self.draft_tokens, config["num_attention_heads"], config["num_key_value_heads"],
+                config["head_dim"], CACHE_LENGTH, self.dtype))
         return need
 
     @torch.inference_mode()

@@ -176,3 +176,23 @@ def test_structs_match_the_header(name, struct, tmp_path):
                     str(tmp_path / "layout")], check=True)
     got = [int(x) for x in subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.split()]
     assert got == [ctypes.sizeof(cls), *(getattr(cls, f).offset for f, _ in cls._fields_)]
+
+
+def test_decoder_workspace_holds_every_pass(lib):
+    """Passes over fewer rows than a bucket's split their choice further."""
+    from types import SimpleNamespace
+
+    from asrback_amd.attention import choice_workspace_size, decode_workspace_size
+    from asrback_amd.drafts import tree_workspace_size
+    from asrback_amd.qwen3_asr import CACHE_LENGTH, TextGreedyDecoder
+
+    for heads in (256, 8):
+        decoder = SimpleNamespace(
+            config={"num_attention_heads": heads, "num_key_value_heads": heads, "head_dim": 64}, buckets=[1, 2, 4, 8],
+            lm_head=SimpleNamespace(weight=torch.empty(151936, 1)), kv_buckets=[CACHE_LENGTH], dtype=torch.float32,
+            draft_tokens=16, max_batch_size=8)
+        held = TextGreedyDecoder._workspace_bytes(decoder)
+        for rows in range(1, 9):
+            assert choice_workspace_size(rows * 16, 151936) <= held
+            assert tree_workspace_size(rows, 16, heads, heads, 64, CACHE_LENGTH, torch.float32) <= held
+        assert all(decode_workspace_size(b, heads, heads, 64, CACHE_LENGTH, torch.float32) <= held for b in (1, 2, 4, 8))

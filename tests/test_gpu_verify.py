@@ -237,3 +237,15 @@ def test_steps_after_rejected_drafts(device):
     results = {}
     _drain(decoder, results)
     assert [results[s] for s in slots] == expected
+
+
+def test_eager_passes_on_the_decoders_workspace(device):
+    """Without graphs, trees of draft_tokens tokens take the decoder's workspace, at row
+    counts between the buckets too."""
+    say("eager, workspace")
+    decoder, prompts, expected = _qwen_decoder(device, False, [], draft_tokens=16)
+    slots = decoder.admit(prompts, 12)
+    assert max(slots) + 1 == 3 not in decoder.buckets
+    results = {}
+    drain_by_drafts(decoder, dict(zip(slots, expected)), 16, torch.Generator().manual_seed(4), results)
+    assert [results[s][0] for s in slots] == expected
