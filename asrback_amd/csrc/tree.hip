@@ -106,12 +106,6 @@ __device__ __forceinline__ f32x4_t mfma_f32(uint32_t a, uint32_t b, const f32x4_
   return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a), __uint_as_float(b), c, 0, 0, 0);
 }
 
-// Waits until a product's result can be read: the compiler puts the wait states of
-// a matrix instruction's result before its first reader in the same block, but has
-// left them out where a branch lay between (the maximum below then read registers
-// not yet written, and results differed in their last bits from run to run).
-__device__ __forceinline__ void settle(f32x4_t& x) { asm volatile("s_nop 15" : "+v"(x)); }
-
 // acc += (16 keys x 64 bytes) (16 rows x 64 bytes)^T
 template <typename T>
 __device__ __forceinline__ f32x4_t score_piece(const uint4& k, const uint4& q, f32x4_t acc) {
@@ -504,11 +498,6 @@ __global__ __launch_bounds__(64 * W, (TreeShape<T, HD>::kWavesPerSimd)) void tre
         for (int h = 0; h < kSub; ++h) s[rt][h] = score_piece<T>(kc[h], qc, s[rt][h]);
       }
     }
-
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int h = 0; h < kSub; ++h) settle(s[rt][h]);
 
     // Keys that a row does not see: past a part's keys, or no ancestor's.
     bool whole = !drafted;

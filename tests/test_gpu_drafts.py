@@ -560,3 +560,25 @@ def test_out_is_written_in_place():
     assert out._version > before and torch.equal(out, linear4(x, weight))
     with torch.inference_mode():
         assert torch.equal(linear4(x, weight, out=torch.empty(3, 64, device="cuda")), out)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_same_bits_call_after_call(dtype, d):
+    """Workgroups of one and two row tiles, of four and eight waves, split and whole,
+    slab and pages, partly filled tiles."""
+    from asrback_amd import drafts
+
+    g = torch.Generator().manual_seed(d)
+    for batch, tokens, heads, kv_heads, length, page in (
+            (1, 1, 16, 8, 480, 0), (8, 16, 16, 8, 576, 64), (2, 64, 8, 4, 1216, 0), (1, 24, 16, 8, 8000, 0),
+            (24, 33, 8, 4, 1536, 16), (70, 3, 8, 4, 48, 0), (5, 7, 6, 6, 448, 64), (16, 40, 8, 4, 1536, 0)):
+        say("repeats", dtype, d, batch, tokens, heads, kv_heads, length, page)
+        q, k, v, kd, vd, pages, _, _ = make(dtype, batch, tokens, heads, kv_heads, d, length, page, g)
+        masks, _ = drafts.tree_masks(torch.tensor([random_parents(tokens, g) for _ in range(batch)]).cuda())
+        lengths = torch.randint(0, length + 1, (batch,), generator=g).cuda()
+        first = drafts.tree_attention(q, k, v, kd, vd, masks, lengths=lengths, pages=pages)
+        differ = torch.zeros((), dtype=torch.int64, device="cuda")
+        for _ in range(30):
+            differ += (drafts.tree_attention(q, k, v, kd, vd, masks, lengths=lengths, pages=pages) != first).any()
+        assert int(differ) == 0
