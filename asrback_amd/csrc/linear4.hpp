@@ -12,8 +12,11 @@
 //     exactly, two elements an instruction (7 for 8 weights).  The 128 and the
 //     zero point leave through the accumulator, which starts at
 //     -(128 + zero) sum(x) of the group: sum x (128 + q) - (128 + zero) sum x.
-//     The sums' float32 rounding is 2^-24 of values up to 143 |x|, some 30 times
-//     the result's own: 2^-19, far below the 2^-8 of the bf16 result.
+//     The sums' float32 rounding is 2^-24 of values up to 143 |x|: with inputs around
+//     zero some 30 times the result's own, 2^-19; with a mean the offset's part grows
+//     faster than the result, whose weights are around zero (of one deviation, the
+//     root mean square over one group of 128: 2^-17).  Both are far below the 2^-8 of
+//     the bf16 result.
 //     float32: x is split into three bf16 whose sum it is, exactly, and nibbles
 //     become bf16 one by one without an offset (only the zero point leaves through
 //     the accumulator): every product is exact, and three bf16 matrix instructions take
@@ -388,9 +391,10 @@ hipError_t launch_l4_group(const asrlayer_linear4_params& p, hipStream_t stream)
   // loads x again, so at fewer blocks it costs (16 rows of 2048 to 12288 outputs, 768
   // blocks: 6.9 us with 512 workgroups, 6.6 with 256; 16384: 7.3 and 7.3; 24576: 8.7 and
   // 9.0; 4 rows to 151936: 34.7 and 43.6; two row tiles, 64 rows to 12288: 12.5 and
-  // 12.2, 33 rows of 1024 to 16384: 9.4 and 10.2).  Workgroups of the same outputs, one
-  // a block of rows, lie a multiple of 8 apart, on one XCD, whose L2 then reads the
-  // weights once (80 rows to 151936: 122.1 us for 124.1).
+  // 12.2, 33 rows of 1024 to 16384: 9.4 and 10.2).  Where the blocks are more than the
+  // workgroups across, workgroups of the same outputs, one a block of rows, lie a multiple of
+  // 8 apart, on one XCD, whose L2 then reads the weights once (80 rows to 151936: 122.1
+  // us for 124.1).
   const bool two = (p.group == 32 ? l4_per_cu<T, W, RT, NB, MB, 32, CHUNKED>()
                                   : l4_per_cu<T, W, RT, NB, MB, 128, CHUNKED>()) > 1 && blocks_n * row_blocks >= (RT == 1 ? 1536 : 2048);
   int64_t across = (two ? 512 : 256) / row_blocks;

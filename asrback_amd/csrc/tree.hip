@@ -830,9 +830,6 @@ TreePlan tree_plan(const asrlayer_tree_params& p) {
   // Two waves gain where keys are few (11.4 there) and lose elsewhere (86.1 at 900
   // keys, 108.4 for 86.2 at 3500).
   plan.waves = bytes > 512 || units > 256 ? 4 : 8;
-  // Splits up to a workgroup a CU, of half a turn's keys at least, where they save two
-  // and a half turns: partials, arrival and fold cost about as much (two splits of
-  // 480 keys 12.9 us, unsplit 11.5; 1216 keys of 512 bytes: four 14.6, unsplit 19.4).
   // The splits of workgroups of so many waves: up to a workgroup a CU, of half a turn's
   // keys at least, where they save two and a half turns: partials, arrival and fold
   // cost about as much (two splits of 480 keys 12.9 us, unsplit 11.5; 1216 keys of 512
@@ -860,9 +857,11 @@ TreePlan tree_plan(const asrlayer_tree_params& p) {
   };
   plan.splits = splits(plan.waves);
   // Rows few enough that their fold costs little are split further, over workgroups
-  // of four waves with half the turn, where CUs are left (2 rows over 480 keys: 7.4 us
-  // with 5 splits of eight waves, 6.9 with 8 of four; over 4000, 10.7 and 9.9; 16 rows
-  // over 1800, 10.1 and 12.2; 2 rows over 16000, all CUs either way, 21.1 and 21.5).
+  // of four waves with half the turn, where CUs are left (8 kv heads of 128 in bf16
+  // over 1800 keys, eight and four waves: 2 rows 9.5 and 8.9 us, 4 rows 9.6 and 9.3, 8
+  // rows 10.0 and 9.8, 12 rows 10.4 and 11.7; over 4000 keys 8 rows 11.5 and 11.5, 12
+  // rows 11.8 and 13.4; 2 rows over 16000, all CUs either way, 21.1 and 21.5.  6 heads
+  // of 64 in float32 over 440 keys gain up to 16 rows: 8.7 and 8.3).
   if (plan.splits > 1 && plan.waves == 8 && rows <= 4) {
     const int more = splits(4);
     if (more > plan.splits && more < by_units) {

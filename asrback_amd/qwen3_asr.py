@@ -775,8 +775,10 @@ class TextGreedyDecoder:
         row's newest token (its entry is not read), the others follow their
         ``parents`` (int64 ``(tokens,)`` or ``(rows, tokens)``; token 0's is -1,
         values below -1 are padding).  Rows advance by at least one token and by
-        as many drafted ones as greedy steps would have produced, with the same
-        results; finished and free rows stay as they are.  Trees of
+        as many drafted ones as greedy steps would have produced, with their
+        results; finished and free rows stay as they are.  A pass and a step round
+        differently (in bf16 the attention's weights too): where two logits lie
+        closer than that, their choices may differ.  Trees of
         ``draft_tokens`` tokens replay captured graphs."""
         if not self.rows:
             raise RuntimeError("no occupied rows")

@@ -272,3 +272,28 @@ def test_one_row_of_any_layout(dtype):
     for x in (buffer[:257].view(1, 257)[:, :256], buffer[3:259].view(1, 256), buffer[3:259], buffer[1:1025].view(2, 2, 256),
               buffer[:514].view(1, 2, 257)[:, :1, :256]):
         assert torch.equal(linear4(x, weight).cpu(), (x.double().cpu() @ matrix(values, scales, points, 64).T).to(dtype))
+
+
+@pytest.mark.parametrize("rows,inputs,outputs,group", SHAPES[::4])
+def test_inputs_with_a_mean(rows, inputs, outputs, group):
+    """Where inputs share a sign, the offset that bf16 weights carry meets their whole
+    sum: the same bound."""
+    from asrback_amd.linear4 import linear4, pack4
+
+    g = torch.Generator().manual_seed(rows * 13 + inputs)
+    say("linear4 mean", rows, inputs, outputs, group)
+    values, scales, points = quantized(outputs, inputs, group, False, BF16, g)
+    weight = pack4(values.cuda(), scales.cuda())
+    x = (torch.randn(rows, inputs, generator=g) + torch.tensor([1.0, -4.0])[torch.arange(rows) % 2, None]).to(BF16)
+    ref = x.double() @ matrix(values, scales, points, group).T
+    sums = x.double().abs() @ scales.double().repeat_interleave(group, 1).T
+    # What is left of the result once it is taken off: the sums' own error.  A group's sums
+    # reach some 143 * 128 (2^14.2), each addition off by half a step of 2^-24 of
+    # that, a dozen of them as their root (2^1.8): 2^-9 of results of some 2^6.2.
+    bias = -ref[0].to(BF16)
+    left = linear4(x[:1].cuda(), weight, bias.cuda()).cpu().double() - (ref[:1] + bias.double())
+    own = 2.0**-24 * (2 * group + inputs // group + 32) * 286 * sums
+    assert (left.abs() <= 2.0**-8 * (ref[:1] + bias.double()).abs() + own[:1]).all()
+    assert float(left.norm() / ref[0].norm()) < 2.0**-15
+    out = linear4(x.cuda(), weight).cpu().double()
+    assert ((out - ref).abs() <= 2.0**-8 * ref.abs() + own).all()
