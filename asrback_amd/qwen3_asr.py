@@ -585,6 +585,7 @@ class TextGreedyDecoder:
         self._drafted = torch.zeros((2, max_batch_size, draft_tokens), dtype=torch.long, device=self.device)
         self.workspace = torch.empty(self._workspace_bytes(), dtype=torch.uint8, device=self.device)
         self.rows: dict[int, dict] = {}
+        self._bounds_ahead = False
         self.graphs: dict[tuple[int, int], CapturedGraph] = {}
         self.verify_graphs: dict[int, CapturedGraph] = {}
         if graphs:
@@ -803,6 +804,7 @@ class TextGreedyDecoder:
             self._verify(self.state.narrow(rows), self.cache.narrow(rows, CACHE_LENGTH), drafted[:rows], parents)
         for r in self.rows.values():
             r["bound"] = min(r["bound"] + width, r["end"])
+        self._bounds_ahead = True
 
     @torch.inference_mode()
     def finished_rows(self) -> dict[int, tuple[list[int], float]]:
@@ -810,9 +812,12 @@ class TextGreedyDecoder:
         which are freed (``qwen3_asr.py:1131-1155``; a trailing EOS is
         dropped)."""
         count = max(self.rows) + 1
-        finished, held = torch.stack((self.state.finished[:count].long(), self.state.position[:count])).tolist()
-        for slot, row in self.rows.items():
-            row["bound"] = held[slot]  # drafted passes leave it above
+        finished = self.state.finished[:count].tolist()
+        if self._bounds_ahead:  # of the positions, by what drafted passes rejected
+            held = self.state.position[:count].tolist()
+            for slot, row in self.rows.items():
+                row["bound"] = held[slot]
+            self._bounds_ahead = False
         done = [slot for slot in self.rows if finished[slot]]
         if not done:
             return {}
