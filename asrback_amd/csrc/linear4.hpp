@@ -8,7 +8,7 @@
 //   * The matrix lies in blocks of 16 outputs x 128 inputs, 1 KB in the order in
 //     which a wave's lanes take it: a load is one 16-byte access per lane over
 //     whole cache lines, and the four dwords are four matrix instructions' operand.
-//   * bf16: a nibble becomes bf16 by an AND and an OR: 0x4300 | q is 128 + q
+//   * bf16: a nibble becomes bf16 by an AND and an OR: 0x3b00 | q is 2^-16 (128 + q)
 //     exactly, two elements an instruction (7 for 8 weights).  The 128 and the
 //     zero point leave through the accumulator, which starts at
 //     -(128 + zero) sum(x) of the group: sum x (128 + q) - (128 + zero) sum x.
@@ -20,15 +20,15 @@
 //     float32: x is split into three bf16 whose sum it is, exactly, and nibbles
 //     become bf16 one by one without an offset (only the zero point leaves through
 //     the accumulator): every product is exact, and three bf16 matrix instructions take
-//     the place of eight float32 ones of twice the time each (16 x 1024 x 40000: 11.5 us
+//     the place of eight float32 ones of twice the time each (16 x 1024 x 40000: 12.0 us
 //     for 20.0).
 //   * A group's sum comes before its scale, and up to 2^15.2 (float32: 2^12) times the
 //     largest |x| passes through the accumulator: 128 inputs, values up to 143 (15) of
 //     weights and of the zero point.  So that no sum overflows that the scale brings
 //     back into range, sums are kept times 2^-16 (2^-12) until the end.  In bf16 that
-//     is in the operand, which is 0x3b00 | q, and costs nothing.  float32 x is multiplied
-//     by it on its way (16 x 1024 x 40000: 12.0 us for 11.7), and what bf16 cannot hold
-//     of it is lost: 2^-121 of an x, so that those below 2^-97 go in with fewer bits.
+//     is in the operand and costs nothing.  float32 x is multiplied by it on its way
+//     (16 x 1024 x 40000: 12.0 us for 11.7), and what bf16 cannot hold of it is lost:
+//     2^-121 of an x, so that those below 2^-97 go in with fewer bits.
 //   * Outputs lie in the rows of the product and x's rows in its columns, so a
 //     lane holds four outputs of one x row: a group's scales are one small load
 //     for four outputs, the group's sum of x one value per lane.
