@@ -334,14 +334,87 @@ class Linear4Params(ctypes.Structure):
     ]
 
 
+class Linear8Params(ctypes.Structure):
+    """``asrlayer_linear8_params`` (csrc/layers.hpp)."""
+
+    _fields_ = [
+        ("x", _ptr),
+        ("x_row_stride", _i64),
+        *[(name, _ptr) for name in ("packed", "scales", "bias", "out")],
+        ("out_row_stride", _i64),
+        ("rows", _i64),
+        *[(name, _i32) for name in ("n", "k", "gated", "dtype")],
+    ]
+
+
+# The fields of ``asrlayer_cache8`` (csrc/layers.hpp), the first of each structure below.
+_CACHE8 = [
+    *[(name, _ptr) for name in ("cache_k", "cache_v", "k_scales", "v_scales")],
+    *[(f"c{t}_{axis}_stride", _i64) for t in ("k", "v") for axis in ("batch", "token", "head")],
+    *[(f"{t}s_{axis}_stride", _i64) for t in ("k", "v") for axis in ("batch", "head")],
+    ("block_table", _ptr),
+    ("bt_stride", _i64),
+    *[(name, _i32) for name in ("page_size", "num_pages", "batch", "heads_kv", "head_dim", "max_len")],
+]
+
+
+class Write8Params(ctypes.Structure):
+    """``asrlayer_write8_params`` (csrc/layers.hpp)."""
+
+    _fields_ = [
+        *_CACHE8,
+        *[(name, _ptr) for name in ("q", "k", "v", "q_out", "k_out")],
+        *[(f"{t}_{axis}_stride", _i64) for t in ("q", "k", "v") for axis in ("token", "head")],
+        *[(name, _ptr) for name in ("rows", "positions", "q_norm", "k_norm", "cos", "sin")],
+        ("rope_stride", _i64),
+        ("tokens", _i64),
+        *[(name, ctypes.c_float) for name in ("q_eps", "k_eps")],
+        *[(name, _i32) for name in ("heads_q", "dtype")],
+    ]
+
+
+class Read8Params(ctypes.Structure):
+    """``asrlayer_read8_params`` (csrc/layers.hpp)."""
+
+    _fields_ = [
+        *_CACHE8,
+        *[(name, _ptr) for name in ("k_out", "v_out", "lengths")],
+        *[(name, _i32) for name in ("lengths64", "dtype")],
+    ]
+
+
+class Decode8Params(ctypes.Structure):
+    """``asrlayer_decode8_params`` (csrc/layers.hpp)."""
+
+    _fields_ = [
+        *_CACHE8,
+        ("q", _ptr),
+        ("out", _ptr),
+        *[(f"{t}_{axis}_stride", _i64) for t in ("q", "o") for axis in ("batch", "head")],
+        ("lengths", _ptr),
+        *[(name, _i32) for name in ("lengths64", "heads_q", "window", "dtype")],
+        ("scale", ctypes.c_float),
+    ]
+
+
 # A NULL pointer is 0 in these.
 pack_tree = Packed(TreeParams).pack
 pack_commit = Packed(CommitParams).pack
 pack_linear4 = Packed(Linear4Params).pack
+pack_linear8 = Packed(Linear8Params).pack
+pack_write8 = Packed(Write8Params).pack
+pack_read8 = Packed(Read8Params).pack
+pack_decode8 = Packed(Decode8Params).pack
 
 # The layers' own entry points (csrc/layers.hpp).
 LAYER_SIGNATURES = {
     "asrlayer_linear4": (ctypes.c_int, [_ptr, _ptr]),
+    "asrlayer_linear8": (ctypes.c_int, [_ptr, _ptr, ctypes.c_size_t, _ptr]),
+    "asrlayer_linear8_workspace_size": (ctypes.c_size_t, [_i64, _i32]),
+    "asrlayer_write8": (ctypes.c_int, [_ptr, _ptr]),
+    "asrlayer_read8": (ctypes.c_int, [_ptr, _ptr]),
+    "asrlayer_decode8": (ctypes.c_int, [_ptr, _ptr, ctypes.c_size_t, _ptr]),
+    "asrlayer_decode8_workspace_size": (ctypes.c_size_t, [_ptr]),
     "asrlayer_tree": (ctypes.c_int, [_ptr, _ptr, ctypes.c_size_t, _ptr]),
     "asrlayer_tree_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(TreeParams)]),
     "asrlayer_tree_masks": (ctypes.c_int, [_ptr, _i64, _i64, _i32, _ptr, _ptr, _ptr]),

@@ -751,4 +751,202 @@ int asrlayer_linear4(const asrlayer_linear4_params* params, void* stream) {
   return from_hip(asrattn::launch_linear4(p, static_cast<hipStream_t>(stream)), "asrlayer_linear4");
 }
 
+size_t asrlayer_linear8_workspace_size(int64_t rows, int32_t k) {
+  if (rows < 0 || k < 1) return (size_t)-1;
+  return asrattn::linear8_workspace(rows, k).total;
+}
+
+int asrlayer_linear8(const asrlayer_linear8_params* params, void* workspace, size_t workspace_bytes, void* stream) {
+  if (params == nullptr) return fail(ASRATTN_ERR_INVALID, "params is NULL");
+  const asrlayer_linear8_params& p = *params;
+  if (p.dtype != ASRATTN_F32 && p.dtype != ASRATTN_BF16) return fail(ASRATTN_ERR_INVALID, "dtype %d", p.dtype);
+  if (p.rows < 0 || p.n < 1 || p.k < 1)
+    return fail(ASRATTN_ERR_INVALID, "rows must be >= 0, n and k positive");
+  if (p.gated != 0 && p.n % 2 != 0)
+    return fail(ASRATTN_ERR_INVALID, "a gated matrix has as many gates as projections, got %d outputs", p.n);
+  if (p.n > (1 << 28) || p.k > (1 << 17) || p.rows > 65535 * 16)
+    return fail(ASRATTN_ERR_UNSUPPORTED, "more than 1048560 rows, 2^28 outputs or 2^17 inputs");
+  if (p.rows == 0) return ok();
+  if (p.x == nullptr || p.packed == nullptr || p.scales == nullptr || p.out == nullptr)
+    return fail(ASRATTN_ERR_INVALID, "x, packed, scales and out must be non-NULL");
+  if ((reinterpret_cast<uintptr_t>(p.packed) & 15u) != 0)
+    return fail(ASRATTN_ERR_INVALID, "packed needs a 16-byte aligned pointer");
+  const size_t need = asrattn::linear8_workspace(p.rows, p.k).total;
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(ASRATTN_ERR_WORKSPACE, "the rows need %zu workspace bytes, got %zu", need,
+                workspace == nullptr ? (size_t)0 : workspace_bytes);
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+    return fail(ASRATTN_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  return from_hip(asrattn::launch_linear8(p, workspace, static_cast<hipStream_t>(stream)), "asrlayer_linear8");
+}
+
+}  // extern "C"
+
+namespace {
+
+// Sizes of an 8-bit cache.
+int check_cache8_sizes(const asrlayer_cache8& c, int dtype) {
+  if (dtype != ASRATTN_F32 && dtype != ASRATTN_BF16) return fail(ASRATTN_ERR_INVALID, "dtype %d", dtype);
+  if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256)
+    return fail(ASRATTN_ERR_UNSUPPORTED, "no 8-bit cache of head_dim %d (supported: 64, 128, 256)", c.head_dim);
+  if (c.batch < 0 || c.max_len < 0 || c.heads_kv < 1)
+    return fail(ASRATTN_ERR_INVALID, "batch and max_len must be >= 0, heads_kv positive");
+  if (c.batch > 65535 || c.heads_kv > 4096 || c.max_len > (1 << 30))
+    return fail(ASRATTN_ERR_UNSUPPORTED, "more than 65535 rows, 4096 heads or 2^30 positions");
+  return ASRATTN_OK;
+}
+
+// Its tensors and pages (of a cache that has positions).
+int check_cache8(const asrlayer_cache8& c) {
+  if (c.k == nullptr || c.v == nullptr || c.k_scales == nullptr || c.v_scales == nullptr)
+    return fail(ASRATTN_ERR_INVALID, "the cache's tensors must be non-NULL");
+  const int64_t bits = c.k_batch_stride | c.k_token_stride | c.k_head_stride | c.v_batch_stride | c.v_token_stride |
+                       c.v_head_stride | (int64_t)reinterpret_cast<uintptr_t>(c.k) |
+                       (int64_t)reinterpret_cast<uintptr_t>(c.v);
+  if ((bits & 15) != 0)
+    return fail(ASRATTN_ERR_INVALID, "keys and values need 16-byte aligned pointers and strides that are multiples of 16");
+  if (c.k_token_stride < 0 || c.v_token_stride < 0 || c.k_token_stride >= (1 << 26) || c.v_token_stride >= (1 << 26))
+    return fail(ASRATTN_ERR_UNSUPPORTED, "positions lie 64 MiB or more apart");
+  if (c.block_table != nullptr) {
+    if (c.page_size < 16 || (c.page_size & (c.page_size - 1)) != 0)
+      return fail(ASRATTN_ERR_UNSUPPORTED, "page_size must be a power of two >= 16, got %d", c.page_size);
+    if (c.num_pages < 0 || c.bt_stride < 1)
+      return fail(ASRATTN_ERR_INVALID, "num_pages must be >= 0 and bt_stride >= 1");
+    if ((long long)c.max_len > c.bt_stride * (long long)c.page_size)
+      return fail(ASRATTN_ERR_INVALID, "max_len (%d) exceeds the block table's reach (%lld pages of %d)", c.max_len,
+                  (long long)c.bt_stride, c.page_size);
+  }
+  return ASRATTN_OK;
+}
+
+// Whether no position holds anything: the tensors may then be NULL.
+bool empty_cache8(const asrlayer_cache8& c) {
+  return c.max_len == 0 || (c.block_table != nullptr && c.num_pages == 0);
+}
+
+int check_decode8(const asrlayer_decode8_params* params) {
+  if (params == nullptr) return fail(ASRATTN_ERR_INVALID, "params is NULL");
+  const asrlayer_decode8_params& p = *params;
+  int rc = check_cache8_sizes(p.cache, p.dtype);
+  if (rc != ASRATTN_OK) return rc;
+  rc = check_common(p.dtype, p.heads_q, p.cache.heads_kv, p.cache.head_dim, p.scale);
+  if (rc != ASRATTN_OK) return rc;
+  if (p.heads_q > 4096) return fail(ASRATTN_ERR_UNSUPPORTED, "more than 4096 heads");
+  if (p.window < 0) return fail(ASRATTN_ERR_INVALID, "window must be >= 0, got %d", p.window);
+  return ASRATTN_OK;
+}
+
+struct Decode8Workspace {
+  size_t stats, arrive, total;
+};
+
+// units: workgroups times splits over all rows; words: units of work.
+Decode8Workspace decode8_workspace(const asrlayer_decode8_params& p, size_t units, size_t words) {
+  const int group = p.heads_q / p.cache.heads_kv;
+  const size_t rows = units * (size_t)(group < 16 ? group : 16);
+  Decode8Workspace w;
+  w.stats = align256(rows * (size_t)p.cache.head_dim * sizeof(float));
+  w.arrive = w.stats + align256(rows * 2 * sizeof(float));
+  w.total = w.arrive + align256(words * sizeof(unsigned long long));
+  return w;
+}
+
+}  // namespace
+
+extern "C" {
+
+int asrlayer_write8(const asrlayer_write8_params* params, void* stream) {
+  if (params == nullptr) return fail(ASRATTN_ERR_INVALID, "params is NULL");
+  const asrlayer_write8_params& p = *params;
+  int rc = check_cache8_sizes(p.cache, p.dtype);
+  if (rc != ASRATTN_OK) return rc;
+  if (p.tokens < 0 || p.heads_q < 0) return fail(ASRATTN_ERR_INVALID, "tokens and heads_q must be >= 0");
+  if (p.tokens > (1 << 23) || p.heads_q > 4096) return fail(ASRATTN_ERR_UNSUPPORTED, "more than 2^23 tokens or 4096 heads");
+  if (p.tokens == 0) return ok();
+  asrlayer_write8_params held = p;
+  if (empty_cache8(p.cache)) {
+    held.cache.max_len = 0;  // no slot is inside
+  } else {
+    rc = check_cache8(p.cache);
+    if (rc != ASRATTN_OK) return rc;
+  }
+  if (p.k == nullptr || p.v == nullptr || p.positions == nullptr || (p.heads_q > 0 && (p.q == nullptr || p.q_out == nullptr)))
+    return fail(ASRATTN_ERR_INVALID, "k, v, positions, and q and q_out of queries must be non-NULL");
+  if ((p.k_norm == nullptr) != (p.q_norm == nullptr) || (p.cos == nullptr) != (p.sin == nullptr))
+    return fail(ASRATTN_ERR_INVALID, "the norms and the tables come in pairs");
+  if (!vec_aligned(p.q, p.dtype, {p.q_token_stride, p.q_head_stride}) ||
+      !vec_aligned(p.k, p.dtype, {p.k_token_stride, p.k_head_stride}) ||
+      !vec_aligned(p.v, p.dtype, {p.v_token_stride, p.v_head_stride}) || !vec_aligned(p.q_out, p.dtype, {}) ||
+      !vec_aligned(p.k_out, p.dtype, {}) || !vec_aligned(p.q_norm, p.dtype, {}) || !vec_aligned(p.k_norm, p.dtype, {}) ||
+      !vec_aligned(p.cos, p.dtype, {p.rope_stride}) || !vec_aligned(p.sin, p.dtype, {}))
+    return fail(ASRATTN_ERR_INVALID, "tensors need 16-byte aligned pointers and strides that are multiples of 16 bytes");
+  return from_hip(asrattn::launch_write8(held, static_cast<hipStream_t>(stream)), "asrlayer_write8");
+}
+
+int asrlayer_read8(const asrlayer_read8_params* params, void* stream) {
+  if (params == nullptr) return fail(ASRATTN_ERR_INVALID, "params is NULL");
+  const asrlayer_read8_params& p = *params;
+  int rc = check_cache8_sizes(p.cache, p.dtype);
+  if (rc != ASRATTN_OK) return rc;
+  const asrlayer_cache8& c = p.cache;
+  if (c.batch == 0 || c.max_len == 0) return ok();
+  // A launch has fewer than 2^32 threads along an axis.
+  if ((long long)c.max_len * c.heads_kv * (c.head_dim / 16) >= (1LL << 31))
+    return fail(ASRATTN_ERR_UNSUPPORTED, "more than 2^35 values a row");
+  if (c.block_table == nullptr || c.num_pages != 0) {
+    rc = check_cache8(c);
+    if (rc != ASRATTN_OK) return rc;
+  }
+  if (p.k_out == nullptr || p.v_out == nullptr) return fail(ASRATTN_ERR_INVALID, "k_out and v_out must be non-NULL");
+  if (!vec_aligned(p.k_out, p.dtype, {}) || !vec_aligned(p.v_out, p.dtype, {}))
+    return fail(ASRATTN_ERR_INVALID, "k_out and v_out need 16-byte aligned pointers");
+  return from_hip(asrattn::launch_read8(p, static_cast<hipStream_t>(stream)), "asrlayer_read8");
+}
+
+size_t asrlayer_decode8_workspace_size(const asrlayer_decode8_params* params) {
+  if (check_decode8(params) != ASRATTN_OK) return (size_t)-1;
+  const asrattn::Decode8Plan plan = asrattn::decode8_plan(*params);
+  if (plan.splits == 1) return 0;
+  // A plan that splits has at most 256 workgroups, whatever its batch.
+  return decode8_workspace(*params, 256, 256).total;
+}
+
+int asrlayer_decode8(const asrlayer_decode8_params* params, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_decode8(params);
+  if (rc != ASRATTN_OK) return rc;
+  asrlayer_decode8_params p = *params;
+  if (p.cache.batch == 0) return ok();
+  if (p.q == nullptr || p.out == nullptr) return fail(ASRATTN_ERR_INVALID, "q and out must be non-NULL");
+  if (!vec_aligned(p.q, p.dtype, {p.q_batch_stride, p.q_head_stride}))
+    return fail(ASRATTN_ERR_INVALID, "q needs a 16-byte aligned pointer and strides that are multiples of 16 bytes");
+  if (empty_cache8(p.cache)) {
+    p.cache.max_len = 0;
+    p.cache.block_table = nullptr;
+  } else {
+    rc = check_cache8(p.cache);
+    if (rc != ASRATTN_OK) return rc;
+  }
+  const asrattn::Decode8Plan plan = asrattn::decode8_plan(p);
+  if ((long long)p.cache.heads_kv * plan.head_tiles > 65535)
+    return fail(ASRATTN_ERR_UNSUPPORTED, "more than 65535 blocks of query heads");
+  float* ws_o = nullptr;
+  float* ws_ml = nullptr;
+  unsigned long long* ws_arrive = nullptr;
+  if (plan.splits > 1) {
+    const size_t words = (size_t)p.cache.batch * p.cache.heads_kv * plan.head_tiles;
+    const Decode8Workspace w = decode8_workspace(p, words * plan.splits, words);
+    if (workspace == nullptr || workspace_bytes < w.total)
+      return fail(ASRATTN_ERR_WORKSPACE, "the step needs %zu workspace bytes, got %zu", w.total,
+                  workspace == nullptr ? (size_t)0 : workspace_bytes);
+    if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+      return fail(ASRATTN_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+    char* base = static_cast<char*>(workspace);
+    ws_o = reinterpret_cast<float*>(base);
+    ws_ml = reinterpret_cast<float*>(base + w.stats);
+    ws_arrive = reinterpret_cast<unsigned long long*>(base + w.arrive);
+  }
+  return from_hip(asrattn::launch_decode8(p, plan, ws_o, ws_ml, ws_arrive, static_cast<hipStream_t>(stream)),
+                  "asrlayer_decode8");
+}
+
 }  // extern "C"

@@ -104,6 +104,27 @@ hipError_t launch_commit(const asrlayer_commit_params& p, hipStream_t stream);
 // Rows through a matrix of 4-bit weights (asrlayer_linear4).
 hipError_t launch_linear4(const asrlayer_linear4_params& p, hipStream_t stream);
 
+// Rows through a matrix of 8-bit weights (asrlayer_linear8); the workspace holds the
+// rounded rows, packed as the matrix is, and behind them their scales.
+struct Linear8Workspace {
+  size_t scales, total;
+};
+Linear8Workspace linear8_workspace(int64_t rows, int k);
+hipError_t launch_linear8(const asrlayer_linear8_params& p, void* workspace, hipStream_t stream);
+
+// The 8-bit cache: writes, reading back (asrlayer_write8, asrlayer_read8) and a
+// decoder step's attention (asrlayer_decode8) over `splits` workgroups per
+// (sequence, kv head, 16 query heads of it), whose partials the last one folds.
+hipError_t launch_write8(const asrlayer_write8_params& p, hipStream_t stream);
+hipError_t launch_read8(const asrlayer_read8_params& p, hipStream_t stream);
+struct Decode8Plan {
+  int head_tiles;  // blocks of 16 query heads of a kv head
+  int splits, waves;
+};
+Decode8Plan decode8_plan(const asrlayer_decode8_params& p);
+hipError_t launch_decode8(const asrlayer_decode8_params& p, const Decode8Plan& plan, float* ws_o, float* ws_ml,
+                          unsigned long long* ws_arrive, hipStream_t stream);
+
 // A tag for a split launch's arrival words that no other launch of the process
 // has (decode.hip).
 unsigned long long launch_tag();

@@ -232,4 +232,130 @@ typedef struct asrlayer_linear4_params {
 
 int asrlayer_linear4(const asrlayer_linear4_params* params, void* stream);
 
+// Rows through a matrix of 8-bit weights with a scale per output, the rows
+// rounded to 8 bits with a scale each:
+//
+//   s[r]    = max_k |x[r, k]| / 127                   (rounded to float32)
+//   a[r, k] = rint(x[r, k] / s[r]), within -127 .. 127 (0 where s[r] is 0)
+//   y[r, n] = s[r] w[n] sum_k a[r, k] q[n, k] (+ bias[n])
+//   out     = y                                       (gated 0)
+//   out[r, i] = silu(y[r, i]) y[r, n / 2 + i]         (gated 1: n / 2 outputs)
+//
+// The rounding is that of the exact quotient, ties to even, and the sum an exact
+// 32-bit integer, so k is at most 2^17; what follows is float32, rounded once.  A
+// row with an infinity or a NaN comes out as NaN.  x rows x_row_stride apart,
+// out rows out_row_stride apart; w and bias in x's type.  The matrix lies in
+// blocks of 16 outputs by 64 inputs, padded to whole blocks with zeros:
+//
+//   packed (n / 16, k / 64, 4, 16, 16) bytes: output 16 i + c, inputs 64 j + 16 g ..
+//     of (i, j, g, c)
+//
+// The workspace holds the rounded rows and their scales (asrlayer_linear8_workspace_size,
+// 256-byte aligned); its contents before the call do not matter, and calls that
+// share it run in stream order.
+typedef struct asrlayer_linear8_params {
+  const void* x;
+  int64_t x_row_stride;
+  const void *packed, *scales, *bias;
+  void* out;
+  int64_t out_row_stride;
+  int64_t rows;
+  int32_t n, k, gated, dtype;
+} asrlayer_linear8_params;
+
+int asrlayer_linear8(const asrlayer_linear8_params* params, void* workspace, size_t workspace_bytes, void* stream);
+
+size_t asrlayer_linear8_workspace_size(int64_t rows, int32_t k);
+
+// A cache of 8-bit keys and values, a float32 scale per position and kv head:
+// key j of sequence b is k_scales[b, h, j] k[b, j, h, :].  k, v (batch,
+// max_len, heads_kv, head_dim), scales (batch, heads_kv, max_len), consecutive
+// positions' next to each other; with a block table (int32, bt_stride entries
+// per sequence) pools (num_pages, page_size, heads_kv, head_dim) and (num_pages,
+// heads_kv, page_size), whose first strides are the batch strides: position j of
+// sequence b is position j % page_size of page block_table[b][j / page_size], and
+// of no page where that is outside [0, num_pages).  head_dim 64, 128 or 256; page
+// sizes powers of two from 16 on.
+typedef struct asrlayer_cache8 {
+  void *k, *v, *k_scales, *v_scales;
+  int64_t k_batch_stride, k_token_stride, k_head_stride;
+  int64_t v_batch_stride, v_token_stride, v_head_stride;
+  int64_t ks_batch_stride, ks_head_stride;
+  int64_t vs_batch_stride, vs_head_stride;
+  const int32_t* block_table;
+  int64_t bt_stride;
+  int32_t page_size, num_pages;
+  int32_t batch, heads_kv, head_dim, max_len;
+} asrlayer_cache8;
+
+// New tokens' keys and values into such a cache, rounded as asrlayer_linear8 rounds
+// rows, after (optionally) the norms and the rotation of asrlayer_prompt_rows:
+//
+//   q' = rot(norm(q, q_norm), cos, sin)   -> q_out              (q given)
+//   k' = rot(norm(k, k_norm), cos, sin)   -> k_out (if given) and the cache
+//   v                                     -> the cache
+//
+// Token t goes to position positions[t] of sequence rows[t] (rows NULL: t); slots
+// outside the cache or on no page are not written.  q (tokens, heads_q,
+// head_dim), k, v (tokens, heads_kv, head_dim) by their strides, q_out and k_out
+// contiguous; the norms (q_norm, k_norm) and the tables (cos, sin (tokens,
+// head_dim), rows rope_stride apart) come in pairs or are NULL.
+typedef struct asrlayer_write8_params {
+  asrlayer_cache8 cache;
+  const void *q, *k, *v;
+  void *q_out, *k_out;
+  int64_t q_token_stride, q_head_stride;
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  const int64_t *rows, *positions;
+  const void *q_norm, *k_norm, *cos, *sin;
+  int64_t rope_stride;
+  int64_t tokens;
+  float q_eps, k_eps;
+  int32_t heads_q, dtype;
+} asrlayer_write8_params;
+
+int asrlayer_write8(const asrlayer_write8_params* params, void* stream);
+
+// The cache read back: k_out[b, j, h, :] = k_scales[b, h, j] k[b, j, h, :] for j <
+// n_b, and v likewise, rounded to the element type; zeros past n_b and on no page.
+// n_b = lengths[b] (int32, or int64 with lengths64; NULL: max_len) clamped to [0,
+// max_len]; k_out and v_out (batch, max_len, heads_kv, head_dim), contiguous.
+typedef struct asrlayer_read8_params {
+  asrlayer_cache8 cache;
+  void *k_out, *v_out;
+  const void* lengths;
+  int32_t lengths64, dtype;
+} asrlayer_read8_params;
+
+int asrlayer_read8(const asrlayer_read8_params* params, void* stream);
+
+// One query per sequence over such a cache: per query head h of kv head h /
+// (heads_q / heads_kv),
+//
+//   out[b, h] = softmax_j(scale q[b, h] . k[b, j]) v[b, j]
+//
+// over the positions j < n_b (as asrlayer_read8's), with a window the last window of
+// them, that lie on a page; zeros where there are none.  The workspace holds
+// the partials of split keys (asrlayer_decode8_workspace_size, 256-byte aligned); its
+// contents before the call do not matter, and calls that share it run in stream
+// order.
+typedef struct asrlayer_decode8_params {
+  asrlayer_cache8 cache;
+  const void* q;
+  void* out;
+  int64_t q_batch_stride, q_head_stride;
+  int64_t o_batch_stride, o_head_stride;
+  const void* lengths;
+  int32_t lengths64, heads_q, window, dtype;
+  float scale;
+} asrlayer_decode8_params;
+
+int asrlayer_decode8(const asrlayer_decode8_params* params, void* workspace, size_t workspace_bytes, void* stream);
+
+// Workspace bytes of these sizes (tensors and strides may be unset): 0 when the
+// call runs unsplit, (size_t)-1 for sizes it does not take; otherwise enough for
+// any smaller batch as well.
+size_t asrlayer_decode8_workspace_size(const asrlayer_decode8_params* params);
+
 }  // extern "C"

@@ -1,0 +1,418 @@
+"""GPU: the 8-bit cache -- writes, reading back, attention -- against plain float64
+on the CPU.
+
+Writes round exactly, so their whole numbers and scales are the reference's.  Reading
+back rounds a product to float32 and that to the type.  Attention's bound, per
+element, with A = the weights times |v| and S the largest sum of |q| |k| scale over a
+row's keys: the products are exact, a score's d additions are each off by 2^-24 of
+at most S, its scales, the maximum's subtraction and the exponential by 8 more;
+weights and their sum both carry them, and the weights' sums over n keys, twice:
+
+    2^-24 A (2 (d + 8) S + 2 n + 64)   float32 work
+    2^-16 A                            bf16: a weight times its scale, as two bf16
+    2^-23 A                            float32: as three
+    2^-8 |ref|, 2^-24 |ref|            the result
+
+times 1.01 for second-order terms."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def say(*args):
+    print(*args, flush=True)
+
+
+def rounded(x):
+    scale = (x.double().abs().amax(-1, keepdim=True) / 127).float().double()
+    q = torch.where(scale > 0, x.double() / scale.where(scale > 0, torch.ones_like(scale)), 0.0)
+    return q.round().clamp(-127, 127).to(torch.int8), scale[..., 0].float()
+
+
+def random_cache(batch, length, heads, head_dim, g, head_major=False):
+    """A Cache8 on the GPU and its tensors on the CPU; with ``head_major`` of the other
+    layout that strides allow."""
+    from asrback_amd.cache8 import Cache8
+
+    shape = (batch, heads, length, head_dim) if head_major else (batch, length, heads, head_dim)
+    held = []
+    for _ in "kv":
+        t = torch.randint(-127, 128, shape, generator=g, dtype=torch.int8)
+        held.append(t.transpose(1, 2) if head_major else t)
+    scales = [(torch.rand(batch, heads, length, generator=g) + 0.5) * 0.02 for _ in "kv"]
+    device = [t.transpose(1, 2).contiguous().cuda().transpose(1, 2) if head_major else t.cuda() for t in held]
+    return Cache8(*device, *(s.cuda() for s in scales)), (*held, *scales)
+
+
+def paged(tensors, page, g, extra=3):
+    """The same positions in pages of a pool in random order; the unowned slots hold the
+    largest values and NaN scales."""
+    from asrback_amd.attention import PageTable
+    from asrback_amd.cache8 import Cache8
+
+    k, v, ks, vs = tensors
+    batch, length, heads, head_dim = k.shape
+    per = -(-length // page)
+    pool = batch * per + extra
+    ids = torch.randperm(pool, generator=g)[: batch * per].view(batch, per)
+    values = [torch.full((pool, page, heads, head_dim), 127, dtype=torch.int8) for _ in "kv"]
+    scales = [torch.full((pool, heads, page), math.nan) for _ in "kv"]
+    for b in range(batch):
+        for i in range(per):
+            n = min(page, length - i * page)
+            for pool_t, t in zip(values, (k, v)):
+                pool_t[ids[b, i], :n] = t[b, i * page : i * page + n]
+            for pool_t, t in zip(scales, (ks, vs)):
+                pool_t[ids[b, i], :, :n] = t[b, :, i * page : i * page + n]
+    table = PageTable(ids.to(torch.int32).cuda(), length)
+    return Cache8(*(t.cuda() for t in (*values, *scales))), table, ids
+
+
+def reference(q, tensors, lengths, scale, window=None):
+    """Output, weights times |v|, the largest |q| |k| scale sum per row and head, key
+    counts."""
+    k, v, ks, vs = (t.double() for t in tensors)
+    batch, heads, d = q.shape
+    group = heads // k.shape[2]
+    out = torch.zeros(batch, heads, d, dtype=torch.float64)
+    weighted, largest = torch.zeros_like(out), torch.zeros(batch, heads, 1, dtype=torch.float64)
+    for b, n in enumerate(lengths):
+        first = max(0, n - window) if window else 0
+        if n <= first:
+            continue
+        kb = (k[b, first:n] * ks[b, :, first:n].T[..., None]).transpose(0, 1).repeat_interleave(group, 0)
+        vb = (v[b, first:n] * vs[b, :, first:n].T[..., None]).transpose(0, 1).repeat_interleave(group, 0)
+        qb = q[b].double()[:, None] * scale
+        w = torch.softmax((qb * kb).sum(-1), -1)[:, None]
+        out[b], weighted[b] = (w @ vb)[:, 0], (w @ vb.abs())[:, 0]
+        largest[b] = (qb.abs() * kb.abs()).sum(-1).amax(-1, keepdim=True)
+    return out, weighted, largest
+
+
+def check(out, q, tensors, lengths, scale=None, window=None):
+    d = q.shape[-1]
+    ref, weighted, largest = reference(q, tensors, lengths, d**-0.5 if scale is None else scale, window)
+    n = torch.tensor([min(x, window or x) for x in lengths]).view(-1, 1, 1).double()
+    step, parts = (2.0**-8, 2.0**-16) if q.dtype == BF16 else (2.0**-24, 2.0**-23)
+    bound = 1.01 * (weighted * (2.0**-24 * (2 * (d + 8) * largest + 2 * n + 64) + parts) + step * ref.abs())
+    out = out.cpu().double()
+    assert torch.isfinite(out).all()
+    worst = ((out - ref).abs() / bound.clamp(min=1e-40)).max()
+    assert worst <= 1, float(worst)
+
+
+def spread(lengths, dtype=torch.int32):
+    return torch.tensor(lengths, dtype=dtype, device="cuda")
+
+
+SHAPES = [
+    # batch, heads, kv heads, head_dim, length
+    (1, 1, 1, 64, 1), (1, 16, 8, 128, 480), (2, 4, 4, 64, 31), (3, 6, 6, 64, 33), (5, 6, 6, 64, 1500), (2, 8, 1, 256, 700),
+    (4, 12, 4, 128, 65), (2, 16, 2, 128, 1000), (1, 17, 1, 64, 300), (2, 40, 1, 128, 200), (40, 16, 8, 128, 100),
+    (3, 5, 1, 256, 260), (1, 8, 8, 64, 9001), (70, 4, 4, 256, 40), (2, 2, 1, 128, 20000),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("batch,heads,kv,head_dim,length", SHAPES)
+def test_attention(dtype, batch, heads, kv, head_dim, length):
+    """Slabs of both layouts and pages, all lengths from none on, int32 and int64."""
+    from asrback_amd.cache8 import decode8
+
+    g = torch.Generator().manual_seed(batch * 1000 + length)
+    q = torch.randn(batch, heads, head_dim, generator=g).to(dtype)
+    lengths = [length] + [int(x) for x in torch.randint(0, length + 1, (batch - 1,), generator=g)]
+    if batch > 2:
+        lengths[1] = 0
+    say("decode8", dtype, batch, heads, kv, head_dim, length)
+    cache, tensors = random_cache(batch, length, kv, head_dim, g, head_major=batch % 2 == 0)
+    out = decode8(q.cuda(), cache, lengths=spread(lengths))
+    check(out, q, tensors, lengths)
+    assert all(not out[b].any() for b, n in enumerate(lengths) if n == 0)
+    if batch == 1:
+        assert torch.equal(decode8(q.cuda(), cache), out)
+    for page in (16, 64):
+        pool, table, _ = paged(tensors, page, g)
+        say("pages of", page)
+        assert torch.equal(decode8(q.cuda(), pool, lengths=spread(lengths, torch.int64), pages=table), out)
+    for window in (1, 30, length + 5):
+        say("window", window)
+        out = decode8(q.cuda(), cache, lengths=spread(lengths), window=window)
+        check(out, q, tensors, lengths, window=window)
+        assert torch.equal(decode8(q.cuda(), pool, lengths=spread(lengths), window=window, pages=table), out)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_masked_places_hold_anything(dtype):
+    """Positions past a row's keys and before its window hold NaN and infinite scales, and
+    table entries outside the pool nothing."""
+    from asrback_amd.attention import PageTable
+    from asrback_amd.cache8 import Cache8, decode8
+
+    g = torch.Generator().manual_seed(4)
+    batch, heads, kv, d, length = 4, 8, 4, 128, 200
+    q = torch.randn(batch, heads, d, generator=g).to(dtype)
+    lengths, window = [0, 77, 128, 200], 50
+    cache, tensors = random_cache(batch, length, kv, d, g)
+    dirty = [t.clone() for t in cache.tensors]
+    for b, n in enumerate(lengths):
+        for t, bad in zip(dirty[2:], (math.nan, math.inf)):
+            t[b, :, n:] = bad
+            t[b, :, : max(0, n - window)] = -bad
+    out = decode8(q.cuda(), Cache8(*dirty), lengths=spread(lengths), window=window)
+    check(out, q, tensors, lengths, window=window)
+    # Lengths outside the cache are clamped to it.
+    ends = decode8(q.cuda(), cache, lengths=spread([-5, 200, 1 << 30, 0]))
+    check(ends, q, tensors, [0, 200, 200, 0])
+    pool, table, ids = paged(tensors, 16, g)
+    broken = ids.clone()
+    broken[1, 2], broken[2, 0], broken[3, 5] = -1, 99999, -7
+    out = decode8(q.cuda(), pool, lengths=spread(lengths), pages=PageTable(broken.to(torch.int32).cuda(), length))
+    for b, gone in ((1, 2), (2, 0), (3, 5)):
+        kept = [j for j in range(lengths[b]) if j // 16 != gone]
+        part = tuple(t[b : b + 1, kept] if i < 2 else t[b : b + 1][..., kept] for i, t in enumerate(tensors))
+        check(out[b : b + 1], q[b : b + 1], part, [len(kept)])
+    none = PageTable(torch.full((4, 13), -1, dtype=torch.int32, device="cuda"), length)
+    assert not decode8(q.cuda(), pool, lengths=spread(lengths), pages=none).any()
+    empty = Cache8(*(t[:0] for t in pool.tensors))
+    assert not decode8(q.cuda(), empty, lengths=spread(lengths), pages=none).any()
+    assert not decode8(q.cuda(), Cache8.allocate(4, 0, kv, d, "cuda")).any()
+    assert decode8(q[:0].cuda(), Cache8.allocate(0, 8, kv, d, "cuda")).shape == (0, heads, d)
+    # A scale of NaN at a key that is seen shows; so does a query that is not finite.
+    seen = [t.clone() for t in cache.tensors]
+    seen[2][3, 1, 10] = math.nan
+    out = decode8(q.cuda(), Cache8(*seen))
+    assert torch.isnan(out[3, 2:4]).all() and torch.isfinite(out[:3]).all() and torch.isfinite(out[3, 4:]).all()
+    bad = q.clone()
+    bad[1, 0, 5] = math.nan
+    out = decode8(bad.cuda(), cache)
+    assert torch.isnan(out[1, 0]).all() and torch.isfinite(out[1, 1:]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_far_scores_and_values(dtype):
+    """One key far above the others, a thousand equal ones, values of very different
+    scales: no weight is lost."""
+    from asrback_amd.cache8 import Cache8, decode8
+
+    g = torch.Generator().manual_seed(9)
+    batch, heads, kv, d, length = 3, 4, 2, 64, 1200
+    q = torch.randn(batch, heads, d, generator=g).to(dtype)
+    cache, tensors = random_cache(batch, length, kv, d, g)
+    k, v, ks, vs = (t.clone() for t in tensors)
+    ks[0, :, 700] *= 40
+    ks[1] *= 1e-6
+    vs[1, :, ::3] *= 1e12
+    ks[2] *= 30
+    for out_scale in (None, 1.0):
+        cache = Cache8(*(t.cuda() for t in (k, v, ks, vs)))
+        check(decode8(q.cuda(), cache, scale=out_scale), q, (k, v, ks, vs), [length] * batch, out_scale)
+
+
+def test_long_cache_past_32_bits():
+    """Positions whose offsets pass 2^31 and 2^32 bytes."""
+    from asrback_amd.cache8 import Cache8, decode8, read8, write8
+
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB of free memory")
+    g = torch.Generator().manual_seed(2)
+    length, kv, d = (1 << 22) + 40, 8, 128  # 4.3 GB each of keys and values
+    say("long cache")
+    cache = Cache8.allocate(1, length, kv, d, "cuda")
+    at = [5, (1 << 21) + 3, (1 << 22) - 1, (1 << 22) + 39]
+    k, v = (torch.randn(len(at), kv, d, generator=g).to(BF16) for _ in "kv")
+    k *= 40  # above the zeros between them
+    q = k[torch.arange(4) % 4][:1].reshape(1, kv, d).clone()
+    write8(cache, k.cuda(), v.cuda(), torch.zeros(4, dtype=torch.int64, device="cuda"), torch.tensor(at, device="cuda"))
+    (qk, sk), (qv, sv) = rounded(k), rounded(v)
+    assert torch.equal(cache.keys[0, at].cpu(), qk) and torch.equal(cache.key_scales[0, :, at].cpu().T, sk)
+    assert torch.equal(cache.values[0, at].cpu(), qv)
+    for seen, n in ((1, 6), (2, (1 << 21) + 4), (4, length)):
+        out = decode8(q.cuda(), cache, lengths=spread([n]), window=n).cpu().double()
+        s = (q.double()[0] * (qk[:seen].double() * sk[:seen, :, None].double())).sum(-1) * d**-0.5  # (seen, heads)
+        e = torch.cat((s, torch.full((1, kv), 0.0, dtype=torch.float64)))
+        top = e.amax(0)
+        w = torch.exp(s - top)
+        total = w.sum(0) + (n - seen) * torch.exp(-top)
+        ref = (w[..., None] * qv[:seen].double() * sv[:seen, :, None].double()).sum(0) / total[:, None]
+        # The first key dwarfs the others: its score is off by at most 2^-24 (2 d) of |q| |k|.
+        assert ((out[0] - ref).abs() <= 2.0**-8 * ref.abs() + 2.0**-7 * ref.abs().amax()).all()
+    two = Cache8(*(t[:, -64:] for t in cache.tensors[:2]), *(t[..., -64:] for t in cache.tensors[2:]))
+    keys, _ = read8(two)
+    assert torch.equal(keys[0, -1].cpu(), (qk[3].float() * sk[3, :, None]).to(BF16))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kv,head_dim", [(6, 64), (8, 128), (1, 256), (5, 128)])
+def test_write_and_read_back(dtype, kv, head_dim):
+    """Slabs and pages, odd strides, slots outside the cache, positions left as they
+    were; ties, rows of zeros, NaN and infinities."""
+    from asrback_amd.attention import PageTable
+    from asrback_amd.cache8 import Cache8, read8, write8
+
+    g = torch.Generator().manual_seed(kv)
+    batch, length, tokens = 3, 96, 50
+    wide = torch.randn(tokens, 2 * kv + 1, head_dim, generator=g).to(dtype)
+    wide[3] = 0
+    wide[4, :, 0] = 127.0
+    wide[4, :, 1:] = (torch.arange(head_dim - 1) % 254 - 126.5).to(dtype)
+    wide[5, 0, 3], wide[6, 0, 4] = math.nan, math.inf
+    k, v = wide[:, :kv], wide[:, kv : 2 * kv]
+    slots = torch.randperm(batch * length, generator=g)[:tokens]
+    rows, positions = slots // length, slots % length
+    rows[7], rows[8], positions[9], positions[10] = -1, batch, -1, length
+    cache, tensors = random_cache(batch, length, kv, head_dim, g)
+    pool, table, ids = paged(tensors, 32, g)
+    broken = ids.clone()
+    broken[1, 1] = -1
+    pool_before = [t.clone() for t in pool.tensors]
+    table = PageTable(broken.to(torch.int32).cuda())
+    say("write8", dtype, kv, head_dim)
+    versions = [t._version for t in cache.tensors]
+    write8(cache, k.cuda(), v.cuda(), rows.cuda(), positions.cuda())
+    write8(pool, k.cuda(), v.cuda(), rows.cuda(), positions.cuda(), pages=table)
+    assert all(t._version > old for t, old in zip(cache.tensors, versions))
+    want = [t.clone() for t in tensors]
+    for t in range(tokens):
+        b, at = int(rows[t]), int(positions[t])
+        if not (0 <= b < batch and 0 <= at < length):
+            continue
+        for x, values, scales in ((k, want[0], want[2]), (v, want[1], want[3])):
+            finite = torch.isfinite(x[t]).all(-1)
+            q, s = rounded(torch.where(finite[:, None], x[t], torch.zeros_like(x[t])))
+            values[b, at] = torch.where(finite[:, None], q, cache.values[b, at].cpu() if x is v else cache.keys[b, at].cpu())
+            scales[b, :, at] = torch.where(finite, s, math.nan)
+    for have, t in zip(cache.tensors, want):
+        assert torch.equal(have.cpu().nan_to_num(7.0) if t.is_floating_point() else have.cpu(),
+                           t.nan_to_num(7.0) if t.is_floating_point() else t)
+    # Pages: the same, but of the page that is not there.
+    back, lengths = read8(cache, dtype=dtype), [96, 50, 0]
+    held = read8(pool, pages=table, dtype=dtype)
+    for a, b in zip(back, held):
+        a = a.clone()
+        a[1, 32:64] = 0
+        assert torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))
+    owned = set(int(x) for x in ids.flatten())
+    for page in range(pool.keys.shape[0]):
+        if page not in owned or page == int(ids[1, 1]):
+            for a, b in zip(pool.tensors, pool_before):
+                assert torch.equal(a[page].nan_to_num(7.0) if a.is_floating_point() else a[page],
+                                   b[page].nan_to_num(7.0) if b.is_floating_point() else b[page])
+    for out, values, scales in zip(back, want[:2], want[2:]):
+        ref = (values.float() * scales.transpose(1, 2)[..., None]).to(dtype)
+        assert torch.equal(out.cpu().nan_to_num(7.0), ref.nan_to_num(7.0))
+    for kind in (torch.int32, torch.int64):
+        part = read8(cache, lengths=spread(lengths, kind), dtype=dtype)
+        for a, b in zip(back, part):
+            for row, n in enumerate(lengths):
+                assert torch.equal(a[row, :n].nan_to_num(7.0), b[row, :n].nan_to_num(7.0)) and not b[row, n:].any()
+    # One token a row, and none.
+    one = Cache8.allocate(4, 9, kv, head_dim, "cuda")
+    write8(one, k[:4].cuda(), v[:4].cuda(), None, torch.tensor([0, 8, 3, 9], device="cuda"))
+    assert torch.equal(one.keys[1, 8].cpu(), rounded(k[1])[0]) and not one.keys[3].any() and not one.keys[0, 1:].any()
+    write8(one, k[:0].cuda(), v[:0].cuda(), None, torch.zeros(0, dtype=torch.int64, device="cuda"))
+    empty = Cache8(*(t[:0] for t in pool.tensors))
+    write8(empty, k.cuda(), v.cuda(), rows.cuda(), positions.cuda(), pages=table)
+    assert not read8(empty, pages=table)[0].any()
+
+
+def test_rows_of_a_decoder():
+    """The norms and the rotation before the write are the prompt pass's: in bf16 to the
+    bit; in float32 the rotation's sum may be contracted with either of its products, so
+    that results differ by a rounding of each of two terms, 2^-24 of at most sqrt(2)
+    times the row's largest, and of the norm's two products."""
+    from asrback_amd.cache8 import Cache8, write8, write_rows8
+    from asrback_amd.layers import prompt_rows
+    from asrback_amd.qwen3_asr import RMSNorm, rope_tables
+
+    for dtype in (BF16, F32):
+        for head_dim, heads, kv in ((128, 16, 8), (64, 3, 3), (256, 8, 1)):
+            torch.manual_seed(head_dim)
+            tokens = 37
+            config = {"head_dim": head_dim, "rope_theta": 1e6}
+            cos, sin = rope_tables(config, tokens, "cuda", dtype)
+            qkv = torch.randn(tokens, heads + 2 * kv, head_dim, device="cuda").to(dtype)
+            q, k, v = qkv.split((heads, kv, kv), 1)
+            norms = [RMSNorm(head_dim, eps).to("cuda", dtype) for eps in (1e-6, 1e-5)]
+            for m in norms:
+                m.weight.data.uniform_(0.5, 1.5)
+            rows = torch.arange(tokens, device="cuda") % 2
+            positions = torch.arange(tokens, device="cuda") // 2
+            scratch = [torch.zeros(2, tokens, kv, head_dim, device="cuda", dtype=dtype) for _ in "kv"]
+            with torch.no_grad():
+                q_ref, k_ref, _ = prompt_rows(q, k, v, *scratch, rows, positions, *norms, cos, sin)
+                want, have = (Cache8.allocate(2, tokens, kv, head_dim, "cuda") for _ in "ab")
+                q_out, k_out = write_rows8(have, q, k, v, rows, positions, q_norm=norms[0].weight, k_norm=norms[1].weight,
+                                           q_eps=norms[0].eps, k_eps=norms[1].eps, cos=cos, sin=sin, keys=True)
+            say("write_rows8", dtype, head_dim)
+            write8(want, k_out, v, rows, positions)
+            for a, b in ((q_out, q_ref), (k_out, k_ref)):
+                if dtype == BF16:
+                    assert torch.equal(a, b)
+                else:
+                    assert ((a - b).abs() <= 2.0**-21 * b.abs().amax(-1, keepdim=True)).all()
+            for a, b in zip(want.tensors, have.tensors):
+                assert torch.equal(a, b)
+
+
+def test_run_of_steps_in_a_graph_and_beside_another():
+    """Write and attention as a decoder runs them, captured and replayed while positions
+    move, two graphs sharing a workspace; an out given, q itself among them."""
+    from asrback_amd.attention import workspace
+    from asrback_amd.cache8 import Cache8, decode8, decode8_workspace_size, write8
+
+    g = torch.Generator().manual_seed(1)
+    batch, heads, kv, d, length = 2, 16, 8, 128, 600
+    cache, _ = random_cache(batch, length, kv, d, g)
+    other = Cache8(*(t.clone() for t in cache.tensors))
+    buffer = torch.full((decode8_workspace_size(batch, heads, kv, d, length),), 255, dtype=torch.uint8, device="cuda")
+    q = torch.randn(batch, heads, d, generator=g).to("cuda", BF16)
+    new = [torch.randn(batch, kv, d, generator=g).to("cuda", BF16) for _ in "kv"]
+    positions = torch.tensor([300, 511], device="cuda")
+
+    def step(cache):
+        write8(cache, *new, None, positions)
+        return decode8(q, cache, lengths=positions + 1)
+
+    graphs, outs = [], []
+    with torch.no_grad(), workspace(buffer):
+        step(cache), step(other)
+        for held in (cache, cache):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                outs.append(step(held))
+            graphs.append(graph)
+    for turn in range(4):
+        q.copy_(torch.randn(batch, heads, d, generator=g))
+        for t in new:
+            t.copy_(torch.randn(batch, kv, d, generator=g))
+        positions += 1
+        with torch.no_grad():
+            want = step(other)
+        for graph, out in zip(graphs, outs):
+            out.zero_()
+            graph.replay()
+            assert torch.equal(out, want)
+        for a, b in zip(cache.tensors, other.tensors):
+            assert torch.equal(a[..., :2], b[..., :2])
+        torch.cuda.synchronize()
+    want = decode8(q, cache)
+    held = torch.zeros(batch, heads, 2 * d, device="cuda", dtype=BF16)
+    out = decode8(q, cache, out=held[..., 1 : d + 1])
+    assert torch.equal(out, want) and not held[..., 0].any() and not held[..., d + 1 :].any()
+    same = q.clone()
+    assert decode8(same, cache, out=same) is same and torch.equal(same, want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        on_side = decode8(q, cache)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(on_side, want)
