@@ -766,6 +766,9 @@ int asrlayer_linear8(const asrlayer_linear8_params* params, void* workspace, siz
     return fail(ASRATTN_ERR_INVALID, "a gated matrix has as many gates as projections, got %d outputs", p.n);
   if (p.n > (1 << 28) || p.k > (1 << 17) || p.rows > 65535 * 16)
     return fail(ASRATTN_ERR_UNSUPPORTED, "more than 1048560 rows, 2^28 outputs or 2^17 inputs");
+  // A launch has fewer than 2^32 threads, 512 a tile of 256 x 128.
+  if ((p.rows + 255) / 256 * ((p.n + 127LL) / 128) >= (1 << 23))
+    return fail(ASRATTN_ERR_UNSUPPORTED, "more than 2^38 sums");
   if (p.rows == 0) return ok();
   if (p.x == nullptr || p.packed == nullptr || p.scales == nullptr || p.out == nullptr)
     return fail(ASRATTN_ERR_INVALID, "x, packed, scales and out must be non-NULL");
