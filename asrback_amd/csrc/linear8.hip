@@ -4,8 +4,16 @@
 // activation happen on the sums.
 //
 // Both operands lie in blocks of 16 (rows, outputs) x 64 inputs, 1 KB in the order in
-// which a wave's lanes take them.  The outputs are the product's rows, so a lane
+// which a wave's lanes take them: a load is 16 bytes a lane over whole cache lines, and
+// a DMA to LDS needs no order of its own.  The outputs are the product's rows, so a lane
 // holds four consecutive outputs of one row.
+//
+// Three ways, by the rows: few rows by workgroups of 16 outputs that read the weights to
+// registers, more by tiles through LDS, of which several sizes (launch_typed says which
+// and why).  One row of 2048 to 2048 outputs takes 4.9 us, of which the launch and
+// two round trips to memory are most; 4099 rows of 2048 to 2 x 6144, gated, 112 us: 206 G
+// operations at 1.85 P/s.  There the matrix cores are busy for half of the time, at a
+// clock that their power holds near 1.7 GHz (a single workgroup runs at 2.3).
 #include "kernels.hpp"
 #include "layers.hpp"
 #include "ring_common.hpp"
@@ -39,7 +47,8 @@ __device__ __forceinline__ void load_inputs(const T* row, int at, int k, bool ve
   }
 }
 
-// ring::dma16 in a kernel that uses M0 for nothing else.
+// ring::dma16 in a kernel where nothing else uses M0 (no LDS instruction of gfx950 does,
+// and the compiler has no use of its own there).
 __device__ __forceinline__ void dma16_m0(__amdgpu_buffer_rsrc_t rsrc, uint32_t lds_base, uint32_t voff) {
   asm volatile(
       "s_mov_b32 m0, %0\n\t"
@@ -47,7 +56,7 @@ __device__ __forceinline__ void dma16_m0(__amdgpu_buffer_rsrc_t rsrc, uint32_t l
       "buffer_load_dwordx4 %1, %2, 0 offen lds"
       :
       : "s"(lds_base), "v"(voff), "s"(rsrc)
-      : "memory", "m0");
+      : "memory");
 }
 
 // acc += (16 outputs x 64 inputs) (16 rows x 64 inputs)^T.  As inline assembly, so that
@@ -67,29 +76,52 @@ __device__ __forceinline__ int sum_of(const i32x4_t& acc, int r) {
 }
 __device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
-// A wave rounds a row: its largest magnitude, then 16 inputs a lane at a time.
-template <typename T>
+// LANES lanes (a wave or the workgroup) round a row, NP pieces of 16 inputs each, which
+// they hold from the one reading for the largest magnitude; longer rows are read again.
+// Bound by a round trip to memory, and by the bytes from some thousand rows on.
+template <typename T, int LANES, int NP>
 __global__ __launch_bounds__(kThreads) void round_rows_kernel(const asrlayer_linear8_params p, uint4* packed, float* scales,
                                                               bool vectors) {
-  const int64_t row = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (row >= p.rows) return;
+  const int lane = threadIdx.x % LANES;
+  const int64_t row = (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
+  if (LANES < kThreads && row >= p.rows) return;  // (uniform over a wave)
   const T* x = static_cast<const T*>(p.x) + row * p.x_row_stride;
   const int pieces = (p.k + 15) / 16, blocks = (p.k + 63) / 64;
+  float v[NP][16];
   uint32_t largest = 0;
-  for (int piece = lane; piece < pieces; piece += 64) {
-    float v[16];
-    load_inputs(x, piece * 16, p.k, vectors, v);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) largest = max(largest, magnitude(v[e]));
+  for (int u = 0; u < NP; ++u) load_inputs(x, (lane + u * LANES) * 16, p.k, vectors, v[u]);
+#pragma unroll
+  for (int u = 0; u < NP; ++u)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) largest = max(largest, magnitude(v[u][e]));
+  for (int piece = lane + NP * LANES; piece < pieces; piece += LANES) {
+    float more[16];
+    load_inputs(x, piece * 16, p.k, vectors, more);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) largest = max(largest, magnitude(more[e]));
   }
-  const Scale8 s = scale8(group_umax<64>(largest));
+  largest = group_umax<64>(largest);
+  if constexpr (LANES == kThreads) {
+    __shared__ uint32_t sm[kThreads / 64];
+    if (threadIdx.x % 64 == 0) sm[threadIdx.x / 64] = largest;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) largest = max(largest, sm[w]);
+  }
+  const Scale8 s = scale8(largest);
   if (lane == 0) scales[row] = s.scale;
   uint4* out = packed + (row / 16) * blocks * 64 + row % 16;
-  for (int piece = lane; piece < pieces; piece += 64) {
-    float v[16];
-    load_inputs(x, piece * 16, p.k, vectors, v);
-    out[piece * 16] = make_uint4(round8x4(v, s), round8x4(v + 4, s), round8x4(v + 8, s), round8x4(v + 12, s));
+  auto store = [&](int piece, const float* y) {
+    if (piece < pieces)
+      out[piece * 16] = make_uint4(round8x4(y, s), round8x4(y + 4, s), round8x4(y + 8, s), round8x4(y + 12, s));
+  };
+#pragma unroll
+  for (int u = 0; u < NP; ++u) store(lane + u * LANES, v[u]);
+  for (int piece = lane + NP * LANES; piece < pieces; piece += LANES) {
+    float more[16];
+    load_inputs(x, piece * 16, p.k, vectors, more);
+    store(piece, more);
   }
 }
 
@@ -103,47 +135,147 @@ __device__ __forceinline__ float scaled(int sum, float row, float output) {
 
 __device__ __forceinline__ float silu(float x) { return x / (1.f + fast_exp2(-kLog2e * x)); }
 
-template <typename T, bool GATED>
-__global__ __launch_bounds__(kThreads) void linear8_kernel(const asrlayer_linear8_params p, const uint4* packed,
-                                                           const float* row_scales) {
-  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+// Few rows: a workgroup takes 16 outputs (gated: and their projections) of 16 RT rows,
+// its eight waves every eighth 64 inputs, whose sums meet in LDS at the end.  Bound
+// by reading the weights, which go straight to registers, kAhead blocks while the ones
+// before are multiplied.  FUSED: up to 16 rows whose values fit LDS are rounded there by
+// every workgroup, while its first weights load, in place of a launch before it.
+constexpr int kFewWaves = 8;
+constexpr int kFusedValues = 16384;  // rounded by every workgroup
+constexpr int kFusedBytes = kFusedValues + 16 * 64;  // rows of whole blocks
+
+template <typename T, bool GATED, int RT, bool FUSED>
+__global__ __launch_bounds__(64 * kFewWaves, 4) void linear8_few_kernel(const asrlayer_linear8_params p, const uint4* packed,
+                                                                        const float* row_scales, bool vectors) {
+  constexpr int W = kFewWaves, NW = GATED ? 2 : 1, kAhead = FUSED || RT == 1 ? 4 : 2;
+  constexpr int kSums = W * NW * RT * 1024;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[FUSED && kFusedBytes > kSums ? kFusedBytes : kSums];
+  __shared__ uint32_t sm_largest[16];
+  __shared__ float sm_scale[16];
   const int outputs = GATED ? p.n / 2 : p.n;
-  const int n0 = (blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6)) * 16;
-  if (n0 >= outputs) return;
+  const int64_t row0 = (int64_t)blockIdx.y * (16 * RT);
+  const int rows = (int)min(p.rows - row0, (int64_t)(16 * RT));
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int n0 = blockIdx.x * 16;
   const int blocks = (p.k + 63) / 64;
-  const int64_t tile = blockIdx.y;
-  const uint4* x = packed + tile * blocks * 64 + lane;
-  const uint4* w[2];
+
+  // The matrix's blocks that hold the workgroup's outputs (projections behind an odd
+  // number of gates lie in two), and the lane's row of them.
+  __amdgpu_buffer_rsrc_t wrs[NW];
+  uint32_t woff[NW];
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int n = min(n0 + i, outputs - 1) + half * outputs * GATED;
-    w[half] = static_cast<const uint4*>(p.packed) + (int64_t)(n / 16) * blocks * 64 + g * 16 + n % 16;
+  for (int h = 0; h < NW; ++h) {
+    const int r = h * outputs + min(n0 + i, outputs - 1), first = (h * outputs + n0) / 16;
+    const int held = min(2, (p.n + 15) / 16 - first);
+    wrs[h] = buffer_rsrc(static_cast<const char*>(p.packed) + (int64_t)first * blocks * 1024, (uint32_t)(held * blocks) * 1024);
+    woff[h] = (uint32_t)((r / 16 - first) * blocks) * 1024 + g * 256 + r % 16 * 16;
   }
-  i32x4_t acc[2] = {};
-  for (int kb = 0; kb < blocks; ++kb) {
-    const i32x4_t xv = __builtin_bit_cast(i32x4_t, x[kb * 64]);
+  const int64_t last = (p.rows - 1) / 16;  // tile of rows (past it: repeated, not stored)
+  struct Ahead {
+    uint4 w[kAhead][NW];
+    uint4 x[FUSED ? 1 : kAhead][FUSED ? 1 : RT];
+  };
+  auto load = [&](int kb, Ahead& v) {
 #pragma unroll
-    for (int half = 0; half <= GATED; ++half)
-      acc[half] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, w[half][kb * 64]), xv, acc[half], 0, 0, 0);
+    for (int u = 0; u < kAhead; ++u) {
+      const int at = kb + u * W;
+      const uint32_t off = at < blocks ? (uint32_t)at * 1024 : 0x7ff00000u;  // past the last: zeros
+#pragma unroll
+      for (int h = 0; h < NW; ++h) v.w[u][h] = buffer_load16(wrs[h], woff[h] + off);
+      if constexpr (!FUSED) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+          v.x[u][t] = packed[(min(row0 / 16 + t, last) * blocks + min(at, blocks - 1)) * 64 + lane];
+      }
+    }
+  };
+  Ahead now;
+  load(wave, now);
+
+  const float* scales = row_scales + row0;
+  if constexpr (FUSED) {
+    // Pieces of 16 inputs, the rows' largest magnitudes first.
+    const int pieces = blocks * 4, all = rows * pieces;
+    if (threadIdx.x < 16) sm_largest[threadIdx.x] = 0;
+    __syncthreads();
+    const T* x = static_cast<const T*>(p.x);
+    for (int at = threadIdx.x; at < all; at += 64 * W) {
+      const int row = at / pieces, piece = at - row * pieces;
+      float v[16];
+      load_inputs(x + row * p.x_row_stride, piece * 16, p.k, vectors, v);
+      uint32_t largest = 0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) largest = max(largest, magnitude(v[e]));
+      // (A row's pieces are a multiple of four.)
+      const bool wide = pieces % 16 == 0;
+      largest = wide ? group_umax<16>(largest) : group_umax<4>(largest);
+      if (lane % (wide ? 16 : 4) == 0) atomicMax(&sm_largest[row], largest);
+    }
+    __syncthreads();
+    if (threadIdx.x < 16) sm_scale[threadIdx.x] = scale8(sm_largest[threadIdx.x]).scale;
+    for (int at = threadIdx.x; at < all; at += 64 * W) {
+      const int row = at / pieces, piece = at - row * pieces;
+      float v[16];
+      load_inputs(x + row * p.x_row_stride, piece * 16, p.k, vectors, v);
+      const Scale8 s = scale8(sm_largest[row]);
+      *reinterpret_cast<uint4*>(lds + (piece * rows + row) * 16) =
+          make_uint4(round8x4(v, s), round8x4(v + 4, s), round8x4(v + 8, s), round8x4(v + 12, s));
+    }
+    __syncthreads();
+    scales = sm_scale;
   }
-  const int64_t row = tile * 16 + i;
-  if (row >= p.rows) return;
-  const float rs = row_scales[row];
-  T* out = static_cast<T*>(p.out) + row * p.out_row_stride;
+  i32x4_t acc[NW][RT] = {};
+  for (int kb = wave; kb < blocks; kb += kAhead * W) {
+    Ahead next;
+    load(kb + kAhead * W, next);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        uint4 x;
+        if constexpr (FUSED)
+          x = *reinterpret_cast<const uint4*>(lds + ((min(kb + u * W, blocks - 1) * 4 + g) * rows + min(i, rows - 1)) * 16);
+        else
+          x = now.x[u][t];
+#pragma unroll
+        for (int h = 0; h < NW; ++h)
+          acc[h][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, now.w[u][h]),
+                                                            __builtin_bit_cast(i32x4_t, x), acc[h][t], 0, 0, 0);
+      }
+    now = next;
+  }
+  if constexpr (FUSED) __syncthreads();  // the rows are used up
+  i32x4_t* const sums = reinterpret_cast<i32x4_t*>(lds);
+#pragma unroll
+  for (int h = 0; h < NW; ++h)
+#pragma unroll
+    for (int t = 0; t < RT; ++t) sums[((wave * NW + h) * RT + t) * 64 + i * 4 + g] = acc[h][t];
+  __syncthreads();
+  // Four outputs of a row a thread.
   const T* ws = static_cast<const T*>(p.scales);
   const T* bias = static_cast<const T*>(p.bias);
+  for (int at = threadIdx.x; at < rows * 4; at += 64 * W) {
+    const int row = at / 4, n = n0 + at % 4 * 4;
+    i32x4_t sum[NW] = {};
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int n = n0 + 4 * g + r;
-    if (n >= outputs) break;
-    float y[2];
+    for (int w = 0; w < W; ++w)
 #pragma unroll
-    for (int half = 0; half <= GATED; ++half) {
-      const int at = n + half * outputs;
-      y[half] = scaled(acc[half][r], rs, Elem<T>::load1(ws + at));
-      if (bias != nullptr) y[half] += Elem<T>::load1(bias + at);
+      for (int h = 0; h < NW; ++h) sum[h] += sums[(w * NW + h) * RT * 64 + at];
+    const float rs = scales[row];
+    T* out = static_cast<T*>(p.out) + (row0 + row) * p.out_row_stride;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (n + r >= outputs) break;
+      float y[NW];
+#pragma unroll
+      for (int h = 0; h < NW; ++h) {
+        const int m = n + r + h * outputs;
+        y[h] = scaled(sum[h][r], rs, Elem<T>::load1(ws + m));
+        if (bias != nullptr) y[h] += Elem<T>::load1(bias + m);
+      }
+      Elem<T>::store1(out + n + r, GATED ? silu(y[0]) * y[NW - 1] : y[0]);
     }
-    Elem<T>::store1(out + n, GATED ? silu(y[0]) * y[1] : y[0]);
   }
 }
 
@@ -161,11 +293,10 @@ __device__ __forceinline__ void store_whole(T* p, const float* x) {
   for (int v = 0; v < N / EPL; ++v) *reinterpret_cast<uint4*>(p + v * EPL) = pack<T>(x + v * EPL);
 }
 
-// Tiles of 256 rows x 256 outputs (gated: 128 gates and their projections), a workgroup
-// a CU that takes one after another: four waves of 128 x 128, the largest that leave
-// room for their operands, since what bounds the product is LDS: a wave reads 16 KB of
-// it for 64 products.  Blocks of both operands, 64 inputs deep, move by DMA into a ring
-// of four stages, 1 KB an instruction, and one barrier a stage separates "landed for
+// Tiles of 32 NA rows x 32 NJ outputs (gated: half of them gates, half projections), as
+// many workgroups as a CU holds, each of which takes one tile after another: four waves
+// of 16 NA x 16 NJ.  Blocks of both operands, 64 inputs deep, move by DMA into a ring
+// of S stages in LDS, 1 KB an instruction, and one barrier a stage separates "landed for
 // every wave" from "free".  A stage's operands are read while the one before is
 // multiplied, and the next tile's first stages load through the end of this one.
 //
@@ -174,16 +305,24 @@ __device__ __forceinline__ void store_whole(T* p, const float* x) {
 // consecutive outputs of a row (8).  Its operand then takes rows of several blocks,
 // which lie 64 bytes more than their size apart, so that the 16 rows a read touches at
 // a time lie in different banks.
-constexpr int kLargeTile = 256, kStages = 4, kPitch = 1024 + 64;
-constexpr int kStageBytes = 2 * (kLargeTile / 16) * kPitch;
+constexpr int kPitch = 1024 + 64;
 // Offset of a DMA that is to write zeros.
 constexpr uint32_t kNowhere = 0x7ff00000u;
 
-template <typename T, bool GATED>
-__global__ __launch_bounds__(256, 1) void linear8_large_kernel(const asrlayer_linear8_params p, const uint4* packed,
-                                                               const float* row_scales, int row_tiles, int col_tiles,
-                                                               bool whole) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds[kStages * kStageBytes];
+template <int NA, int NJ, int S>
+struct LargeShape {
+  static constexpr int kRows = 32 * NA, kOutputs = 32 * NJ;
+  static constexpr int kStageBytes = 2 * (NA + NJ) * kPitch;
+  static constexpr int kDmas = (NA + NJ) / 2;  // of a wave and stage
+  static constexpr int kPerCu = 163840 / (S * kStageBytes) < 2 ? 1 : 2;
+};
+
+template <typename T, bool GATED, int NA, int NJ, int S>
+__global__ __launch_bounds__(256, (LargeShape<NA, NJ, S>::kPerCu)) void linear8_large_kernel(
+    const asrlayer_linear8_params p, const uint4* packed, const float* row_scales, int row_tiles, int col_tiles, bool whole) {
+  using Shape = LargeShape<NA, NJ, S>;
+  constexpr int kStageBytes = Shape::kStageBytes, kRows = Shape::kRows, kOutputs = Shape::kOutputs, kDmas = Shape::kDmas;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[S * kStageBytes];
   const int outputs = GATED ? p.n / 2 : p.n;
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -204,20 +343,21 @@ __global__ __launch_bounds__(256, 1) void linear8_large_kernel(const asrlayer_li
     constexpr int kGroup = 8;
     const int band = item / (kGroup * col_tiles), first = band * kGroup, within = item - first * col_tiles;
     const int tall = min(kGroup, row_tiles - first);
-    return {(int64_t)(first + within % tall) * kLargeTile, within / tall * (GATED ? kLargeTile / 2 : kLargeTile)};
+    return {(int64_t)(first + within % tall) * kRows, within / tall * (GATED ? kOutputs / 2 : kOutputs)};
   };
   const int turns = tiles / (int)gridDim.x + ((int)blockIdx.x < tiles % (int)gridDim.x ? 1 : 0);
 
-  // A wave's DMAs of a stage: four blocks of rows, four of outputs.
-  uint32_t xoff[4], woff[4];
+  // A wave's DMAs of a stage: NA / 2 blocks of rows, NJ / 2 of outputs.
+  uint32_t xoff[NA / 2], woff[NJ / 2];
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int block = 4 * wave + u;
-    xoff[u] = (uint32_t)block * (uint32_t)blocks * 1024 + lane * 16;
+  for (int u = 0; u < NA / 2; ++u) xoff[u] = (uint32_t)(NA / 2 * wave + u) * (uint32_t)blocks * 1024 + lane * 16;
+#pragma unroll
+  for (int u = 0; u < NJ / 2; ++u) {
     // Rows of the matrix, 16 from a multiple of 16 on but for projections behind an odd
     // number of gates.
+    const int block = NJ / 2 * wave + u;
     int r = block * 16 + i;
-    if (GATED && block >= 8) r = r - 128 + outputs % 16;
+    if (GATED && block >= NJ) r = r - 16 * NJ + outputs % 16;
     woff[u] = (uint32_t)(r / 16) * (uint32_t)blocks * 1024 + g * 256 + r % 16 * 16;
   }
   const int w_blocks = (p.n + 15) / 16;
@@ -226,25 +366,25 @@ __global__ __launch_bounds__(256, 1) void linear8_large_kernel(const asrlayer_li
   auto aim = [&](int turn) {
     const Tile tile = tile_of(turn);
     const int64_t row_block = tile.row0 / 16;
-    const int left = (int)min((int64_t)16, (p.rows + 15) / 16 - row_block);
+    const int left = (int)min((int64_t)(2 * NA), (p.rows + 15) / 16 - row_block);
     xrs = buffer_rsrc(packed + row_block * blocks * 64, (uint32_t)left * block_bytes);
     const int first = (GATED && wave >= 2 ? outputs + tile.n0 : tile.n0) / 16;
     wrs = buffer_rsrc(static_cast<const char*>(p.packed) + (int64_t)first * block_bytes,
-                      (uint32_t)min(17, w_blocks - first) * block_bytes);
+                      (uint32_t)min(2 * NJ + 1, w_blocks - first) * block_bytes);
   };
   const uint32_t lds_base = (uint32_t)(uintptr_t)lds;
-  constexpr uint32_t kW = kLargeTile / 16 * kPitch;  // the outputs' blocks of a stage
+  constexpr uint32_t kW = 2 * NA * kPitch;  // the outputs' blocks of a stage
   int issue_turn = 0, issue_step = 0;
   uint32_t issue_stage = 0, issue_at = 0;
   auto issue = [&](int u) {
-    const uint32_t base = lds_base + issue_stage + (4 * wave + u % 4) * kPitch;
-    if (u < 4)
-      dma16_m0(xrs, base, xoff[u] + issue_at);
+    if (u < NA / 2)
+      dma16_m0(xrs, lds_base + issue_stage + (NA / 2 * wave + u) * kPitch, xoff[u % (NA / 2)] + issue_at);
     else
-      dma16_m0(wrs, base + kW, woff[u - 4] + issue_at);
+      dma16_m0(wrs, lds_base + issue_stage + kW + (NJ / 2 * wave + u - NA / 2) * kPitch,
+               woff[(u - NA / 2) % (NJ / 2)] + issue_at);
   };
   auto issue_next = [&] {
-    issue_stage = issue_stage == (kStages - 1) * kStageBytes ? 0 : issue_stage + kStageBytes;
+    issue_stage = issue_stage == (S - 1) * kStageBytes ? 0 : issue_stage + kStageBytes;
     issue_at += 1024;
     if (++issue_step == steps) {
       issue_step = 0;
@@ -255,27 +395,20 @@ __global__ __launch_bounds__(256, 1) void linear8_large_kernel(const asrlayer_li
   };
 
   // Operand addresses in stage 0.
-  const uint32_t xaddr = (lds_base + 8 * wm * kPitch + lane * 16) & 0x3ffffu;
+  const uint32_t xaddr = (lds_base + NA * wm * kPitch + lane * 16) & 0x3ffffu;
   const int q = i >> 2;
-  uint32_t waddr[2];
-  if constexpr (GATED) {
-    const uint32_t at = kW + (4 * wn + (q >> 1)) * kPitch + g * 256 + (8 * (q & 1) + (i & 3)) * 16;
-    waddr[0] = (lds_base + at) & 0x3ffffu;
-    waddr[1] = (lds_base + at + 8 * kPitch) & 0x3ffffu;
-  } else {
-    const uint32_t at = kW + (8 * wn + q) * kPitch + g * 256 + (i & 3) * 16;
-    waddr[0] = (lds_base + at) & 0x3ffffu;
-    waddr[1] = (lds_base + at + 4 * kPitch) & 0x3ffffu;
-  }
-  // Product j of a wave's 128 outputs: two times 64 (gated: two times 32 gates, two
-  // times 32 projections).
+  const uint32_t waddr =
+      (lds_base + kW + g * 256 + (i & 3) * 16 +
+       (GATED ? (NJ / 2 * wn + (q >> 1)) * kPitch + (q & 1) * 128 : (NJ * wn + q) * kPitch)) & 0x3ffffu;
+  // Product j: of 64 outputs, four of them (gated: of 32 gates two, and two of the
+  // projections).
   auto read_w = [&](int j, uint32_t so) {
     if constexpr (GATED)
-      return lds_read(waddr[(j >> 1) & 1] + so + (j >> 2) * 2 * kPitch + (j & 1) * 64);
+      return lds_read(waddr + so + (j >> 2) * 2 * kPitch + ((j >> 1) & 1) * NJ * kPitch + (j & 1) * 64);
     else
-      return lds_read(waddr[j >> 2] + so + (j & 3) * 64);
+      return lds_read(waddr + so + (j >> 2) * 4 * kPitch + (j & 3) * 64);
   };
-  i32x4_t acc[8][8], xv[8], w0[8], w1[8];
+  i32x4_t acc[NA][NJ], xv[NA], w0[NJ], w1[NJ];
   // A stage is multiplied, whose operands are held but for the last rows', and the next
   // one's read.  A wave has 16 cycles for each product, the time of a few instructions of
   // others: those go between the products one by one (behind each eight of them a
@@ -283,25 +416,30 @@ __global__ __launch_bounds__(256, 1) void linear8_large_kernel(const asrlayer_li
   uint32_t so = 0;
   auto half = [&](const i32x4_t* now, i32x4_t* next) {
     const uint32_t held = so;
-    so = so == (kStages - 1) * kStageBytes ? 0 : so + kStageBytes;
+    so = so == (S - 1) * kStageBytes ? 0 : so + kStageBytes;
 #pragma unroll
-    for (int a = 0; a < 8; ++a)
+    for (int a = 0; a < NA; ++a)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < NJ; ++j) {
         multiply(now[j], xv[a], acc[a][j]);
-        if (a == 0 && j == 1) xv[7] = lds_read(xaddr + held + 7 * kPitch);
-        if (a == 0 && j == 7) {
+        const int m = a * NJ + j;
+        if (m == 1) xv[NA - 1] = lds_read(xaddr + held + (NA - 1) * kPitch);
+        if (m == NJ - 1) {
           // The next stage has landed for every wave, and every wave has the operands of
           // the one before this, whose place the DMAs take.
-          wait_vmcnt<8>();
+          wait_vmcnt<kDmas * (S - 3)>();
           asm volatile("" ::: "memory");
           __builtin_amdgcn_s_barrier();
           asm volatile("" ::: "memory");
         }
         if (a > 0 && j == 1) xv[a - 1] = lds_read(xaddr + so + (a - 1) * kPitch);
-        if (a > 0 && a < 5 && (j == 3 || j == 5)) next[2 * a - 2 + j / 5] = read_w(2 * a - 2 + j / 5, so);
-        if (a > 0 && j == 6) issue(a - 1);
-        if (a == 7 && j == 7) issue(7);
+        constexpr int kReads = (NA - 1) * NJ - 3 < 4 * NJ ? (NA - 1) * NJ - 3 : 4 * NJ, kIssues = (NA - 1) * NJ - 3;
+#pragma unroll
+        for (int u = 0; u < NJ; ++u)
+          if (m == NJ + 2 + u * kReads / NJ) next[u] = read_w(u, so);
+#pragma unroll
+        for (int u = 0; u < kDmas; ++u)
+          if (m == NJ + 3 + u * kIssues / kDmas) issue(u);
       }
     issue_next();
   };
@@ -309,23 +447,23 @@ __global__ __launch_bounds__(256, 1) void linear8_large_kernel(const asrlayer_li
   const T* ws = static_cast<const T*>(p.scales);
   const T* bias = static_cast<const T*>(p.bias);
   aim(0);
-  for (int s = 0; s < kStages - 1; ++s) {
+  for (int s = 0; s < S - 1; ++s) {
 #pragma unroll
-    for (int u = 0; u < 8; ++u) issue(u);
+    for (int u = 0; u < kDmas; ++u) issue(u);
     issue_next();
   }
-  wait_vmcnt<16>();
+  wait_vmcnt<kDmas * (S - 2)>();
   __syncthreads();
-#pragma unroll
-  for (int a = 0; a < 8; ++a) {
-    if (a < 7) xv[a] = lds_read(xaddr + a * kPitch);
-    w0[a] = read_w(a, 0);
-  }
   for (int turn = 0; turn < turns; ++turn) {
+    // (Again, behind the end of a tile, which needs the registers.)
 #pragma unroll
-    for (int a = 0; a < 8; ++a)
+    for (int a = 0; a < NA - 1; ++a) xv[a] = lds_read(xaddr + so + a * kPitch);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[a][j] = i32x4_t{0, 0, 0, 0};
+    for (int j = 0; j < NJ; ++j) w0[j] = read_w(j, so);
+#pragma unroll
+    for (int a = 0; a < NA; ++a)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[a][j] = i32x4_t{0, 0, 0, 0};
     settle();
     for (int t = 0; t < steps; t += 2) {
       half(w0, w1);
@@ -340,11 +478,11 @@ __global__ __launch_bounds__(256, 1) void linear8_large_kernel(const asrlayer_li
     const int ri = at_lane & 15, rg = at_lane >> 4;
     const Tile tile = tile_of(turn);
     constexpr int N = GATED ? 8 : 16;
-    const int64_t row_at = tile.row0 + 128 * wm + ri;
-    const int n_at = tile.n0 + (GATED ? 64 : 128) * wn + N * rg;
-    float rs[8], far = 0.f;
+    const int64_t row_at = tile.row0 + 16 * NA * wm + ri;
+    const int n_at = tile.n0 + (GATED ? 8 : 16) * NJ * wn + N * rg;
+    float rs[NA], far = 0.f;
 #pragma unroll
-    for (int a = 0; a < 8; ++a) {
+    for (int a = 0; a < NA; ++a) {
       rs[a] = row_scales[min(row_at + 16 * a, p.rows - 1)];
       far = fmaxf(far, rs[a]);
     }
@@ -352,7 +490,7 @@ __global__ __launch_bounds__(256, 1) void linear8_large_kernel(const asrlayer_li
       // As short as it can be, since it runs once a tile, at the pace its instructions
       // come from memory.
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < NJ / 4; ++c) {
         const int n = n_at + (GATED ? 32 : 64) * c;
         if (n >= outputs) break;
         float scale[16], add[16];
@@ -364,7 +502,7 @@ __global__ __launch_bounds__(256, 1) void linear8_large_kernel(const asrlayer_li
         }
         T* out = static_cast<T*>(p.out) + row_at * p.out_row_stride + n;
 #pragma unroll
-        for (int a = 0; a < 8; ++a) {
+        for (int a = 0; a < NA; ++a) {
           float y[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) y[e] = (float)sum_of(acc[a][4 * c + e / 4], e % 4) * rs[a] * scale[e];
@@ -386,14 +524,14 @@ __global__ __launch_bounds__(256, 1) void linear8_large_kernel(const asrlayer_li
     // Outputs that end inside a lane's, or rows that vectors do not write: 16 rows and 64
     // outputs at a time, in a loop.
 #pragma unroll 1
-    for (int ca = 0; ca < 16; ++ca) {
-      const int n = n_at + (GATED ? 32 : 64) * (ca / 8);
-      const int64_t row = row_at + 16 * (ca % 8);
+    for (int ca = 0; ca < NA * NJ / 4; ++ca) {
+      const int n = n_at + (GATED ? 32 : 64) * (ca / NA);
+      const int64_t row = row_at + 16 * (ca % NA);
       int sums[16];
       switch (ca) {
 #define ASR_SUMS(at)                                                                                            \
   case at:                                                                                                      \
-    for (int e = 0; e < 16; ++e) sums[e] = sum_of(acc[at % 8][4 * (at / 8) + e / 4], e % 4);                    \
+    for (int e = 0; e < 16; ++e) sums[e] = sum_of(acc[at % NA][at / NA * 4 % NJ + e / 4], e % 4);               \
     break;
         ASR_SUMS(0) ASR_SUMS(1) ASR_SUMS(2) ASR_SUMS(3) ASR_SUMS(4) ASR_SUMS(5) ASR_SUMS(6) ASR_SUMS(7)
         ASR_SUMS(8) ASR_SUMS(9) ASR_SUMS(10) ASR_SUMS(11) ASR_SUMS(12) ASR_SUMS(13) ASR_SUMS(14)
@@ -422,40 +560,88 @@ __global__ __launch_bounds__(256, 1) void linear8_large_kernel(const asrlayer_li
   wait_vmcnt<0>();  // the surplus DMAs, before the workgroup's LDS is another's
 }
 
+template <typename T, int NA, int NJ, int S>
+hipError_t launch_large(const asrlayer_linear8_params& p, const uint4* packed, const float* scales, hipStream_t stream) {
+  using Shape = LargeShape<NA, NJ, S>;
+  const int outputs = p.gated ? p.n / 2 : p.n, wide = p.gated ? Shape::kOutputs / 2 : Shape::kOutputs;
+  const int row_tiles = (int)((p.rows + Shape::kRows - 1) / Shape::kRows), col_tiles = (outputs + wide - 1) / wide;
+  // Whether a lane's outputs are vectors, of the scales and the bias as well.
+  const bool whole = (reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.scales) |
+                      reinterpret_cast<uintptr_t>(p.bias)) % 16 == 0 &&
+                     p.out_row_stride % Elem<T>::kPerVec == 0 && outputs % (p.gated ? 8 : 16) == 0;
+  const long long tiles = (long long)row_tiles * col_tiles, most = 256 * Shape::kPerCu;
+  const dim3 grid((unsigned)(tiles < most ? tiles : most));
+  if (p.gated)
+    hipLaunchKernelGGL((linear8_large_kernel<T, true, NA, NJ, S>), grid, dim3(256), 0, stream, p, packed, scales, row_tiles,
+                       col_tiles, whole);
+  else
+    hipLaunchKernelGGL((linear8_large_kernel<T, false, NA, NJ, S>), grid, dim3(256), 0, stream, p, packed, scales, row_tiles,
+                       col_tiles, whole);
+  return hipGetLastError();
+}
+
+template <typename T, int LANES, int NP>
+hipError_t launch_round(const asrlayer_linear8_params& p, uint4* packed, float* scales, bool vectors, hipStream_t stream) {
+  constexpr int kRows = kThreads / LANES;
+  hipLaunchKernelGGL((round_rows_kernel<T, LANES, NP>), dim3((unsigned)((p.rows + kRows - 1) / kRows)), dim3(kThreads), 0,
+                     stream, p, packed, scales, vectors);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_rounding(const asrlayer_linear8_params& p, uint4* packed, float* scales, bool vectors,
+                           hipStream_t stream) {
+  const int pieces = (p.k + 15) / 16;
+  if (pieces <= 64) return launch_round<T, 64, 1>(p, packed, scales, vectors, stream);
+  if (pieces <= 128) return launch_round<T, 64, 2>(p, packed, scales, vectors, stream);
+  if (pieces <= 256) return launch_round<T, kThreads, 1>(p, packed, scales, vectors, stream);
+  if (pieces <= 512) return launch_round<T, kThreads, 2>(p, packed, scales, vectors, stream);
+  return launch_round<T, kThreads, 4>(p, packed, scales, vectors, stream);
+}
+
+template <typename T, int RT, bool FUSED>
+hipError_t launch_few(const asrlayer_linear8_params& p, const uint4* packed, const float* scales, bool vectors,
+                      hipStream_t stream) {
+  const int outputs = p.gated ? p.n / 2 : p.n;
+  const dim3 grid((outputs + 15) / 16, (unsigned)((p.rows + 16 * RT - 1) / (16 * RT))), block(64 * kFewWaves);
+  if (p.gated)
+    hipLaunchKernelGGL((linear8_few_kernel<T, true, RT, FUSED>), grid, block, 0, stream, p, packed, scales, vectors);
+  else
+    hipLaunchKernelGGL((linear8_few_kernel<T, false, RT, FUSED>), grid, block, 0, stream, p, packed, scales, vectors);
+  return hipGetLastError();
+}
+
 template <typename T>
 hipError_t launch_typed(const asrlayer_linear8_params& p, void* workspace, hipStream_t stream) {
   const Linear8Workspace ws = linear8_workspace(p.rows, p.k);
   uint4* packed = static_cast<uint4*>(workspace);
   float* scales = reinterpret_cast<float*>(static_cast<char*>(workspace) + ws.scales);
   const bool vectors = reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.x_row_stride % Elem<T>::kPerVec == 0;
-  hipLaunchKernelGGL((round_rows_kernel<T>), dim3((unsigned)((p.rows + 3) / 4)), dim3(kThreads), 0, stream, p, packed,
-                     scales, vectors);
-  hipError_t err = hipGetLastError();
-  if (err != hipSuccess) return err;
   const int outputs = p.gated ? p.n / 2 : p.n;
-  if (p.rows > 64) {
-    const int row_tiles = (int)((p.rows + kLargeTile - 1) / kLargeTile);
-    const int wide = p.gated ? kLargeTile / 2 : kLargeTile, col_tiles = (outputs + wide - 1) / wide;
-    // Whether a lane's outputs are vectors, of the scales and the bias as well.
-    const bool whole = (reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.scales) |
-                        reinterpret_cast<uintptr_t>(p.bias)) % 16 == 0 &&
-                       p.out_row_stride % Elem<T>::kPerVec == 0 && outputs % (p.gated ? 8 : 16) == 0;
-    const long long tiles = (long long)row_tiles * col_tiles;
-    const dim3 grid((unsigned)(tiles < 256 ? tiles : 256));
-    if (p.gated)
-      hipLaunchKernelGGL((linear8_large_kernel<T, true>), grid, dim3(256), 0, stream, p, packed, scales, row_tiles,
-                         col_tiles, whole);
-    else
-      hipLaunchKernelGGL((linear8_large_kernel<T, false>), grid, dim3(256), 0, stream, p, packed, scales, row_tiles,
-                         col_tiles, whole);
-    return hipGetLastError();
-  }
-  const dim3 grid((outputs + 63) / 64, (unsigned)((p.rows + 15) / 16));
-  if (p.gated)
-    hipLaunchKernelGGL((linear8_kernel<T, true>), grid, dim3(kThreads), 0, stream, p, packed, scales);
-  else
-    hipLaunchKernelGGL((linear8_kernel<T, false>), grid, dim3(kThreads), 0, stream, p, packed, scales);
-  return hipGetLastError();
+  // Few values are rounded by every workgroup, while a CU holds all of its workgroups at
+  // once: 4 x 2048 to 2 x 6144 outputs (gated) 8.2 us, with a launch before it 10.7; 8 x
+  // 2048 10.1 and 10.2; 16 x 2048 13.0 and 9.4; 1 x 2048 to 40000 23.0 and 18.1.
+  if (p.rows <= 16 && p.rows * p.k <= kFusedValues && outputs <= 512 * 16)
+    return launch_few<T, 1, true>(p, nullptr, nullptr, vectors, stream);
+  const hipError_t err = launch_rounding<T>(p, packed, scales, vectors, stream);
+  if (err != hipSuccess) return err;
+  if (p.rows <= 16) return launch_few<T, 1, false>(p, packed, scales, vectors, stream);
+  if (p.rows <= 32) return launch_few<T, 2, false>(p, packed, scales, vectors, stream);
+  const auto tiles = [&](int rows, int wide) { return (p.rows + rows - 1) / rows * (((long long)outputs + wide - 1) / wide); };
+  // Workgroups of 16 outputs and all inputs read the rows anew each: two a CU (128 rows
+  // of 2048 to 4096 outputs, 512 of them: 12.0 us, 14.1 in tiles of 64 x 128; 256 to
+  // 2048, 512: 11.8 and 13.9; 200 to 4096, 1024: 17.7 and 15.7).
+  if (tiles(64, 16) <= 512) return launch_few<T, 4, false>(p, packed, scales, vectors, stream);
+  // Tiles of 64 x 128 while each has a CU, and a ring of eight stages, to itself (512
+  // rows of 6144 to 2048: 27.7 us, 33.6 in tiles of 128 x 128; 1024 of 2048 to 4096, two
+  // rounds: 23.9 and 21.1).
+  const int wide = p.gated ? 64 : 128;
+  if (tiles(64, wide) <= 256) return launch_large<T, 2, 4, 8>(p, packed, scales, stream);
+  // Tiles of 128 x 256 from three rounds of workgroups on (1880 of them, 12000 rows of
+  // 1280 to 5120: 99.5 us, 105.1 in tiles of 128 x 128; 1584, gated 4099 of 2048 to 2 x
+  // 6144: 111.8 and 118.7; 624, 1537 rows of it: 57.7 and 51.1).
+  if (tiles(128, 2 * wide) >= 1536) return launch_large<T, 4, 8, 3>(p, packed, scales, stream);
+  return launch_large<T, 4, 4, 4>(p, packed, scales, stream);
 }
 
 }  // namespace
