@@ -843,10 +843,10 @@ struct Decode8Workspace {
   size_t stats, arrive, total;
 };
 
-// units: workgroups times splits over all rows; words: units of work.
-Decode8Workspace decode8_workspace(const asrlayer_decode8_params& p, size_t units, size_t words) {
+// groups: workgroups; words: sequences times blocks of query heads.
+Decode8Workspace decode8_workspace(const asrlayer_decode8_params& p, size_t groups, size_t words) {
   const int group = p.heads_q / p.cache.heads_kv;
-  const size_t rows = units * (size_t)(group < 16 ? group : 16);
+  const size_t rows = groups * (size_t)(group < 16 ? group : 16);
   Decode8Workspace w;
   w.stats = align256(rows * (size_t)p.cache.head_dim * sizeof(float));
   w.arrive = w.stats + align256(rows * 2 * sizeof(float));
@@ -909,9 +909,10 @@ int asrlayer_read8(const asrlayer_read8_params* params, void* stream) {
 size_t asrlayer_decode8_workspace_size(const asrlayer_decode8_params* params) {
   if (check_decode8(params) != ASRATTN_OK) return (size_t)-1;
   const asrattn::Decode8Plan plan = asrattn::decode8_plan(*params);
-  if (plan.splits == 1) return 0;
-  // A plan that splits has at most 256 workgroups, whatever its batch.
-  return decode8_workspace(*params, 256, 256).total;
+  if (plan.share == 0) return 0;
+  // A plan that splits has at most 256 workgroups and 128 sequences' blocks of heads,
+  // whatever its batch.
+  return decode8_workspace(*params, 256, 128).total;
 }
 
 int asrlayer_decode8(const asrlayer_decode8_params* params, void* workspace, size_t workspace_bytes, void* stream) {
@@ -935,9 +936,9 @@ int asrlayer_decode8(const asrlayer_decode8_params* params, void* workspace, siz
   float* ws_o = nullptr;
   float* ws_ml = nullptr;
   unsigned long long* ws_arrive = nullptr;
-  if (plan.splits > 1) {
-    const size_t words = (size_t)p.cache.batch * p.cache.heads_kv * plan.head_tiles;
-    const Decode8Workspace w = decode8_workspace(p, words * plan.splits, words);
+  if (plan.share > 0) {
+    const size_t blocks = (size_t)p.cache.heads_kv * plan.head_tiles;
+    const Decode8Workspace w = decode8_workspace(p, blocks * plan.share, blocks * p.cache.batch);
     if (workspace == nullptr || workspace_bytes < w.total)
       return fail(ASRATTN_ERR_WORKSPACE, "the step needs %zu workspace bytes, got %zu", w.total,
                   workspace == nullptr ? (size_t)0 : workspace_bytes);

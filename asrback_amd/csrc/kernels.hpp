@@ -113,13 +113,14 @@ Linear8Workspace linear8_workspace(int64_t rows, int k);
 hipError_t launch_linear8(const asrlayer_linear8_params& p, void* workspace, hipStream_t stream);
 
 // The 8-bit cache: writes, reading back (asrlayer_write8, asrlayer_read8) and a
-// decoder step's attention (asrlayer_decode8) over `splits` workgroups per
-// (sequence, kv head, 16 query heads of it), whose partials the last one folds.
+// decoder step's attention (asrlayer_decode8).
 hipError_t launch_write8(const asrlayer_write8_params& p, hipStream_t stream);
 hipError_t launch_read8(const asrlayer_read8_params& p, hipStream_t stream);
 struct Decode8Plan {
   int head_tiles;  // blocks of 16 query heads of a kv head
-  int splits, waves;
+  int waves;       // of a workgroup
+  int share;       // workgroups that share all sequences' keys of their heads (0: one a sequence)
+  int splits;      // of each sequence among them (0: by their lengths)
 };
 Decode8Plan decode8_plan(const asrlayer_decode8_params& p);
 hipError_t launch_decode8(const asrlayer_decode8_params& p, const Decode8Plan& plan, float* ws_o, float* ws_ml,

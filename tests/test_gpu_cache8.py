@@ -13,7 +13,15 @@ weights and their sum both carry them, and the weights' sums over n keys, twice:
     2^-23 A                            float32: as three
     2^-8 |ref|, 2^-24 |ref|            the result
 
-times 1.01 for second-order terms."""
+times 1.01 for second-order terms.  In bf16 the products are of the stored numbers plus
+128, between 0 and 255, and the same sums of 128 are taken off again: both pass through
+the float32 accumulator, so that an addition is off by 2^-24 of at most 255 in a stored
+number's place, twice.  With B = the weights times the values' scales and Q the largest
+sum of |q| times a key's scale and the scale, that adds
+
+    2^-24 (n + 64) 510 B               to the output (n additions on a weight's way)
+    2^-24 (d + 8) 510 Q                to a score: 2 A times it to the output
+"""
 
 from __future__ import annotations
 
@@ -77,13 +85,14 @@ def paged(tensors, page, g, extra=3):
 
 
 def reference(q, tensors, lengths, scale, window=None):
-    """Output, weights times |v|, the largest |q| |k| scale sum per row and head, key
-    counts."""
+    """Output, weights times |v|, the largest |q| |k| scale sum per row and head, weights
+    times v's scales, the largest |q| sum times a key's scale and the scale."""
     k, v, ks, vs = (t.double() for t in tensors)
     batch, heads, d = q.shape
     group = heads // k.shape[2]
     out = torch.zeros(batch, heads, d, dtype=torch.float64)
     weighted, largest = torch.zeros_like(out), torch.zeros(batch, heads, 1, dtype=torch.float64)
+    units, queries = torch.zeros_like(largest), torch.zeros_like(largest)
     for b, n in enumerate(lengths):
         first = max(0, n - window) if window else 0
         if n <= first:
@@ -94,15 +103,19 @@ def reference(q, tensors, lengths, scale, window=None):
         w = torch.softmax((qb * kb).sum(-1), -1)[:, None]
         out[b], weighted[b] = (w @ vb)[:, 0], (w @ vb.abs())[:, 0]
         largest[b] = (qb.abs() * kb.abs()).sum(-1).amax(-1, keepdim=True)
-    return out, weighted, largest
+        units[b] = (w[:, 0] * vs[b, :, first:n].repeat_interleave(group, 0)).sum(-1, keepdim=True)
+        queries[b] = qb.abs().sum(-1) * ks[b, :, first:n].repeat_interleave(group, 0).amax(-1, keepdim=True)
+    return out, weighted, largest, units, queries
 
 
 def check(out, q, tensors, lengths, scale=None, window=None):
     d = q.shape[-1]
-    ref, weighted, largest = reference(q, tensors, lengths, d**-0.5 if scale is None else scale, window)
+    ref, weighted, largest, units, queries = reference(q, tensors, lengths, d**-0.5 if scale is None else scale, window)
     n = torch.tensor([min(x, window or x) for x in lengths]).view(-1, 1, 1).double()
     step, parts = (2.0**-8, 2.0**-16) if q.dtype == BF16 else (2.0**-24, 2.0**-23)
     bound = 1.01 * (weighted * (2.0**-24 * (2 * (d + 8) * largest + 2 * n + 64) + parts) + step * ref.abs())
+    if q.dtype == BF16:
+        bound += 1.01 * 2.0**-24 * 510 * ((n + 64) * units + 2 * weighted * (d + 8) * queries)
     out = out.cpu().double()
     assert torch.isfinite(out).all()
     worst = ((out - ref).abs() / bound.clamp(min=1e-40)).max()
