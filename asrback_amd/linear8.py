@@ -25,7 +25,7 @@ from torch import Tensor, nn
 
 from . import _lib
 from .attention import _DTYPES, _check_device
-from .layers import _increment_version, check_out, refuse_unseen
+from .layers import _increment_version, check_out, computes, refuse_unseen
 from .linear4 import _as_built
 
 _BLOCK_N, _BLOCK_K = 16, 64
@@ -184,6 +184,7 @@ def _product(what: str, x: Tensor, packed: Tensor, scales: Tensor, outputs: int,
     return out
 
 
+@computes
 class Linear8(nn.Module):
     """``nn.Linear`` with 8-bit weights (:func:`linear8`); made by
     :meth:`from_linear` or from a :class:`Weight8`.  The matrix lies in

@@ -24,6 +24,10 @@ decode loop around them (``DecodeState``, ``choose``, ``TextGreedyDecoder``:
   rows hold the pages their prompt and generation limit need.  Its layers
   index like the slab (``keys[rows, positions] = k``), so the attention
   modules take either cache.
+* :class:`KVCache8` and :class:`PagedKVCache8` hold 8-bit keys and values
+  (``TextGreedyDecoder(cache_bits=8)``, :mod:`asrback_amd.cache8`), and 8-bit
+  layers (:func:`asrback_amd.linear8.quantize_linears8`) run the gated
+  feed-forward block as one product.
 * Drafted tokens, which the reference has not: ``verify`` of ``TextAttention``,
   ``TextModel`` and ``TextGreedyDecoder`` runs a tree of them through the model
   in one pass (:mod:`asrback_amd.drafts`) and keeps those that greedy steps
@@ -44,8 +48,10 @@ from torch import Tensor, nn
 from . import attention
 from .attention import KeyPrefix, PageTable, decode, decode_append, greedy_choice, varlen_attn
 from .drafts import MAX_TOKENS, accept_drafts, commit_drafts, tree_attention, tree_masks, tree_workspace_size
-from .layers import computes, prompt_rows, prompt_rows_takes
+from .cache8 import Cache8, decode8, decode8_workspace_size, read8, write8, write_rows8
+from .layers import computes, prompt_rows, prompt_rows_takes, unhooked
 from .linear4 import Linear4
+from .linear8 import Linear8
 from .transcription import CapturedGraph, to_device
 
 # Positions per row of the KV cache (qwen3_asr.py:57-59).
@@ -243,6 +249,61 @@ class PagedKVCache:
         self.free_pages.extend(reversed(pages))
 
 
+class Layer8:
+    """One layer's keys and values of a :class:`KVCache8` or :class:`PagedKVCache8`."""
+
+    def __init__(self, cache: Cache8, pages: PageTable | None = None) -> None:
+        self.cache = cache
+        self.pages = pages
+        batch, length, *heads = cache.keys.shape
+        if pages is not None:
+            batch, length = pages.block_table.shape[0], pages.max_len
+        self.shape = (batch, length, *heads)
+
+
+class KVCache8:
+    """:class:`KVCache` with 8-bit values and a float32 scale per position and kv
+    head: ``keys[i]`` and ``values[i]`` are both layer ``i``'s :class:`Layer8`."""
+
+    def __init__(self, layers: list[Cache8]) -> None:
+        self.layers = layers
+        self.keys = self.values = [Layer8(layer) for layer in layers]
+
+    @classmethod
+    def allocate(cls, config: dict, batch: int, length: int, device) -> KVCache8:
+        return cls([Cache8.allocate(batch, length, config["num_key_value_heads"], config["head_dim"], device)
+                    for _ in range(config["num_hidden_layers"])])
+
+    def narrow(self, batch_size: int, length: int) -> KVCache8:
+        return KVCache8([Cache8(layer.keys[:batch_size, :length], layer.values[:batch_size, :length],
+                                layer.key_scales[:batch_size, :, :length], layer.value_scales[:batch_size, :, :length])
+                         for layer in self.layers])
+
+
+class PagedKVCache8(PagedKVCache):
+    """:class:`PagedKVCache` over pools of 8-bit values, one
+    :class:`~asrback_amd.cache8.Cache8` a layer.  Without a sink page: the writes leave
+    alone what has no page."""
+
+    def __init__(self, layers: list[Cache8], block_table: Tensor, page_size: int, free_pages: list[int]) -> None:
+        self.layers, self.block_table, self.page_size, self.free_pages = layers, block_table, page_size, free_pages
+        table = PageTable(block_table, CACHE_LENGTH)
+        self.keys = self.values = [Layer8(layer, table) for layer in layers]
+
+    @classmethod
+    def allocate(cls, config: dict, batch: int, num_pages: int, page_size: int, device) -> PagedKVCache8:
+        if CACHE_LENGTH % page_size:
+            raise ValueError(f"page_size must divide {CACHE_LENGTH}")
+        layers = [Cache8.allocate(num_pages, page_size, config["num_key_value_heads"], config["head_dim"], device)
+                  for _ in range(config["num_hidden_layers"])]
+        table = torch.full((batch, CACHE_LENGTH // page_size), -1, dtype=torch.int32, device=device)
+        return cls(layers, table, page_size, list(range(num_pages - 1, -1, -1)))
+
+    def narrow(self, batch_size: int, length: int) -> PagedKVCache8:
+        del length  # every row reads only its own pages
+        return PagedKVCache8(self.layers, self.block_table[:batch_size], self.page_size, self.free_pages)
+
+
 @dataclass
 class DraftCache:
     """Keys and values of drafted tokens, ``(layers, batch, tokens, kv_heads,
@@ -259,10 +320,20 @@ class DraftCache:
     def narrow(self, batch_size: int, tokens: int) -> DraftCache:
         return DraftCache(self.keys[:, :batch_size, :tokens], self.values[:, :batch_size, :tokens])
 
-    def commit(self, cache: KVCache | PagedKVCache, path: Tensor, count: Tensor, lengths: Tensor) -> None:
+    def commit(self, cache: KVCache | PagedKVCache | KVCache8, path: Tensor, count: Tensor, lengths: Tensor) -> None:
         """Write the accepted tokens into ``cache``
-        (:func:`~asrback_amd.drafts.commit_drafts`)."""
-        if isinstance(cache, PagedKVCache):
+        (:func:`~asrback_amd.drafts.commit_drafts`, :func:`~asrback_amd.cache8.write8`)."""
+        if isinstance(cache, (KVCache8, PagedKVCache8)):
+            batch, width = path.shape
+            step = torch.arange(width, device=path.device)
+            there = (step < count[:, None]) & (path >= 0) & (path < self.keys.shape[2])
+            # (outside the cache: not written)
+            positions = torch.where(there, lengths[:, None] + step, -1).flatten()
+            rows = torch.arange(batch, device=path.device).repeat_interleave(width)
+            drafted = path.clamp(0, self.keys.shape[2] - 1).flatten()
+            for layer, k, v in zip(cache.keys, self.keys, self.values):
+                write8(layer.cache, k[rows, drafted], v[rows, drafted], rows, positions, pages=layer.pages)
+        elif isinstance(cache, PagedKVCache):
             pages = PageTable(cache.block_table, CACHE_LENGTH)
             commit_drafts(cache.pool_keys, cache.pool_values, self.keys, self.values, path, count, lengths, pages=pages)
         else:
@@ -334,13 +405,32 @@ class TextAttention(nn.Module):
         values[rows, positions] = v
         return q, k, v
 
+    def _rows8(self, x, layer: Layer8, rows, positions, cos, sin, prompt: bool) -> tuple[Tensor, ...]:
+        """The queries of ``x``, the rounded keys and values written to an 8-bit cache,
+        and for a prompt the keys and values as they were."""
+        qkv = self.qkv_proj(x)
+        norms = q_norm, k_norm = self.q_norm, self.k_norm
+        if type(q_norm) is RMSNorm and type(k_norm) is RMSNorm and unhooked(*norms):
+            q, k, v = (t.view(len(x), -1, self.head_dim) for t in qkv.split(self.sizes, dim=-1))
+            q, k = write_rows8(layer.cache, q, k, v, rows, positions, q_norm=q_norm.weight, k_norm=k_norm.weight,
+                               q_eps=q_norm.eps, k_eps=k_norm.eps, cos=cos, sin=sin, pages=layer.pages, keys=prompt)
+        else:
+            q, k, v = self._norm_rotate(qkv, cos, sin)
+            write8(layer.cache, k, v, rows, positions, pages=layer.pages)
+        return q, k, v
+
     def prefill(self, x, keys, values, rows, positions, segments: Segments, cos, sin) -> Tensor:
         """The prompt pass (``:374-390``): keys and values of the packed
         prompts are stored at (row, position) in the cache, then each prompt
         attends causally within itself.  The norms, the rotation and the
         cache writes are one kernel on the tensors it takes
-        (:func:`~asrback_amd.layers.prompt_rows`)."""
-        q, k, v = self._prompt_rows(x, keys, values, rows, positions, cos, sin)
+        (:func:`~asrback_amd.layers.prompt_rows`,
+        :func:`~asrback_amd.cache8.write_rows8`: prompts attend to their own
+        keys and values as they were before an 8-bit cache's rounding)."""
+        if isinstance(keys, Layer8):
+            q, k, v = self._rows8(x, keys, rows, positions, cos, sin, True)
+        else:
+            q, k, v = self._prompt_rows(x, keys, values, rows, positions, cos, sin)
         return self.o_proj(attend(q, k, v, segments, causal=True).flatten(1))
 
     def _fused_step(self, x: Tensor, keys: Tensor) -> bool:
@@ -358,7 +448,13 @@ class TextAttention(nn.Module):
         :class:`KeyPrefix` of ``positions``, as :meth:`TextModel.step`
         passes), the norms, the rotation, the cache write and the attention
         run as one kernel (:func:`~asrback_amd.attention.decode_append`);
-        other mask forms take the reference's sequence of ops."""
+        other mask forms take the reference's sequence of ops.  Over an 8-bit
+        cache it is a write (:func:`~asrback_amd.cache8.write_rows8`) and the
+        attention (:func:`~asrback_amd.cache8.decode8`), with any mask form."""
+        if isinstance(keys, Layer8):
+            q, _, _ = self._rows8(x, keys, None, positions, cos, sin, False)
+            output = decode8(q, keys.cache, lengths=_step_lengths(mask, positions, keys.shape[1]), pages=keys.pages)
+            return self.o_proj(output.flatten(1))
         key_cache, pages = _cache_layer(keys)
         value_cache, _ = _cache_layer(values)
         if isinstance(mask, KeyPrefix) and mask.positions is positions and self._fused_step(x, key_cache):
@@ -389,9 +485,14 @@ class TextAttention(nn.Module):
         :func:`~asrback_amd.drafts.tree_masks`), whose keys and values go to
         ``k_draft``/``v_draft`` ``(batch, tokens, kv_heads, head_dim)``; the cache
         stays as it is.  ``cos``/``sin`` ``(batch, tokens, head_dim)`` at each
-        token's position, ``rows`` 0 .. batch - 1 (int64)."""
-        key_cache, pages = _cache_layer(keys)
-        value_cache, _ = _cache_layer(values)
+        token's position, ``rows`` 0 .. batch - 1 (int64).  An 8-bit cache is read
+        back for it (:func:`~asrback_amd.cache8.read8`)."""
+        if isinstance(keys, Layer8):
+            pages = None
+            key_cache, value_cache = read8(keys.cache, lengths=lengths, pages=keys.pages, dtype=x.dtype)
+        else:
+            key_cache, pages = _cache_layer(keys)
+            value_cache, _ = _cache_layer(values)
         batch, tokens, _ = x.shape
         qkv = self.qkv_proj(x)
         q, k, v = (t.view(batch, tokens, -1, self.head_dim) for t in qkv.split(self.sizes, dim=-1))
@@ -414,6 +515,8 @@ class TextMLP(nn.Module):
         self.down_proj = nn.Linear(hidden, width, bias=False)
 
     def forward(self, x: Tensor) -> Tensor:
+        if type(self.gate_up_proj) is Linear8 and unhooked(self.gate_up_proj):
+            return self.down_proj(self.gate_up_proj.gated(x))
         gate, up = self.gate_up_proj(x).chunk(2, dim=-1)
         return self.down_proj(F.silu(gate) * up)
 
@@ -446,7 +549,8 @@ class TextModel(nn.Module):
             x = layer(x, lambda attention, h: attention.prefill(h, keys, values, rows, positions, segments, cos, sin))
         return self.norm(x)
 
-    def step(self, tokens, positions, cache: KVCache, cos, sin, varlen: bool = True) -> Tensor:
+    def step(self, tokens, positions, cache: KVCache | PagedKVCache | KVCache8, cos, sin,
+             varlen: bool = True) -> Tensor:
         """Hidden states for one token per row over a fixed-shape cache view;
         ``cos``/``sin`` are the full tables.  Each row reads its keys
         ``0 .. position`` whatever the view's length (``varlen`` is kept for
@@ -455,13 +559,15 @@ class TextModel(nn.Module):
         x = self.embed_tokens(tokens)
         cos, sin = cos[positions], sin[positions]
         mask = KeyPrefix(positions=positions)
+        if isinstance(cache, (KVCache8, PagedKVCache8)):  # counted once for all layers
+            mask = KeyPrefix(lengths=_step_lengths(None, positions, cache.keys[0].shape[1]))
         for index, layer in enumerate(self.layers):
             keys, values = cache.keys[index], cache.values[index]
             x = layer(x, lambda attention, h: attention.step(h, keys, values, positions, mask, cos, sin))
         return self.norm(x)
 
 
-    def verify(self, tokens, lengths, cache: KVCache | PagedKVCache, drafts: DraftCache, masks, depths, cos,
+    def verify(self, tokens, lengths, cache: KVCache | PagedKVCache | KVCache8, drafts: DraftCache, masks, depths, cos,
                sin) -> Tensor:
         """Hidden states ``(batch, tokens, width)`` of drafted trees
         ``tokens`` ``(batch, tokens)`` behind the ``lengths`` (int64) keys each row
@@ -553,14 +659,18 @@ class TextGreedyDecoder:
     reference's varlen path.  With ``page_size`` the cache is a
     :class:`PagedKVCache` of ``num_pages`` pages (default: as many
     positions as the slab): a row holds the pages for its prompt and its
-    generation limit from admission until it finishes.  :meth:`verify` takes
+    generation limit from admission until it finishes.  With ``cache_bits=8``
+    the cache is a :class:`KVCache8` (:class:`PagedKVCache8`), in about half of
+    bf16's memory.  :meth:`verify` takes
     drafted trees instead of single steps; ``draft_tokens`` is the tree size
     whose passes are captured in graphs as well.
     """
 
     def __init__(self, text: TextModel, lm_head: nn.Module, config: dict, max_batch_size: int,
                  eos_ids: list[int], graphs: bool = True, page_size: int | None = None,
-                 num_pages: int | None = None, draft_tokens: int = 0) -> None:
+                 num_pages: int | None = None, draft_tokens: int = 0, cache_bits: int | None = None) -> None:
+        if cache_bits not in (None, 8):
+            raise ValueError(f"the cache holds the model's type (None) or 8 bits, got cache_bits={cache_bits}")
         self.text = text
         self.lm_head = lm_head
         self.config = config
@@ -572,11 +682,12 @@ class TextGreedyDecoder:
             {min(2**p, max_batch_size) for p in range(max_batch_size.bit_length())} | {max_batch_size}
         )
         self.kv_buckets = [CACHE_LENGTH]
+        slab, paged, dtype = (KVCache, PagedKVCache, (self.dtype,)) if cache_bits is None else (KVCache8, PagedKVCache8, ())
         if page_size is None:
-            self.cache = KVCache.allocate(config, max_batch_size, CACHE_LENGTH, self.device, self.dtype)
+            self.cache = slab.allocate(config, max_batch_size, CACHE_LENGTH, self.device, *dtype)
         else:
             pages = max_batch_size * CACHE_LENGTH // page_size if num_pages is None else num_pages
-            self.cache = PagedKVCache.allocate(config, max_batch_size, pages, page_size, self.device, self.dtype)
+            self.cache = paged.allocate(config, max_batch_size, pages, page_size, self.device, *dtype)
         self.state = DecodeState.allocate(max_batch_size, self.device)
         self.eos_ids = torch.tensor(eos_ids, dtype=torch.long, device=self.device)
         self.draft_tokens = draft_tokens
@@ -596,11 +707,14 @@ class TextGreedyDecoder:
         launch per layer and the greedy choice over the logits, and of the
         largest pass over drafted trees."""
         config = self.config
-        vocab = self.lm_head.out_features if isinstance(self.lm_head, Linear4) else self.lm_head.weight.shape[0]
+        quantized = isinstance(self.lm_head, (Linear4, Linear8))
+        vocab = self.lm_head.out_features if quantized else self.lm_head.weight.shape[0]
+        step = (decode8_workspace_size if isinstance(self.cache, (KVCache8, PagedKVCache8)) else
+                attention.decode_workspace_size)
         need = 256
         for batch in self.buckets:
             for length in self.kv_buckets:
-                need = max(need, attention.decode_workspace_size(
+                need = max(need, step(
                     batch, config["num_attention_heads"], config["num_key_value_heads"], config["head_dim"],
                     length, self.dtype))
             need = max(need, attention.choice_workspace_size(batch, vocab))
@@ -695,7 +809,7 @@ class TextGreedyDecoder:
             self.rows[slot] = {"prompt_length": length, "end": end_position, "bound": length, "pages": pages}
         return slots
 
-    def step(self, state: DecodeState, cache: KVCache, temperatures: Tensor | None = None) -> None:
+    def step(self, state: DecodeState, cache: KVCache | PagedKVCache | KVCache8, temperatures: Tensor | None = None) -> None:
         """Decode ``state.tokens`` and select every row's next token
         (``qwen3_asr.py:1179-1198``).  Split partials go to the decoder's
         own workspace, sized at construction for the largest bucket."""
@@ -734,7 +848,8 @@ class TextGreedyDecoder:
             r["bound"] = min(r["bound"] + count, r["end"])
         return count
 
-    def _verify(self, state: DecodeState, cache: KVCache | PagedKVCache, drafted: Tensor, parents: Tensor) -> Tensor:
+    def _verify(self, state: DecodeState, cache: KVCache | PagedKVCache | KVCache8, drafted: Tensor,
+                parents: Tensor) -> Tensor:
         """:meth:`step` over drafted trees: every row advances by the tokens the
         model's own greedy choices accept; returns how many per row."""
         batch, width = drafted.shape
