@@ -410,7 +410,7 @@ pack_decode8 = Packed(Decode8Params).pack
 LAYER_SIGNATURES = {
     "asrlayer_linear4": (ctypes.c_int, [_ptr, _ptr]),
     "asrlayer_linear8": (ctypes.c_int, [_ptr, _ptr, ctypes.c_size_t, _ptr]),
-    "asrlayer_linear8_workspace_size": (ctypes.c_size_t, [_i64, _i32]),
+    "asrlayer_linear8_workspace_size": (ctypes.c_size_t, [_i64, _i32, _i32, _i32]),
     "asrlayer_write8": (ctypes.c_int, [_ptr, _ptr]),
     "asrlayer_read8": (ctypes.c_int, [_ptr, _ptr]),
     "asrlayer_decode8": (ctypes.c_int, [_ptr, _ptr, ctypes.c_size_t, _ptr]),

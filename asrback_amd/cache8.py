@@ -21,13 +21,14 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .attention import _DTYPES, PageTable, _aligned, _check_device, _dtype_code, _split_workspace
+from .attention import _DTYPES, PageTable, _aligned, _check_device, _split_workspace
 from .drafts import _lengths, _on
 from .layers import _increment_version, check_out, refuse_unseen
 
 HEAD_DIMS = (64, 128, 256)
-# The current stream's handle on a device.
+# The current stream's handle on a device; the current device (once a tensor is on one).
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 @dataclass(frozen=True)
@@ -69,6 +70,10 @@ class Cache8:
                 raise ValueError(f"{name} needs a unit last stride")
         if any(t.device != self.keys.device for t in self.tensors):
             raise RuntimeError("a cache's tensors must be on one device")
+        # The strides as the kernels take them (asking for them is a third of a call's time).
+        strides = (*self.keys.stride()[:3], *self.values.stride()[:3], *self.key_scales.stride()[:2],
+                   *self.value_scales.stride()[:2])
+        object.__setattr__(self, "_strides", strides)
 
     @property
     def tensors(self) -> tuple[Tensor, Tensor, Tensor, Tensor]:
@@ -85,7 +90,7 @@ class Cache8:
 
 def _cache_fields(cache: Cache8, pages: PageTable | None, batch: int, index: int) -> tuple:
     """The fields of ``asrlayer_cache8`` over ``batch`` rows, on GPU ``index``."""
-    k, v, ks, vs = cache.keys, cache.values, cache.key_scales, cache.value_scales
+    k = cache.keys
     lead, length, heads, head_dim = k.shape
     if k.get_device() != index:
         _on(index, k)
@@ -105,27 +110,30 @@ def _cache_fields(cache: Cache8, pages: PageTable | None, batch: int, index: int
             raise ValueError(f"max_len {length} outside the table's reach {reach}")
         # (a table that reaches nothing is no table)
         paged = (table.data_ptr(), table.stride(0), page_size, lead) if length else (0, 0, 0, 0)
-    k0, k1, k2, _ = k.stride()
-    v0, v1, v2, _ = v.stride()
-    a0, a1, _ = ks.stride()
-    b0, b1, _ = vs.stride()
-    return (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), k0, k1, k2, v0, v1, v2, a0, a1, b0, b1, *paged,
-            batch, heads, head_dim, length)
+    return (k.data_ptr(), cache.values.data_ptr(), cache.key_scales.data_ptr(), cache.value_scales.data_ptr(),
+            *cache._strides, *paged, batch, heads, head_dim, length)
 
 
 def _ready(what: str, first: Tensor, *others: Tensor | None) -> int:
     """The index of the current GPU, which must hold these float tensors of one
     supported type, none of which may need a gradient."""
-    index = first.get_device()
-    tensors = [t for t in (first, *others) if t is not None]
-    if first.dtype not in _DTYPES or any(t.dtype is not first.dtype for t in tensors) or index < 0:
-        if first.dtype in _DTYPES and all(t.dtype is first.dtype for t in tensors):
-            raise RuntimeError(f"{what} runs on the GPU only; got tensors on {first.device}")
-        _dtype_code(*tensors)
-    if index != torch.cuda.current_device() or any(t.get_device() != index for t in tensors):
-        _check_device(*tensors)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no gradient; call it under torch.no_grad() or on detached tensors")
+    index, dtype, grad = first.get_device(), first.dtype, torch.is_grad_enabled()
+    if dtype not in _DTYPES:
+        raise TypeError(f"{what} supports float32 and bfloat16, got {dtype}")
+    elsewhere = index >= 0 and index != _current_device()
+    for t in (first, *others):
+        if t is None:
+            continue
+        if t.dtype is not dtype:
+            raise TypeError(f"mixed dtypes: {dtype} and {t.dtype}")
+        if t.get_device() != index:
+            elsewhere = True
+        if grad and t.requires_grad and index >= 0:
+            raise RuntimeError(f"{what} has no gradient; call it under torch.no_grad() or on detached tensors")
+    if index < 0:
+        raise RuntimeError(f"{what} runs on the GPU only; got tensors on {first.device}")
+    if elsewhere:
+        _check_device(first, *others)  # says what is wrong
     return index
 
 
@@ -224,12 +232,13 @@ def read8(cache: Cache8, *, lengths: Tensor | None = None, pages: PageTable | No
     index = cache.keys.get_device()
     if index < 0:
         raise RuntimeError(f"read8 runs on the GPU only; got tensors on {cache.keys.device}")
-    if index != torch.cuda.current_device():
+    if index != _current_device():
         _check_device(cache.keys)
     _on(index, lengths)
     fields = _cache_fields(cache, pages, batch, index)
     shape = (batch, fields[-1], *cache.keys.shape[2:])
-    k_out, v_out = (torch.empty(shape, dtype=dtype, device=cache.keys.device) for _ in "kv")
+    k_out = torch.empty(shape, dtype=dtype, device=cache.keys.device)
+    v_out = torch.empty_like(k_out)
     params = _lib.pack_read8(*fields, k_out.data_ptr(), v_out.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
                              lengths is not None and lengths.dtype is torch.int64, _DTYPES[dtype])
     status = _lib.load().asrlayer_read8(params, _raw_stream(index))
@@ -299,7 +308,7 @@ def decode8(q: Tensor, cache: Cache8, *, lengths: Tensor | None = None, scale: f
     _on(index, lengths, out)
     fields = _cache_fields(cache, pages, batch, index)
     if not given:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(shape)
     code, span = _DTYPES[q.dtype], window or 0
     params = _lib.pack_decode8(
         *fields, q.data_ptr(), out.data_ptr(), *q.stride()[:2], *out.stride()[:2],

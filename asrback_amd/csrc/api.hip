@@ -751,9 +751,9 @@ int asrlayer_linear4(const asrlayer_linear4_params* params, void* stream) {
   return from_hip(asrattn::launch_linear4(p, static_cast<hipStream_t>(stream)), "asrlayer_linear4");
 }
 
-size_t asrlayer_linear8_workspace_size(int64_t rows, int32_t k) {
-  if (rows < 0 || k < 1) return (size_t)-1;
-  return asrattn::linear8_workspace(rows, k).total;
+size_t asrlayer_linear8_workspace_size(int64_t rows, int32_t n, int32_t k, int32_t gated) {
+  if (rows < 0 || n < 1 || k < 1) return (size_t)-1;
+  return asrattn::linear8_workspace(rows, n, k, gated != 0).total;
 }
 
 int asrlayer_linear8(const asrlayer_linear8_params* params, void* workspace, size_t workspace_bytes, void* stream) {
@@ -774,8 +774,8 @@ int asrlayer_linear8(const asrlayer_linear8_params* params, void* workspace, siz
     return fail(ASRATTN_ERR_INVALID, "x, packed, scales and out must be non-NULL");
   if ((reinterpret_cast<uintptr_t>(p.packed) & 15u) != 0)
     return fail(ASRATTN_ERR_INVALID, "packed needs a 16-byte aligned pointer");
-  const size_t need = asrattn::linear8_workspace(p.rows, p.k).total;
-  if (workspace == nullptr || workspace_bytes < need)
+  const size_t need = asrattn::linear8_workspace(p.rows, p.n, p.k, p.gated != 0).total;
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(ASRATTN_ERR_WORKSPACE, "the rows need %zu workspace bytes, got %zu", need,
                 workspace == nullptr ? (size_t)0 : workspace_bytes);
   if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)

@@ -109,7 +109,7 @@ hipError_t launch_linear4(const asrlayer_linear4_params& p, hipStream_t stream);
 struct Linear8Workspace {
   size_t scales, total;
 };
-Linear8Workspace linear8_workspace(int64_t rows, int k);
+Linear8Workspace linear8_workspace(int64_t rows, int n, int k, bool gated);
 hipError_t launch_linear8(const asrlayer_linear8_params& p, void* workspace, hipStream_t stream);
 
 // The 8-bit cache: writes, reading back (asrlayer_write8, asrlayer_read8) and a

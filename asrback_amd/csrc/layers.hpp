@@ -265,7 +265,8 @@ typedef struct asrlayer_linear8_params {
 
 int asrlayer_linear8(const asrlayer_linear8_params* params, void* workspace, size_t workspace_bytes, void* stream);
 
-size_t asrlayer_linear8_workspace_size(int64_t rows, int32_t k);
+// (size_t)-1 for sizes it does not take; 0 where a call needs none.
+size_t asrlayer_linear8_workspace_size(int64_t rows, int32_t n, int32_t k, int32_t gated);
 
 // A cache of 8-bit keys and values, a float32 scale per position and kv head:
 // key j of sequence b is k_scales[b, h, j] k[b, j, h, :].  k, v (batch,

@@ -613,16 +613,12 @@ hipError_t launch_few(const asrlayer_linear8_params& p, const uint4* packed, con
 
 template <typename T>
 hipError_t launch_typed(const asrlayer_linear8_params& p, void* workspace, hipStream_t stream) {
-  const Linear8Workspace ws = linear8_workspace(p.rows, p.k);
+  const Linear8Workspace ws = linear8_workspace(p.rows, p.n, p.k, p.gated != 0);
   uint4* packed = static_cast<uint4*>(workspace);
   float* scales = reinterpret_cast<float*>(static_cast<char*>(workspace) + ws.scales);
   const bool vectors = reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.x_row_stride % Elem<T>::kPerVec == 0;
   const int outputs = p.gated ? p.n / 2 : p.n;
-  // Few values are rounded by every workgroup, while a CU holds all of its workgroups at
-  // once: 4 x 2048 to 2 x 6144 outputs (gated) 8.2 us, with a launch before it 10.7; 8 x
-  // 2048 10.1 and 10.2; 16 x 2048 13.0 and 9.4; 1 x 2048 to 40000 23.0 and 18.1.
-  if (p.rows <= 16 && p.rows * p.k <= kFusedValues && outputs <= 512 * 16)
-    return launch_few<T, 1, true>(p, nullptr, nullptr, vectors, stream);
+  if (ws.total == 0) return launch_few<T, 1, true>(p, nullptr, nullptr, vectors, stream);
   const hipError_t err = launch_rounding<T>(p, packed, scales, vectors, stream);
   if (err != hipSuccess) return err;
   if (p.rows <= 16) return launch_few<T, 1, false>(p, packed, scales, vectors, stream);
@@ -646,7 +642,11 @@ hipError_t launch_typed(const asrlayer_linear8_params& p, void* workspace, hipSt
 
 }  // namespace
 
-Linear8Workspace linear8_workspace(int64_t rows, int k) {
+Linear8Workspace linear8_workspace(int64_t rows, int n, int k, bool gated) {
+  // Few values are rounded by every workgroup, while a CU holds all of its workgroups at
+  // once: 4 x 2048 to 2 x 6144 outputs (gated) 8.2 us, with a launch before it 10.7; 8 x
+  // 2048 10.1 and 10.2; 16 x 2048 13.0 and 9.4; 1 x 2048 to 40000 23.0 and 18.1.
+  if (rows <= 16 && rows * k <= kFusedValues && (gated ? n / 2 : n) <= 512 * 16) return {0, 0};
   const size_t tiles = (size_t)(rows + 15) / 16;
   Linear8Workspace w;
   w.scales = tiles * ((size_t)(k + 63) / 64) * 1024;

@@ -18,6 +18,7 @@ would need one, in forward mode too, or that a tracer records are refused.
 
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -31,8 +32,9 @@ from .linear4 import _as_built
 _BLOCK_N, _BLOCK_K = 16, 64
 # Inputs of a row: the sum of their products stays within 32 bits.
 MAX_INPUTS = 1 << 17
-# The current stream's handle on a device.
+# The current stream's handle on a device; the current device (once a tensor is on one).
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 @dataclass(frozen=True)
@@ -135,6 +137,11 @@ def gated8(x: Tensor, weight: Weight8, bias: Tensor | None = None, *, out: Tenso
     return _product("gated8", x, weight.packed, weight.scales, weight.outputs, weight.inputs, bias, out, True)
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace(rows: int, outputs: int, inputs: int, gated: bool) -> int:
+    return _lib.load().asrlayer_linear8_workspace_size(rows, outputs, inputs, gated)
+
+
 def _product(what: str, x: Tensor, packed: Tensor, scales: Tensor, outputs: int, inputs: int, bias: Tensor | None,
              out: Tensor | None, gated: bool) -> Tensor:
     shape = x.shape
@@ -158,9 +165,9 @@ def _product(what: str, x: Tensor, packed: Tensor, scales: Tensor, outputs: int,
         raise RuntimeError(f"{what} runs on the GPU only; got a tensor on {x.device}")
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         raise RuntimeError(f"{what} has no gradient; call it under torch.no_grad() or on detached tensors")
-    others = (packed, scales, bias, out)
-    if index != torch.cuda.current_device() or any(t is not None and t.get_device() != index for t in others):
-        _check_device(x, *others)  # says what is wrong
+    if (index != _current_device() or packed.get_device() != index or scales.get_device() != index
+            or (bias is not None and bias.get_device() != index) or (given and out.get_device() != index)):
+        _check_device(x, packed, scales, bias, out)  # says what is wrong
     if not given:
         out = x.new_empty((*shape[:-1], width))
     rows = x if len(shape) == 2 else x.reshape(-1, inputs)
@@ -168,15 +175,14 @@ def _product(what: str, x: Tensor, packed: Tensor, scales: Tensor, outputs: int,
         rows = rows.contiguous()
     if bias is not None:
         bias = bias.contiguous()
-    lib = _lib.load()
     count = rows.shape[0]
-    # Rounded rows, 16 to a block, and their scales.
-    size = lib.asrlayer_linear8_workspace_size(count, inputs)
-    held = torch.empty(size, dtype=torch.uint8, device=x.device)
+    # Rounded rows, 16 to a block, and their scales, where a launch of its own rounds them.
+    size = _workspace(count, outputs, inputs, gated)
+    held = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
     params = _lib.pack_linear8(
         rows.data_ptr(), rows.stride(0), packed.data_ptr(), scales.data_ptr(), 0 if bias is None else bias.data_ptr(),
         out.data_ptr(), width, count, outputs, inputs, gated, _DTYPES[dtype])
-    status = lib.asrlayer_linear8(params, held.data_ptr(), size, _raw_stream(index))
+    status = _lib.load().asrlayer_linear8(params, held.data_ptr() if size else None, size, _raw_stream(index))
     if status:
         _lib.check(status, "asrlayer_linear8")
     if given:

@@ -694,7 +694,8 @@ class TextGreedyDecoder:
         self.drafts = DraftCache.allocate(config, max_batch_size, draft_tokens, self.device, self.dtype)
         # The drafted tokens and parents of the captured passes.
         self._drafted = torch.zeros((2, max_batch_size, draft_tokens), dtype=torch.long, device=self.device)
-        self.workspace = torch.empty(self._workspace_bytes(), dtype=torch.uint8, device=self.device)
+        step = attention.decode_workspace_size if cache_bits is None else decode8_workspace_size
+        self.workspace = torch.empty(self._workspace_bytes(step), dtype=torch.uint8, device=self.device)
         self.rows: dict[int, dict] = {}
         self._bounds_ahead = False
         self.graphs: dict[tuple[int, int], CapturedGraph] = {}
@@ -702,15 +703,13 @@ class TextGreedyDecoder:
         if graphs:
             self._capture_graphs()
 
-    def _workspace_bytes(self) -> int:
+    def _workspace_bytes(self, step: Callable[..., int] = attention.decode_workspace_size) -> int:
         """Split partials of the largest step over the buckets, the decode
-        launch per layer and the greedy choice over the logits, and of the
+        launch per layer (``step`` bytes) and the greedy choice over the logits, and of the
         largest pass over drafted trees."""
         config = self.config
         quantized = isinstance(self.lm_head, (Linear4, Linear8))
         vocab = self.lm_head.out_features if quantized else self.lm_head.weight.shape[0]
-        step = (decode8_workspace_size if isinstance(self.cache, (KVCache8, PagedKVCache8)) else
-                attention.decode_workspace_size)
         need = 256
         for batch in self.buckets:
             for length in self.kv_buckets:
