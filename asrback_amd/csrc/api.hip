@@ -865,6 +865,8 @@ int asrlayer_write8(const asrlayer_write8_params* params, void* stream) {
   if (rc != ASRATTN_OK) return rc;
   if (p.tokens < 0 || p.heads_q < 0) return fail(ASRATTN_ERR_INVALID, "tokens and heads_q must be >= 0");
   if (p.tokens > (1 << 23) || p.heads_q > 4096) return fail(ASRATTN_ERR_UNSUPPORTED, "more than 2^23 tokens or 4096 heads");
+  if (p.tokens * (p.heads_q + 2LL * p.cache.heads_kv) >= (1LL << 32))
+    return fail(ASRATTN_ERR_UNSUPPORTED, "2^32 rows of heads or more");
   if (p.tokens == 0) return ok();
   asrlayer_write8_params held = p;
   if (empty_cache8(p.cache)) {
@@ -893,9 +895,9 @@ int asrlayer_read8(const asrlayer_read8_params* params, void* stream) {
   if (rc != ASRATTN_OK) return rc;
   const asrlayer_cache8& c = p.cache;
   if (c.batch == 0 || c.max_len == 0) return ok();
-  // A launch has fewer than 2^32 threads along an axis.
-  if ((long long)c.max_len * c.heads_kv * (c.head_dim / 16) >= (1LL << 31))
-    return fail(ASRATTN_ERR_UNSUPPORTED, "more than 2^35 values a row");
+  // Pieces of four values count to 2^31.
+  if ((long long)c.max_len * c.heads_kv * (c.head_dim / 4) >= (1LL << 31))
+    return fail(ASRATTN_ERR_UNSUPPORTED, "2^33 values a row or more");
   if (c.block_table == nullptr || c.num_pages != 0) {
     rc = check_cache8(c);
     if (rc != ASRATTN_OK) return rc;

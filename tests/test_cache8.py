@@ -253,11 +253,12 @@ def test_what_the_library_refuses():
     ]
     for make, own in (
         (write, [({"tokens": -1}, _lib.ERR_INVALID, b"tokens"), ({"tokens": 1 << 24}, _lib.ERR_UNSUPPORTED, b"2^23"),
+                 ({"tokens": 1 << 23, "heads_q": 4096}, _lib.ERR_UNSUPPORTED, b"2^32"),
                  ({"positions": 0}, _lib.ERR_INVALID, b"positions"), ({"heads_q": 1}, _lib.ERR_INVALID, b"queries"),
                  ({"k_norm": 4096}, _lib.ERR_INVALID, b"pairs"), ({"sin": 4096}, _lib.ERR_INVALID, b"pairs"),
                  ({"k_token_stride": 4}, _lib.ERR_INVALID, b"16-byte"), ({"v": 4100}, _lib.ERR_INVALID, b"16-byte")]),
         (read, [({"v_out": 0}, _lib.ERR_INVALID, b"non-NULL"), ({"k_out": 4104}, _lib.ERR_INVALID, b"aligned"),
-                ({"max_len": 1 << 30, "heads_kv": 4}, _lib.ERR_UNSUPPORTED, b"2^35")]),
+                ({"max_len": 1 << 30, "heads_kv": 4}, _lib.ERR_UNSUPPORTED, b"2^33")]),
         (decode, [({"heads_q": 3}, _lib.ERR_INVALID, b"multiple"), ({"heads_q": 8192}, _lib.ERR_UNSUPPORTED, b"4096"),
                   ({"window": -1}, _lib.ERR_INVALID, b"window"), ({"scale": float("nan")}, _lib.ERR_INVALID, b"scale"),
                   ({"q": 0}, _lib.ERR_INVALID, b"non-NULL"), ({"q_head_stride": 4}, _lib.ERR_INVALID, b"16-byte"),
