@@ -34,13 +34,33 @@ __device__ __forceinline__ i32x4_t lds_read(uint32_t addr) { return *(lds_i32x4_
 
 constexpr int kThreads = 256;
 
+// N consecutive elements at any address of them: global memory takes vectors there
+// (2791 rows of 320 inputs to 21497 bf16 outputs 85 us, stored one by one 219; to 21504 50).
+template <typename T, int N>
+__device__ __forceinline__ void load_whole(const T* p, float* x) {
+  constexpr int EPL = Elem<T>::kPerVec;
+#pragma unroll
+  for (int v = 0; v < N / EPL; ++v) {
+    uint4 raw;
+    __builtin_memcpy(&raw, p + v * EPL, 16);
+    unpack<T>(raw, x + v * EPL);
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_whole(T* p, const float* x) {
+  constexpr int EPL = Elem<T>::kPerVec;
+#pragma unroll
+  for (int v = 0; v < N / EPL; ++v) {
+    const uint4 raw = pack<T>(x + v * EPL);
+    __builtin_memcpy(p + v * EPL, &raw, 16);
+  }
+}
+
 // 16 inputs of a row from `at` on, zeros past k.
 template <typename T>
-__device__ __forceinline__ void load_inputs(const T* row, int at, int k, bool vectors, float* x) {
-  constexpr int EPL = Elem<T>::kPerVec;
-  if (vectors && at + 16 <= k) {
-#pragma unroll
-    for (int v = 0; v < 16 / EPL; ++v) Elem<T>::load16(row + at + v * EPL, x + v * EPL);
+__device__ __forceinline__ void load_inputs(const T* row, int at, int k, float* x) {
+  if (at + 16 <= k) {
+    load_whole<T, 16>(row + at, x);
   } else {
 #pragma unroll
     for (int e = 0; e < 16; ++e) x[e] = at + e < k ? Elem<T>::load1(row + at + e) : 0.f;
@@ -80,8 +100,7 @@ __device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" :
 // they hold from the one reading for the largest magnitude; longer rows are read again.
 // Bound by a round trip to memory, and by the bytes from some thousand rows on.
 template <typename T, int LANES, int NP>
-__global__ __launch_bounds__(kThreads) void round_rows_kernel(const asrlayer_linear8_params p, uint4* packed, float* scales,
-                                                              bool vectors) {
+__global__ __launch_bounds__(kThreads) void round_rows_kernel(const asrlayer_linear8_params p, uint4* packed, float* scales) {
   const int lane = threadIdx.x % LANES;
   const int64_t row = (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
   if (LANES < kThreads && row >= p.rows) return;  // (uniform over a wave)
@@ -90,14 +109,14 @@ __global__ __launch_bounds__(kThreads) void round_rows_kernel(const asrlayer_lin
   float v[NP][16];
   uint32_t largest = 0;
 #pragma unroll
-  for (int u = 0; u < NP; ++u) load_inputs(x, (lane + u * LANES) * 16, p.k, vectors, v[u]);
+  for (int u = 0; u < NP; ++u) load_inputs(x, (lane + u * LANES) * 16, p.k, v[u]);
 #pragma unroll
   for (int u = 0; u < NP; ++u)
 #pragma unroll
     for (int e = 0; e < 16; ++e) largest = max(largest, magnitude(v[u][e]));
   for (int piece = lane + NP * LANES; piece < pieces; piece += LANES) {
     float more[16];
-    load_inputs(x, piece * 16, p.k, vectors, more);
+    load_inputs(x, piece * 16, p.k, more);
 #pragma unroll
     for (int e = 0; e < 16; ++e) largest = max(largest, magnitude(more[e]));
   }
@@ -120,7 +139,7 @@ __global__ __launch_bounds__(kThreads) void round_rows_kernel(const asrlayer_lin
   for (int u = 0; u < NP; ++u) store(lane + u * LANES, v[u]);
   for (int piece = lane + NP * LANES; piece < pieces; piece += LANES) {
     float more[16];
-    load_inputs(x, piece * 16, p.k, vectors, more);
+    load_inputs(x, piece * 16, p.k, more);
     store(piece, more);
   }
 }
@@ -146,7 +165,7 @@ constexpr int kFusedBytes = kFusedValues + 16 * 64;  // rows of whole blocks
 
 template <typename T, bool GATED, int RT, bool FUSED>
 __global__ __launch_bounds__(64 * kFewWaves, 4) void linear8_few_kernel(const asrlayer_linear8_params p, const uint4* packed,
-                                                                        const float* row_scales, bool vectors) {
+                                                                        const float* row_scales) {
   constexpr int W = kFewWaves, NW = GATED ? 2 : 1, kAhead = FUSED || RT == 1 ? 4 : 2;
   constexpr int kSums = W * NW * RT * 1024;
   __shared__ __attribute__((aligned(16))) unsigned char lds[FUSED && kFusedBytes > kSums ? kFusedBytes : kSums];
@@ -203,7 +222,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 4) void linear8_few_kernel(const as
     for (int at = threadIdx.x; at < all; at += 64 * W) {
       const int row = at / pieces, piece = at - row * pieces;
       float v[16];
-      load_inputs(x + row * p.x_row_stride, piece * 16, p.k, vectors, v);
+      load_inputs(x + row * p.x_row_stride, piece * 16, p.k, v);
       uint32_t largest = 0;
 #pragma unroll
       for (int e = 0; e < 16; ++e) largest = max(largest, magnitude(v[e]));
@@ -217,7 +236,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 4) void linear8_few_kernel(const as
     for (int at = threadIdx.x; at < all; at += 64 * W) {
       const int row = at / pieces, piece = at - row * pieces;
       float v[16];
-      load_inputs(x + row * p.x_row_stride, piece * 16, p.k, vectors, v);
+      load_inputs(x + row * p.x_row_stride, piece * 16, p.k, v);
       const Scale8 s = scale8(sm_largest[row]);
       *reinterpret_cast<uint4*>(lds + (piece * rows + row) * 16) =
           make_uint4(round8x4(v, s), round8x4(v + 4, s), round8x4(v + 8, s), round8x4(v + 12, s));
@@ -279,20 +298,6 @@ __global__ __launch_bounds__(64 * kFewWaves, 4) void linear8_few_kernel(const as
   }
 }
 
-// N consecutive elements.
-template <typename T, int N>
-__device__ __forceinline__ void load_whole(const T* p, float* x) {
-  constexpr int EPL = Elem<T>::kPerVec;
-#pragma unroll
-  for (int v = 0; v < N / EPL; ++v) Elem<T>::load16(p + v * EPL, x + v * EPL);
-}
-template <typename T, int N>
-__device__ __forceinline__ void store_whole(T* p, const float* x) {
-  constexpr int EPL = Elem<T>::kPerVec;
-#pragma unroll
-  for (int v = 0; v < N / EPL; ++v) *reinterpret_cast<uint4*>(p + v * EPL) = pack<T>(x + v * EPL);
-}
-
 // Tiles of 32 NA rows x 32 NJ outputs (gated: half of them gates, half projections), as
 // many workgroups as a CU holds, each of which takes one tile after another: four waves
 // of 16 NA x 16 NJ.  Blocks of both operands, 64 inputs deep, move by DMA into a ring
@@ -319,7 +324,7 @@ struct LargeShape {
 
 template <typename T, bool GATED, int NA, int NJ, int S>
 __global__ __launch_bounds__(256, (LargeShape<NA, NJ, S>::kPerCu)) void linear8_large_kernel(
-    const asrlayer_linear8_params p, const uint4* packed, const float* row_scales, int row_tiles, int col_tiles, bool whole) {
+    const asrlayer_linear8_params p, const uint4* packed, const float* row_scales, int row_tiles, int col_tiles) {
   using Shape = LargeShape<NA, NJ, S>;
   constexpr int kStageBytes = Shape::kStageBytes, kRows = Shape::kRows, kOutputs = Shape::kOutputs, kDmas = Shape::kDmas;
   __shared__ __attribute__((aligned(16))) unsigned char lds[S * kStageBytes];
@@ -486,13 +491,14 @@ __global__ __launch_bounds__(256, (LargeShape<NA, NJ, S>::kPerCu)) void linear8_
       rs[a] = row_scales[min(row_at + 16 * a, p.rows - 1)];
       far = fmaxf(far, rs[a]);
     }
-    if (whole && !__any(far >= kFar)) {
+    const bool near = !__any(far >= kFar);
+    if (near) {
       // As short as it can be, since it runs once a tile, at the pace its instructions
       // come from memory.
 #pragma unroll
       for (int c = 0; c < NJ / 4; ++c) {
         const int n = n_at + (GATED ? 32 : 64) * c;
-        if (n >= outputs) break;
+        if (n + N > outputs) break;
         float scale[16], add[16];
 #pragma unroll
         for (int e = 0; e < 16; e += N) load_whole<T, N>(ws + (e != 0 ? outputs : 0) + n, scale + e);
@@ -519,10 +525,10 @@ __global__ __launch_bounds__(256, (LargeShape<NA, NJ, S>::kPerCu)) void linear8_
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-      continue;
+      if (outputs % N == 0 || tile.n0 + (GATED ? kOutputs / 2 : kOutputs) <= outputs) continue;
     }
-    // Outputs that end inside a lane's, or rows that vectors do not write: 16 rows and 64
-    // outputs at a time, in a loop.
+    // Lanes inside whose outputs they end, or rows of far scales: 16 rows and 64 outputs at a
+    // time, in a loop.
 #pragma unroll 1
     for (int ca = 0; ca < NA * NJ / 4; ++ca) {
       const int n = n_at + (GATED ? 32 : 64) * (ca / NA);
@@ -554,7 +560,7 @@ __global__ __launch_bounds__(256, (LargeShape<NA, NJ, S>::kPerCu)) void linear8_
       T* out = static_cast<T*>(p.out) + row * p.out_row_stride + n;
 #pragma unroll
       for (int e = 0; e < N; ++e)
-        if (row < p.rows && n + e < outputs) Elem<T>::store1(out + e, y[e]);
+        if (row < p.rows && n + e < outputs && !(near && n + N <= outputs)) Elem<T>::store1(out + e, y[e]);
     }
   }
   wait_vmcnt<0>();  // the surplus DMAs, before the workgroup's LDS is another's
@@ -565,49 +571,44 @@ hipError_t launch_large(const asrlayer_linear8_params& p, const uint4* packed, c
   using Shape = LargeShape<NA, NJ, S>;
   const int outputs = p.gated ? p.n / 2 : p.n, wide = p.gated ? Shape::kOutputs / 2 : Shape::kOutputs;
   const int row_tiles = (int)((p.rows + Shape::kRows - 1) / Shape::kRows), col_tiles = (outputs + wide - 1) / wide;
-  // Whether a lane's outputs are vectors, of the scales and the bias as well.
-  const bool whole = (reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.scales) |
-                      reinterpret_cast<uintptr_t>(p.bias)) % 16 == 0 &&
-                     p.out_row_stride % Elem<T>::kPerVec == 0 && outputs % (p.gated ? 8 : 16) == 0;
   const long long tiles = (long long)row_tiles * col_tiles, most = 256 * Shape::kPerCu;
   const dim3 grid((unsigned)(tiles < most ? tiles : most));
   if (p.gated)
     hipLaunchKernelGGL((linear8_large_kernel<T, true, NA, NJ, S>), grid, dim3(256), 0, stream, p, packed, scales, row_tiles,
-                       col_tiles, whole);
+                       col_tiles);
   else
     hipLaunchKernelGGL((linear8_large_kernel<T, false, NA, NJ, S>), grid, dim3(256), 0, stream, p, packed, scales, row_tiles,
-                       col_tiles, whole);
+                       col_tiles);
   return hipGetLastError();
 }
 
 template <typename T, int LANES, int NP>
-hipError_t launch_round(const asrlayer_linear8_params& p, uint4* packed, float* scales, bool vectors, hipStream_t stream) {
+hipError_t launch_round(const asrlayer_linear8_params& p, uint4* packed, float* scales, hipStream_t stream) {
   constexpr int kRows = kThreads / LANES;
   hipLaunchKernelGGL((round_rows_kernel<T, LANES, NP>), dim3((unsigned)((p.rows + kRows - 1) / kRows)), dim3(kThreads), 0,
-                     stream, p, packed, scales, vectors);
+                     stream, p, packed, scales);
   return hipGetLastError();
 }
 
 template <typename T>
-hipError_t launch_rounding(const asrlayer_linear8_params& p, uint4* packed, float* scales, bool vectors,
-                           hipStream_t stream) {
+hipError_t launch_rounding(const asrlayer_linear8_params& p, uint4* packed, float* scales, hipStream_t stream) {
   const int pieces = (p.k + 15) / 16;
-  if (pieces <= 64) return launch_round<T, 64, 1>(p, packed, scales, vectors, stream);
-  if (pieces <= 128) return launch_round<T, 64, 2>(p, packed, scales, vectors, stream);
-  if (pieces <= 256) return launch_round<T, kThreads, 1>(p, packed, scales, vectors, stream);
-  if (pieces <= 512) return launch_round<T, kThreads, 2>(p, packed, scales, vectors, stream);
-  return launch_round<T, kThreads, 4>(p, packed, scales, vectors, stream);
+  if (pieces <= 64) return launch_round<T, 64, 1>(p, packed, scales, stream);
+  if (pieces <= 128) return launch_round<T, 64, 2>(p, packed, scales, stream);
+  if (pieces <= 256) return launch_round<T, kThreads, 1>(p, packed, scales, stream);
+  if (pieces <= 512) return launch_round<T, kThreads, 2>(p, packed, scales, stream);
+  return launch_round<T, kThreads, 4>(p, packed, scales, stream);
 }
 
 template <typename T, int RT, bool FUSED>
-hipError_t launch_few(const asrlayer_linear8_params& p, const uint4* packed, const float* scales, bool vectors,
+hipError_t launch_few(const asrlayer_linear8_params& p, const uint4* packed, const float* scales,
                       hipStream_t stream) {
   const int outputs = p.gated ? p.n / 2 : p.n;
   const dim3 grid((outputs + 15) / 16, (unsigned)((p.rows + 16 * RT - 1) / (16 * RT))), block(64 * kFewWaves);
   if (p.gated)
-    hipLaunchKernelGGL((linear8_few_kernel<T, true, RT, FUSED>), grid, block, 0, stream, p, packed, scales, vectors);
+    hipLaunchKernelGGL((linear8_few_kernel<T, true, RT, FUSED>), grid, block, 0, stream, p, packed, scales);
   else
-    hipLaunchKernelGGL((linear8_few_kernel<T, false, RT, FUSED>), grid, block, 0, stream, p, packed, scales, vectors);
+    hipLaunchKernelGGL((linear8_few_kernel<T, false, RT, FUSED>), grid, block, 0, stream, p, packed, scales);
   return hipGetLastError();
 }
 
@@ -616,18 +617,17 @@ hipError_t launch_typed(const asrlayer_linear8_params& p, void* workspace, hipSt
   const Linear8Workspace ws = linear8_workspace(p.rows, p.n, p.k, p.gated != 0);
   uint4* packed = static_cast<uint4*>(workspace);
   float* scales = reinterpret_cast<float*>(static_cast<char*>(workspace) + ws.scales);
-  const bool vectors = reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.x_row_stride % Elem<T>::kPerVec == 0;
   const int outputs = p.gated ? p.n / 2 : p.n;
-  if (ws.total == 0) return launch_few<T, 1, true>(p, nullptr, nullptr, vectors, stream);
-  const hipError_t err = launch_rounding<T>(p, packed, scales, vectors, stream);
+  if (ws.total == 0) return launch_few<T, 1, true>(p, nullptr, nullptr, stream);
+  const hipError_t err = launch_rounding<T>(p, packed, scales, stream);
   if (err != hipSuccess) return err;
-  if (p.rows <= 16) return launch_few<T, 1, false>(p, packed, scales, vectors, stream);
-  if (p.rows <= 32) return launch_few<T, 2, false>(p, packed, scales, vectors, stream);
+  if (p.rows <= 16) return launch_few<T, 1, false>(p, packed, scales, stream);
+  if (p.rows <= 32) return launch_few<T, 2, false>(p, packed, scales, stream);
   const auto tiles = [&](int rows, int wide) { return (p.rows + rows - 1) / rows * (((long long)outputs + wide - 1) / wide); };
   // Workgroups of 16 outputs and all inputs read the rows anew each: two a CU (128 rows
   // of 2048 to 4096 outputs, 512 of them: 12.0 us, 14.1 in tiles of 64 x 128; 256 to
   // 2048, 512: 11.8 and 13.9; 200 to 4096, 1024: 17.7 and 15.7).
-  if (tiles(64, 16) <= 512) return launch_few<T, 4, false>(p, packed, scales, vectors, stream);
+  if (tiles(64, 16) <= 512) return launch_few<T, 4, false>(p, packed, scales, stream);
   // Tiles of 64 x 128 while each has a CU, and a ring of eight stages, to itself (512
   // rows of 6144 to 2048: 27.7 us, 33.6 in tiles of 128 x 128; 1024 of 2048 to 4096, two
   // rounds: 23.9 and 21.1).
