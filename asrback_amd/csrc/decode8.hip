@@ -383,13 +383,13 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
   };
-  float key_unit = a.c;  // what a key's scale is multiplied by
-  bool exact_keys = true;
+  // What a key's scale is multiplied by: where bytes are converted and where they are
+  // biased.
+  float unit = a.c, biased_unit = 0.f;
   f32x4_t bias{0.f, 0.f, 0.f, 0.f};
   if constexpr (S::kBiased) {
     // The queries times a power of two that puts their largest near 2^100, so that
-    // products with u 2^-133 are ordinary numbers (past 2^60, where that power would be
-    // too small, keys are converted).
+    // products with u 2^-133 are ordinary numbers.
     uint32_t largest = 0;
 #pragma unroll
     for (int turn = 0; turn < kQTurns; ++turn) {
@@ -404,8 +404,9 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
 #pragma unroll
     for (int u = 0; u < W; ++u) largest = max(largest, sm_largest[u]);
     const int e = (int)(__builtin_amdgcn_readfirstlane(largest) >> 23) - 127, up = 100 - e;
-    exact_keys = e > 60;
-    key_unit = __builtin_ldexpf(a.c, exact_keys ? -up : 133 - up);
+    auto scalar = [](float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); };
+    unit = scalar(__builtin_ldexpf(a.c, -up));
+    biased_unit = scalar(__builtin_ldexpf(a.c, 133 - up));
 #pragma unroll
     for (int turn = 0; turn < kQTurns; ++turn) {
       float x[8];
@@ -445,9 +446,11 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
         for (int u = 0; u < kKP; ++u)
           sm_k[lds_piece<S::kLPR>(16 * h + u * (64 / S::kLPR) + lane / S::kLPR, lane % S::kLPR)] = k[h][u];
       if (!(i < ((lane & 16) != 0 ? keys[1] : keys[0]) && t * kKeys + (lane & 31) >= first)) scale = 0.f;
-      // Weights of values with a scale above 128 would not stay within range.
-      const bool exact_values = !S::kBiased || __any(lane >= 32 && !(scale <= 128.f));
-      sm_scale[wave][lane] = scale * (lane < 32 ? key_unit : !S::kBiased ? 1.f : exact_values ? 0x1p-13f : 0x1p120f);
+      // Scales that the powers of two would put out of range (a value's above 128, a key's
+      // above some 2^95 over the largest query): the tile's bytes are converted.
+      const float biased = scale * (lane < 32 ? biased_unit : 0x1p120f);
+      const bool convert = !S::kBiased || __any(!(biased <= 0x1p127f));
+      sm_scale[wave][lane] = convert ? scale * (lane < 32 ? unit : S::kBiased ? 0x1p-13f : 1.f) : biased;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
       __builtin_amdgcn_wave_barrier();
       f32x4_t s[2];
@@ -467,7 +470,7 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
           }
           return sum;
         };
-        if (S::kBiased && !exact_keys)
+        if (S::kBiased && !convert)
           s[h] = scores([](uint32_t x) { return widen_biased(x ^ kBias); }, bias);
         else
           s[h] = scores([](uint32_t x) { return widen(x); }, f32x4_t{0.f, 0.f, 0.f, 0.f});
@@ -522,7 +525,7 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
         w[part] = make_uint4(take(x[0][0], x[0][1]), take(x[0][2], x[0][3]), take(x[1][0], x[1][1]), take(x[1][2], x[1][3]));
       }
       // O^T += V^T P^T
-      if (S::kBiased && !exact_values) {
+      if (S::kBiased && !convert) {
         constexpr uint32_t kZeros = 0x00800080u;
 #pragma unroll
         for (int part = kWP - 1; part >= 0; --part)
