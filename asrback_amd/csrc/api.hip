@@ -824,7 +824,7 @@ int check_cache8(const asrlayer_cache8& c) {
 
 // Whether no position holds anything: the tensors may then be NULL.
 bool empty_cache8(const asrlayer_cache8& c) {
-  return c.max_len == 0 || (c.block_table != nullptr && c.num_pages == 0);
+  return c.max_len == 0 || (c.block_table != nullptr ? c.num_pages == 0 : c.batch == 0);
 }
 
 int check_decode8(const asrlayer_decode8_params* params) {

@@ -38,7 +38,7 @@ from __future__ import annotations
 
 import contextlib
 from dataclasses import dataclass
-from typing import Callable
+from typing import Callable, Union
 
 import numpy as np
 import torch
@@ -189,8 +189,36 @@ class PagedLayer:
         self.pool[pages, positions % self.page_size] = value
 
 
+class RowPages:
+    """Hands a pool's pages out to rows: the free ones on the host, a row's in its
+    ``block_table``."""
+
+    block_table: Tensor
+    page_size: int
+    free_pages: list[int]
+
+    def pages_for(self, positions: int) -> int:
+        return -(-positions // self.page_size)
+
+    def assign(self, row: int, positions: int) -> list[int]:
+        """Pages for positions ``0 .. positions - 1`` of ``row`` (whose
+        previous pages must have been released)."""
+        count = self.pages_for(positions)
+        if count > len(self.free_pages):
+            raise RuntimeError(f"paged cache exhausted: {count} pages wanted, {len(self.free_pages)} free")
+        pages = [self.free_pages.pop() for _ in range(count)]
+        entries = torch.full((self.block_table.shape[1],), -1, dtype=torch.int32)
+        entries[:count] = torch.tensor(pages, dtype=torch.int32)
+        self.block_table[row].copy_(entries.to(self.block_table.device))
+        return pages
+
+    def release(self, row: int, pages: list[int]) -> None:
+        self.block_table[row].fill_(-1)
+        self.free_pages.extend(reversed(pages))
+
+
 @dataclass
-class PagedKVCache:
+class PagedKVCache(RowPages):
     """Keys and values in pages of ``page_size`` positions from one pool per
     layer, ``(layers, num_pages + 1, page_size, kv_heads, head_dim)`` (the
     last page a write sink that no row owns), and a block
@@ -229,25 +257,6 @@ class PagedKVCache:
         return PagedKVCache(self.pool_keys, self.pool_values, self.block_table[:batch_size], self.page_size,
                             self.free_pages)
 
-    def pages_for(self, positions: int) -> int:
-        return -(-positions // self.page_size)
-
-    def assign(self, row: int, positions: int) -> list[int]:
-        """Pages for positions ``0 .. positions - 1`` of ``row`` (whose
-        previous pages must have been released)."""
-        count = self.pages_for(positions)
-        if count > len(self.free_pages):
-            raise RuntimeError(f"paged cache exhausted: {count} pages wanted, {len(self.free_pages)} free")
-        pages = [self.free_pages.pop() for _ in range(count)]
-        entries = torch.full((self.block_table.shape[1],), -1, dtype=torch.int32)
-        entries[:count] = torch.tensor(pages, dtype=torch.int32)
-        self.block_table[row].copy_(entries.to(self.block_table.device))
-        return pages
-
-    def release(self, row: int, pages: list[int]) -> None:
-        self.block_table[row].fill_(-1)
-        self.free_pages.extend(reversed(pages))
-
 
 class Layer8:
     """One layer's keys and values of a :class:`KVCache8` or :class:`PagedKVCache8`."""
@@ -280,7 +289,7 @@ class KVCache8:
                          for layer in self.layers])
 
 
-class PagedKVCache8(PagedKVCache):
+class PagedKVCache8(RowPages):
     """:class:`PagedKVCache` over pools of 8-bit values, one
     :class:`~asrback_amd.cache8.Cache8` a layer.  Without a sink page: the writes leave
     alone what has no page."""
@@ -304,6 +313,9 @@ class PagedKVCache8(PagedKVCache):
         return PagedKVCache8(self.layers, self.block_table[:batch_size], self.page_size, self.free_pages)
 
 
+DecoderCache = Union[KVCache, PagedKVCache, KVCache8, PagedKVCache8]
+
+
 @dataclass
 class DraftCache:
     """Keys and values of drafted tokens, ``(layers, batch, tokens, kv_heads,
@@ -320,7 +332,7 @@ class DraftCache:
     def narrow(self, batch_size: int, tokens: int) -> DraftCache:
         return DraftCache(self.keys[:, :batch_size, :tokens], self.values[:, :batch_size, :tokens])
 
-    def commit(self, cache: KVCache | PagedKVCache | KVCache8, path: Tensor, count: Tensor, lengths: Tensor) -> None:
+    def commit(self, cache: DecoderCache, path: Tensor, count: Tensor, lengths: Tensor) -> None:
         """Write the accepted tokens into ``cache``
         (:func:`~asrback_amd.drafts.commit_drafts`, :func:`~asrback_amd.cache8.write8`)."""
         if isinstance(cache, (KVCache8, PagedKVCache8)):
@@ -549,7 +561,7 @@ class TextModel(nn.Module):
             x = layer(x, lambda attention, h: attention.prefill(h, keys, values, rows, positions, segments, cos, sin))
         return self.norm(x)
 
-    def step(self, tokens, positions, cache: KVCache | PagedKVCache | KVCache8, cos, sin,
+    def step(self, tokens, positions, cache: DecoderCache, cos, sin,
              varlen: bool = True) -> Tensor:
         """Hidden states for one token per row over a fixed-shape cache view;
         ``cos``/``sin`` are the full tables.  Each row reads its keys
@@ -567,7 +579,7 @@ class TextModel(nn.Module):
         return self.norm(x)
 
 
-    def verify(self, tokens, lengths, cache: KVCache | PagedKVCache | KVCache8, drafts: DraftCache, masks, depths, cos,
+    def verify(self, tokens, lengths, cache: DecoderCache, drafts: DraftCache, masks, depths, cos,
                sin) -> Tensor:
         """Hidden states ``(batch, tokens, width)`` of drafted trees
         ``tokens`` ``(batch, tokens)`` behind the ``lengths`` (int64) keys each row
@@ -682,7 +694,9 @@ class TextGreedyDecoder:
             {min(2**p, max_batch_size) for p in range(max_batch_size.bit_length())} | {max_batch_size}
         )
         self.kv_buckets = [CACHE_LENGTH]
-        slab, paged, dtype = (KVCache, PagedKVCache, (self.dtype,)) if cache_bits is None else (KVCache8, PagedKVCache8, ())
+        slab, paged, dtype = KVCache8, PagedKVCache8, ()
+        if cache_bits is None:
+            slab, paged, dtype = KVCache, PagedKVCache, (self.dtype,)
         if page_size is None:
             self.cache = slab.allocate(config, max_batch_size, CACHE_LENGTH, self.device, *dtype)
         else:
@@ -777,7 +791,7 @@ class TextGreedyDecoder:
         limits = [min(n, CACHE_LENGTH - length) for n, length in zip(max_new_tokens, lengths)]
         ends = [length - 1 + limit for length, limit in zip(lengths, limits)]
         audio = np.flatnonzero(ids == audio_id) if audio_id is not None else None
-        if isinstance(self.cache, PagedKVCache):
+        if isinstance(self.cache, RowPages):
             wanted = sum(self.cache.pages_for(end + 1) for end in ends)
             if wanted > len(self.cache.free_pages):
                 raise RuntimeError(f"paged cache exhausted: {wanted} pages wanted, {len(self.cache.free_pages)} free")
@@ -808,7 +822,7 @@ class TextGreedyDecoder:
             self.rows[slot] = {"prompt_length": length, "end": end_position, "bound": length, "pages": pages}
         return slots
 
-    def step(self, state: DecodeState, cache: KVCache | PagedKVCache | KVCache8, temperatures: Tensor | None = None) -> None:
+    def step(self, state: DecodeState, cache: DecoderCache, temperatures: Tensor | None = None) -> None:
         """Decode ``state.tokens`` and select every row's next token
         (``qwen3_asr.py:1179-1198``).  Split partials go to the decoder's
         own workspace, sized at construction for the largest bucket."""
@@ -847,8 +861,7 @@ class TextGreedyDecoder:
             r["bound"] = min(r["bound"] + count, r["end"])
         return count
 
-    def _verify(self, state: DecodeState, cache: KVCache | PagedKVCache | KVCache8, drafted: Tensor,
-                parents: Tensor) -> Tensor:
+    def _verify(self, state: DecodeState, cache: DecoderCache, drafted: Tensor, parents: Tensor) -> Tensor:
         """:meth:`step` over drafted trees: every row advances by the tokens the
         model's own greedy choices accept; returns how many per row."""
         batch, width = drafted.shape
@@ -944,7 +957,7 @@ class TextGreedyDecoder:
         out = {}
         for slot, position, total, tokens in zip(done, positions, sums, generated):
             row = self.rows.pop(slot)
-            if isinstance(self.cache, PagedKVCache):
+            if isinstance(self.cache, RowPages):
                 self.cache.release(slot, row["pages"])
             tokens = tokens[row["prompt_length"] : position + 1]
             if tokens and tokens[-1] in eos:

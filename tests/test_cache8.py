@@ -289,7 +289,7 @@ def test_what_the_library_refuses():
 
 def test_decoder_caches():
     """Slab and pages, as the decoder narrows them and hands pages out."""
-    from asrback_amd.qwen3_asr import CACHE_LENGTH, KVCache8, Layer8, PagedKVCache, PagedKVCache8
+    from asrback_amd.qwen3_asr import CACHE_LENGTH, KVCache8, Layer8, PagedKVCache8, RowPages
 
     slab = KVCache8.allocate(CONFIG, 4, 96, "cpu")
     part = slab.narrow(3, 32)
@@ -299,7 +299,7 @@ def test_decoder_caches():
     assert slab.layers[1].value_scales[2, 1, 31] == 7
     assert slab.narrow(3, 32).layers[0].keys.data_ptr() == slab.layers[0].keys.data_ptr()
     paged = PagedKVCache8.allocate(CONFIG, 4, 6, 64, "cpu")
-    assert isinstance(paged, PagedKVCache) and paged.layers[0].keys.shape == (6, 64, 2, 64)
+    assert isinstance(paged, RowPages) and "PagedKVCache8" in repr(paged) and paged.layers[0].keys.shape == (6, 64, 2, 64)
     pages = paged.assign(1, 65)
     assert len(pages) == 2 and paged.block_table[1, :3].tolist() == [*pages, -1]
     part = paged.narrow(2, 100)

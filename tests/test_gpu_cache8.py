@@ -230,6 +230,26 @@ def test_far_scores_and_values(dtype):
         check(decode8(q.cuda(), cache, scale=out_scale), q, (k, v, ks, vs), [length] * batch, out_scale)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_queries_and_scales_far_from_one(dtype):
+    """Powers of two that take the products out of range, by themselves or together, where
+    the scores are not: ordinary scores, and ones so far apart that one key is left."""
+    from asrback_amd.cache8 import Cache8, decode8
+
+    g = torch.Generator().manual_seed(19)
+    batch, heads, kv, d, length = 2, 4, 2, 64, 300
+    _, (k, v, ks, vs) = random_cache(batch, length, kv, d, g)
+    plain = torch.randn(batch, heads, d, generator=g)
+    for queries, keys in ((-60, 53), (-100, 93), (50, -57), (62, -69), (100, -107), (0, 90), (40, 60), (70, 30), (-30, -60)):
+        q = (plain * 2.0**queries).to(dtype)
+        tensors = k, v, ks * 2.0**keys, vs
+        # One row's scale alone far off.
+        tensors[2][1, 0, 5] *= 2.0**-40
+        say("far", dtype, queries, keys)
+        out = decode8(q.cuda(), Cache8(*(t.cuda() for t in tensors)), lengths=spread([length, 250]))
+        check(out, q, tensors, [length, 250])
+
+
 def test_long_cache_past_32_bits():
     """Positions whose offsets pass 2^31 and 2^32 bytes."""
     from asrback_amd.cache8 import Cache8, decode8, read8, write8
@@ -335,6 +355,7 @@ def test_write_and_read_back(dtype, kv, head_dim):
     empty = Cache8(*(t[:0] for t in pool.tensors))
     write8(empty, k.cuda(), v.cuda(), rows.cuda(), positions.cuda(), pages=table)
     assert not read8(empty, pages=table)[0].any()
+    write8(Cache8.allocate(0, 9, kv, head_dim, "cuda"), k.cuda(), v.cuda(), rows.cuda(), positions.cuda())  # of no rows
 
 
 def test_rows_of_a_decoder():
