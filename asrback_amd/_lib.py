@@ -397,6 +397,20 @@ class Decode8Params(ctypes.Structure):
     ]
 
 
+class Append8Params(ctypes.Structure):
+    """``asrlayer_append8_params`` (csrc/layers.hpp)."""
+
+    _fields_ = [
+        *Decode8Params._fields_,
+        ("padding", _i32),  # of the structure above
+        *[(name, _ptr) for name in ("k", "v")],
+        *[(f"{t}_{axis}_stride", _i64) for t in ("k", "v") for axis in ("batch", "head")],
+        *[(name, _ptr) for name in ("positions", "q_norm", "k_norm", "cos", "sin")],
+        ("rope_stride", _i64),
+        *[(name, ctypes.c_float) for name in ("q_eps", "k_eps")],
+    ]
+
+
 # A NULL pointer is 0 in these.
 pack_tree = Packed(TreeParams).pack
 pack_commit = Packed(CommitParams).pack
@@ -405,6 +419,7 @@ pack_linear8 = Packed(Linear8Params).pack
 pack_write8 = Packed(Write8Params).pack
 pack_read8 = Packed(Read8Params).pack
 pack_decode8 = Packed(Decode8Params).pack
+pack_append8 = Packed(Append8Params).pack
 
 # The layers' own entry points (csrc/layers.hpp).
 LAYER_SIGNATURES = {
@@ -414,6 +429,7 @@ LAYER_SIGNATURES = {
     "asrlayer_write8": (ctypes.c_int, [_ptr, _ptr]),
     "asrlayer_read8": (ctypes.c_int, [_ptr, _ptr]),
     "asrlayer_decode8": (ctypes.c_int, [_ptr, _ptr, ctypes.c_size_t, _ptr]),
+    "asrlayer_append8": (ctypes.c_int, [_ptr, _ptr, ctypes.c_size_t, _ptr]),
     "asrlayer_decode8_workspace_size": (ctypes.c_size_t, [_ptr]),
     "asrlayer_tree": (ctypes.c_int, [_ptr, _ptr, ctypes.c_size_t, _ptr]),
     "asrlayer_tree_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(TreeParams)]),

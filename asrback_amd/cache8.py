@@ -4,7 +4,8 @@ A decoder step is bound by reading the cache; with 8 bits a value (and a float32
 per position and kv head) there is half as much of it to read as in bfloat16, and
 twice as many positions fit.  :class:`Cache8` is one layer's cache, a slab or a page
 pool; :func:`write8` rounds new tokens' keys and values into it, :func:`decode8` is
-the attention of one query a row over it, and :func:`read8` gives it back in a float
+the attention of one query a row over it, :func:`decode_append8` both for a
+decoder's step, and :func:`read8` gives it back in a float
 type, for what attends over it in another way.
 
 As in :mod:`asrback_amd.attention`, calls launch on the current HIP stream, never
@@ -285,6 +286,37 @@ def decode8(q: Tensor, cache: Cache8, *, lengths: Tensor | None = None, scale: f
     and exact, sums float32.  ``out`` is written in place; it may be ``q`` itself.
     ``workspace``: the split partials' memory (:func:`decode8_workspace_size`,
     :func:`asrback_amd.attention.workspace`).  Returns ``(batch, heads_q, head_dim)``."""
+    return _decode("decode8", q, cache, lengths, scale, out, workspace, pages, window)
+
+
+def decode_append8(q: Tensor, k: Tensor, v: Tensor, cache: Cache8, positions: Tensor, *, q_norm: Tensor, k_norm: Tensor,
+                   q_eps: float, k_eps: float, cos: Tensor, sin: Tensor, scale: float | None = None,
+                   out: Tensor | None = None, workspace: Tensor | None = None, pages: PageTable | None = None,
+                   window: int | None = None) -> Tensor:
+    """A decoder step in one launch (``asrlayer_append8``): :func:`write_rows8` of one token a
+    row, ``k``/``v`` ``(batch, heads_kv, head_dim)`` at ``positions`` (int64), and
+    :func:`decode8` of the queries ``q`` ``(batch, heads_q, head_dim)`` over positions ``0 ..
+    positions[b]`` (the whole cache where that is past its end, without the new key,
+    which is dropped there as it is where there is no page; none below 0).  Returns
+    ``(batch, heads_q, head_dim)``."""
+    batch, heads, head_dim = q.shape[0], *cache.keys.shape[2:]
+    for name, t in (("k", k), ("v", v)):
+        if t.shape != (batch, heads, head_dim):
+            raise ValueError(f"{name} must be ({batch}, {heads}, {head_dim}), got {tuple(t.shape)}")
+    for name, t, shape in (("q_norm", q_norm, (head_dim,)), ("k_norm", k_norm, (head_dim,)),
+                           ("cos", cos, (batch, head_dim)), ("sin", sin, (batch, head_dim))):
+        if t.shape != shape:
+            raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+    positions = _index(positions, "positions", batch)
+    if positions is None:
+        raise TypeError("positions must be a tensor")
+    return _decode("decode_append8", q, cache, None, scale, out, workspace, pages, window,
+                   (k, v, q_norm, k_norm, cos, sin), positions, q_eps, k_eps)
+
+
+def _decode(what: str, q: Tensor, cache: Cache8, lengths: Tensor | None, scale: float | None, out: Tensor | None,
+            workspace: Tensor | None, pages: PageTable | None, window: int | None, new: tuple = (),
+            positions: Tensor | None = None, q_eps: float = 0.0, k_eps: float = 0.0) -> Tensor:
     shape = q.shape
     heads_kv, head_dim = cache.keys.shape[2:]
     if len(shape) != 3 or shape[2] != head_dim:
@@ -295,25 +327,24 @@ def decode8(q: Tensor, cache: Cache8, *, lengths: Tensor | None = None, scale: f
     if window is not None and window < 1:
         raise ValueError(f"a window holds at least one position, got {window}")
     lengths = _lengths(lengths, batch)
-    refuse_unseen("decode8", q, *cache.tensors)
+    refuse_unseen(what, q, *new, *cache.tensors)
     given = out is not None
     if given:
         if out.shape != shape or out.dtype != q.dtype or out.stride(-1) != 1:
             raise ValueError("out must match q's shape and dtype, with a unit last stride")
         # A row's queries are read before any of its outputs is written.
         in_place = out.data_ptr() == q.data_ptr() and out.stride() == q.stride()
-        check_out("decode8", out, None if in_place else q, *cache.tensors, lengths)
-    index = _ready("decode8", q)
+        check_out(what, out, None if in_place else q, *new, *cache.tensors, lengths, positions)
+    index = _ready(what, q, *new)
     q = _aligned(q)
-    _on(index, lengths, out)
+    _on(index, lengths, out, positions)
     fields = _cache_fields(cache, pages, batch, index)
     if not given:
         out = q.new_empty(shape)
     code, span = _DTYPES[q.dtype], window or 0
-    params = _lib.pack_decode8(
-        *fields, q.data_ptr(), out.data_ptr(), *q.stride()[:2], *out.stride()[:2],
-        0 if lengths is None else lengths.data_ptr(), lengths is not None and lengths.dtype is torch.int64, heads_q, span,
-        code, head_dim**-0.5 if scale is None else scale)
+    step = (*fields, q.data_ptr(), out.data_ptr(), *q.stride()[:2], *out.stride()[:2],
+            0 if lengths is None else lengths.data_ptr(), lengths is not None and lengths.dtype is torch.int64, heads_q, span,
+            code, head_dim**-0.5 if scale is None else scale)
     need = _workspace(batch, heads_q, heads_kv, head_dim, fields[-1], span, code)
     size = 0
     if need > 0:
@@ -321,9 +352,22 @@ def decode8(q: Tensor, cache: Cache8, *, lengths: Tensor | None = None, scale: f
     if workspace is not None:
         size, workspace = workspace.numel(), workspace.data_ptr()
     # Sizes that the library does not take (need -1): the call says why.
-    status = _lib.load().asrlayer_decode8(params, workspace, size, _raw_stream(index))
+    lib = _lib.load()
+    if not new:
+        status = lib.asrlayer_decode8(_lib.pack_decode8(*step), workspace, size, _raw_stream(index))
+    else:
+        if not torch.is_inference_mode_enabled() and any(t.is_inference() for t in cache.tensors):
+            raise RuntimeError("inplace update to inference tensors outside InferenceMode is not allowed")
+        k, v = _aligned(new[0]), _aligned(new[1])
+        q_norm, k_norm, cos, sin = (_aligned(t if t.is_contiguous() else t.contiguous()) for t in new[2:])
+        status = lib.asrlayer_append8(
+            _lib.pack_append8(*step, 0, k.data_ptr(), v.data_ptr(), *k.stride()[:2], *v.stride()[:2], positions.data_ptr(),
+                              q_norm.data_ptr(), k_norm.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.stride(0), q_eps, k_eps),
+            workspace, size, _raw_stream(index))
     if status:
-        _lib.check(status, "asrlayer_decode8")
+        _lib.check(status, "asrlayer_append8" if new else "asrlayer_decode8")
+    if new:
+        _increment_version(cache.tensors)
     if given:
         _increment_version(out)
     return out

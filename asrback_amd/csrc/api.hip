@@ -854,6 +854,57 @@ Decode8Workspace decode8_workspace(const asrlayer_decode8_params& p, size_t grou
   return w;
 }
 
+// append: of asrlayer_append8, whose step params is.
+int run_decode8(const asrlayer_decode8_params* params, const asrlayer_append8_params* append, void* workspace,
+                size_t workspace_bytes, void* stream) {
+  int rc = check_decode8(params);
+  if (rc != ASRATTN_OK) return rc;
+  asrlayer_decode8_params p = *params;
+  if (p.cache.batch == 0) return ok();
+  if (p.q == nullptr || p.out == nullptr) return fail(ASRATTN_ERR_INVALID, "q and out must be non-NULL");
+  if (!vec_aligned(p.q, p.dtype, {p.q_batch_stride, p.q_head_stride}))
+    return fail(ASRATTN_ERR_INVALID, "q needs a 16-byte aligned pointer and strides that are multiples of 16 bytes");
+  if (append != nullptr) {
+    const asrlayer_append8_params& n = *append;
+    if (n.k == nullptr || n.v == nullptr || n.positions == nullptr || n.q_norm == nullptr || n.k_norm == nullptr ||
+        n.cos == nullptr || n.sin == nullptr)
+      return fail(ASRATTN_ERR_INVALID, "k, v, positions, the norms and the tables must be non-NULL");
+    if (!vec_aligned(n.k, p.dtype, {n.k_batch_stride, n.k_head_stride}) ||
+        !vec_aligned(n.v, p.dtype, {n.v_batch_stride, n.v_head_stride}) || !vec_aligned(n.q_norm, p.dtype, {}) ||
+        !vec_aligned(n.k_norm, p.dtype, {}) || !vec_aligned(n.cos, p.dtype, {n.rope_stride}) ||
+        !vec_aligned(n.sin, p.dtype, {}))
+      return fail(ASRATTN_ERR_INVALID, "tensors need 16-byte aligned pointers and strides that are multiples of 16 bytes");
+  }
+  if (empty_cache8(p.cache)) {
+    p.cache.max_len = 0;
+    p.cache.block_table = nullptr;
+  } else {
+    rc = check_cache8(p.cache);
+    if (rc != ASRATTN_OK) return rc;
+  }
+  const asrattn::Decode8Plan plan = asrattn::decode8_plan(p);
+  if ((long long)p.cache.heads_kv * plan.head_tiles > 65535)
+    return fail(ASRATTN_ERR_UNSUPPORTED, "more than 65535 blocks of query heads");
+  float* ws_o = nullptr;
+  float* ws_ml = nullptr;
+  unsigned long long* ws_arrive = nullptr;
+  if (plan.share > 0) {
+    const size_t blocks = (size_t)p.cache.heads_kv * plan.head_tiles;
+    const Decode8Workspace w = decode8_workspace(p, blocks * plan.share, blocks * p.cache.batch);
+    if (workspace == nullptr || workspace_bytes < w.total)
+      return fail(ASRATTN_ERR_WORKSPACE, "the step needs %zu workspace bytes, got %zu", w.total,
+                  workspace == nullptr ? (size_t)0 : workspace_bytes);
+    if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+      return fail(ASRATTN_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+    char* base = static_cast<char*>(workspace);
+    ws_o = reinterpret_cast<float*>(base);
+    ws_ml = reinterpret_cast<float*>(base + w.stats);
+    ws_arrive = reinterpret_cast<unsigned long long*>(base + w.arrive);
+  }
+  return from_hip(asrattn::launch_decode8(p, append, plan, ws_o, ws_ml, ws_arrive, static_cast<hipStream_t>(stream)),
+                  append != nullptr ? "asrlayer_append8" : "asrlayer_decode8");
+}
+
 }  // namespace
 
 extern "C" {
@@ -918,41 +969,12 @@ size_t asrlayer_decode8_workspace_size(const asrlayer_decode8_params* params) {
 }
 
 int asrlayer_decode8(const asrlayer_decode8_params* params, void* workspace, size_t workspace_bytes, void* stream) {
-  int rc = check_decode8(params);
-  if (rc != ASRATTN_OK) return rc;
-  asrlayer_decode8_params p = *params;
-  if (p.cache.batch == 0) return ok();
-  if (p.q == nullptr || p.out == nullptr) return fail(ASRATTN_ERR_INVALID, "q and out must be non-NULL");
-  if (!vec_aligned(p.q, p.dtype, {p.q_batch_stride, p.q_head_stride}))
-    return fail(ASRATTN_ERR_INVALID, "q needs a 16-byte aligned pointer and strides that are multiples of 16 bytes");
-  if (empty_cache8(p.cache)) {
-    p.cache.max_len = 0;
-    p.cache.block_table = nullptr;
-  } else {
-    rc = check_cache8(p.cache);
-    if (rc != ASRATTN_OK) return rc;
-  }
-  const asrattn::Decode8Plan plan = asrattn::decode8_plan(p);
-  if ((long long)p.cache.heads_kv * plan.head_tiles > 65535)
-    return fail(ASRATTN_ERR_UNSUPPORTED, "more than 65535 blocks of query heads");
-  float* ws_o = nullptr;
-  float* ws_ml = nullptr;
-  unsigned long long* ws_arrive = nullptr;
-  if (plan.share > 0) {
-    const size_t blocks = (size_t)p.cache.heads_kv * plan.head_tiles;
-    const Decode8Workspace w = decode8_workspace(p, blocks * plan.share, blocks * p.cache.batch);
-    if (workspace == nullptr || workspace_bytes < w.total)
-      return fail(ASRATTN_ERR_WORKSPACE, "the step needs %zu workspace bytes, got %zu", w.total,
-                  workspace == nullptr ? (size_t)0 : workspace_bytes);
-    if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
-      return fail(ASRATTN_ERR_WORKSPACE, "workspace must be 256-byte aligned");
-    char* base = static_cast<char*>(workspace);
-    ws_o = reinterpret_cast<float*>(base);
-    ws_ml = reinterpret_cast<float*>(base + w.stats);
-    ws_arrive = reinterpret_cast<unsigned long long*>(base + w.arrive);
-  }
-  return from_hip(asrattn::launch_decode8(p, plan, ws_o, ws_ml, ws_arrive, static_cast<hipStream_t>(stream)),
-                  "asrlayer_decode8");
+  return run_decode8(params, nullptr, workspace, workspace_bytes, stream);
+}
+
+int asrlayer_append8(const asrlayer_append8_params* params, void* workspace, size_t workspace_bytes, void* stream) {
+  if (params == nullptr) return fail(ASRATTN_ERR_INVALID, "params is NULL");
+  return run_decode8(&params->step, params, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -1,5 +1,5 @@
 // A decoder step's attention over a cache of 8-bit keys and values
-// (asrlayer_decode8).
+// (asrlayer_decode8), with the step's write and what comes before it (asrlayer_append8).
 //
 // One query per sequence: g query heads share a kv head's n keys, each of which is
 // read once, 2 (head_dim + 4) bytes with its value and scales, for 4 g head_dim
@@ -61,6 +61,7 @@ constexpr int kNontemporal = 2;
 
 struct Decode8Args {
   asrlayer_decode8_params p;
+  asrlayer_append8_params n;  // of the variant that appends (its step is p)
   int page_shift, head_tiles;
   int share;       // workgroups of a block of heads, that share all sequences' keys (0: one each)
   int splits;      // of every sequence (0: by their lengths)
@@ -172,7 +173,12 @@ __device__ __forceinline__ int lanes_prefix(int x, int lanes) {
   return x;
 }
 
-template <typename T, int HD, int W, bool PAGED>
+// APPEND: the queries get their norm and rotation here, and the sequence's new key and
+// value are rounded, written, and attended to beside the tiles: the softmax of the last
+// split's last wave, which has the fewest, begins with them.  One of 480 keys (16 heads
+// over 8 of 128) 9.5 us, with a launch before it 12.1; 64 of them 18.5 and 20.2; one
+// of 16 000 19.1 and 21.1.
+template <typename T, int HD, int W, bool PAGED, bool APPEND>
 __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decode8_kernel(const Decode8Args a) {
   using S = Decode8Shape<T, HD>;
   constexpr int kQP = S::kQP, kWP = S::kWP, kKP = S::kKP, kVB = S::kVB, kVD = S::kVD;
@@ -187,18 +193,25 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
   // The workgroup's sequence, its keys, and its split of them.
   auto keys_of = [&](int64_t have) { return have < 0 ? 0 : have < c.max_len ? (int)have : c.max_len; };
   auto first_of = [&](int n) { return p.window > 0 && n > p.window ? n - p.window : 0; };
-  int b = blockIdx.z, n = c.max_len, split = 0, splits = 1;
+  // Keys of sequence j, the new one among them, where `load` reads a number.
+  auto have_of = [&](int j, auto load) {
+    if constexpr (APPEND) {
+      const int64_t pos = load(a.n.positions + j);
+      return pos < c.max_len ? keys_of(pos + 1) : c.max_len;
+    }
+    if (p.lengths == nullptr) return c.max_len;
+    return keys_of(p.lengths64 ? load(static_cast<const int64_t*>(p.lengths) + j)
+                               : (int64_t)load(static_cast<const int32_t*>(p.lengths) + j));
+  };
+  auto uniformly = [](auto* p) { return load_uniform(p); };
+  int b = blockIdx.z, n, split = 0, splits = 1;
   if (a.share == 0) {
-    if (p.lengths != nullptr)
-      n = keys_of(p.lengths64 ? load_uniform(static_cast<const int64_t*>(p.lengths) + b)
-                              : (int64_t)load_uniform(static_cast<const int32_t*>(p.lengths) + b));
+    n = have_of(b, uniformly);
   } else if (a.splits > 0) {
     b = blockIdx.x / a.splits;
     split = blockIdx.x - b * a.splits;
     splits = a.splits;
-    if (p.lengths != nullptr)
-      n = keys_of(p.lengths64 ? load_uniform(static_cast<const int64_t*>(p.lengths) + b)
-                              : (int64_t)load_uniform(static_cast<const int32_t*>(p.lengths) + b));
+    n = have_of(b, uniformly);
   } else {
     // Sequences get workgroups by their tiles: every `per` of them one, where per is whole
     // turns of the waves, and about the fewest for which the workgroups do not run out (they
@@ -208,9 +221,7 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int j = 2 * lane + s;
-      int have = j < c.batch ? c.max_len : 0;
-      if (p.lengths != nullptr && j < c.batch)
-        have = keys_of(p.lengths64 ? static_cast<const int64_t*>(p.lengths)[j] : (int64_t)static_cast<const int32_t*>(p.lengths)[j]);
+      const int have = j < c.batch ? have_of(j, [](auto* p) { return *p; }) : 0;
       held_keys[s] = have;
       count[s] = have / kKeys + (have % kKeys != 0) - first_of(have) / kKeys;
       tiles += count[s];
@@ -258,21 +269,57 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
   __shared__ uint32_t sm_largest[W];
   __shared__ int sm_last;
 
+  constexpr int EPL = Elem<T>::kPerVec, LPK = HD / EPL, kGroups = 64 * W / LPK;
+  constexpr int kRowTurns = APPEND ? (16 + 2 + kGroups - 1) / kGroups : 1;
+  const int sub = threadIdx.x % LPK;
+  __shared__ uint4 sm_new[APPEND ? 2 * HD / 16 : 1];  // the new key's and value's bytes
+  __shared__ float sm_new_scale[2];
+  uint4 row[kRowTurns], weights[kRowTurns], cs{}, sn{};
+  int new_page = 0, new_pos = -1;  // where the new key goes (-1: nowhere)
+  if constexpr (APPEND) {
+    // Rows of LPK lanes: the queries', and the new key and value of the last split.
+    cs = reinterpret_cast<const uint4*>(static_cast<const T*>(a.n.cos) + b * a.n.rope_stride)[sub];
+    sn = reinterpret_cast<const uint4*>(static_cast<const T*>(a.n.sin) + b * a.n.rope_stride)[sub];
+#pragma unroll
+    for (int turn = 0; turn < kRowTurns; ++turn) {
+      const int r = min(turn * kGroups + (int)threadIdx.x / LPK, split == splits - 1 ? held + 1 : held - 1);
+      const T* from = r < held ? static_cast<const T*>(p.q) + (int64_t)b * p.q_batch_stride + (int64_t)(head0 + r) * p.q_head_stride
+                      : r == held ? static_cast<const T*>(a.n.k) + (int64_t)b * a.n.k_batch_stride + hkv * a.n.k_head_stride
+                                  : static_cast<const T*>(a.n.v) + (int64_t)b * a.n.v_batch_stride + hkv * a.n.v_head_stride;
+      row[turn] = reinterpret_cast<const uint4*>(from)[sub];
+      weights[turn] = static_cast<const uint4*>(r < held ? a.n.q_norm : a.n.k_norm)[sub];
+    }
+    const int64_t pos = load_uniform(a.n.positions + b);
+    if (pos >= 0 && pos < c.max_len) {
+      new_pos = (int)pos;
+      if constexpr (PAGED) {
+        new_page = load_uniform(c.block_table + (int64_t)b * c.bt_stride + (new_pos >> a.page_shift));
+        if (new_page < 0 || new_page >= c.num_pages) new_pos = -1;
+      }
+    }
+  }
+
   // The queries' pieces, 8 dimensions each: lane's piece u of its head (heads past the
   // last repeat it) goes to (u, part, lane) of LDS.
   constexpr int kQTurns = (2 * kKP + W - 1) / W, kQVecs = sizeof(T) / 2;
   uint4 raw_q[kQTurns][kQVecs];
+  auto read_queries = [&](const T* at, int64_t head_step) {
 #pragma unroll
-  for (int turn = 0; turn < kQTurns; ++turn) {
-    const int u = min(turn * W + wave, 2 * kKP - 1);
-    const T* from = static_cast<const T*>(p.q) + (int64_t)b * p.q_batch_stride +
-                    (int64_t)(head0 + min(i, held - 1)) * p.q_head_stride + 64 * (u / 2) + 16 * g + 8 * (u % 2);
+    for (int turn = 0; turn < kQTurns; ++turn) {
+      const int u = min(turn * W + wave, 2 * kKP - 1);
+      const T* from = at + min(i, held - 1) * head_step + 64 * (u / 2) + 16 * g + 8 * (u % 2);
 #pragma unroll
-    for (int x = 0; x < kQVecs; ++x) raw_q[turn][x] = reinterpret_cast<const uint4*>(from)[x];
-  }
+      for (int x = 0; x < kQVecs; ++x) raw_q[turn][x] = reinterpret_cast<const uint4*>(from)[x];
+    }
+  };
+  if constexpr (!APPEND)
+    read_queries(static_cast<const T*>(p.q) + (int64_t)b * p.q_batch_stride + (int64_t)head0 * p.q_head_stride,
+                 p.q_head_stride);
 
-  // The positions: from a multiple of a tile on.
-  const int first = first_of(n), tile0 = first / kKeys, tiles = n / kKeys + (n % kKeys != 0) - tile0;
+  // The positions: from a multiple of a tile on, up to the new key.
+  const int first = first_of(n);
+  if (APPEND && new_pos >= 0) n = new_pos;
+  const int tile0 = first / kKeys, tiles = n / kKeys + (n % kKeys != 0) - tile0;
   const int per = (tiles + splits - 1) / splits;
   const int t0 = tile0 + min(tiles, split * per), t1 = min(tile0 + tiles, t0 + per);
 
@@ -383,6 +430,53 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
   };
+  if constexpr (APPEND) {
+    uint4* const rows = sm_pool;
+    uint32_t largest_q = 0;
+#pragma unroll
+    for (int turn = 0; turn < kRowTurns; ++turn) {
+      const int r = turn * kGroups + (int)threadIdx.x / LPK;
+      const bool is_v = r == held + 1;
+      const uint4 out = prologue_row<T, HD, LPK>(row[turn], true, !is_v, true, weights[turn], true, !is_v, cs, sn,
+                                                 r < held ? a.n.q_eps : a.n.k_eps, sub);
+      float x[EPL];
+      unpack<T>(out, x);
+      uint32_t largest = 0;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) largest = max(largest, magnitude(x[e]));
+      const Scale8 s = scale8(group_umax<LPK>(largest));
+      if (r < held) {
+        rows[r * LPK + sub] = out;
+        largest_q = max(largest_q, largest);
+      } else if (split == splits - 1 && r <= held + 1) {
+        uint32_t bytes[EPL / 4];
+#pragma unroll
+        for (int e = 0; e < EPL; e += 4) bytes[e / 4] = round8x4(x + e, s);
+        __builtin_memcpy(reinterpret_cast<char*>(sm_new) + (is_v ? HD : 0) + sub * EPL, bytes, EPL);
+        if (sub == 0) sm_new_scale[is_v] = s.scale;
+        if (ht == 0 && new_pos >= 0) {
+          const int64_t entry = PAGED ? new_page : b;
+          const int64_t at = PAGED ? new_pos & ((1 << a.page_shift) - 1) : new_pos;
+          int8_t* to = static_cast<int8_t*>(is_v ? c.v : c.k) + entry * (is_v ? c.v_batch_stride : c.k_batch_stride) +
+                       at * (is_v ? c.v_token_stride : c.k_token_stride) + hkv * (is_v ? c.v_head_stride : c.k_head_stride);
+          if constexpr (EPL == 8)
+            reinterpret_cast<uint2*>(to)[sub] = make_uint2(bytes[0], bytes[EPL / 4 - 1]);
+          else
+            reinterpret_cast<uint32_t*>(to)[sub] = bytes[0];
+          if (sub == 0)
+            static_cast<float*>(is_v ? c.v_scales : c.k_scales)
+                [entry * (is_v ? c.vs_batch_stride : c.ks_batch_stride) + hkv * (is_v ? c.vs_head_stride : c.ks_head_stride) +
+                 at] = s.scale;
+        }
+      }
+    }
+    if constexpr (S::kBiased) {
+      largest_q = group_umax<64>(largest_q);
+      if (lane == 0) sm_largest[wave] = largest_q;
+    }
+    lds_barrier();
+    read_queries(reinterpret_cast<const T*>(rows), HD);
+  }
   // What a key's scale is multiplied by: where bytes are converted and where they are
   // biased.
   float unit = a.c, biased_unit = 0.f;
@@ -391,16 +485,18 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
     // The queries times a power of two that puts their largest near 2^100, so that
     // products with u 2^-133 are ordinary numbers.
     uint32_t largest = 0;
+    if constexpr (!APPEND) {
 #pragma unroll
-    for (int turn = 0; turn < kQTurns; ++turn) {
-      float x[8];
-      unpack<bf16_raw>(raw_q[turn][0], x);
+      for (int turn = 0; turn < kQTurns; ++turn) {
+        float x[8];
+        unpack<bf16_raw>(raw_q[turn][0], x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) largest = max(largest, magnitude(x[e]));
+        for (int e = 0; e < 8; ++e) largest = max(largest, magnitude(x[e]));
+      }
+      largest = group_umax<64>(largest);
+      if (lane == 0) sm_largest[wave] = largest;
+      lds_barrier();
     }
-    largest = group_umax<64>(largest);
-    if (lane == 0) sm_largest[wave] = largest;
-    lds_barrier();
 #pragma unroll
     for (int u = 0; u < W; ++u) largest = max(largest, sm_largest[u]);
     const int e = (int)(__builtin_amdgcn_readfirstlane(largest) >> 23) - 127, up = 100 - e;
@@ -437,6 +533,38 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
     lds_barrier();
   }
   f32x4_t weighed{0.f, 0.f, 0.f, 0.f};  // products of the weights with biased zeros
+  // Scores of 16 keys of the wave's LDS.
+  auto scores_of = [&](int h, auto widened, f32x4_t sum) {
+#pragma unroll
+    for (int u = 0; u < kKP; ++u) {
+      const uint4 raw = sm_k[lds_piece<S::kLPR>(16 * h + i, 4 * u + g)];
+      const uint2 w0 = widened(raw.x), w1 = widened(raw.y), w2 = widened(raw.z), w3 = widened(raw.w);
+      const uint4 lo = make_uint4(w0.x, w0.y, w1.x, w1.y), hi = make_uint4(w2.x, w2.y, w3.x, w3.y);
+#pragma unroll
+      for (int part = kQP - 1; part >= 0; --part) {
+        sum = mfma_bf16(lo, sm_q[(2 * u * kQP + part) * 64 + lane], sum);
+        sum = mfma_bf16(hi, sm_q[((2 * u + 1) * kQP + part) * 64 + lane], sum);
+      }
+    }
+    return sum;
+  };
+  if (APPEND && new_pos >= 0 && split == splits - 1 && wave == W - 1) {
+    // The new key as the first of 16 (the others are whatever lies there, and not looked at).
+    if (lane < S::kLPR) sm_k[lds_piece<S::kLPR>(0, lane)] = sm_new[lane];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    const f32x4_t s = scores_of(0, [](uint32_t x) { return widen(x); }, f32x4_t{0.f, 0.f, 0.f, 0.f});
+    m = __shfl(s[0] * (sm_new_scale[0] * unit), i, 64);
+    l = g == 0 ? 1.f : 0.f;
+    const float vs = sm_new_scale[1] * (1.f / S::kUnit);
+    const uint32_t* value = reinterpret_cast<const uint32_t*>(sm_new + HD / 16) + g * kVB;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int e = 0; e < kVB; ++e) o[e][r] = byte_of(value[(r * kVB + e) / 4], e % 4) * vs;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+  }
   {
     while (t < t1) {
       // The keys and the scales change lanes through the wave's own LDS.
@@ -456,24 +584,10 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
       f32x4_t s[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        auto scores = [&](auto widened, f32x4_t sum) {
-#pragma unroll
-          for (int u = 0; u < kKP; ++u) {
-            const uint4 raw = sm_k[lds_piece<S::kLPR>(16 * h + i, 4 * u + g)];
-            const uint2 w0 = widened(raw.x), w1 = widened(raw.y), w2 = widened(raw.z), w3 = widened(raw.w);
-            const uint4 lo = make_uint4(w0.x, w0.y, w1.x, w1.y), hi = make_uint4(w2.x, w2.y, w3.x, w3.y);
-#pragma unroll
-            for (int part = kQP - 1; part >= 0; --part) {
-              sum = mfma_bf16(lo, sm_q[(2 * u * kQP + part) * 64 + lane], sum);
-              sum = mfma_bf16(hi, sm_q[((2 * u + 1) * kQP + part) * 64 + lane], sum);
-            }
-          }
-          return sum;
-        };
         if (S::kBiased && !convert)
-          s[h] = scores([](uint32_t x) { return widen_biased(x ^ kBias); }, bias);
+          s[h] = scores_of(h, [](uint32_t x) { return widen_biased(x ^ kBias); }, bias);
         else
-          s[h] = scores([](uint32_t x) { return widen(x); }, f32x4_t{0.f, 0.f, 0.f, 0.f});
+          s[h] = scores_of(h, [](uint32_t x) { return widen(x); }, f32x4_t{0.f, 0.f, 0.f, 0.f});
       }
       const int pos = t * kKeys + 4 * g;
       float x[2][4], vs[2][4];
@@ -694,29 +808,35 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
   }
 }
 
-template <typename T, int HD, int W>
+template <typename T, int HD, int W, bool APPEND>
 hipError_t launch_waves(const Decode8Args& a, hipStream_t stream) {
   const bool split = a.share > 0;
   const dim3 grid(split ? a.share : 1, a.p.cache.heads_kv * a.head_tiles, split ? 1 : a.p.cache.batch), block(64 * W);
   if (a.p.cache.block_table != nullptr)
-    hipLaunchKernelGGL((decode8_kernel<T, HD, W, true>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((decode8_kernel<T, HD, W, true, APPEND>), grid, block, 0, stream, a);
   else
-    hipLaunchKernelGGL((decode8_kernel<T, HD, W, false>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((decode8_kernel<T, HD, W, false, APPEND>), grid, block, 0, stream, a);
   return hipGetLastError();
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool APPEND>
 hipError_t launch_head(const Decode8Args& a, const Decode8Plan& plan, hipStream_t stream) {
-  return plan.waves == 8 ? launch_waves<T, HD, 8>(a, stream) : launch_waves<T, HD, 4>(a, stream);
+  return plan.waves == 8 ? launch_waves<T, HD, 8, APPEND>(a, stream) : launch_waves<T, HD, 4, APPEND>(a, stream);
 }
 
-template <typename T>
+template <typename T, bool APPEND>
 hipError_t launch_typed(const Decode8Args& a, const Decode8Plan& plan, hipStream_t stream) {
   switch (a.p.cache.head_dim) {
-    case 64: return launch_head<T, 64>(a, plan, stream);
-    case 128: return launch_head<T, 128>(a, plan, stream);
-    default: return launch_head<T, 256>(a, plan, stream);
+    case 64: return launch_head<T, 64, APPEND>(a, plan, stream);
+    case 128: return launch_head<T, 128, APPEND>(a, plan, stream);
+    default: return launch_head<T, 256, APPEND>(a, plan, stream);
   }
+}
+
+template <bool APPEND>
+hipError_t launch_step(const Decode8Args& a, const Decode8Plan& plan, hipStream_t stream) {
+  return a.p.dtype == ASRATTN_BF16 ? launch_typed<bf16_raw, APPEND>(a, plan, stream)
+                                   : launch_typed<float, APPEND>(a, plan, stream);
 }
 
 }  // namespace
@@ -752,10 +872,11 @@ Decode8Plan decode8_plan(const asrlayer_decode8_params& p) {
   return plan;
 }
 
-hipError_t launch_decode8(const asrlayer_decode8_params& p, const Decode8Plan& plan, float* ws_o, float* ws_ml,
-                          unsigned long long* ws_arrive, hipStream_t stream) {
-  Decode8Args a;
+hipError_t launch_decode8(const asrlayer_decode8_params& p, const asrlayer_append8_params* append, const Decode8Plan& plan,
+                          float* ws_o, float* ws_ml, unsigned long long* ws_arrive, hipStream_t stream) {
+  Decode8Args a{};
   a.p = p;
+  if (append != nullptr) a.n = *append;
   a.page_shift = 0;
   while (p.cache.block_table != nullptr && (1 << a.page_shift) < p.cache.page_size) ++a.page_shift;
   a.head_tiles = plan.head_tiles;
@@ -768,8 +889,7 @@ hipError_t launch_decode8(const asrlayer_decode8_params& p, const Decode8Plan& p
   a.ws_ml = ws_ml;
   a.ws_arrive = ws_arrive;
   a.tag = plan.share > 0 ? launch_tag() : 0;
-  return p.dtype == ASRATTN_BF16 ? launch_typed<bf16_raw>(a, plan, stream)
-                                 : launch_typed<float>(a, plan, stream);
+  return append != nullptr ? launch_step<true>(a, plan, stream) : launch_step<false>(a, plan, stream);
 }
 
 }  // namespace asrattn

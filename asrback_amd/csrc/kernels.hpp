@@ -113,7 +113,7 @@ Linear8Workspace linear8_workspace(int64_t rows, int n, int k, bool gated);
 hipError_t launch_linear8(const asrlayer_linear8_params& p, void* workspace, hipStream_t stream);
 
 // The 8-bit cache: writes, reading back (asrlayer_write8, asrlayer_read8) and a
-// decoder step's attention (asrlayer_decode8).
+// decoder step's attention (asrlayer_decode8, asrlayer_append8).
 hipError_t launch_write8(const asrlayer_write8_params& p, hipStream_t stream);
 hipError_t launch_read8(const asrlayer_read8_params& p, hipStream_t stream);
 struct Decode8Plan {
@@ -123,8 +123,9 @@ struct Decode8Plan {
   int splits;      // of each sequence among them (0: by their lengths)
 };
 Decode8Plan decode8_plan(const asrlayer_decode8_params& p);
-hipError_t launch_decode8(const asrlayer_decode8_params& p, const Decode8Plan& plan, float* ws_o, float* ws_ml,
-                          unsigned long long* ws_arrive, hipStream_t stream);
+// (append: NULL where the keys are all there)
+hipError_t launch_decode8(const asrlayer_decode8_params& p, const asrlayer_append8_params* append, const Decode8Plan& plan,
+                          float* ws_o, float* ws_ml, unsigned long long* ws_arrive, hipStream_t stream);
 
 // A tag for a split launch's arrival words that no other launch of the process
 // has (decode.hip).

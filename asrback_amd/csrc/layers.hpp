@@ -359,4 +359,23 @@ int asrlayer_decode8(const asrlayer_decode8_params* params, void* workspace, siz
 // any smaller batch as well.
 size_t asrlayer_decode8_workspace_size(const asrlayer_decode8_params* params);
 
+// asrlayer_write8 and asrlayer_decode8 of a decoder step in one launch: sequence b's
+// query heads and new key k (batch, heads_kv, head_dim) get the norms and the rotation,
+// key and value v go to the cache at positions[b], and the queries attend the positions up
+// to it (step.lengths is not read; a position past the cache: all of it, and the key is
+// dropped, as it is where there is no page; below 0: none).  cos, sin (batch,
+// head_dim), rows rope_stride apart.  The workspace is that of step.
+typedef struct asrlayer_append8_params {
+  asrlayer_decode8_params step;
+  const void *k, *v;
+  int64_t k_batch_stride, k_head_stride;
+  int64_t v_batch_stride, v_head_stride;
+  const int64_t* positions;
+  const void *q_norm, *k_norm, *cos, *sin;
+  int64_t rope_stride;
+  float q_eps, k_eps;
+} asrlayer_append8_params;
+
+int asrlayer_append8(const asrlayer_append8_params* params, void* workspace, size_t workspace_bytes, void* stream);
+
 }  // extern "C"

@@ -48,7 +48,7 @@ from torch import Tensor, nn
 from . import attention
 from .attention import KeyPrefix, PageTable, decode, decode_append, greedy_choice, varlen_attn
 from .drafts import MAX_TOKENS, accept_drafts, commit_drafts, tree_attention, tree_masks, tree_workspace_size
-from .cache8 import Cache8, decode8, decode8_workspace_size, read8, write8, write_rows8
+from .cache8 import Cache8, decode8, decode8_workspace_size, decode_append8, read8, write8, write_rows8
 from .layers import computes, prompt_rows, prompt_rows_takes, unhooked
 from .linear4 import Linear4
 from .linear8 import Linear8
@@ -417,15 +417,17 @@ class TextAttention(nn.Module):
         values[rows, positions] = v
         return q, k, v
 
+    def _plain_norms(self) -> bool:
+        return type(self.q_norm) is RMSNorm and type(self.k_norm) is RMSNorm and unhooked(self.q_norm, self.k_norm)
+
     def _rows8(self, x, layer: Layer8, rows, positions, cos, sin, prompt: bool) -> tuple[Tensor, ...]:
         """The queries of ``x``, the rounded keys and values written to an 8-bit cache,
         and for a prompt the keys and values as they were."""
         qkv = self.qkv_proj(x)
-        norms = q_norm, k_norm = self.q_norm, self.k_norm
-        if type(q_norm) is RMSNorm and type(k_norm) is RMSNorm and unhooked(*norms):
+        if self._plain_norms():
             q, k, v = (t.view(len(x), -1, self.head_dim) for t in qkv.split(self.sizes, dim=-1))
-            q, k = write_rows8(layer.cache, q, k, v, rows, positions, q_norm=q_norm.weight, k_norm=k_norm.weight,
-                               q_eps=q_norm.eps, k_eps=k_norm.eps, cos=cos, sin=sin, pages=layer.pages, keys=prompt)
+            q, k = write_rows8(layer.cache, q, k, v, rows, positions, q_norm=self.q_norm.weight, k_norm=self.k_norm.weight,
+                               q_eps=self.q_norm.eps, k_eps=self.k_norm.eps, cos=cos, sin=sin, pages=layer.pages, keys=prompt)
         else:
             q, k, v = self._norm_rotate(qkv, cos, sin)
             write8(layer.cache, k, v, rows, positions, pages=layer.pages)
@@ -460,10 +462,16 @@ class TextAttention(nn.Module):
         :class:`KeyPrefix` of ``positions``, as :meth:`TextModel.step`
         passes), the norms, the rotation, the cache write and the attention
         run as one kernel (:func:`~asrback_amd.attention.decode_append`);
-        other mask forms take the reference's sequence of ops.  Over an 8-bit
-        cache it is a write (:func:`~asrback_amd.cache8.write_rows8`) and the
-        attention (:func:`~asrback_amd.cache8.decode8`), with any mask form."""
+        other mask forms take the reference's sequence of ops.  So it is over
+        an 8-bit cache (:func:`~asrback_amd.cache8.decode_append8`, or
+        :func:`~asrback_amd.cache8.write_rows8` and
+        :func:`~asrback_amd.cache8.decode8`)."""
         if isinstance(keys, Layer8):
+            if isinstance(mask, KeyPrefix) and mask.positions is positions and self._plain_norms():
+                q, k, v = (t.view(len(x), -1, self.head_dim) for t in self.qkv_proj(x).split(self.sizes, dim=-1))
+                output = decode_append8(q, k, v, keys.cache, positions, q_norm=self.q_norm.weight, k_norm=self.k_norm.weight,
+                                        q_eps=self.q_norm.eps, k_eps=self.k_norm.eps, cos=cos, sin=sin, pages=keys.pages)
+                return self.o_proj(output.flatten(1))
             q, _, _ = self._rows8(x, keys, None, positions, cos, sin, False)
             output = decode8(q, keys.cache, lengths=_step_lengths(mask, positions, keys.shape[1]), pages=keys.pages)
             return self.o_proj(output.flatten(1))
@@ -571,8 +579,6 @@ class TextModel(nn.Module):
         x = self.embed_tokens(tokens)
         cos, sin = cos[positions], sin[positions]
         mask = KeyPrefix(positions=positions)
-        if isinstance(cache, (KVCache8, PagedKVCache8)):  # counted once for all layers
-            mask = KeyPrefix(lengths=_step_lengths(None, positions, cache.keys[0].shape[1]))
         for index, layer in enumerate(self.layers):
             keys, values = cache.keys[index], cache.values[index]
             x = layer(x, lambda attention, h: attention.step(h, keys, values, positions, mask, cos, sin))

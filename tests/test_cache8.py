@@ -15,7 +15,8 @@ CONFIG = {"num_hidden_layers": 2, "num_key_value_heads": 2, "head_dim": 64}
 
 
 @pytest.mark.parametrize("name,struct", [("Linear8Params", "asrlayer_linear8_params"), ("Write8Params", "asrlayer_write8_params"),
-                                         ("Read8Params", "asrlayer_read8_params"), ("Decode8Params", "asrlayer_decode8_params")])
+                                         ("Read8Params", "asrlayer_read8_params"), ("Decode8Params", "asrlayer_decode8_params"),
+                                         ("Append8Params", "asrlayer_append8_params")])
 def test_structs_match_the_header(name, struct, tmp_path):
     """The cache's fields come first, one by one."""
     from asrback_amd import _lib
@@ -28,6 +29,10 @@ def test_structs_match_the_header(name, struct, tmp_path):
     if name != "Linear8Params":
         assert len(_lib._CACHE8) == len(inner)
         fields = [f"cache.{f}" for f in inner] + fields[len(inner):]
+    if name == "Append8Params":  # the step's fields and its padding first
+        step = len(_lib.Decode8Params._fields_)
+        assert fields[step] == "padding" and ctypes.sizeof(_lib.Decode8Params) == cls.padding.offset + cls.padding.size
+        fields = [f"step.{f}" for f in fields[:step]] + fields[step + 1:]
     lines = [f'printf("%zu\\n", sizeof({struct}));', *(f'printf("%zu\\n", offsetof({struct}, {f}));' for f in fields)]
     source = tmp_path / "layout.cpp"
     source.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "layers.hpp"\nint main() {\n'
@@ -35,7 +40,7 @@ def test_structs_match_the_header(name, struct, tmp_path):
     subprocess.run(["g++", f"-I{ROOT / 'include'}", f"-I{ROOT / 'asrback_amd' / 'csrc'}", str(source), "-o",
                     str(tmp_path / "layout")], check=True)
     got = [int(x) for x in subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.split()]
-    assert got == [ctypes.sizeof(cls), *(getattr(cls, f).offset for f, _ in cls._fields_)]
+    assert got == [ctypes.sizeof(cls), *(getattr(cls, f).offset for f, _ in cls._fields_ if f != "padding")]
 
 
 def test_caches():
@@ -66,7 +71,7 @@ def test_caches():
 
 def calls():
     """Name, call of one float tensor, that tensor."""
-    from asrback_amd.cache8 import Cache8, decode8, read8, write8, write_rows8
+    from asrback_amd.cache8 import Cache8, decode8, decode_append8, read8, write8, write_rows8
 
     cache = Cache8.allocate(2, 8, 3, 64)
     k, positions, weight, table = torch.zeros(2, 3, 64), torch.zeros(2, dtype=torch.int64), torch.zeros(64), torch.zeros(2, 64)
@@ -74,6 +79,10 @@ def calls():
     def rows(q, k=k, weight=weight, table=table):
         return write_rows8(cache, q, k, k, None, positions, q_norm=weight, k_norm=weight, q_eps=1e-6, k_eps=1e-6, cos=table,
                            sin=table)
+
+    def append(q, k=k, weight=weight, table=table):
+        return decode_append8(q, k, k, cache, positions, q_norm=weight, k_norm=weight, q_eps=1e-6, k_eps=1e-6, cos=table,
+                              sin=table)
 
     def scaled(x, f):
         return f(Cache8(cache.keys, cache.values, cache.key_scales, x))
@@ -87,13 +96,16 @@ def calls():
         ("write_rows8", lambda x: rows(torch.zeros(2, 6, 64), weight=x), weight),
         ("write_rows8", lambda x: rows(torch.zeros(2, 6, 64), table=x), table),
         ("read8", lambda x: scaled(x, read8), s),
+        ("decode_append8", append, torch.zeros(2, 6, 64)),
+        ("decode_append8", lambda x: append(torch.zeros(2, 6, 64), k=x), k),
+        ("decode_append8", lambda x: append(torch.zeros(2, 6, 64), table=x), table),
         ("decode8", lambda x: decode8(x, cache), torch.zeros(2, 6, 64)),
         ("decode8", lambda x: scaled(x, lambda c: decode8(torch.zeros(2, 6, 64), c)), s),
     ]
 
 
 @pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning", "ignore::DeprecationWarning")
-@pytest.mark.parametrize("index", range(9))
+@pytest.mark.parametrize("index", range(12))
 def test_unseen(index):
     """Forward mode, function transforms and tracers do not see what a kernel computes."""
     from torch.fx.experimental.proxy_tensor import make_fx
@@ -140,7 +152,7 @@ def test_linear8_unseen():
 
 @pytest.mark.filterwarnings("ignore::DeprecationWarning")
 def test_refusals():
-    from asrback_amd.cache8 import Cache8, decode8, decode8_workspace_size, read8, write8, write_rows8
+    from asrback_amd.cache8 import Cache8, decode8, decode8_workspace_size, decode_append8, read8, write8, write_rows8
 
     cache = Cache8.allocate(2, 8, 3, 64)
     k, positions = torch.zeros(2, 3, 64), torch.zeros(2, dtype=torch.int64)
@@ -164,9 +176,20 @@ def test_refusals():
                                  (torch.zeros(2, 6, 128), {}, "q_norm|q must")):
         with pytest.raises(ValueError, match=match):
             write_rows8(cache, query, k, k, None, positions, **(good | change))
-    with torch.inference_mode():
-        held = Cache8.allocate(2, 8, 3, 64)
-    assert all(t.is_inference() for t in held.tensors)
+    for args, change, match in (((q, k[:1], k, positions), {}, "k must"), ((q, k, k[:, :1], positions), {}, "v must"),
+                                ((q, k, k, positions[:1]), {}, "positions"), ((q, k, k, positions.int()), {}, "positions"),
+                                ((q, k, k, positions), {"k_norm": norm[:32]}, "k_norm"),
+                                ((q, k, k, positions), {"cos": table[:1]}, "cos"), ((q[0], k, k, positions), {}, "must"),
+                                ((q[:, :4], k, k, positions), {}, "multiple"), ((q, k, k, positions), {"window": 0}, "window")):
+        with pytest.raises(ValueError, match=match):
+            decode_append8(args[0], args[1], args[2], cache, args[3], **(good | change))
+    with pytest.raises(TypeError, match="positions"):
+        decode_append8(q, k, k, cache, None, **good)
+    with pytest.raises(TypeError, match="mixed"):
+        decode_append8(q, k.bfloat16(), k, cache, positions, **good)
+    buffer = torch.zeros(2, 12, 64)
+    with pytest.raises(ValueError, match="shares memory"):
+        decode_append8(buffer[:, :6], buffer[:, 6:9], buffer[:, 9:], cache, positions, out=buffer[:, 5:11], **good)
     with pytest.raises(TypeError, match="float32 and bfloat16"):
         read8(cache, dtype=torch.float16)
     for bad in (positions[:1], positions.float()):
@@ -233,7 +256,15 @@ def test_what_the_library_refuses():
         p.heads_q, p.scale = 4, 0.125
         return p
 
+    def append():
+        p = cache(_lib.Append8Params())
+        p.q = p.out = p.k = p.v = p.positions = p.q_norm = p.k_norm = p.cos = p.sin = 4096
+        p.heads_q, p.scale = 4, 0.125
+        return p
+
     def run(p):
+        if isinstance(p, _lib.Append8Params):
+            return lib.asrlayer_append8(bytes(p), 0, 0, None)
         if isinstance(p, _lib.Write8Params):
             return lib.asrlayer_write8(bytes(p), None)
         if isinstance(p, _lib.Read8Params):
@@ -259,6 +290,10 @@ def test_what_the_library_refuses():
                  ({"k_token_stride": 4}, _lib.ERR_INVALID, b"16-byte"), ({"v": 4100}, _lib.ERR_INVALID, b"16-byte")]),
         (read, [({"v_out": 0}, _lib.ERR_INVALID, b"non-NULL"), ({"k_out": 4104}, _lib.ERR_INVALID, b"aligned"),
                 ({"max_len": 1 << 30, "heads_kv": 4}, _lib.ERR_UNSUPPORTED, b"2^33")]),
+        (append, [({"heads_q": 3}, _lib.ERR_INVALID, b"multiple"), ({"positions": 0}, _lib.ERR_INVALID, b"non-NULL"),
+                  ({"cos": 0}, _lib.ERR_INVALID, b"non-NULL"), ({"k": 4100}, _lib.ERR_INVALID, b"16-byte"),
+                  ({"v_head_stride": 4}, _lib.ERR_INVALID, b"16-byte"), ({"rope_stride": 4}, _lib.ERR_INVALID, b"16-byte"),
+                  ({"max_len": 4096}, _lib.ERR_WORKSPACE, b"workspace")]),
         (decode, [({"heads_q": 3}, _lib.ERR_INVALID, b"multiple"), ({"heads_q": 8192}, _lib.ERR_UNSUPPORTED, b"4096"),
                   ({"window": -1}, _lib.ERR_INVALID, b"window"), ({"scale": float("nan")}, _lib.ERR_INVALID, b"scale"),
                   ({"q": 0}, _lib.ERR_INVALID, b"non-NULL"), ({"q_head_stride": 4}, _lib.ERR_INVALID, b"16-byte"),
@@ -282,7 +317,7 @@ def test_what_the_library_refuses():
     assert 0 < need < 1 << 24
     assert lib.asrlayer_decode8(bytes(p), 4096 + 64, need, None) == _lib.ERR_WORKSPACE
     for f in (lambda: lib.asrlayer_write8(None, None), lambda: lib.asrlayer_read8(None, None),
-              lambda: lib.asrlayer_decode8(None, 0, 0, None)):
+              lambda: lib.asrlayer_decode8(None, 0, 0, None), lambda: lib.asrlayer_append8(None, 0, 0, None)):
         assert f() == _lib.ERR_INVALID
     assert lib.asrlayer_decode8_workspace_size(None) == (1 << 64) - 1
 

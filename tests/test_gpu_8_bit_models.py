@@ -206,6 +206,11 @@ def plain_decode(q, cache, *, lengths, pages=None):
     return out
 
 
+def plain_append(q, k, v, cache, positions, *, pages=None, **more):
+    q, _ = plain_write_rows(cache, q, k, v, None, positions, pages=pages, **more)
+    return plain_decode(q, cache, lengths=positions + 1, pages=pages)
+
+
 @pytest.fixture
 def plainly(monkeypatch):
     """A context in which the decoder calls the plain forms."""
@@ -215,7 +220,7 @@ def plainly(monkeypatch):
         patched = monkeypatch.context()
         m = patched.__enter__()
         for name, f in (("write8", plain_write), ("write_rows8", plain_write_rows), ("read8", plain_read),
-                        ("decode8", plain_decode)):
+                        ("decode8", plain_decode), ("decode_append8", plain_append)):
             m.setattr(aq, name, f)
         return patched
 

@@ -108,18 +108,28 @@ def reference(q, tensors, lengths, scale, window=None):
     return out, weighted, largest, units, queries
 
 
-def check(out, q, tensors, lengths, scale=None, window=None):
+def check(out, q, tensors, lengths, scale=None, window=None, queries_off=0.0):
+    """queries_off: how far the call's own queries are from q, of a head's largest."""
     d = q.shape[-1]
     ref, weighted, largest, units, queries = reference(q, tensors, lengths, d**-0.5 if scale is None else scale, window)
     n = torch.tensor([min(x, window or x) for x in lengths]).view(-1, 1, 1).double()
     step, parts = (2.0**-8, 2.0**-16) if q.dtype == BF16 else (2.0**-24, 2.0**-23)
     bound = 1.01 * (weighted * (2.0**-24 * (2 * (d + 8) * largest + 2 * n + 64) + parts) + step * ref.abs())
+    bound += 1.01 * weighted * 2 * queries_off * q.double().abs().amax(-1, keepdim=True) * keys_sum(tensors, q, lengths, scale)
     if q.dtype == BF16:
         bound += 1.01 * 2.0**-24 * 510 * ((n + 64) * units + 2 * weighted * (d + 8) * queries)
     out = out.cpu().double()
     assert torch.isfinite(out).all()
     worst = ((out - ref).abs() / bound.clamp(min=1e-40)).max()
     assert worst <= 1, float(worst)
+
+
+def keys_sum(tensors, q, lengths, scale):
+    """The largest sum of |k| times the scale over a row's keys, per query head."""
+    k, _, ks, _ = (t.double() for t in tensors)
+    group, d = q.shape[1] // k.shape[2], q.shape[2]
+    sums = [((k[b, :n].abs().sum(-1) * ks[b, :, :n].T).amax(0) if n else k.new_zeros(k.shape[2])) for b, n in enumerate(lengths)]
+    return torch.stack(sums).repeat_interleave(group, 1)[..., None] * (d**-0.5 if scale is None else scale)
 
 
 def spread(lengths, dtype=torch.int32):
@@ -395,6 +405,79 @@ def test_rows_of_a_decoder():
                     assert ((a - b).abs() <= 2.0**-21 * b.abs().amax(-1, keepdim=True)).all()
             for a, b in zip(want.tensors, have.tensors):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads,kv,head_dim,length,page,window", [
+    (16, 8, 128, 1024, 0, None), (4, 2, 128, 200, 16, None), (3, 3, 64, 512, 0, None), (8, 1, 256, 640, 64, None),
+    (40, 2, 64, 300, 0, 33), (16, 8, 128, 8192, 0, None), (4, 4, 256, 96, 32, 1), (34, 1, 128, 5000, 128, 700),
+])
+def test_steps_that_append(dtype, heads, kv, head_dim, length, page, window):
+    """A step in one launch against its write and attention: positions at both ends of the
+    cache, outside it, on no page and inside pages.  Both round the same rows; in float32
+    the rotation's sum may be contracted differently (2^-21 of a row's largest, as in
+    test_rows_of_a_decoder), so that scales and numbers at a border may differ."""
+    from asrback_amd.attention import PageTable
+    from asrback_amd.cache8 import Cache8, decode8, decode_append8, write_rows8
+    from asrback_amd.qwen3_asr import rope_tables
+
+    g = torch.Generator().manual_seed(heads * length)
+    where = [0, length - 1, length // 2, 31, 32, -1, length, length + 700, -4, length // 3, 2**62]
+    batch = len(where)
+    _, tensors = random_cache(batch, length, kv, head_dim, g)
+    tensors = list(tensors)
+    for b, p in enumerate(where):  # what is not held yet may be anything
+        if 0 <= p < length:
+            tensors[2][b, :, p:] = math.nan
+            tensors[3][b, :, p:] = math.inf
+    pages = None
+    if page:
+        cache, pages, ids = paged(tensors, page, g)
+        ids = ids.clone()
+        ids[2, (length // 2) // page] = -1  # the new key's page
+        ids[9, 0] = -1 if length // 3 >= page else ids[9, 0]
+        pages = PageTable(ids.to(torch.int32).cuda(), length)
+        both = [Cache8(*(t.clone() for t in cache.tensors)) for _ in "ab"]
+    else:
+        both = [Cache8(*(t.cuda() for t in tensors)) for _ in "ab"]
+    q, k, v = (torch.randn(batch, n, head_dim, generator=g).to("cuda", dtype) for n in (heads, kv, kv))
+    norms = [(torch.rand(head_dim, generator=g) + 0.5).to("cuda", dtype) for _ in "qk"]
+    cos, sin = (t[:batch].flip(0) for t in rope_tables({"head_dim": head_dim, "rope_theta": 1e4}, batch, "cuda", dtype))
+    more = {"q_norm": norms[0], "k_norm": norms[1], "q_eps": 1e-6, "k_eps": 1e-5, "cos": cos, "sin": sin}
+    positions = torch.tensor(where, device="cuda")
+    say("append", dtype, heads, kv, head_dim, length, page, window)
+    # (The queries written over, and strided keys.)
+    given = q.clone()
+    strided = torch.stack((k, v), 2).flatten(1, 2)
+    out = decode_append8(given, strided[:, ::2], strided[:, 1::2], both[1], positions, pages=pages, window=window,
+                         out=given, **more)
+    assert out is given
+    queries, _ = write_rows8(both[0], q, k, v, None, positions, pages=pages, **more)
+    counts = [min(max(p + 1, 0), length) for p in where]
+    want = decode8(queries, both[0], lengths=spread(counts), pages=pages, window=window)
+    for a, b in zip(*(c.tensors for c in both)):
+        if dtype == BF16:
+            assert torch.equal(a, b) if a.dtype == torch.int8 else torch.equal(a.nan_to_num(5.0), b.nan_to_num(5.0))
+        elif a.dtype == torch.int8:
+            assert (a.int() - b.int()).abs().max() <= 1
+        else:
+            assert ((a - b).abs() <= 2.0**-21 * b.abs()).logical_or(a.isnan() & b.isnan()).logical_or(a == b).all()
+    for b, n in enumerate(counts):
+        if n == 0:
+            assert not out[b].any()
+    # Rows whose pages are all there, against float64 of the step's own cache.
+    rows = [b for b in range(batch) if not page or b not in (2, 9)]
+    if page:
+        held = [t.cpu() for t in both[1].tensors]
+        whole = [torch.stack([t[ids[b]].flatten(0, 1)[:length] for b in rows]) for t in held[:2]]
+        whole += [torch.stack([t[ids[b]].transpose(0, 1).flatten(1)[:, :length] for b in rows]) for t in held[2:]]
+    else:
+        whole = [t.cpu()[rows] for t in both[1].tensors]
+    check(out[rows], queries[rows].cpu(), whole, [counts[b] for b in rows], window=window,
+          queries_off=0.0 if dtype == BF16 else 2.0**-21)
+    # Rows with a page missing: the other call's answer, both within their bounds.
+    for b in set(range(batch)) - set(rows):
+        assert (out[b].double() - want[b].double()).abs().max() <= 2.0**-6 * want[b].double().abs().max()
 
 
 def test_run_of_steps_in_a_graph_and_beside_another():
