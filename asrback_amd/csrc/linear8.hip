@@ -56,15 +56,28 @@ __device__ __forceinline__ void store_whole(T* p, const float* x) {
   }
 }
 
-// 16 inputs of a row from `at` on, zeros past k.
+// 16 inputs of a row from `at` on, zeros past k, as vectors.
 template <typename T>
-__device__ __forceinline__ void load_inputs(const T* row, int at, int k, float* x) {
+__device__ __forceinline__ void load_inputs(const T* row, int at, int k, uint4* raw) {
+  constexpr int EPL = Elem<T>::kPerVec;
   if (at + 16 <= k) {
-    load_whole<T, 16>(row + at, x);
+#pragma unroll
+    for (int v = 0; v < 16 / EPL; ++v) __builtin_memcpy(raw + v, row + at + v * EPL, 16);
   } else {
+    float x[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) x[e] = at + e < k ? Elem<T>::load1(row + at + e) : 0.f;
+#pragma unroll
+    for (int v = 0; v < 16 / EPL; ++v) raw[v] = pack<T>(x + v * EPL);
   }
+}
+template <typename T>
+__device__ __forceinline__ void load_inputs(const T* row, int at, int k, float* x) {
+  constexpr int EPL = Elem<T>::kPerVec;
+  uint4 raw[16 / EPL];
+  load_inputs(row, at, k, raw);
+#pragma unroll
+  for (int v = 0; v < 16 / EPL; ++v) unpack<T>(raw[v], x + v * EPL);
 }
 
 // ring::dma16 in a kernel where nothing else uses M0 (no LDS instruction of gfx950 does,
@@ -98,27 +111,32 @@ __device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" :
 
 // LANES lanes (a wave or the workgroup) round a row, NP pieces of 16 inputs each, which
 // they hold from the one reading for the largest magnitude; longer rows are read again.
-// Bound by a round trip to memory, and by the bytes from some thousand rows on.
+// Bound by a round trip to memory, and by the bytes from some thousand rows on.  Eight
+// rows share a line of the packed blocks, so an XCD takes neighbouring ones (12000 rows of
+// 5120 with a product to 16 outputs 57 us; dealt out one by one, each XCD writes parts of
+// every line: 81).
 template <typename T, int LANES, int NP>
 __global__ __launch_bounds__(kThreads) void round_rows_kernel(const asrlayer_linear8_params p, uint4* packed, float* scales) {
   const int lane = threadIdx.x % LANES;
-  const int64_t row = (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
+  const int64_t row = (int64_t)xcd_remap((int)blockIdx.x, (int)gridDim.x) * (kThreads / LANES) + threadIdx.x / LANES;
   if (LANES < kThreads && row >= p.rows) return;  // (uniform over a wave)
   const T* x = static_cast<const T*>(p.x) + row * p.x_row_stride;
   const int pieces = (p.k + 15) / 16, blocks = (p.k + 63) / 64;
-  float v[NP][16];
+  constexpr int EPL = Elem<T>::kPerVec, kVecs = 16 / EPL;
+  uint4 v[NP][kVecs];
   uint32_t largest = 0;
+  auto take = [&](const uint4* raw) {
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) largest = max(largest, largest_of(raw[i], T{}));
+  };
 #pragma unroll
   for (int u = 0; u < NP; ++u) load_inputs(x, (lane + u * LANES) * 16, p.k, v[u]);
 #pragma unroll
-  for (int u = 0; u < NP; ++u)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) largest = max(largest, magnitude(v[u][e]));
+  for (int u = 0; u < NP; ++u) take(v[u]);
   for (int piece = lane + NP * LANES; piece < pieces; piece += LANES) {
-    float more[16];
+    uint4 more[kVecs];
     load_inputs(x, piece * 16, p.k, more);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) largest = max(largest, magnitude(more[e]));
+    take(more);
   }
   largest = group_umax<64>(largest);
   if constexpr (LANES == kThreads) {
@@ -131,14 +149,17 @@ __global__ __launch_bounds__(kThreads) void round_rows_kernel(const asrlayer_lin
   const Scale8 s = scale8(largest);
   if (lane == 0) scales[row] = s.scale;
   uint4* out = packed + (row / 16) * blocks * 64 + row % 16;
-  auto store = [&](int piece, const float* y) {
-    if (piece < pieces)
-      out[piece * 16] = make_uint4(round8x4(y, s), round8x4(y + 4, s), round8x4(y + 8, s), round8x4(y + 12, s));
+  auto store = [&](int piece, const uint4* raw) {
+    if (piece >= pieces) return;
+    float y[16];
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) unpack<T>(raw[i], y + i * EPL);
+    out[piece * 16] = make_uint4(round8x4(y, s), round8x4(y + 4, s), round8x4(y + 8, s), round8x4(y + 12, s));
   };
 #pragma unroll
   for (int u = 0; u < NP; ++u) store(lane + u * LANES, v[u]);
   for (int piece = lane + NP * LANES; piece < pieces; piece += LANES) {
-    float more[16];
+    uint4 more[kVecs];
     load_inputs(x, piece * 16, p.k, more);
     store(piece, more);
   }

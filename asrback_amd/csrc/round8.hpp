@@ -65,21 +65,35 @@ __device__ __forceinline__ float round8_any(float x, const Scale8& s) {
 
 // Four values x / scale rounded to whole numbers, the first in the low byte.
 __device__ __forceinline__ uint32_t round8x4(const float* x, const Scale8& s) {
+  // Added to 3 2^22, a number this small is rounded to a whole one, which is the low bits.
+  constexpr float kWhole = 0x1.8p23f;
   float q[4], most = 0.f;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    q[e] = __builtin_rintf(x[e] * s.inverse);
-    most = fmaxf(most, fabsf(fmaf(-q[e], s.scale, x[e])));
+    q[e] = fmaf(x[e], s.inverse, kWhole);
+    most = fmaxf(most, fabsf(fmaf(kWhole - q[e], s.scale, x[e])));
   }
   // Some value at a border, or none found by the reciprocal.
   if (!(most < 0.5f * s.scale)) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) q[e] = round8_any(x[e], s);
+    for (int e = 0; e < 4; ++e) q[e] = round8_any(x[e], s) + kWhole;
   }
-  uint32_t r = 0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) r |= (uint32_t)((int)q[e] & 0xff) << (8 * e);
-  return r;
+  const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(q[1]), __float_as_uint(q[0]), 0x0c0c0400u);
+  const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(q[3]), __float_as_uint(q[2]), 0x0c0c0400u);
+  return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+}
+
+// The largest magnitude of a vector of elements.
+__device__ __forceinline__ uint32_t largest_of(const uint4& raw, float) {
+  auto bits = [](uint32_t x) { return x & 0x7fffffffu; };
+  return max(max(bits(raw.x), bits(raw.y)), max(bits(raw.z), bits(raw.w)));
+}
+__device__ __forceinline__ uint32_t largest_of(const uint4& raw, bf16_raw) {
+  typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+  auto bits = [](uint32_t x) { return __builtin_bit_cast(u16x2_t, x & 0x7fff7fffu); };
+  const u16x2_t a = __builtin_elementwise_max(bits(raw.x), bits(raw.y)), b = __builtin_elementwise_max(bits(raw.z), bits(raw.w)),
+                c = __builtin_elementwise_max(a, b);
+  return (uint32_t)max(c[0], c[1]) << 16;
 }
 
 }  // namespace
