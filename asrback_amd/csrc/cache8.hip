@@ -10,10 +10,10 @@
 // values of four heads, so that its scales lie next to each other in memory, a token's
 // slot and tables are looked up for four rows, and what tells queries, keys and values
 // apart is uniform, which leaves per row little but the loads, the rounding and the
-// stores.  Two prompts of 20 000 tokens, 8 heads of 128, bf16: 50 us (4.9 TB/s; a workgroup
-// per token, its rows one by one: 79), with 16 heads of queries and the norms 129 (157).
-// 8 of 430 into pages: 11.1 us, with queries 16.5; below 10 us the chain of position, page
-// and stores is most of it.  A step's few rows spread over the card, 3.9 us.  Reading back
+// stores.  Two prompts of 20 000 tokens, 8 heads of 128, bf16: 49.5 us (5.0 TB/s; a workgroup
+// per token, its rows one by one: 79), with 16 heads of queries and the norms 126 (157).
+// 8 of 430 into pages: 9.2 us, with queries 15.1, of which the chain of position, page
+// and stores is a good part.  A step's few rows spread over the card, 3.3 us.  Reading back
 // two of 20 000 of 32768: 69 us (5.1 TB/s); 8 of 430 of 1024: 9.8 us.
 #include "kernels.hpp"
 #include "layers.hpp"
@@ -110,10 +110,12 @@ __global__ __launch_bounds__(kThreads) void write8_kernel(const asrlayer_write8_
     for (int e = 0; e < EPL; ++e) largest = max(largest, magnitude(x[e]));
     const Scale8 s = scale8(group_umax<LPK>(largest));
     if (!held) continue;
+    uint32_t bytes[EPL / 4];
+    round8<T>(x, s, bytes);
     if constexpr (EPL == 8)
-      *reinterpret_cast<uint2*>(to + u * to_step) = make_uint2(round8x4(x, s), round8x4(x + 4, s));
+      *reinterpret_cast<uint2*>(to + u * to_step) = make_uint2(bytes[0], bytes[EPL / 4 - 1]);
     else
-      *reinterpret_cast<uint32_t*>(to + u * to_step) = round8x4(x, s);
+      *reinterpret_cast<uint32_t*>(to + u * to_step) = bytes[0];
     if (sub == 0) scale[u * scale_step] = s.scale;
   }
 }

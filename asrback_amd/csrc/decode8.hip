@@ -450,8 +450,7 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
         largest_q = max(largest_q, largest);
       } else if (split == splits - 1 && r <= held + 1) {
         uint32_t bytes[EPL / 4];
-#pragma unroll
-        for (int e = 0; e < EPL; e += 4) bytes[e / 4] = round8x4(x + e, s);
+        round8<T>(x, s, bytes);
         __builtin_memcpy(reinterpret_cast<char*>(sm_new) + (is_v ? HD : 0) + sub * EPL, bytes, EPL);
         if (sub == 0) sm_new_scale[is_v] = s.scale;
         if (ht == 0 && new_pos >= 0) {
@@ -584,7 +583,7 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
       f32x4_t s[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (S::kBiased && !convert)
+        if (S::kBiased && __builtin_expect(!convert, 1))
           s[h] = scores_of(h, [](uint32_t x) { return widen_biased(x ^ kBias); }, bias);
         else
           s[h] = scores_of(h, [](uint32_t x) { return widen(x); }, f32x4_t{0.f, 0.f, 0.f, 0.f});
@@ -639,7 +638,7 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
         w[part] = make_uint4(take(x[0][0], x[0][1]), take(x[0][2], x[0][3]), take(x[1][0], x[1][1]), take(x[1][2], x[1][3]));
       }
       // O^T += V^T P^T
-      if (S::kBiased && !convert) {
+      if (S::kBiased && __builtin_expect(!convert, 1)) {
         constexpr uint32_t kZeros = 0x00800080u;
 #pragma unroll
         for (int part = kWP - 1; part >= 0; --part)

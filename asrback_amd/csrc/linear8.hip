@@ -59,25 +59,35 @@ __device__ __forceinline__ void store_whole(T* p, const float* x) {
 // 16 inputs of a row from `at` on, zeros past k, as vectors.
 template <typename T>
 __device__ __forceinline__ void load_inputs(const T* row, int at, int k, uint4* raw) {
-  constexpr int EPL = Elem<T>::kPerVec;
-  if (at + 16 <= k) {
+  constexpr int EPL = Elem<T>::kPerVec, kWords = 4 * (16 / EPL);
+  if (__builtin_expect(at + 16 <= k, 1)) {
 #pragma unroll
     for (int v = 0; v < 16 / EPL; ++v) __builtin_memcpy(raw + v, row + at + v * EPL, 16);
   } else {
-    float x[16];
+    uint32_t words[kWords] = {};
+#pragma unroll 1
+    for (int e = 0; e < 16 && at + e < k; ++e) {
+      uint32_t bits = 0;
+      __builtin_memcpy(&bits, row + at + e, sizeof(T));
+      if constexpr (EPL == 8) bits <<= e % 2 * 16;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = at + e < k ? Elem<T>::load1(row + at + e) : 0.f;
+      for (int i = 0; i < kWords; ++i) words[i] |= i == e * kWords / 16 ? bits : 0;
+    }
 #pragma unroll
-    for (int v = 0; v < 16 / EPL; ++v) raw[v] = pack<T>(x + v * EPL);
+    for (int v = 0; v < 16 / EPL; ++v) raw[v] = make_uint4(words[4 * v], words[4 * v + 1], words[4 * v + 2], words[4 * v + 3]);
   }
 }
+
+// 16 inputs rounded.
 template <typename T>
-__device__ __forceinline__ void load_inputs(const T* row, int at, int k, float* x) {
+__device__ __forceinline__ uint4 round_inputs(const uint4* raw, const Scale8& s) {
   constexpr int EPL = Elem<T>::kPerVec;
-  uint4 raw[16 / EPL];
-  load_inputs(row, at, k, raw);
+  float x[16];
+  uint32_t w[4];
 #pragma unroll
   for (int v = 0; v < 16 / EPL; ++v) unpack<T>(raw[v], x + v * EPL);
+  round8<T>(x, s, w);
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // ring::dma16 in a kernel where nothing else uses M0 (no LDS instruction of gfx950 does,
@@ -113,7 +123,7 @@ __device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" :
 // they hold from the one reading for the largest magnitude; longer rows are read again.
 // Bound by a round trip to memory, and by the bytes from some thousand rows on.  Eight
 // rows share a line of the packed blocks, so an XCD takes neighbouring ones (12000 rows of
-// 5120 with a product to 16 outputs 57 us; dealt out one by one, each XCD writes parts of
+// 5120 with a product to 16 outputs 56 us; dealt out one by one, each XCD writes parts of
 // every line: 81).
 template <typename T, int LANES, int NP>
 __global__ __launch_bounds__(kThreads) void round_rows_kernel(const asrlayer_linear8_params p, uint4* packed, float* scales) {
@@ -150,11 +160,7 @@ __global__ __launch_bounds__(kThreads) void round_rows_kernel(const asrlayer_lin
   if (lane == 0) scales[row] = s.scale;
   uint4* out = packed + (row / 16) * blocks * 64 + row % 16;
   auto store = [&](int piece, const uint4* raw) {
-    if (piece >= pieces) return;
-    float y[16];
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) unpack<T>(raw[i], y + i * EPL);
-    out[piece * 16] = make_uint4(round8x4(y, s), round8x4(y + 4, s), round8x4(y + 8, s), round8x4(y + 12, s));
+    if (piece < pieces) out[piece * 16] = round_inputs<T>(raw, s);
   };
 #pragma unroll
   for (int u = 0; u < NP; ++u) store(lane + u * LANES, v[u]);
@@ -242,11 +248,11 @@ __global__ __launch_bounds__(64 * kFewWaves, 4) void linear8_few_kernel(const as
     const T* x = static_cast<const T*>(p.x);
     for (int at = threadIdx.x; at < all; at += 64 * W) {
       const int row = at / pieces, piece = at - row * pieces;
-      float v[16];
+      uint4 v[16 / Elem<T>::kPerVec];
       load_inputs(x + row * p.x_row_stride, piece * 16, p.k, v);
       uint32_t largest = 0;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) largest = max(largest, magnitude(v[e]));
+      for (int e = 0; e < 16 / Elem<T>::kPerVec; ++e) largest = max(largest, largest_of(v[e], T{}));
       // (A row's pieces are a multiple of four.)
       const bool wide = pieces % 16 == 0;
       largest = wide ? group_umax<16>(largest) : group_umax<4>(largest);
@@ -256,11 +262,9 @@ __global__ __launch_bounds__(64 * kFewWaves, 4) void linear8_few_kernel(const as
     if (threadIdx.x < 16) sm_scale[threadIdx.x] = scale8(sm_largest[threadIdx.x]).scale;
     for (int at = threadIdx.x; at < all; at += 64 * W) {
       const int row = at / pieces, piece = at - row * pieces;
-      float v[16];
+      uint4 v[16 / Elem<T>::kPerVec];
       load_inputs(x + row * p.x_row_stride, piece * 16, p.k, v);
-      const Scale8 s = scale8(sm_largest[row]);
-      *reinterpret_cast<uint4*>(lds + (piece * rows + row) * 16) =
-          make_uint4(round8x4(v, s), round8x4(v + 4, s), round8x4(v + 8, s), round8x4(v + 12, s));
+      *reinterpret_cast<uint4*>(lds + (piece * rows + row) * 16) = round_inputs<T>(v, scale8(sm_largest[row]));
     }
     __syncthreads();
     scales = sm_scale;
@@ -646,17 +650,17 @@ hipError_t launch_typed(const asrlayer_linear8_params& p, void* workspace, hipSt
   if (p.rows <= 32) return launch_few<T, 2, false>(p, packed, scales, stream);
   const auto tiles = [&](int rows, int wide) { return (p.rows + rows - 1) / rows * (((long long)outputs + wide - 1) / wide); };
   // Workgroups of 16 outputs and all inputs read the rows anew each: two a CU (128 rows
-  // of 2048 to 4096 outputs, 512 of them: 12.0 us, 14.1 in tiles of 64 x 128; 256 to
-  // 2048, 512: 11.8 and 13.9; 200 to 4096, 1024: 17.7 and 15.7).
+  // of 2048 to 4096 outputs, 512 of them: 11.8 us, 13.8 in tiles of 64 x 128; 256 to
+  // 2048, 512: 12.0 and 14.0; 200 to 4096, 1024: 16.1 and 14.0).
   if (tiles(64, 16) <= 512) return launch_few<T, 4, false>(p, packed, scales, stream);
   // Tiles of 64 x 128 while each has a CU, and a ring of eight stages, to itself (512
-  // rows of 6144 to 2048: 27.7 us, 33.6 in tiles of 128 x 128; 1024 of 2048 to 4096, two
-  // rounds: 23.9 and 21.1).
+  // rows of 6144 to 2048: 26.8 us, 32.5 in tiles of 128 x 128; 1024 of 2048 to 4096, two
+  // rounds: 24.4 and 20.8).
   const int wide = p.gated ? 64 : 128;
   if (tiles(64, wide) <= 256) return launch_large<T, 2, 4, 8>(p, packed, scales, stream);
   // Tiles of 128 x 256 from three rounds of workgroups on (1880 of them, 12000 rows of
-  // 1280 to 5120: 99.5 us, 105.1 in tiles of 128 x 128; 1584, gated 4099 of 2048 to 2 x
-  // 6144: 111.8 and 118.7; 624, 1537 rows of it: 57.7 and 51.1).
+  // 1280 to 5120: 100.8 us, 104.8 in tiles of 128 x 128; 1584, gated 4099 of 2048 to 2 x
+  // 6144: 112.7 and 118.1; 624, 1537 rows of it: 55.2 and 48.8).
   if (tiles(128, 2 * wide) >= 1536) return launch_large<T, 4, 8, 3>(p, packed, scales, stream);
   return launch_large<T, 4, 4, 4>(p, packed, scales, stream);
 }
@@ -665,8 +669,8 @@ hipError_t launch_typed(const asrlayer_linear8_params& p, void* workspace, hipSt
 
 Linear8Workspace linear8_workspace(int64_t rows, int n, int k, bool gated) {
   // Few values are rounded by every workgroup, while a CU holds all of its workgroups at
-  // once: 4 x 2048 to 2 x 6144 outputs (gated) 8.2 us, with a launch before it 10.7; 8 x
-  // 2048 10.1 and 10.2; 16 x 2048 13.0 and 9.4; 1 x 2048 to 40000 23.0 and 18.1.
+  // once: 4 x 2048 to 2 x 6144 outputs (gated) 10.9 us, with a launch before it 12.0; 8 x
+  // 2048 to 2048 6.4 and 7.6; 16 x 2048 8.4 and 7.8; 1 x 2048 to 151936 70.3 and 63.8.
   if (rows <= 16 && rows * k <= kFusedValues && (gated ? n / 2 : n) <= 512 * 16) return {0, 0};
   const size_t tiles = (size_t)(rows + 15) / 16;
   Linear8Workspace w;

@@ -56,31 +56,58 @@ __device__ __forceinline__ float round8_any(float x, const Scale8& s) {
   if (s.inverse == 0.f && !s.tiny) return 0.f;
   float q = __builtin_rintf(s.tiny ? x / s.scale : x * s.inverse);
   const float two = 2.f * fmaf(-q, s.scale, x);  // twice the remainder
-  if (fabsf(two) > s.scale)
-    q += two > 0.f ? 1.f : -1.f;
-  else if (fabsf(two) == s.scale && ((int)q & 1))
-    q += two > 0.f ? 1.f : -1.f;
+  if (fabsf(two) > s.scale || (fabsf(two) == s.scale && ((int)q & 1))) q += two > 0.f ? 1.f : -1.f;
   return fminf(fmaxf(q, -127.f), 127.f);
 }
 
-// Four values x / scale rounded to whole numbers, the first in the low byte.
-__device__ __forceinline__ uint32_t round8x4(const float* x, const Scale8& s) {
+// N values x / scale of elements T rounded to whole numbers, the first in the low byte of
+// w[0].
+//
+// A row of bf16 has values next to a border all the time (254 x / largest is odd for many
+// numbers of eight bits), so they are taken without a branch: the remainder times the
+// reciprocal is added to the whole number found first, rounded with it.  With the scale
+// S 2^k, S below 2^24, twice the remainder is a multiple of 2^k, so that it differs from the
+// scale by one S-th of it or is equal; the reciprocal is off by at most S 2^-48 of
+// itself, and S (S + 1) < 2^48, so the sum falls on the side of the border that x
+// lies on.  Equal it is only where (2 q + 1) S has as few bits as x.  With eight that
+// takes a scale of a power of two, whose reciprocal is exact, and then the even one is
+// taken (a scale that is the 127th part of a number of eight bits is that or has no such S).
+// In float32 a loop over one value at a time decides, as for tiny and non-finite rows: written
+// out for all it would be most of a kernel's instructions, which come from memory
+// anew at each launch (16 rows of 2048 and a product 7.3 us, so written 8.3).
+template <typename T, int N>
+__device__ __forceinline__ void round8(const float (&x)[N], const Scale8& s, uint32_t (&w)[N / 4]) {
   // Added to 3 2^22, a number this small is rounded to a whole one, which is the low bits.
   constexpr float kWhole = 0x1.8p23f;
-  float q[4], most = 0.f;
+  constexpr bool kShort = sizeof(T) == 2;
+  const float half = 0.5f * s.scale;
+  float q[N];
+  bool tie = false;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < N; ++e) {
     q[e] = fmaf(x[e], s.inverse, kWhole);
-    most = fmaxf(most, fabsf(fmaf(kWhole - q[e], s.scale, x[e])));
+    const float rest = fmaf(kWhole - q[e], s.scale, x[e]);
+    q[e] = fmaf(rest, s.inverse, q[e]);
+    if constexpr (!kShort) tie = tie || fabsf(rest) == half;
   }
-  // Some value at a border, or none found by the reciprocal.
-  if (!(most < 0.5f * s.scale)) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) q[e] = round8_any(x[e], s) + kWhole;
+  for (int e = 0; e < N; e += 4) {
+    const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(q[e + 1]), __float_as_uint(q[e]), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(q[e + 3]), __float_as_uint(q[e + 2]), 0x0c0c0400u);
+    w[e / 4] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
   }
-  const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(q[1]), __float_as_uint(q[0]), 0x0c0c0400u);
-  const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(q[3]), __float_as_uint(q[2]), 0x0c0c0400u);
-  return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+  if (__builtin_expect(s.scale != 0.f && (s.inverse == 0.f || tie), 0)) {
+#pragma unroll 1
+    for (int e = 0; e < N; ++e) {
+      float one = x[0];
+#pragma unroll
+      for (int i = 1; i < N; ++i) one = i == e ? x[i] : one;
+      const uint32_t byte = (uint32_t)(int)round8_any(one, s) & 0xff;
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i)
+        w[i] = i == e / 4 ? (w[i] & ~(0xffu << (e % 4 * 8))) | byte << (e % 4 * 8) : w[i];
+    }
+  }
 }
 
 // The largest magnitude of a vector of elements.

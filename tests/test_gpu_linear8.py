@@ -132,6 +132,24 @@ def test_borders_of_the_rounding(dtype, rows):
     assert torch.equal(out, ref)
 
 
+def test_every_quotient_of_bf16_numbers():
+    """Rows of each largest mantissa, of all mantissas at ten exponents: many lie within
+    2^-24 of a border, and those of the largest 254 on one."""
+    from asrback_amd.linear8 import linear8, pack8
+
+    mantissas = torch.arange(128, 256).double()
+    values = torch.cat([mantissas * 2.0**-j for j in range(1, 11)])
+    rows = torch.cat([torch.cat((m[None], values, -values)) * 2.0 ** (int(m) % 5 - 2) for m in mantissas]).view(128, -1)
+    x = rows.to(BF16)
+    assert torch.equal(x.double(), rows)
+    weight = pack8(torch.eye(x.shape[1], dtype=torch.int8).cuda(), torch.ones(x.shape[1], dtype=BF16).cuda())
+    q, scale = rounded(x)
+    for part in (x, x[:3]):  # rounded by a launch of its own and by the product
+        say("quotients", len(part))
+        out = linear8(part.cuda(), weight).cpu()
+        assert torch.equal(out, (q[: len(part)].float() * scale[: len(part)].float()).to(BF16))
+
+
 def test_layouts_of_x_out_and_other_rows():
     """Leading dimensions, strided and misaligned rows, a given out, no rows; rows do
     not touch each other, NaN and infinities included."""
