@@ -533,3 +533,117 @@ def test_run_of_steps_in_a_graph_and_beside_another():
         on_side = decode8(q, cache)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(on_side, want)
+
+
+def test_appending_steps_in_graphs():
+    """decode_append8 captured twice over one workspace, replayed while positions move past a
+    page's end, eager calls between; and on two streams at once, each with memory of its
+    own."""
+    from asrback_amd.attention import PageTable, workspace
+    from asrback_amd.cache8 import Cache8, decode_append8, decode8_workspace_size
+    from asrback_amd.qwen3_asr import rope_tables
+
+    g = torch.Generator().manual_seed(7)
+    batch, heads, kv, d, page, length = 3, 16, 8, 128, 64, 1024
+    _, tensors = random_cache(batch, length, kv, d, g)
+    first, pages, _ = paged(tensors, page, g)
+    caches = [Cache8(*(t.clone() for t in first.tensors)) for _ in range(3)]
+    buffer = torch.full((decode8_workspace_size(batch, heads, kv, d, length),), 255, dtype=torch.uint8, device="cuda")
+    q, k, v = (torch.randn(batch, n, d, generator=g).to("cuda", BF16) for n in (heads, kv, kv))
+    norm = torch.ones(d, device="cuda", dtype=BF16)
+    tables = rope_tables({"head_dim": d, "rope_theta": 1e6}, length, "cuda", BF16)
+    positions = torch.tensor([300, 509, 1021], device="cuda")
+
+    def step(cache):
+        cos, sin = (t[positions.clamp(max=length - 1)] for t in tables)
+        return decode_append8(q, k, v, cache, positions, q_norm=norm, k_norm=norm, q_eps=1e-6, k_eps=1e-6, cos=cos, sin=sin,
+                              pages=PageTable(pages.block_table, length))
+
+    def follow():
+        for t in (q, k, v):
+            t.copy_(torch.randn(t.shape, generator=g))
+        positions.add_(1)
+
+    graphs, outs = [], []
+    with torch.no_grad(), workspace(buffer):
+        for cache in caches:
+            step(cache)
+        for cache in caches[:2]:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                outs.append(step(cache))
+            graphs.append(graph)
+    for turn in range(5):  # the last row's position leaves the cache
+        follow()
+        with torch.no_grad():
+            want = step(caches[2])
+        for graph, out in zip(graphs, outs):
+            out.zero_()
+            graph.replay()
+            assert torch.equal(out, want)
+        for cache in caches[:2]:
+            for a, b in zip(cache.tensors, caches[2].tensors):
+                assert torch.equal(a.nan_to_num(5.0) if a.is_floating_point() else a,
+                                   b.nan_to_num(5.0) if a.is_floating_point() else b)
+        torch.cuda.synchronize()
+    follow()
+    streams, got = [torch.cuda.Stream() for _ in "ab"], []
+    with torch.no_grad():
+        for _ in range(3):
+            for stream, cache in zip(streams, caches):
+                stream.wait_stream(torch.cuda.current_stream())
+                with torch.cuda.stream(stream):
+                    got.append(step(cache))
+        for stream in streams:
+            torch.cuda.current_stream().wait_stream(stream)
+        want = step(caches[2])
+    assert all(torch.equal(out, want) for out in got)
+
+
+def test_most_rows_and_a_far_position():
+    """As many rows as a call takes, and a step at an offset past 2^32 bytes."""
+    from asrback_amd.cache8 import Cache8, decode8, decode_append8, write_rows8
+
+    g = torch.Generator(device="cuda").manual_seed(3)
+    batch, length, d = 65535, 16, 64
+    cache = Cache8.allocate(batch, length, 1, d, "cuda")
+    for t in cache.tensors[:2]:
+        t.random_(-127, 128, generator=g)
+    for t in cache.tensors[2:]:
+        t.uniform_(0.01, 0.02, generator=g)
+    q, k, v = (torch.randn(batch, n, d, device="cuda", generator=g).to(BF16) for n in (2, 1, 1))
+    table, norm = torch.ones(batch, d, device="cuda", dtype=BF16), torch.ones(d, device="cuda", dtype=BF16)
+    more = {"q_norm": norm, "k_norm": norm, "q_eps": 1e-6, "k_eps": 1e-6}
+    positions = torch.arange(batch, device="cuda") % length
+    say("most rows")
+    out = decode_append8(q, k, v, cache, positions, cos=table, sin=table, **more)
+    for part in (slice(0, 400), slice(batch - 400, batch)):  # over 256 rows: unsplit as well
+        held = Cache8(*(t[part].clone() for t in cache.tensors))
+        queries, _ = write_rows8(held, q[part], k[part], v[part], None, positions[part], cos=table[part], sin=table[part], **more)
+        check(out[part], queries.cpu(), [t.cpu() for t in held.tensors], (positions[part] + 1).tolist())
+        assert all(torch.equal(a, b[part]) for a, b in zip(held.tensors, cache.tensors))
+        assert torch.equal(decode8(queries, held, lengths=positions[part] + 1),
+                           decode8(queries, cache_part(cache, part), lengths=positions[part] + 1))
+    del cache
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB of free memory")
+    length, kv, d = (1 << 22) + 40, 8, 128
+    say("far position")
+    cache = Cache8.allocate(1, length, kv, d, "cuda")
+    q, k, v = (torch.randn(1, n, d, device="cuda", generator=g).to(BF16) for n in (16, kv, kv))
+    table, norm = torch.ones(1, d, device="cuda", dtype=BF16), torch.ones(d, device="cuda", dtype=BF16)
+    at = torch.tensor([length - 3], device="cuda")
+    more |= {"q_norm": norm, "k_norm": norm, "cos": table, "sin": table}
+    out = decode_append8(q, k, v, cache, at, window=40, **more)
+    tail = Cache8(*(t[:, -64:].clone() for t in cache.tensors[:2]), *(t[..., -64:].clone() for t in cache.tensors[2:]))
+    assert tail.keys[0, 61].any() and not tail.keys[0, :61].any() and not tail.keys[0, 62:].any()
+    queries, _ = write_rows8(tail, q, k, v, None, at - length + 64, **more)
+    assert all(torch.equal(a, b) for a, b in zip((tail.keys[0, 61], tail.key_scales[..., 61]),
+                                                 (cache.keys[0, -3], cache.key_scales[..., -3])))
+    check(out, queries.cpu(), [t.cpu() for t in tail.tensors], [62], window=40)
+
+
+def cache_part(cache, part):
+    from asrback_amd.cache8 import Cache8
+
+    return Cache8(*(t[part] for t in cache.tensors))

@@ -249,3 +249,21 @@ def test_module_quantization_and_graph():
             graph.replay()
             assert torch.equal(out, model(x))
             torch.cuda.synchronize()
+
+
+def test_most_rows():
+    """As many rows as a call takes, some of them checked."""
+    from asrback_amd.linear8 import gated8, linear8, pack8
+
+    g = torch.Generator().manual_seed(8)
+    rows, inputs, outputs = 65535 * 16, 64, 18
+    values, scales = matrix(outputs, inputs, BF16, g)
+    weight = pack8(values.cuda(), scales.cuda())
+    x = torch.randn(rows, inputs, device="cuda").to(BF16)
+    at = torch.tensor([0, 1, 4095, 300_007, 777_777, rows - 2, rows - 1], device="cuda")
+    say("most rows")
+    check(linear8(x, weight)[at], x[at].cpu(), values, scales, None)
+    small = x / 32
+    check(gated8(small, weight)[at], small[at].cpu(), values, scales, None, gated=True)
+    with pytest.raises(RuntimeError, match="1048560 rows"):
+        linear8(torch.zeros(rows + 1, 64, device="cuda", dtype=BF16), weight)
