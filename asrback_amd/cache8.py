@@ -71,10 +71,14 @@ class Cache8:
                 raise ValueError(f"{name} needs a unit last stride")
         if any(t.device != self.keys.device for t in self.tensors):
             raise RuntimeError("a cache's tensors must be on one device")
-        # The strides as the kernels take them (asking for them is a third of a call's time).
+        # What a call needs to know of the tensors besides their addresses (asking anew is a
+        # third of its time): sizes, the strides as the kernels take them, and whether they
+        # are inference tensors.
+        object.__setattr__(self, "_sizes", (batch, length, heads, head_dim))
         strides = (*self.keys.stride()[:3], *self.values.stride()[:3], *self.key_scales.stride()[:2],
                    *self.value_scales.stride()[:2])
         object.__setattr__(self, "_strides", strides)
+        object.__setattr__(self, "_inference", any(t.is_inference() for t in self.tensors))
 
     @property
     def tensors(self) -> tuple[Tensor, Tensor, Tensor, Tensor]:
@@ -92,7 +96,7 @@ class Cache8:
 def _cache_fields(cache: Cache8, pages: PageTable | None, batch: int, index: int) -> tuple:
     """The fields of ``asrlayer_cache8`` over ``batch`` rows, on GPU ``index``."""
     k = cache.keys
-    lead, length, heads, head_dim = k.shape
+    lead, length, heads, head_dim = cache._sizes
     if k.get_device() != index:
         _on(index, k)
     if pages is None:
@@ -178,10 +182,11 @@ def write_rows8(cache: Cache8, q: Tensor, k: Tensor, v: Tensor, rows: Tensor | N
 
 def _write(what: str, cache: Cache8, k: Tensor, v: Tensor, rows: Tensor | None, positions: Tensor,
            pages: PageTable | None, q: Tensor | None = None, prologue: tuple | None = None, keys: bool = False):
-    heads, head_dim = cache.keys.shape[2:]
-    if k.dim() != 3 or k.shape[1:] != (heads, head_dim) or v.shape != k.shape:
-        raise ValueError(f"k and v must be (tokens, {heads}, {head_dim}); got {tuple(k.shape)}, {tuple(v.shape)}")
-    tokens = k.shape[0]
+    lead, _, heads, head_dim = cache._sizes
+    shape = k.shape
+    if len(shape) != 3 or shape != (shape[0], heads, head_dim) or v.shape != shape:
+        raise ValueError(f"k and v must be (tokens, {heads}, {head_dim}); got {tuple(shape)}, {tuple(v.shape)}")
+    tokens = shape[0]
     if q is not None and (q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != head_dim):
         raise ValueError(f"q must be ({tokens}, heads, {head_dim}), got {tuple(q.shape)}")
     rows, positions = _index(rows, "rows", tokens), _index(positions, "positions", tokens)
@@ -190,10 +195,10 @@ def _write(what: str, cache: Cache8, k: Tensor, v: Tensor, rows: Tensor | None, 
     weights = () if prologue is None else (*prologue[:2], *prologue[4:])
     refuse_unseen(what, k, v, q, *weights, *cache.tensors)
     index = _ready(what, k, v, q, *weights)
-    if not torch.is_inference_mode_enabled() and any(t.is_inference() for t in cache.tensors):
+    if cache._inference and not torch.is_inference_mode_enabled():
         raise RuntimeError("inplace update to inference tensors outside InferenceMode is not allowed")
     _on(index, rows, positions)
-    batch = cache.keys.shape[0] if pages is None else pages.block_table.shape[0]
+    batch = lead if pages is None else pages.block_table.shape[0]
     if rows is None and tokens > batch:
         raise ValueError(f"{tokens} tokens without rows for a cache of {batch}")
     k, v = _aligned(k), _aligned(v)
@@ -227,7 +232,8 @@ def read8(cache: Cache8, *, lengths: Tensor | None = None, pages: PageTable | No
     there is no page."""
     if dtype not in _DTYPES:
         raise TypeError(f"read8 gives float32 and bfloat16, not {dtype}")
-    batch = cache.keys.shape[0] if pages is None else pages.block_table.shape[0]
+    lead, _, heads, head_dim = cache._sizes
+    batch = lead if pages is None else pages.block_table.shape[0]
     lengths = _lengths(lengths, batch)
     refuse_unseen("read8", *cache.tensors)
     index = cache.keys.get_device()
@@ -237,8 +243,7 @@ def read8(cache: Cache8, *, lengths: Tensor | None = None, pages: PageTable | No
         _check_device(cache.keys)
     _on(index, lengths)
     fields = _cache_fields(cache, pages, batch, index)
-    shape = (batch, fields[-1], *cache.keys.shape[2:])
-    k_out = torch.empty(shape, dtype=dtype, device=cache.keys.device)
+    k_out = torch.empty((batch, fields[-1], heads, head_dim), dtype=dtype, device=cache.keys.device)
     v_out = torch.empty_like(k_out)
     params = _lib.pack_read8(*fields, k_out.data_ptr(), v_out.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
                              lengths is not None and lengths.dtype is torch.int64, _DTYPES[dtype])
@@ -318,7 +323,7 @@ def _decode(what: str, q: Tensor, cache: Cache8, lengths: Tensor | None, scale: 
             workspace: Tensor | None, pages: PageTable | None, window: int | None, new: tuple = (),
             positions: Tensor | None = None, q_eps: float = 0.0, k_eps: float = 0.0) -> Tensor:
     shape = q.shape
-    heads_kv, head_dim = cache.keys.shape[2:]
+    _, _, heads_kv, head_dim = cache._sizes
     if len(shape) != 3 or shape[2] != head_dim:
         raise ValueError(f"q must be (batch, heads, {head_dim}), got {tuple(shape)}")
     batch, heads_q, _ = shape
@@ -356,7 +361,7 @@ def _decode(what: str, q: Tensor, cache: Cache8, lengths: Tensor | None, scale: 
     if not new:
         status = lib.asrlayer_decode8(_lib.pack_decode8(*step), workspace, size, _raw_stream(index))
     else:
-        if not torch.is_inference_mode_enabled() and any(t.is_inference() for t in cache.tensors):
+        if cache._inference and not torch.is_inference_mode_enabled():
             raise RuntimeError("inplace update to inference tensors outside InferenceMode is not allowed")
         k, v = _aligned(new[0]), _aligned(new[1])
         q_norm, k_norm, cos, sin = (_aligned(t if t.is_contiguous() else t.contiguous()) for t in new[2:])
