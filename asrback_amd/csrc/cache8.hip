@@ -17,7 +17,7 @@
 // two of 20 000 of 32768: 69 us (5.1 TB/s); 8 of 430 of 1024: 9.8 us.
 #include "kernels.hpp"
 #include "layers.hpp"
-#include "round8.hpp"
+#include "quantize8.hpp"
 #include "row_ops.hpp"
 
 namespace asrattn {
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(kThreads) void write8_kernel(const asrlayer_write8_
     const Scale8 s = scale8(group_umax<LPK>(largest));
     if (!held) continue;
     uint32_t bytes[EPL / 4];
-    round8<T>(x, s, bytes);
+    bytes_of<T>(x, s, bytes);
     if constexpr (EPL == 8)
       *reinterpret_cast<uint2*>(to + u * to_step) = make_uint2(bytes[0], bytes[EPL / 4 - 1]);
     else

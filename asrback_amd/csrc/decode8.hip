@@ -42,7 +42,7 @@
 // arrival, fold.
 #include "common.hpp"
 #include "kernels.hpp"
-#include "round8.hpp"
+#include "quantize8.hpp"
 #include "row_ops.hpp"
 
 namespace asrattn {
@@ -450,7 +450,7 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
         largest_q = max(largest_q, largest);
       } else if (split == splits - 1 && r <= held + 1) {
         uint32_t bytes[EPL / 4];
-        round8<T>(x, s, bytes);
+        bytes_of<T>(x, s, bytes);
         __builtin_memcpy(reinterpret_cast<char*>(sm_new) + (is_v ? HD : 0) + sub * EPL, bytes, EPL);
         if (sub == 0) sm_new_scale[is_v] = s.scale;
         if (ht == 0 && new_pos >= 0) {

@@ -10,14 +10,14 @@
 //
 // Three ways, by the rows: few rows by workgroups of 16 outputs that read the weights to
 // registers, more by tiles through LDS, of which several sizes (launch_typed says which
-// and why).  One row of 2048 to 2048 outputs takes 4.9 us, of which the launch and
-// two round trips to memory are most; 4099 rows of 2048 to 2 x 6144, gated, 112 us: 206 G
-// operations at 1.85 P/s.  There the matrix cores are busy for half of the time, at a
+// and why).  One row of 2048 to 2048 outputs takes 4.4 us, of which the launch and
+// two round trips to memory are most; 4099 rows of 2048 to 2 x 6144, gated, 111 us: 206 G
+// operations at 1.86 P/s.  There the matrix cores are busy for 60% of the time, at a
 // clock that their power holds near 1.7 GHz (a single workgroup runs at 2.3).
 #include "kernels.hpp"
 #include "layers.hpp"
 #include "ring_common.hpp"
-#include "round8.hpp"
+#include "quantize8.hpp"
 #include "row_ops.hpp"
 
 namespace asrattn {
@@ -86,7 +86,7 @@ __device__ __forceinline__ uint4 round_inputs(const uint4* raw, const Scale8& s)
   uint32_t w[4];
 #pragma unroll
   for (int v = 0; v < 16 / EPL; ++v) unpack<T>(raw[v], x + v * EPL);
-  round8<T>(x, s, w);
+  bytes_of<T>(x, s, w);
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 

@@ -52,7 +52,7 @@ __device__ __forceinline__ Scale8 scale8(uint32_t largest) {
 }
 
 // x / scale rounded to a whole number, for any scale.
-__device__ __forceinline__ float round8_any(float x, const Scale8& s) {
+__device__ __forceinline__ float whole_of(float x, const Scale8& s) {
   if (s.inverse == 0.f && !s.tiny) return 0.f;
   float q = __builtin_rintf(s.tiny ? x / s.scale : x * s.inverse);
   const float two = 2.f * fmaf(-q, s.scale, x);  // twice the remainder
@@ -76,7 +76,7 @@ __device__ __forceinline__ float round8_any(float x, const Scale8& s) {
 // out for all it would be most of a kernel's instructions, which come from memory
 // anew at each launch (16 rows of 2048 and a product 7.3 us, so written 8.3).
 template <typename T, int N>
-__device__ __forceinline__ void round8(const float (&x)[N], const Scale8& s, uint32_t (&w)[N / 4]) {
+__device__ __forceinline__ void bytes_of(const float (&x)[N], const Scale8& s, uint32_t (&w)[N / 4]) {
   // Added to 3 2^22, a number this small is rounded to a whole one, which is the low bits.
   constexpr float kWhole = 0x1.8p23f;
   constexpr bool kShort = sizeof(T) == 2;
@@ -102,7 +102,7 @@ __device__ __forceinline__ void round8(const float (&x)[N], const Scale8& s, uin
       float one = x[0];
 #pragma unroll
       for (int i = 1; i < N; ++i) one = i == e ? x[i] : one;
-      const uint32_t byte = (uint32_t)(int)round8_any(one, s) & 0xff;
+      const uint32_t byte = (uint32_t)(int)whole_of(one, s) & 0xff;
 #pragma unroll
       for (int i = 0; i < N / 4; ++i)
         w[i] = i == e / 4 ? (w[i] & ~(0xffu << (e % 4 * 8))) | byte << (e % 4 * 8) : w[i];
