@@ -35,7 +35,7 @@ __device__ __forceinline__ i32x4_t lds_read(uint32_t addr) { return *(lds_i32x4_
 constexpr int kThreads = 256;
 
 // N consecutive elements at any address of them: global memory takes vectors there
-// (2791 rows of 320 inputs to 21497 bf16 outputs 85 us, stored one by one 219; to 21504 50).
+// (2791 rows of 320 inputs to 21497 bf16 outputs 77 us, stored one by one 219; to 21504 49).
 template <typename T, int N>
 __device__ __forceinline__ void load_whole(const T* p, float* x) {
   constexpr int EPL = Elem<T>::kPerVec;
@@ -558,6 +558,8 @@ __global__ __launch_bounds__(256, (LargeShape<NA, NJ, S>::kPerCu)) void linear8_
     for (int ca = 0; ca < NA * NJ / 4; ++ca) {
       const int n = n_at + (GATED ? 32 : 64) * (ca / NA);
       const int64_t row = row_at + 16 * (ca % NA);
+      const bool left = row < p.rows && n < outputs && !(near && n + N <= outputs);
+      if (!__any(left)) continue;
       int sums[16];
       switch (ca) {
 #define ASR_SUMS(at)                                                                                            \
@@ -585,7 +587,7 @@ __global__ __launch_bounds__(256, (LargeShape<NA, NJ, S>::kPerCu)) void linear8_
       T* out = static_cast<T*>(p.out) + row * p.out_row_stride + n;
 #pragma unroll
       for (int e = 0; e < N; ++e)
-        if (row < p.rows && n + e < outputs && !(near && n + N <= outputs)) Elem<T>::store1(out + e, y[e]);
+        if (left && n + e < outputs) Elem<T>::store1(out + e, y[e]);
     }
   }
   wait_vmcnt<0>();  // the surplus DMAs, before the workgroup's LDS is another's
@@ -658,10 +660,13 @@ hipError_t launch_typed(const asrlayer_linear8_params& p, void* workspace, hipSt
   // rounds: 24.4 and 20.8).
   const int wide = p.gated ? 64 : 128;
   if (tiles(64, wide) <= 256) return launch_large<T, 2, 4, 8>(p, packed, scales, stream);
-  // Tiles of 128 x 256 from three rounds of workgroups on (1880 of them, 12000 rows of
-  // 1280 to 5120: 100.8 us, 104.8 in tiles of 128 x 128; 1584, gated 4099 of 2048 to 2 x
-  // 6144: 112.7 and 118.1; 624, 1537 rows of it: 55.2 and 48.8).
-  if (tiles(128, 2 * wide) >= 1536) return launch_large<T, 4, 8, 3>(p, packed, scales, stream);
+  // Tiles of 128 x 256 where the last round of the 512 workgroups that the card holds is
+  // nearly full, or two full ones go before (3440 rows of 2048 to 4096, 432 of them: 39.9
+  // us, 42.9 in tiles of 128 x 128; 7300, 928: 72.1 and 79.4; 9600, 1200: 93.0 and 99.0;
+  // 4099 of 2048 to 2 x 6144, gated, 1584: 112.7 and 118.1; but 6800 to 4096, 864: 70.5 and
+  // 70.1; 3291 of 6397 to 3149, 338: 119.6 and 106.5; 1537 gated, 624: 55.2 and 48.8).
+  const long long big = tiles(128, 2 * wide);
+  if (big >= 1200 || (big - 1) % 512 >= 399) return launch_large<T, 4, 8, 3>(p, packed, scales, stream);
   return launch_large<T, 4, 4, 4>(p, packed, scales, stream);
 }
 

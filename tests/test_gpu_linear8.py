@@ -67,6 +67,7 @@ SHAPES = [
     (130, 1152, 514), (200, 64, 1000), (255, 512, 256), (256, 1024, 1026), (257, 130, 700), (300, 2048, 96), (513, 1280, 258),
     (1, 20000, 50), (4, 2048, 30001), (1000, 512, 1536), (1537, 2048, 514), (2100, 100, 260), (40, 100001, 18),
     (12, 2049, 4096), (9, 4096, 2050), (129, 4096, 4100), (700, 1280, 5120), (1300, 193, 5007), (2600, 77, 9001),
+    (3300, 100, 4096), (3231, 67, 4111),
 ]
 
 
