@@ -11,8 +11,8 @@
 // Three ways, by the rows: few rows by workgroups of 16 outputs that read the weights to
 // registers, more by tiles through LDS, of which several sizes (launch_typed says which
 // and why).  One row of 2048 to 2048 outputs takes 4.4 us, of which the launch and
-// two round trips to memory are most; 4099 rows of 2048 to 2 x 6144, gated, 111 us: 206 G
-// operations at 1.86 P/s.  There the matrix cores are busy for 60% of the time, at a
+// two round trips to memory are most; 4099 rows of 2048 to 2 x 6144, gated, 109 us: 206 G
+// operations at 1.90 P/s.  There the matrix cores are busy for 60% of the time, at a
 // clock that their power holds near 1.7 GHz (a single workgroup runs at 2.3).
 #include "kernels.hpp"
 #include "layers.hpp"
