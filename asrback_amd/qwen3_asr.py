@@ -47,8 +47,8 @@ from torch import Tensor, nn
 
 from . import attention
 from .attention import KeyPrefix, PageTable, decode, decode_append, greedy_choice, varlen_attn
-from .drafts import MAX_TOKENS, accept_drafts, commit_drafts, tree_attention, tree_masks, tree_workspace_size
 from .cache8 import Cache8, decode8, decode8_workspace_size, decode_append8, read8, write8, write_rows8
+from .drafts import MAX_TOKENS, accept_drafts, commit_drafts, tree_attention, tree_masks, tree_workspace_size
 from .layers import computes, prompt_rows, prompt_rows_takes, unhooked
 from .linear4 import Linear4
 from .linear8 import Linear8
