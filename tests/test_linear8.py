@@ -2,8 +2,6 @@
 
 from __future__ import annotations
 
-import ctypes
-
 import pytest
 import torch
 from torch.autograd import forward_ad
