@@ -24,7 +24,7 @@ from torch import Tensor
 from . import _lib
 from .attention import _DTYPES, PageTable, _aligned, _check_device, _split_workspace
 from .drafts import _lengths, _on
-from .layers import _increment_version, check_out, refuse_unseen
+from .layers import _increment_version, check_out, refuse_gradient, refuse_unseen
 
 HEAD_DIMS = (64, 128, 256)
 # The current stream's handle on a device; the current device (once a tensor is on one).
@@ -194,6 +194,7 @@ def _write(what: str, cache: Cache8, k: Tensor, v: Tensor, rows: Tensor | None, 
         raise TypeError("positions must be a tensor")
     weights = () if prologue is None else (*prologue[:2], *prologue[4:])
     refuse_unseen(what, k, v, q, *weights, *cache.tensors)
+    refuse_gradient(what, cache.key_scales, cache.value_scales)
     index = _ready(what, k, v, q, *weights)
     if cache._inference and not torch.is_inference_mode_enabled():
         raise RuntimeError("inplace update to inference tensors outside InferenceMode is not allowed")
@@ -236,6 +237,7 @@ def read8(cache: Cache8, *, lengths: Tensor | None = None, pages: PageTable | No
     batch = lead if pages is None else pages.block_table.shape[0]
     lengths = _lengths(lengths, batch)
     refuse_unseen("read8", *cache.tensors)
+    refuse_gradient("read8", cache.key_scales, cache.value_scales)
     index = cache.keys.get_device()
     if index < 0:
         raise RuntimeError(f"read8 runs on the GPU only; got tensors on {cache.keys.device}")
@@ -333,6 +335,7 @@ def _decode(what: str, q: Tensor, cache: Cache8, lengths: Tensor | None, scale: 
         raise ValueError(f"a window holds at least one position, got {window}")
     lengths = _lengths(lengths, batch)
     refuse_unseen(what, q, *new, *cache.tensors)
+    refuse_gradient(what, cache.key_scales, cache.value_scales)
     given = out is not None
     if given:
         if out.shape != shape or out.dtype != q.dtype or out.stride(-1) != 1:

@@ -73,6 +73,14 @@ def refuse_unseen(what: str, *tensors: Tensor | None) -> None:
             raise RuntimeError(f"{what} has no gradient, in forward mode neither; call it on primal tensors")
 
 
+def refuse_gradient(what: str, *tensors: Tensor | None) -> None:
+    """Raise where autograd would follow ``what``, which has no gradient, to one of these."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no gradient; call it under torch.no_grad() or on detached tensors")
+
+
 def overlap(a: Tensor, b: Tensor) -> bool:
     """Whether two tensors may share memory: the ranges from their first to their last
     elements meet, and they are not different parts of the same rows (a stride of ``a``

@@ -26,7 +26,7 @@ from torch import Tensor, nn
 
 from . import _lib
 from .attention import _DTYPES, _check_device
-from .layers import _increment_version, check_out, computes, refuse_unseen
+from .layers import _increment_version, check_out, computes, refuse_gradient, refuse_unseen
 from .linear4 import _as_built
 
 _BLOCK_N, _BLOCK_K = 16, 64
@@ -155,6 +155,7 @@ def _product(what: str, x: Tensor, packed: Tensor, scales: Tensor, outputs: int,
     if bias is not None and (bias.shape != (outputs,) or bias.dtype is not dtype):
         raise ValueError(f"bias must be {dtype} ({outputs},), got {bias.dtype} {tuple(bias.shape)}")
     refuse_unseen(what, x, scales, bias)
+    refuse_gradient(what, scales)
     width = outputs // 2 if gated else outputs
     given = out is not None
     if given:
@@ -163,8 +164,7 @@ def _product(what: str, x: Tensor, packed: Tensor, scales: Tensor, outputs: int,
         check_out(what, out, x, bias, packed, scales)
     if index < 0:
         raise RuntimeError(f"{what} runs on the GPU only; got a tensor on {x.device}")
-    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
-        raise RuntimeError(f"{what} has no gradient; call it under torch.no_grad() or on detached tensors")
+    refuse_gradient(what, x, bias)
     if (index != _current_device() or packed.get_device() != index or scales.get_device() != index
             or (bias is not None and bias.get_device() != index) or (given and out.get_device() != index)):
         _check_device(x, packed, scales, bias, out)  # says what is wrong

@@ -150,6 +150,30 @@ def test_linear8_unseen():
                 make_fx(lambda t: call(t))(t)
 
 
+def test_scales_that_require_a_gradient():
+    """No op drops the gradient of a cache's scales, or writes over such a leaf."""
+    from asrback_amd.cache8 import Cache8, decode8, decode_append8, read8, write8, write_rows8
+
+    k, q, positions = torch.zeros(2, 3, 64), torch.zeros(2, 6, 64), torch.zeros(2, dtype=torch.int64)
+    norm, table = torch.zeros(64), torch.zeros(2, 64)
+    more = {"q_norm": norm, "k_norm": norm, "q_eps": 1e-6, "k_eps": 1e-6, "cos": table, "sin": table}
+    for field in ("key_scales", "value_scales"):
+        cache = Cache8.allocate(2, 8, 3, 64)
+        getattr(cache, field).requires_grad_()
+        for name, call in (("write8", lambda: write8(cache, k, k, None, positions)), ("read8", lambda: read8(cache)),
+                           ("write_rows8", lambda: write_rows8(cache, q, k, k, None, positions, **more)),
+                           ("decode8", lambda: decode8(q, cache)),
+                           ("decode_append8", lambda: decode_append8(q, k, k, cache, positions, **more))):
+            with pytest.raises(RuntimeError, match=f"{name} has no gradient"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="GPU only"):
+                call()
+    # One that takes part in a graph without being a leaf.
+    cache = Cache8(cache.keys, cache.values, torch.zeros(2, 3, 8, requires_grad=True) * 2, torch.zeros(2, 3, 8))
+    with pytest.raises(RuntimeError, match="decode8 has no gradient"):
+        decode8(q, cache)
+
+
 @pytest.mark.filterwarnings("ignore::DeprecationWarning")
 def test_refusals():
     from asrback_amd.cache8 import Cache8, decode8, decode8_workspace_size, decode_append8, read8, write8, write_rows8

@@ -138,6 +138,21 @@ def test_refusals():
     assert lib.asrlayer_linear8(bytes(p), 0, 0, None) == _lib.OK
 
 
+def test_scales_that_require_a_gradient():
+    from asrback_amd.linear8 import Linear8, Weight8, gated8, linear8, pack8
+
+    held = pack8(torch.zeros(8, 64, dtype=torch.int8), torch.ones(8))
+    weight = Weight8(held.packed, held.scales.clone().requires_grad_(), 8, 64)
+    layer, x = Linear8(held), torch.zeros(3, 64)
+    layer.scales = weight.scales
+    for name, call in (("linear8", lambda: linear8(x, weight)), ("gated8", lambda: gated8(x, weight)),
+                       ("linear8", lambda: layer(x)), ("gated8", lambda: layer.gated(x))):
+        with pytest.raises(RuntimeError, match=f"{name} has no gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="GPU only"):
+            call()
+
+
 @pytest.mark.filterwarnings("ignore::DeprecationWarning")
 @pytest.mark.parametrize("gated", [False, True])
 def test_out(gated):
