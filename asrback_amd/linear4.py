@@ -22,7 +22,7 @@ from torch import Tensor, nn
 
 from . import _lib
 from .attention import _DTYPES, _aligned, _check_device
-from .layers import _FORWARDS, _increment_version, check_out, refuse_unseen
+from .layers import _FORWARDS, _increment_version, check_out, refuse_gradient, refuse_unseen
 
 GROUPS = (32, 64, 128)
 _BLOCK_N, _BLOCK_K = 16, 128
@@ -192,6 +192,7 @@ def _product(x: Tensor, packed: Tensor, scales: Tensor, zeros: Tensor | None, ou
     if bias is not None and (bias.shape != (outputs,) or bias.dtype is not dtype):
         raise ValueError(f"bias must be {dtype} ({outputs},), got {bias.dtype} {tuple(bias.shape)}")
     refuse_unseen("linear4", x, scales, bias)
+    refuse_gradient("linear4", scales)
     given = out is not None
     if given:
         if out.shape != (*shape[:-1], outputs) or out.dtype is not dtype or not out.is_contiguous():
@@ -199,8 +200,7 @@ def _product(x: Tensor, packed: Tensor, scales: Tensor, zeros: Tensor | None, ou
         check_out("linear4", out, x, bias)
     if index < 0:
         raise RuntimeError(f"linear4 runs on the GPU only; got a tensor on {x.device}")
-    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
-        raise RuntimeError("linear4 has no gradient; call it under torch.no_grad() or on detached tensors")
+    refuse_gradient("linear4", x, bias)
     if not given:
         out = x.new_empty((*shape[:-1], outputs))
     rows = _aligned(x if len(shape) == 2 else x.reshape(-1, inputs))

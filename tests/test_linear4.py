@@ -137,6 +137,20 @@ def test_refusals():
     assert lib.asrlayer_linear4(ctypes.byref(p), None) == _lib.OK
 
 
+def test_scales_that_require_a_gradient():
+    from asrback_amd.linear4 import Linear4, Weight4, linear4, pack4
+
+    held = pack4(torch.zeros(8, 64, dtype=torch.uint8), torch.ones(8, 2))
+    weight = Weight4(held.packed, held.scales.clone().requires_grad_(), None, 8, 64, 32)
+    layer, x = Linear4(held), torch.zeros(3, 64)
+    layer.scales = weight.scales
+    for call in (lambda: linear4(x, weight), lambda: layer(x)):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="GPU only"):
+            call()
+
+
 def test_quantize_linears_replaces_every_name():
     """A layer under two names of one parent, and under another parent, is rounded once
     and stays shared."""
