@@ -41,7 +41,9 @@ class Cache8:
     whole 16-byte vectors with a unit last one; the scales float32 ``(batch, heads_kv,
     length)`` with a unit last stride.  With a :class:`~asrback_amd.attention.PageTable`
     at a call they are pools, ``(num_pages, page_size, heads_kv, head_dim)`` and
-    ``(num_pages, heads_kv, page_size)``."""
+    ``(num_pages, heads_kv, page_size)``.  As a view of them would, it keeps the memory
+    and the layout that they have when it is made: a tensor that is resized or set to
+    another memory afterwards does not change it."""
 
     keys: Tensor
     values: Tensor
@@ -71,7 +73,10 @@ class Cache8:
                 raise ValueError(f"{name} needs a unit last stride")
         if any(t.device != self.keys.device for t in self.tensors):
             raise RuntimeError("a cache's tensors must be on one device")
-        # What a call needs to know of the tensors besides their addresses (asking anew is a
+        # What the kernels read and write: views of the cache's own, which nothing done to the
+        # tensors given can resize.
+        object.__setattr__(self, "_held", tuple(t.view(t.shape) for t in self.tensors))
+        # What a call needs to know of them besides their addresses (asking anew is a
         # third of its time): sizes, the strides as the kernels take them, and whether they
         # are inference tensors.
         object.__setattr__(self, "_sizes", (batch, length, heads, head_dim))
@@ -79,6 +84,9 @@ class Cache8:
                    *self.value_scales.stride()[:2])
         object.__setattr__(self, "_strides", strides)
         object.__setattr__(self, "_inference", any(t.is_inference() for t in self.tensors))
+
+    def __reduce__(self):
+        return Cache8, self.tensors  # (a copy holds views of its own)
 
     @property
     def tensors(self) -> tuple[Tensor, Tensor, Tensor, Tensor]:
@@ -95,7 +103,7 @@ class Cache8:
 
 def _cache_fields(cache: Cache8, pages: PageTable | None, batch: int, index: int) -> tuple:
     """The fields of ``asrlayer_cache8`` over ``batch`` rows, on GPU ``index``."""
-    k = cache.keys
+    k, v, key_scales, value_scales = cache._held
     lead, length, heads, head_dim = cache._sizes
     if k.get_device() != index:
         _on(index, k)
@@ -115,8 +123,8 @@ def _cache_fields(cache: Cache8, pages: PageTable | None, batch: int, index: int
             raise ValueError(f"max_len {length} outside the table's reach {reach}")
         # (a table that reaches nothing is no table)
         paged = (table.data_ptr(), table.stride(0), page_size, lead) if length else (0, 0, 0, 0)
-    return (k.data_ptr(), cache.values.data_ptr(), cache.key_scales.data_ptr(), cache.value_scales.data_ptr(),
-            *cache._strides, *paged, batch, heads, head_dim, length)
+    return (k.data_ptr(), v.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), *cache._strides, *paged, batch, heads,
+            head_dim, length)
 
 
 def _ready(what: str, first: Tensor, *others: Tensor | None) -> int:
@@ -221,7 +229,7 @@ def _write(what: str, cache: Cache8, k: Tensor, v: Tensor, rows: Tensor | None, 
     status = _lib.load().asrlayer_write8(params, _raw_stream(index))
     if status:
         _lib.check(status, "asrlayer_write8")
-    _increment_version(cache.tensors)
+    _increment_version(cache._held)
     return q_out, k_out
 
 
@@ -238,14 +246,15 @@ def read8(cache: Cache8, *, lengths: Tensor | None = None, pages: PageTable | No
     lengths = _lengths(lengths, batch)
     refuse_unseen("read8", *cache.tensors)
     refuse_gradient("read8", cache.key_scales, cache.value_scales)
-    index = cache.keys.get_device()
+    keys = cache._held[0]
+    index = keys.get_device()
     if index < 0:
-        raise RuntimeError(f"read8 runs on the GPU only; got tensors on {cache.keys.device}")
+        raise RuntimeError(f"read8 runs on the GPU only; got tensors on {keys.device}")
     if index != _current_device():
-        _check_device(cache.keys)
+        _check_device(keys)
     _on(index, lengths)
     fields = _cache_fields(cache, pages, batch, index)
-    k_out = torch.empty((batch, fields[-1], heads, head_dim), dtype=dtype, device=cache.keys.device)
+    k_out = torch.empty((batch, fields[-1], heads, head_dim), dtype=dtype, device=keys.device)
     v_out = torch.empty_like(k_out)
     params = _lib.pack_read8(*fields, k_out.data_ptr(), v_out.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
                              lengths is not None and lengths.dtype is torch.int64, _DTYPES[dtype])
@@ -306,7 +315,7 @@ def decode_append8(q: Tensor, k: Tensor, v: Tensor, cache: Cache8, positions: Te
     positions[b]`` (the whole cache where that is past its end, without the new key,
     which is dropped there as it is where there is no page; none below 0).  Returns
     ``(batch, heads_q, head_dim)``."""
-    batch, heads, head_dim = q.shape[0], *cache.keys.shape[2:]
+    batch, heads, head_dim = q.shape[0], *cache._sizes[2:]
     for name, t in (("k", k), ("v", v)):
         if t.shape != (batch, heads, head_dim):
             raise ValueError(f"{name} must be ({batch}, {heads}, {head_dim}), got {tuple(t.shape)}")
@@ -342,7 +351,7 @@ def _decode(what: str, q: Tensor, cache: Cache8, lengths: Tensor | None, scale: 
             raise ValueError("out must match q's shape and dtype, with a unit last stride")
         # A row's queries are read before any of its outputs is written.
         in_place = out.data_ptr() == q.data_ptr() and out.stride() == q.stride()
-        check_out(what, out, None if in_place else q, *new, *cache.tensors, lengths, positions)
+        check_out(what, out, None if in_place else q, *new, *cache._held, lengths, positions)
     index = _ready(what, q, *new)
     q = _aligned(q)
     _on(index, lengths, out, positions)
@@ -375,7 +384,7 @@ def _decode(what: str, q: Tensor, cache: Cache8, lengths: Tensor | None, scale: 
     if status:
         _lib.check(status, "asrlayer_append8" if new else "asrlayer_decode8")
     if new:
-        _increment_version(cache.tensors)
+        _increment_version(cache._held)
     if given:
         _increment_version(out)
     return out

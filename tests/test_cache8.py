@@ -69,6 +69,38 @@ def test_caches():
             Cache8(*bad)
 
 
+def test_tensors_that_change_after_a_cache_is_made():
+    """A cache keeps the memory and the layout that its tensors had, so that no call reads past
+    what a resized or re-set one has; a copy has its own."""
+    import copy
+    import pickle
+
+    from asrback_amd.cache8 import Cache8, _cache_fields
+
+    def small(i, dtype):
+        return torch.zeros((1, 1, 3, 64) if i < 2 else (1, 3, 1), dtype=dtype)
+
+    for i in range(4):
+        for change in (lambda t: t.set_(small(i, t.dtype)), lambda t: setattr(t, "data", small(i, t.dtype)),
+                       lambda t: t.resize_(small(i, t.dtype).shape), lambda t: t.resize_(16, *t.shape[1:]),
+                       lambda t: t.transpose_(0, 1), lambda t: setattr(t, "data", t.data.double())):
+            tensors = Cache8.allocate(2, 8, 3, 64).tensors
+            cache, other = Cache8(*tensors), Cache8(*tensors)
+            before = _cache_fields(cache, None, 2, -1)
+            change(tensors[i])
+            after, sizes = _cache_fields(cache, None, 2, -1), [t.untyped_storage().nbytes() for t in other._held]
+            # (A storage that grows may move.)
+            assert after[:4] == tuple(t.data_ptr() for t in other._held) and after[4:] == before[4:]
+            assert all(n >= need for n, need in zip(sizes, (2 * 8 * 3 * 64, 2 * 8 * 3 * 64, 2 * 8 * 3 * 4, 2 * 8 * 3 * 4)))
+    cache = Cache8.allocate(2, 8, 3, 64)
+    for twin in (copy.deepcopy(cache), pickle.loads(pickle.dumps(cache))):
+        assert all(a.data_ptr() == b.data_ptr() != c.data_ptr() for a, b, c in zip(twin._held, twin.tensors, cache.tensors))
+    assert copy.copy(cache).keys is cache.keys
+    for t in cache.tensors:
+        t += 1
+    assert all((t == 1).all() for t in cache._held)
+
+
 def calls():
     """Name, call of one float tensor, that tensor."""
     from asrback_amd.cache8 import Cache8, decode8, decode_append8, read8, write8, write_rows8
