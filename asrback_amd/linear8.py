@@ -41,7 +41,8 @@ _current_device = torch._C._cuda_getDevice
 class Weight8:
     """A matrix ``(outputs, inputs)`` of 8-bit values with a scale per output, in
     the kernel's layout (``asrlayer_linear8_params``).  Made by :func:`pack8` or
-    :func:`quantize8`."""
+    :func:`quantize8`.  As a view of them would, it keeps the memory and the layout that
+    its tensors have when it is made."""
 
     packed: Tensor
     scales: Tensor
@@ -50,6 +51,12 @@ class Weight8:
 
     def __post_init__(self) -> None:
         _check_layout(self.packed, self.scales, self.outputs, self.inputs)
+        # What the kernel reads: views of its own, which nothing done to the tensors given
+        # can resize.
+        object.__setattr__(self, "_held", (self.packed.view(self.packed.shape), self.scales.view(self.scales.shape)))
+
+    def __reduce__(self):
+        return Weight8, (self.packed, self.scales, self.outputs, self.inputs)  # (a copy holds views of its own)
 
 
 def _check_layout(packed: Tensor, scales: Tensor, outputs: int, inputs: int) -> None:
@@ -124,7 +131,8 @@ def linear8(x: Tensor, weight: Weight8, bias: Tensor | None = None, *, out: Tens
     products is exact, what follows float32, rounded once.  A row with an infinity or
     a NaN comes out as NaN.  ``out`` is written in place and must not share
     memory with ``x`` or ``bias``.  Returns ``(..., outputs)``."""
-    return _product("linear8", x, weight.packed, weight.scales, weight.outputs, weight.inputs, bias, out, False)
+    refuse_gradient("linear8", weight.scales)
+    return _product("linear8", x, *weight._held, weight.outputs, weight.inputs, bias, out, False)
 
 
 def gated8(x: Tensor, weight: Weight8, bias: Tensor | None = None, *, out: Tensor | None = None) -> Tensor:
@@ -134,7 +142,8 @@ def gated8(x: Tensor, weight: Weight8, bias: Tensor | None = None, *, out: Tenso
     for :func:`linear8`.  Returns ``(..., n)``."""
     if weight.outputs % 2:
         raise ValueError(f"a gated matrix has as many gates as projections, got {weight.outputs} outputs")
-    return _product("gated8", x, weight.packed, weight.scales, weight.outputs, weight.inputs, bias, out, True)
+    refuse_gradient("gated8", weight.scales)
+    return _product("gated8", x, *weight._held, weight.outputs, weight.inputs, bias, out, True)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -155,7 +164,6 @@ def _product(what: str, x: Tensor, packed: Tensor, scales: Tensor, outputs: int,
     if bias is not None and (bias.shape != (outputs,) or bias.dtype is not dtype):
         raise ValueError(f"bias must be {dtype} ({outputs},), got {bias.dtype} {tuple(bias.shape)}")
     refuse_unseen(what, x, scales, bias)
-    refuse_gradient(what, scales)
     width = outputs // 2 if gated else outputs
     given = out is not None
     if given:
@@ -214,6 +222,7 @@ class Linear8(nn.Module):
 
     def forward(self, x: Tensor) -> Tensor:
         _check_layout(self.packed, self.scales, self.out_features, self.in_features)
+        refuse_gradient("linear8", self.scales)
         return _product("linear8", x, self.packed, self.scales, self.out_features, self.in_features, self.bias, None, False)
 
     def gated(self, x: Tensor) -> Tensor:

@@ -138,6 +138,32 @@ def test_refusals():
     assert lib.asrlayer_linear8(bytes(p), 0, 0, None) == _lib.OK
 
 
+def test_tensors_that_change_after_a_weight_is_made(monkeypatch):
+    """A weight keeps the memory that its tensors had: a call hands that to the kernel."""
+    import copy
+    import pickle
+
+    from asrback_amd import linear8 as module
+    from asrback_amd.linear8 import Weight8, gated8, linear8, pack8
+
+    seen = []
+    monkeypatch.setattr(module, "_product", lambda what, x, packed, scales, *args: seen.append((packed, scales)))
+    for name in ("packed", "scales"):
+        for change in (lambda t: t.set_(torch.zeros(1, dtype=t.dtype)), lambda t: t.resize_(1),
+                       lambda t: setattr(t, "data", torch.zeros(1, dtype=t.dtype))):
+            weight = pack8(torch.full((8, 64), 3, dtype=torch.int8), torch.ones(8))
+            held = [t.clone() for t in (weight.packed, weight.scales)]
+            change(getattr(weight, name))
+            for f in (linear8, gated8):
+                f(torch.zeros(3, 64), weight)
+                assert all(torch.equal(a, b) for a, b in zip(seen.pop(), held))
+    weight = pack8(torch.zeros(8, 64, dtype=torch.int8), torch.ones(8))
+    for twin in (copy.deepcopy(weight), pickle.loads(pickle.dumps(weight))):
+        assert isinstance(twin, Weight8) and (twin.outputs, twin.inputs) == (8, 64)
+        assert all(a.data_ptr() == b.data_ptr() for a, b in zip(twin._held, (twin.packed, twin.scales)))
+        assert twin.packed.data_ptr() != weight.packed.data_ptr()
+
+
 def test_scales_that_require_a_gradient():
     from asrback_amd.linear8 import Linear8, Weight8, gated8, linear8, pack8
 
