@@ -37,7 +37,8 @@ class Weight4:
     """A matrix ``(outputs, inputs)`` of 4-bit values with a scale (and a zero
     point) per ``group`` inputs of an output, in the kernel's layout
     (``asrlayer_linear4_params``).  Made by :func:`pack4` or
-    :func:`quantize4`."""
+    :func:`quantize4`.  As a view of them would, it keeps the memory and the layout
+    that its tensors have when it is made."""
 
     packed: Tensor
     scales: Tensor
@@ -48,6 +49,14 @@ class Weight4:
 
     def __post_init__(self) -> None:
         _check_layout(self.packed, self.scales, self.zeros, self.outputs, self.inputs, self.group)
+        # What the kernel reads: views of its own, which nothing done to the tensors given
+        # can resize.
+        held = tuple(None if t is None else t.view(t.shape) for t in (self.packed, self.scales, self.zeros))
+        object.__setattr__(self, "_held", held)
+
+    def __reduce__(self):
+        # (a copy holds views of its own)
+        return Weight4, (self.packed, self.scales, self.zeros, self.outputs, self.inputs, self.group)
 
 
 def _check_layout(packed: Tensor, scales: Tensor, zeros: Tensor | None, outputs: int, inputs: int, group: int) -> None:
@@ -176,7 +185,8 @@ def linear4(x: Tensor, weight: Weight4, bias: Tensor | None = None, *, out: Tens
     drafted tree (up to 32 are read against the weights in one pass); more rows
     are right, the weights being read again for each 32.  ``out`` is written in
     place and must not share memory with ``x`` or ``bias``.  Returns ``(..., outputs)``."""
-    return _product(x, weight.packed, weight.scales, weight.zeros, weight.outputs, weight.inputs, weight.group, bias, out)
+    refuse_gradient("linear4", weight.scales)
+    return _product(x, *weight._held, weight.outputs, weight.inputs, weight.group, bias, out)
 
 
 def _product(x: Tensor, packed: Tensor, scales: Tensor, zeros: Tensor | None, outputs: int, inputs: int, group: int,
@@ -192,7 +202,6 @@ def _product(x: Tensor, packed: Tensor, scales: Tensor, zeros: Tensor | None, ou
     if bias is not None and (bias.shape != (outputs,) or bias.dtype is not dtype):
         raise ValueError(f"bias must be {dtype} ({outputs},), got {bias.dtype} {tuple(bias.shape)}")
     refuse_unseen("linear4", x, scales, bias)
-    refuse_gradient("linear4", scales)
     given = out is not None
     if given:
         if out.shape != (*shape[:-1], outputs) or out.dtype is not dtype or not out.is_contiguous():
@@ -245,6 +254,7 @@ class Linear4(nn.Module):
 
     def forward(self, x: Tensor) -> Tensor:
         _check_layout(self.packed, self.scales, self.zeros, self.out_features, self.in_features, self.group)
+        refuse_gradient("linear4", self.scales)
         return _product(x, self.packed, self.scales, self.zeros, self.out_features, self.in_features, self.group, self.bias,
                         None)
 

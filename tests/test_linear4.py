@@ -137,6 +137,32 @@ def test_refusals():
     assert lib.asrlayer_linear4(ctypes.byref(p), None) == _lib.OK
 
 
+def test_tensors_that_change_after_a_weight_is_made(monkeypatch):
+    """A weight keeps the memory that its tensors had: a call hands that to the kernel."""
+    import copy
+    import pickle
+
+    from asrback_amd import linear4 as module
+    from asrback_amd.linear4 import Weight4, linear4, pack4
+
+    seen = []
+    monkeypatch.setattr(module, "_product", lambda x, packed, scales, zeros, *args: seen.append((packed, scales, zeros)))
+    values, zeros = torch.full((8, 64), 3, dtype=torch.uint8), torch.full((8, 2), 5, dtype=torch.uint8)
+    for name in ("packed", "scales", "zeros"):
+        for change in (lambda t: t.set_(torch.zeros(1, dtype=t.dtype)), lambda t: t.resize_(1),
+                       lambda t: setattr(t, "data", torch.zeros(1, dtype=t.dtype))):
+            weight = pack4(values, torch.ones(8, 2), zeros)
+            held = [t.clone() for t in (weight.packed, weight.scales, weight.zeros)]
+            change(getattr(weight, name))
+            linear4(torch.zeros(3, 64), weight)
+            assert all(torch.equal(a, b) for a, b in zip(seen.pop(), held))
+    for weight in (pack4(values, torch.ones(8, 2), zeros), pack4(values, torch.ones(8, 2))):
+        for twin in (copy.deepcopy(weight), pickle.loads(pickle.dumps(weight))):
+            assert isinstance(twin, Weight4) and (twin.outputs, twin.inputs, twin.group) == (8, 64, 32)
+            assert twin._held[0].data_ptr() == twin.packed.data_ptr() != weight.packed.data_ptr()
+            assert (twin._held[2] is None) == (weight.zeros is None)
+
+
 def test_scales_that_require_a_gradient():
     from asrback_amd.linear4 import Linear4, Weight4, linear4, pack4
 
