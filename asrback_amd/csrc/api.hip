@@ -766,7 +766,12 @@ int asrlayer_linear8(const asrlayer_linear8_params* params, void* workspace, siz
     return fail(ASRATTN_ERR_INVALID, "a gated matrix has as many gates as projections, got %d outputs", p.n);
   if (p.n > (1 << 28) || p.k > (1 << 17) || p.rows > 65535 * 16)
     return fail(ASRATTN_ERR_UNSUPPORTED, "more than 1048560 rows, 2^28 outputs or 2^17 inputs");
-  // A launch has fewer than 2^32 threads, 512 a tile of 256 x 128.
+  // Up to 32 rows are taken by workgroups of 512 threads to 16 outputs, and a launch has
+  // fewer than 2^32 threads.
+  if (p.rows <= 32 && (p.gated != 0 ? p.n / 2 : p.n) > (1 << 27) - 16)
+    return fail(ASRATTN_ERR_UNSUPPORTED, "2^27 outputs or more of up to 32 rows");
+  // More rows' tiles (the smallest of 64 x 128, where they are few, else 128 x 128) are
+  // counted in 32 bits.
   if ((p.rows + 255) / 256 * ((p.n + 127LL) / 128) >= (1 << 23))
     return fail(ASRATTN_ERR_UNSUPPORTED, "more than 2^38 sums");
   if (p.rows == 0) return ok();

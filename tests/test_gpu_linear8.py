@@ -268,3 +268,18 @@ def test_most_rows():
     check(gated8(small, weight)[at], small[at].cpu(), values, scales, None, gated=True)
     with pytest.raises(RuntimeError, match="1048560 rows"):
         linear8(torch.zeros(rows + 1, 64, device="cuda", dtype=BF16), weight)
+
+
+def test_most_outputs():
+    """As many outputs as few rows' launch takes, some of them checked."""
+    from asrback_amd.linear8 import linear8, pack8
+
+    g = torch.Generator().manual_seed(9)
+    outputs = (1 << 27) - 16
+    values = torch.randint(-127, 128, (outputs, 1), device="cuda", dtype=torch.int8)
+    scales = (torch.rand(outputs, device="cuda") * 0.02 + 0.001).to(BF16)
+    x = torch.randn(1, 1, generator=g).to(BF16)
+    say("most outputs")
+    out = linear8(x.cuda(), pack8(values, scales))
+    at = torch.tensor([0, 1, 15, 16, 9_999_999, 77_777_777, outputs - 17, outputs - 1], device="cuda")
+    check(out[:, at], x, values[at].cpu(), scales[at].cpu(), None)

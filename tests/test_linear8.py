@@ -138,6 +138,23 @@ def test_refusals():
     assert lib.asrlayer_linear8(bytes(p), 0, 0, None) == _lib.OK
 
 
+def test_most_outputs_of_few_rows():
+    """What a launch could not hold is refused before anything is launched."""
+    from asrback_amd import _lib
+
+    lib = _lib.load()
+    p = _lib.Linear8Params()
+    p.k, p.x_row_stride, p.dtype = 1, 1, _lib.BF16
+    p.x = p.packed = p.scales = p.out = 4096
+    for rows, n, gated, taken in ((1, (1 << 27) - 16, 0, True), (32, (1 << 27) - 15, 0, False), (1, 1 << 28, 0, False),
+                                  (5, (1 << 28) - 32, 1, True), (5, (1 << 28) - 30, 1, False), (33, 1 << 28, 0, True)):
+        p.rows, p.n, p.gated = rows, n, gated
+        # (Enough of a workspace, but misaligned: what the sizes allow is refused for that.)
+        code = lib.asrlayer_linear8(bytes(p), 4096 + 16, 1 << 40, None)
+        assert code == (_lib.ERR_WORKSPACE if taken else _lib.ERR_UNSUPPORTED)
+        assert (b"aligned" if taken else b"2^27 outputs") in lib.asrattn_last_error()
+
+
 def test_tensors_that_change_after_a_weight_is_made(monkeypatch):
     """A weight keeps the memory that its tensors had: a call hands that to the kernel."""
     import copy
