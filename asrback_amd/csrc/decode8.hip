@@ -40,6 +40,8 @@
 // of the keys and a merge of one head at a time 20.5); two of about 52 000, 47.8 us
 // (5.0 TB/s; 64.9); one of 480, 8.2 us, a chain of round trips: length, keys, LDS, partials,
 // arrival, fold.
+#include <cmath>
+
 #include "common.hpp"
 #include "kernels.hpp"
 #include "quantize8.hpp"
@@ -66,7 +68,9 @@ struct Decode8Args {
   int share;       // workgroups of a block of heads, that share all sequences' keys (0: one each)
   int splits;      // of every sequence (0: by their lengths)
   int tile_heads;  // query heads of a block, at most 16
-  float c;         // scale * log2(e)
+  float c;         // scale * log2(e): c_part 2^c_power
+  float c_part;
+  int c_power;
   float* ws_o;     // [block][workgroup][tile_heads][head_dim]
   float* ws_ml;    // [block][workgroup][tile_heads][2]
   unsigned long long* ws_arrive;  // [block][sequence]
@@ -476,9 +480,14 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
     lds_barrier();
     read_queries(reinterpret_cast<const T*>(rows), HD);
   }
-  // What a key's scale is multiplied by: where bytes are converted and where they are
-  // biased.
-  float unit = a.c, biased_unit = 0.f;
+  // What a key's scale is multiplied by where bytes are biased, and what the queries are
+  // (2^up): where bytes are converted, that is taken off together with the scales, since by
+  // itself it has powers of two that float32 has not.
+  float biased_unit = 0.f;
+  int up = 0;
+  auto key_unit = [&](float key_scale) {
+    return S::kBiased ? __builtin_ldexpf(key_scale * a.c_part, a.c_power - up) : key_scale * a.c;
+  };
   f32x4_t bias{0.f, 0.f, 0.f, 0.f};
   if constexpr (S::kBiased) {
     // The queries times a power of two that puts their largest near 2^100, so that
@@ -498,9 +507,8 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
     }
 #pragma unroll
     for (int u = 0; u < W; ++u) largest = max(largest, sm_largest[u]);
-    const int e = (int)(__builtin_amdgcn_readfirstlane(largest) >> 23) - 127, up = 100 - e;
+    up = 100 - ((int)(__builtin_amdgcn_readfirstlane(largest) >> 23) - 127);
     auto scalar = [](float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); };
-    unit = scalar(__builtin_ldexpf(a.c, -up));
     biased_unit = scalar(__builtin_ldexpf(a.c, 133 - up));
 #pragma unroll
     for (int turn = 0; turn < kQTurns; ++turn) {
@@ -553,7 +561,7 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
     __builtin_amdgcn_wave_barrier();
     const f32x4_t s = scores_of(0, [](uint32_t x) { return widen(x); }, f32x4_t{0.f, 0.f, 0.f, 0.f});
-    m = __shfl(s[0] * (sm_new_scale[0] * unit), i, 64);
+    m = __shfl(s[0] * key_unit(sm_new_scale[0]), i, 64);
     l = g == 0 ? 1.f : 0.f;
     const float vs = sm_new_scale[1] * (1.f / S::kUnit);
     const uint32_t* value = reinterpret_cast<const uint32_t*>(sm_new + HD / 16) + g * kVB;
@@ -577,7 +585,7 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
       // above some 2^95 over the largest query): the tile's bytes are converted.
       const float biased = scale * (lane < 32 ? biased_unit : 0x1p120f);
       const bool convert = !S::kBiased || __any(!(biased <= 0x1p127f));
-      sm_scale[wave][lane] = convert ? scale * (lane < 32 ? unit : S::kBiased ? 0x1p-13f : 1.f) : biased;
+      sm_scale[wave][lane] = convert ? (lane < 32 ? key_unit(scale) : scale * (S::kBiased ? 0x1p-13f : 1.f)) : biased;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
       __builtin_amdgcn_wave_barrier();
       f32x4_t s[2];
@@ -884,6 +892,7 @@ hipError_t launch_decode8(const asrlayer_decode8_params& p, const asrlayer_appen
   const int group = p.heads_q / p.cache.heads_kv;
   a.tile_heads = group < 16 ? group : 16;
   a.c = p.scale * kLog2e;
+  a.c_part = std::frexp(p.scale, &a.c_power) * kLog2e;
   a.ws_o = ws_o;
   a.ws_ml = ws_ml;
   a.ws_arrive = ws_arrive;

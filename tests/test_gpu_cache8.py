@@ -260,6 +260,38 @@ def test_queries_and_scales_far_from_one(dtype):
         check(out, q, tensors, [length, 250])
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_tiny_queries_beside_large_values(dtype):
+    """Ordinary scores of tiny queries and huge keys, in tiles whose values' scales are large
+    as well: those are converted, and the queries' power of two is far from 1."""
+    from asrback_amd.cache8 import Cache8, decode8, decode_append8, write_rows8
+
+    g = torch.Generator().manual_seed(23)
+    batch, heads, kv, d, length = 2, 4, 2, 64, 300
+    _, (k, v, ks, vs) = random_cache(batch, length, kv, d, g)
+    plain, lengths = torch.randn(batch, heads, d, generator=g), [length, 250]
+    rows = [torch.randn(batch, n, d, generator=g).to(dtype) for n in (heads, kv, kv)]
+    norms = [(torch.rand(d, generator=g) + 0.5) for _ in "qk"]
+    angles = torch.rand(batch, d // 2, generator=g).repeat(1, 2)
+    for power in (20, 30, 40, 60, 100):
+        q = (plain * 2.0**-power).to(dtype)
+        tensors = k, v, ks * 2.0 ** (power - 7), vs.clone()
+        tensors[3][:, :, 64:96] *= 2.0**20  # one tile's
+        tensors[3][1, 1, 200] *= 2.0**20
+        say("tiny queries", dtype, power)
+        cache = Cache8(*(t.cuda() for t in tensors))
+        check(decode8(q.cuda(), cache, lengths=spread(lengths)), q, tensors, lengths)
+        # A step whose new key and value are such ones.
+        new = {"q_norm": (norms[0] * 2.0**-power).to(dtype).cuda(), "k_norm": (norms[1] * 2.0 ** (power - 3)).to(dtype).cuda(),
+               "q_eps": 1e-6, "k_eps": 1e-6, "cos": angles.cos().to(dtype).cuda(), "sin": angles.sin().to(dtype).cuda()}
+        x = rows[0].cuda(), rows[1].cuda(), (rows[2] * 2.0**20).cuda()
+        positions = torch.tensor([n - 1 for n in lengths], device="cuda")
+        out = decode_append8(*x, cache, positions, **new)
+        queries, _ = write_rows8(Cache8.allocate(batch, length, kv, d, "cuda"), *x, None, positions, **new)
+        # (Queries rounded by another kernel: 2^-21 of their largest in float32.)
+        check(out, queries.cpu(), [t.cpu() for t in cache.tensors], lengths, queries_off=0.0 if dtype == BF16 else 2.0**-21)
+
+
 def test_long_cache_past_32_bits():
     """Positions whose offsets pass 2^31 and 2^32 bytes."""
     from asrback_amd.cache8 import Cache8, decode8, read8, write8
