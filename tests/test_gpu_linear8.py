@@ -283,3 +283,68 @@ def test_most_outputs():
     out = linear8(x.cuda(), pack8(values, scales))
     at = torch.tensor([0, 1, 15, 16, 9_999_999, 77_777_777, outputs - 17, outputs - 1], device="cuda")
     check(out[:, at], x, values[at].cpu(), scales[at].cpu(), None)
+
+
+def check_here(out, x, values, scales, bias, gated=False):
+    """:func:`check` where the tensors are, for many outputs.  Below 2^-126 the numbers of both
+    types are evenly spaced, 2^-133 apart in bf16 (8 bits from 2^-126 down) and 2^-149 in
+    float32, so a rounding there is off by up to half of that whatever the value: 2^-134
+    (4.6e-41), and less than 1e-44."""
+    y, error = reference(x, values, scales, bias)
+    if gated:
+        (g, u), (eg, eu) = y.chunk(2, -1), error.chunk(2, -1)
+        s = g * torch.sigmoid(g)
+        y = s * u
+        error = u.abs() * (1.1 * eg + s.abs() * (2 * g.abs() + 8) * 2.0**-24 + 1e-36) + s.abs() * eu
+    bound = 1.01 * (error + STEP[out.dtype] * y.abs()) + (1.01 * 2.0**-134 if out.dtype == BF16 else 1e-44)
+    worst = ((out.double() - y).abs() / bound).max()
+    assert worst <= 1, float(worst)
+
+
+# Tiles of 64 x 128, of 128 x 128 and of 128 x 256 (gated: half as many outputs), the last
+# two in more tiles than the card's 512 workgroups; an odd and an even number of blocks of
+# 64 inputs, and widths that end inside a vector.
+TILED = [
+    # rows, inputs, outputs
+    (1000, 512, 1541), (970, 700, 1536), (2600, 650, 9006), (2500, 1280, 9008), (3500, 700, 8450), (3457, 1024, 8706),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,inputs,outputs", TILED)
+@pytest.mark.parametrize("gated", [False, True])
+def test_deep_products_of_many_tiles(dtype, rows, inputs, outputs, gated):
+    """Every output of tiles whose ring of stages turns over several times, from a tile into the
+    next; then rows of far scales in some waves only, of NaN and of infinities."""
+    from asrback_amd.linear8 import gated8, linear8, pack8
+
+    g = torch.Generator().manual_seed(rows + inputs)
+    if gated:
+        outputs = outputs // 2 * 2
+    call = gated8 if gated else linear8
+    values, scales = (t.cuda() for t in matrix(outputs, inputs, dtype, g))
+    bias = torch.randn(outputs, generator=g).to("cuda", dtype)
+    x = torch.randn(rows, inputs, generator=g).to("cuda", dtype) / (4 * math.sqrt(inputs))
+    say("tiled", dtype, rows, inputs, outputs, gated)
+    weight = pack8(values, scales)
+    check_here(call(x, weight, bias), x, values, scales, bias, gated)
+    # Scales from 2^90 on are multiplied in another order; with an output's own far below, the
+    # results are ordinary.
+    far = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    far[:16] = far[rows // 2] = far[-1] = True
+    small = (scales.float() * 2.0**-110).to(dtype)
+    mixed = torch.where(far[:, None], x.float() * 2.0**115, x.float()).to(dtype)
+    say("far rows")
+    weight = pack8(values, small)
+    out = call(mixed, weight)
+    check_here(out, mixed, values, small, None, gated)
+    at = torch.tensor([5, 40, rows // 3, rows - 1], device="cuda")
+    bad = mixed.clone()
+    bad[at, torch.tensor([0, 63, 64, inputs - 1], device="cuda")] = torch.tensor(
+        [math.nan, math.inf, math.nan, -math.inf], device="cuda", dtype=dtype)
+    say("rows without numbers")
+    have = call(bad, weight)
+    assert torch.isnan(have[at]).all()
+    others = torch.ones(rows, dtype=torch.bool, device="cuda")
+    others[at] = False
+    assert torch.equal(have[others], out[others])
