@@ -173,6 +173,80 @@ def test_attention(dtype, batch, heads, kv, head_dim, length):
         assert torch.equal(decode8(q.cuda(), pool, lengths=spread(lengths), window=window, pages=table), out)
 
 
+LONG = [
+    # heads, kv heads, head_dim, room, lengths: splits by lengths, equal splits, none
+    (4, 2, 128, 20000, (20000, 4097, 9031)), (16, 8, 128, 40032, (31999, 40032)), (6, 6, 64, 9000, (9000, 1, 0, 8801, 33)),
+    (8, 1, 256, 6000, (5999, 6000, 4512)), (17, 1, 64, 12000, (11999, 7)), (16, 8, 128, 9001, (9001,)),
+    (4, 4, 64, 1500, (1500, 700, 1499)), (2, 2, 128, 300, tuple(300 - 2 * b for b in range(140))),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads,kv,head_dim,room,lengths", LONG)
+@pytest.mark.parametrize("page", [0, 16])
+def test_every_key_counts_once(dtype, heads, kv, head_dim, room, lengths, page):
+    """Queries of zeros weigh every key 1, and keys have values at one dimension each: an output
+    is the number of keys at its dimension over that of all.  Sums of whole numbers below 2^24
+    are exact, so that only the quotient's two roundings are left, and a key (a tile) that is
+    lost or taken twice stands out of the keys of its dimension."""
+    from asrback_amd.attention import PageTable
+    from asrback_amd.cache8 import Cache8, decode8
+
+    g = torch.Generator().manual_seed(room)
+    batch, scale = len(lengths), 0.25
+    q = torch.zeros(batch, heads, head_dim, device="cuda", dtype=dtype)
+    step = 2.0**-8 if dtype == BF16 else 2.0**-23
+    at, table = torch.arange(room), None
+    # By keys, and by tiles of 32.
+    for dims in (at % head_dim, at // 32 % head_dim):
+        values = torch.zeros(batch, room, kv, head_dim, dtype=torch.int8)
+        values[:, at, :, dims] = 127
+        tensors = [torch.randint(-127, 128, values.shape, generator=g, dtype=torch.int8), values,
+                   *(torch.full((batch, kv, room), scale) for _ in "kv")]
+        if page:
+            cache, table, _ = paged(tensors, page, g)
+            table = PageTable(table.block_table, room)
+        else:
+            cache = Cache8(*(t.cuda() for t in tensors))
+        for window in (None, 1000, 4100):
+            say("counts", dtype, heads, kv, head_dim, room, page, window)
+            out = decode8(q, cache, lengths=spread(lengths), pages=table, window=window).cpu().double()
+            for b, n in enumerate(lengths):
+                first = max(0, n - window) if window else 0
+                counts = torch.bincount(dims[first:n], minlength=head_dim).double()
+                ref = counts * 127 * scale / max(1, n - first)
+                assert ((out[b] - ref).abs() <= 1.01 * step * ref).all(), (b, n)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("head_dim,room", [(128, 20000), (64, 40000), (256, 5000)])
+def test_one_key_among_many(dtype, head_dim, room):
+    """A key that dwarfs the others, at both ends of halves, tiles, turns of the waves and
+    about everywhere else: its value comes out, whichever workgroup holds it."""
+    from asrback_amd.cache8 import Cache8, decode8
+
+    g = torch.Generator().manual_seed(head_dim)
+    batch, kv = 2, 8
+    near = [p + d for p in (0, 16, 32, 64, 128, 256, 512, 1024, 4096, room // 2 // 32 * 32) for d in (-1, 0, 1)]
+    near += [*range(room // 40, room - 40, room // 40), room - 33, room - 32, room - 1]
+    near = [p for p in near if 0 <= p < room]
+    q = torch.zeros(batch, 2 * kv, head_dim)
+    q[..., 0] = 1
+    values = torch.randint(-127, 128, (batch, room, kv, head_dim), generator=g, dtype=torch.int8).cuda()
+    ones = torch.ones(batch, kv, room, device="cuda")
+    for first in range(0, len(near), kv):
+        places = [near[(first + h) % len(near)] for h in range(kv)]
+        keys = torch.zeros(batch, room, kv, head_dim, dtype=torch.int8, device="cuda")
+        for h, p in enumerate(places):
+            keys[:, p, h, 0] = 127
+        lengths = [room, max(places) + 1]
+        say("one key", dtype, head_dim, places)
+        out = decode8(q.to("cuda", dtype), Cache8(keys, values, ones, ones / 8), lengths=spread(lengths), scale=1.0)
+        # The others' weights are e^-127 each.
+        ref = torch.stack([values[:, p, h].float() / 8 for h, p in enumerate(places)], 1).repeat_interleave(2, 1)
+        assert torch.equal(out.float(), ref)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_masked_places_hold_anything(dtype):
     """Positions past a row's keys and before its window hold NaN and infinite scales, and
