@@ -660,13 +660,22 @@ hipError_t launch_typed(const asrlayer_linear8_params& p, void* workspace, hipSt
   // rounds: 24.4 and 20.8).
   const int wide = p.gated ? 64 : 128;
   if (tiles(64, wide) <= 256) return launch_large<T, 2, 4, 8>(p, packed, scales, stream);
-  // Tiles of 128 x 256 where the last round of the 512 workgroups that the card holds is
-  // nearly full, or two full ones go before (3440 rows of 2048 to 4096, 432 of them: 39.9
-  // us, 42.9 in tiles of 128 x 128; 7300, 928: 72.1 and 79.4; 9600, 1200: 93.0 and 99.0;
-  // 4099 of 2048 to 2 x 6144, gated, 1584: 112.7 and 118.1; but 6800 to 4096, 864: 70.5 and
-  // 70.1; 3291 of 6397 to 3149, 338: 119.6 and 106.5; 1537 gated, 624: 55.2 and 48.8).
+  // Tiles of 128 x 256 against ones of 128 x 128: the same work in 92% of the time.  The card
+  // holds 512 workgroups of either, two a CU, and 256 more take a CU each, so a kernel's
+  // time goes up with every 256 workgroups: with an even number of steps of the smaller
+  // tiles the larger ones have half as many and win, with an odd one they do half a step
+  // for nothing, which they have made up for after five of their own.  2048 inputs to 4096
+  // outputs, us in the larger and in the smaller tiles:
+  //   3035 rows (384 of the larger)   39.5 and 37.3     3163 (400)    40.1 and 43.0
+  //   5083 (640)                      58.8 and 54.9     5211 (656)    59.6 and 62.0
+  //   7003 (880)                      73.2 and 72.5     7259 (912)    74.6 and 81.0
+  //   9051 (1136)                     89.5 and 90.3     9307 (1168)   89.5 and 99.9
+  //  10971 (1376)                    109.7 and 111.8   12379 (1552)  122.2 and 127.3
+  // of 6144 inputs, gated: 640 of them 148.3 and 134.7, 656 149.3 and 154.4; 880 188.8 and
+  // 185.2, 912 191.1 and 208.6; 1376 286.2 and 287.0.  Up to 256 of the larger, a CU to
+  // themselves, have too few waves (1755 rows, 224: 30.6 and 27.0).
   const long long big = tiles(128, 2 * wide);
-  if (big >= 1200 || (big - 1) % 512 >= 399) return launch_large<T, 4, 8, 3>(p, packed, scales, stream);
+  if (big > 5 * 256 || (big > 256 && (big - 1) % 256 >= 128)) return launch_large<T, 4, 8, 3>(p, packed, scales, stream);
   return launch_large<T, 4, 4, 4>(p, packed, scales, stream);
 }
 

@@ -307,6 +307,7 @@ def check_here(out, x, values, scales, bias, gated=False):
 TILED = [
     # rows, inputs, outputs
     (1000, 512, 1541), (970, 700, 1536), (2600, 650, 9006), (2500, 1280, 9008), (3500, 700, 8450), (3457, 1024, 8706),
+    (2600, 650, 6606), (2500, 1280, 6608), (5200, 330, 8450),
 ]
 
 
