@@ -86,7 +86,7 @@ class Cache8:
         object.__setattr__(self, "_inference", any(t.is_inference() for t in self.tensors))
 
     def __reduce__(self):
-        return Cache8, self.tensors  # (a copy holds views of its own)
+        return type(self), self.tensors  # (a copy holds views of its own)
 
     @property
     def tensors(self) -> tuple[Tensor, Tensor, Tensor, Tensor]:

@@ -56,7 +56,7 @@ class Weight4:
 
     def __reduce__(self):
         # (a copy holds views of its own)
-        return Weight4, (self.packed, self.scales, self.zeros, self.outputs, self.inputs, self.group)
+        return type(self), (self.packed, self.scales, self.zeros, self.outputs, self.inputs, self.group)
 
 
 def _check_layout(packed: Tensor, scales: Tensor, zeros: Tensor | None, outputs: int, inputs: int, group: int) -> None:

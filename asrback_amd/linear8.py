@@ -56,7 +56,7 @@ class Weight8:
         object.__setattr__(self, "_held", (self.packed.view(self.packed.shape), self.scales.view(self.scales.shape)))
 
     def __reduce__(self):
-        return Weight8, (self.packed, self.scales, self.outputs, self.inputs)  # (a copy holds views of its own)
+        return type(self), (self.packed, self.scales, self.outputs, self.inputs)  # (a copy holds views of its own)
 
 
 def _check_layout(packed: Tensor, scales: Tensor, outputs: int, inputs: int) -> None:
@@ -140,8 +140,6 @@ def gated8(x: Tensor, weight: Weight8, bias: Tensor | None = None, *, out: Tenso
     ``2 n`` outputs, the gates before the projections, in one product
     (``asrlayer_linear8``): float32 until the one rounding at the end.  Arguments as
     for :func:`linear8`.  Returns ``(..., n)``."""
-    if weight.outputs % 2:
-        raise ValueError(f"a gated matrix has as many gates as projections, got {weight.outputs} outputs")
     refuse_gradient("gated8", weight.scales)
     return _product("gated8", x, *weight._held, weight.outputs, weight.inputs, bias, out, True)
 
@@ -157,6 +155,8 @@ def _product(what: str, x: Tensor, packed: Tensor, scales: Tensor, outputs: int,
     if not shape or shape[-1] != inputs:
         raise ValueError(f"x must be (..., {inputs}), got {tuple(shape)}")
     dtype, index = x.dtype, x.get_device()
+    if gated and outputs % 2:
+        raise ValueError(f"a gated matrix has as many gates as projections, got {outputs} outputs")
     if dtype is not scales.dtype:
         raise TypeError(f"x is {dtype}, the weight's scales {scales.dtype}")
     if dtype not in _DTYPES:
@@ -227,7 +227,9 @@ class Linear8(nn.Module):
 
     def gated(self, x: Tensor) -> Tensor:
         """:func:`gated8` over this layer's matrix and bias."""
-        return gated8(x, self.weight8, self.bias)
+        _check_layout(self.packed, self.scales, self.out_features, self.in_features)
+        refuse_gradient("gated8", self.scales)
+        return _product("gated8", x, self.packed, self.scales, self.out_features, self.in_features, self.bias, None, True)
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
