@@ -36,10 +36,13 @@
 // words).  Maxima, sums and outputs are float32 until the one rounding at the end.
 //
 // Measured with 16 heads over 8 of 128, bf16, every call on another cache: 64 sequences
-// of 400 to 560 keys, pages of 64, 18.0 us (4.5 TB/s; with conversions, an unshuffled load
-// of the keys and a merge of one head at a time 20.5); two of about 52 000, 47.8 us
-// (5.0 TB/s; 64.9); one of 480, 8.2 us, a chain of round trips: length, keys, LDS, partials,
-// arrival, fold.
+// of 400 to 560 keys, pages of 64, 17.2 us (65 MB at 3.8 TB/s; where it took 18.0, with
+// conversions, an unshuffled load of the keys and a merge of one head at a time 20.5); two
+// of about 52 000, 45.9 us (223 MB at 4.9 TB/s; 47.8 and 64.9); one of 480, 7.9 us, a chain
+// of round trips: length, keys, LDS, partials, arrival, fold.  Heads of 64 have half as many
+// bytes a tile for the same exchange through LDS: 16 sequences of 1500 keys, 12 heads, take
+// 17.2 us (39 MB at 2.3 TB/s), 16.1 with keys loaded straight into the operand and bytes
+// converted.
 #include <cmath>
 
 #include "common.hpp"
@@ -56,8 +59,6 @@ typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kKeys = 32;  // of a tile, in two halves
-// Cache policy of device scope (sc1).
-constexpr int kDeviceScope = 16;
 // Cache policy of data read once (common.hpp, buffer_load16_stream).
 constexpr int kNontemporal = 2;
 
@@ -180,8 +181,8 @@ __device__ __forceinline__ int lanes_prefix(int x, int lanes) {
 // APPEND: the queries get their norm and rotation here, and the sequence's new key and
 // value are rounded, written, and attended to beside the tiles: the softmax of the last
 // split's last wave, which has the fewest, begins with them.  One of 480 keys (16 heads
-// over 8 of 128) 9.5 us, with a launch before it 12.1; 64 of them 18.5 and 20.2; one
-// of 16 000 19.1 and 21.1.
+// over 8 of 128) 9.3 us, in two launches 11.2; 64 of them 18.4 and 19.5; one of 16 000
+// 19.2 and 21.1.
 template <typename T, int HD, int W, bool PAGED, bool APPEND>
 __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decode8_kernel(const Decode8Args a) {
   using S = Decode8Shape<T, HD>;

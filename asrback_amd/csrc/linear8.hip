@@ -10,9 +10,9 @@
 //
 // Three ways, by the rows: few rows by workgroups of 16 outputs that read the weights to
 // registers, more by tiles through LDS, of which several sizes (launch_typed says which
-// and why).  One row of 2048 to 2048 outputs takes 4.4 us, of which the launch and
-// two round trips to memory are most; 4099 rows of 2048 to 2 x 6144, gated, 109 us: 206 G
-// operations at 1.90 P/s.  There the matrix cores are busy for 60% of the time, at a
+// and why).  One row of 2048 to 2048 outputs takes 4.5 us, of which the launch and
+// two round trips to memory are most; 4099 rows of 2048 to 2 x 6144, gated, 109 to 113 us
+// from card to card: 206 G operations at 1.83 to 1.89 P/s.  There the matrix cores are busy for 60% of the time, at a
 // clock that their power holds near 1.7 GHz (a single workgroup runs at 2.3).
 #include "kernels.hpp"
 #include "layers.hpp"
@@ -35,7 +35,7 @@ __device__ __forceinline__ i32x4_t lds_read(uint32_t addr) { return *(lds_i32x4_
 constexpr int kThreads = 256;
 
 // N consecutive elements at any address of them: global memory takes vectors there
-// (2791 rows of 320 inputs to 21497 bf16 outputs 77 us, stored one by one 219; to 21504 49).
+// (2791 rows of 320 inputs to 21497 bf16 outputs 73 us, stored one by one 219; to 21504 45).
 template <typename T, int N>
 __device__ __forceinline__ void load_whole(const T* p, float* x) {
   constexpr int EPL = Elem<T>::kPerVec;
@@ -652,12 +652,12 @@ hipError_t launch_typed(const asrlayer_linear8_params& p, void* workspace, hipSt
   if (p.rows <= 32) return launch_few<T, 2, false>(p, packed, scales, stream);
   const auto tiles = [&](int rows, int wide) { return (p.rows + rows - 1) / rows * (((long long)outputs + wide - 1) / wide); };
   // Workgroups of 16 outputs and all inputs read the rows anew each: two a CU (128 rows
-  // of 2048 to 4096 outputs, 512 of them: 11.8 us, 13.8 in tiles of 64 x 128; 256 to
-  // 2048, 512: 12.0 and 14.0; 200 to 4096, 1024: 16.1 and 14.0).
+  // of 2048 to 4096 outputs, 512 of them: 10.6 us, 12.5 in tiles of 64 x 128; 256 to
+  // 2048, 512: 10.8 and 12.8; 200 to 4096, 1024: 15.0 and 12.7).
   if (tiles(64, 16) <= 512) return launch_few<T, 4, false>(p, packed, scales, stream);
   // Tiles of 64 x 128 while each has a CU, and a ring of eight stages, to itself (512
-  // rows of 6144 to 2048: 26.8 us, 32.5 in tiles of 128 x 128; 1024 of 2048 to 4096, two
-  // rounds: 24.4 and 20.8).
+  // rows of 6144 to 2048: 25.9 us, 31.4 in tiles of 128 x 128; 512 of 2048 to 4096 14.2 and
+  // 16.0; 576, two rounds: 20.7 and 16.2).
   const int wide = p.gated ? 64 : 128;
   if (tiles(64, wide) <= 256) return launch_large<T, 2, 4, 8>(p, packed, scales, stream);
   // Tiles of 128 x 256 against ones of 128 x 128: the same work in 92% of the time.  The card
@@ -683,8 +683,9 @@ hipError_t launch_typed(const asrlayer_linear8_params& p, void* workspace, hipSt
 
 Linear8Workspace linear8_workspace(int64_t rows, int n, int k, bool gated) {
   // Few values are rounded by every workgroup, while a CU holds all of its workgroups at
-  // once: 4 x 2048 to 2 x 6144 outputs (gated) 10.9 us, with a launch before it 12.0; 8 x
-  // 2048 to 2048 6.4 and 7.6; 16 x 2048 8.4 and 7.8; 1 x 2048 to 151936 70.3 and 63.8.
+  // once: 4 x 2048 to 2 x 6144 outputs (gated) 9.7 us, with a launch before it 10.8; 8 x
+  // 2048 to 2048 5.9 and 6.7, to 8192 8.8 and 8.6; 1 x 2048 to 8192 6.9 and 8.2, to 151936
+  // 64.2 and 59.8.
   if (rows <= 16 && rows * k <= kFusedValues && (gated ? n / 2 : n) <= 512 * 16) return {0, 0};
   const size_t tiles = (size_t)(rows + 15) / 16;
   Linear8Workspace w;

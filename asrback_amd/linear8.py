@@ -239,7 +239,16 @@ def quantize_linears8(module: nn.Module) -> int:
     """Replace every ``nn.Linear`` under ``module`` (not ``module`` itself) by a
     :class:`Linear8` of its rounded weights, in place; returns how many.  A layer that
     appears in several places is rounded once and stays shared; one that carries
-    hooks or a forward of its own stays as it is."""
+    hooks or a forward of its own stays as it is.
+
+    Prompts and steps gain where their layers are calls, as Qwen3's are.  An encoder of
+    inputs of 768 to 1280 gains 3 to 12% (four Whisper layers of 1280 in bf16: 2.43 ms
+    for 2.51 over 8 x 1500 frames, 0.57 for 0.64 over 1500): the rounding of its rows
+    takes most of what the products save.  Kernels that read a layer's matrix in place
+    of its call run for ``nn.Linear`` only, so that a Whisper decoder's step, whose layers
+    take six launches, goes op by op and is slower (12 layers of 768 in bf16: 810 us for
+    394 at one row, 1026 for 774 at 16; 4 layers of 1280: 300 for 159 and 445 for 417; 12
+    of 768 in float32 801 for 456 and 1224 for 903): quantize the encoder alone there."""
     places = [(parent, name, child) for parent in module.modules()
               # (named_children leaves out a child's second name)
               for name, child in parent._modules.items()

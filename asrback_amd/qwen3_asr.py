@@ -31,7 +31,8 @@ decode loop around them (``DecodeState``, ``choose``, ``TextGreedyDecoder``:
 * Drafted tokens, which the reference has not: ``verify`` of ``TextAttention``,
   ``TextModel`` and ``TextGreedyDecoder`` runs a tree of them through the model
   in one pass (:mod:`asrback_amd.drafts`) and keeps those that greedy steps
-  would have produced.
+  would have produced (over an 8-bit cache but for its rounding, which steps and
+  passes see differently: ``TextAttention.verify``).
 """
 
 from __future__ import annotations
@@ -506,7 +507,9 @@ class TextAttention(nn.Module):
         ``k_draft``/``v_draft`` ``(batch, tokens, kv_heads, head_dim)``; the cache
         stays as it is.  ``cos``/``sin`` ``(batch, tokens, head_dim)`` at each
         token's position, ``rows`` 0 .. batch - 1 (int64).  An 8-bit cache is read
-        back for it (:func:`~asrback_amd.cache8.read8`)."""
+        back for it (:func:`~asrback_amd.cache8.read8`): its keys and values are rounded
+        to ``x``'s type, in bf16 by up to 2^-8 of each, which a step takes exactly, and
+        drafted ones are attended to as they are, which steps find rounded to 8 bits."""
         if isinstance(keys, Layer8):
             pages = None
             key_cache, value_cache = read8(keys.cache, lengths=lengths, pages=keys.pages, dtype=x.dtype)
