@@ -16,6 +16,7 @@ that would need one, in forward mode too, or that a tracer records are refused.
 from __future__ import annotations
 
 import functools
+import itertools
 from dataclasses import dataclass
 
 import torch
@@ -24,7 +25,7 @@ from torch import Tensor
 from . import _lib
 from .attention import _DTYPES, PageTable, _aligned, _check_device, _split_workspace
 from .drafts import _lengths, _on
-from .layers import _increment_version, check_out, refuse_gradient, refuse_unseen
+from .layers import _increment_version, check_out, overlap, refuse_gradient, refuse_unseen, repeats
 
 HEAD_DIMS = (64, 128, 256)
 # The current stream's handle on a device; the current device (once a tensor is on one).
@@ -41,7 +42,8 @@ class Cache8:
     whole 16-byte vectors with a unit last one; the scales float32 ``(batch, heads_kv,
     length)`` with a unit last stride.  With a :class:`~asrback_amd.attention.PageTable`
     at a call they are pools, ``(num_pages, page_size, heads_kv, head_dim)`` and
-    ``(num_pages, heads_kv, page_size)``.  As a view of them would, it keeps the memory
+    ``(num_pages, heads_kv, page_size)``.  Tensors that hold an element more than once, as
+    expanded ones do, or share memory can be read but not written.  As a view of them would, it keeps the memory
     and the layout that they have when it is made: a tensor that is resized or set to
     another memory afterwards does not change it."""
 
@@ -84,6 +86,12 @@ class Cache8:
                    *self.value_scales.stride()[:2])
         object.__setattr__(self, "_strides", strides)
         object.__setattr__(self, "_inference", any(t.is_inference() for t in self.tensors))
+
+    @functools.cached_property
+    def _repeats(self) -> bool:
+        apart = len({t.untyped_storage().data_ptr() for t in self._held}) == len(self._held)
+        return any(repeats(t) for t in self._held) or \
+            not apart and any(overlap(*pair) for pair in itertools.combinations(self._held, 2))
 
     def __reduce__(self):
         return type(self), self.tensors  # (a copy holds views of its own)
@@ -150,6 +158,13 @@ def _ready(what: str, first: Tensor, *others: Tensor | None) -> int:
     return index
 
 
+def _check_written(what: str, cache: Cache8) -> None:
+    if cache._repeats:
+        raise ValueError(f"{what} cannot write a cache that holds elements more than once")
+    if cache._inference and not torch.is_inference_mode_enabled():
+        raise RuntimeError("inplace update to inference tensors outside InferenceMode is not allowed")
+
+
 def _index(t: Tensor | None, name: str, tokens: int) -> Tensor | None:
     if t is None:
         return None
@@ -203,9 +218,8 @@ def _write(what: str, cache: Cache8, k: Tensor, v: Tensor, rows: Tensor | None, 
     weights = () if prologue is None else (*prologue[:2], *prologue[4:])
     refuse_unseen(what, k, v, q, *weights, *cache.tensors)
     refuse_gradient(what, cache.key_scales, cache.value_scales)
+    _check_written(what, cache)
     index = _ready(what, k, v, q, *weights)
-    if cache._inference and not torch.is_inference_mode_enabled():
-        raise RuntimeError("inplace update to inference tensors outside InferenceMode is not allowed")
     _on(index, rows, positions)
     batch = lead if pages is None else pages.block_table.shape[0]
     if rows is None and tokens > batch:
@@ -352,6 +366,8 @@ def _decode(what: str, q: Tensor, cache: Cache8, lengths: Tensor | None, scale: 
         # A row's queries are read before any of its outputs is written.
         in_place = out.data_ptr() == q.data_ptr() and out.stride() == q.stride()
         check_out(what, out, None if in_place else q, *new, *cache._held, lengths, positions)
+    if new:
+        _check_written(what, cache)
     index = _ready(what, q, *new)
     q = _aligned(q)
     _on(index, lengths, out, positions)
@@ -373,8 +389,6 @@ def _decode(what: str, q: Tensor, cache: Cache8, lengths: Tensor | None, scale: 
     if not new:
         status = lib.asrlayer_decode8(_lib.pack_decode8(*step), workspace, size, _raw_stream(index))
     else:
-        if cache._inference and not torch.is_inference_mode_enabled():
-            raise RuntimeError("inplace update to inference tensors outside InferenceMode is not allowed")
         k, v = _aligned(new[0]), _aligned(new[1])
         q_norm, k_norm, cos, sin = (_aligned(t if t.is_contiguous() else t.contiguous()) for t in new[2:])
         status = lib.asrlayer_append8(

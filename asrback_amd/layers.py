@@ -105,6 +105,17 @@ def overlap(a: Tensor, b: Tensor) -> bool:
     return True
 
 
+def repeats(t: Tensor) -> bool:
+    """Whether ``t`` may hold an element more than once (a larger stride does not pass what
+    the smaller ones reach), so that writing it writes places twice."""
+    reach = 1
+    for stride, size in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if stride < reach and t.numel():
+            return True
+        reach += stride * (size - 1)
+    return False
+
+
 def check_out(what: str, out: Tensor, *inputs: Tensor | None) -> None:
     """Raise for a given ``out`` that a kernel cannot fill: one that autograd or
     inference mode guards, one that holds an element twice, or one that shares
@@ -114,11 +125,8 @@ def check_out(what: str, out: Tensor, *inputs: Tensor | None) -> None:
         raise RuntimeError(f"{what} has no gradient: out must not require one")
     if out.is_inference() and not torch.is_inference_mode_enabled():
         raise RuntimeError("inplace update to inference tensors outside InferenceMode is not allowed")
-    reach = 1
-    for stride, size in sorted((s, n) for n, s in zip(out.shape, out.stride()) if n > 1):
-        if stride < reach and out.numel():
-            raise ValueError(f"out of strides {out.stride()} holds elements more than once")
-        reach += stride * (size - 1)
+    if repeats(out):
+        raise ValueError(f"out of strides {out.stride()} holds elements more than once")
     for t in inputs:
         if t is not None and overlap(out, t):
             raise ValueError(f"out shares memory with what {what} reads")

@@ -206,6 +206,40 @@ def test_scales_that_require_a_gradient():
         decode8(q, cache)
 
 
+def test_caches_that_hold_elements_twice():
+    """Read, but not written: heads, rows and positions that share places."""
+    from asrback_amd.cache8 import Cache8, decode8, decode_append8, read8, write8, write_rows8
+
+    k, q, positions = torch.zeros(2, 3, 64), torch.zeros(2, 6, 64), torch.zeros(2, dtype=torch.int64)
+    norm, table = torch.zeros(64), torch.zeros(2, 64)
+    more = {"q_norm": norm, "k_norm": norm, "q_eps": 1e-6, "k_eps": 1e-6, "cos": table, "sin": table}
+    whole = Cache8.allocate(2, 8, 3, 64).tensors
+    for i, shared in ((0, torch.zeros(1, 8, 3, 64, dtype=torch.int8).expand(2, 8, 3, 64)),
+                      (1, torch.zeros(2, 8, 1, 64, dtype=torch.int8).expand(2, 8, 3, 64)),
+                      (1, torch.zeros(2 * 8 * 3 * 64, dtype=torch.int8).as_strided((2, 8, 3, 64), (1536, 16, 512, 1))),
+                      (2, torch.zeros(2, 1, 8).expand(2, 3, 8)), (3, torch.zeros(2, 3, 1).expand(2, 3, 1))):
+        if i == 3:  # one position: nothing is held twice
+            cache = Cache8(*(t[:, :1] for t in whole[:2]), whole[2][..., :1], shared)
+        else:
+            cache = Cache8(*(shared if j == i else t for j, t in enumerate(whole)))
+        word, kind = ("GPU only", RuntimeError) if i == 3 else ("more than once", ValueError)
+        for call in (lambda: write8(cache, k, k, None, positions), lambda: write_rows8(cache, q, k, k, None, positions, **more),
+                     lambda: decode_append8(q, k, k, cache, positions, **more)):
+            with pytest.raises(kind, match=word):
+                call()
+        for call in (lambda: read8(cache), lambda: decode8(q, cache)):
+            with pytest.raises(RuntimeError, match="GPU only"):
+                call()
+    # Keys that are the values, too, or reach into them; parts of the same pages are apart.
+    flat, pool = torch.zeros(2 * 1536 + 64, dtype=torch.int8), torch.zeros(2, 2, 8, 3, 64, dtype=torch.int8)
+    scales = torch.zeros(2, 2, 3, 8)
+    for tensors, taken in (((whole[0], whole[0], *whole[2:]), False), ((*whole[:2], whole[2], whole[2]), False),
+                           ((flat[:3072].view(2, 8, 3, 64), flat[64:].view(2, 8, 3, 64), *whole[2:]), False),
+                           ((pool[:, 0], pool[:, 1], scales[:, 0], scales[:, 1]), True)):
+        with pytest.raises(RuntimeError if taken else ValueError, match="GPU only" if taken else "more than once"):
+            write8(Cache8(*tensors), k, k, None, positions)
+
+
 @pytest.mark.filterwarnings("ignore::DeprecationWarning")
 def test_refusals():
     from asrback_amd.cache8 import Cache8, decode8, decode8_workspace_size, decode_append8, read8, write8, write_rows8
