@@ -243,7 +243,8 @@ int asrlayer_linear4(const asrlayer_linear4_params* params, void* stream);
 //
 // The rounding is that of the exact quotient, ties to even, and the sum an exact
 // 32-bit integer, so k is at most 2^17; what follows is float32, rounded once.  A
-// row with an infinity or a NaN comes out as NaN.  x rows x_row_stride apart,
+// row with an infinity or a NaN comes out as NaN.  At most 65535 * 16 rows, and fewer than
+// 2^27 outputs of up to 32 rows or 2^38 sums of more.  x rows x_row_stride apart,
 // out rows out_row_stride apart; w and bias in x's type.  The matrix lies in
 // blocks of 16 outputs by 64 inputs, padded to whole blocks with zeros:
 //
