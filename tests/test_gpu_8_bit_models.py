@@ -346,6 +346,32 @@ def test_drafts(device, dtype, page):
                         close(tensors[row, n:n + new], step[row, n:n + new], bound)
 
 
+@pytest.mark.parametrize("page", [None, 16])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_drafts_see_the_cache_as_it_reads_back(device, dtype, page):
+    """A pass over an 8-bit cache is one over a cache of the model's type that holds what
+    reading the 8-bit one back gives, to the bit."""
+    from asrback_amd import qwen3_asr as aq
+    from asrback_amd.cache8 import read8
+    from asrback_amd.drafts import tree_masks
+
+    say("8-bit drafts read back", dtype, page)
+    with torch.inference_mode():
+        text, prompt, cos, sin, held, _, g = setting(device, dtype, False)
+        mine = caches(page, 3, device)
+        prompt(text, mine)
+        plain = aq.KVCache.allocate(QWEN3, 3, mine.keys[0].shape[1], device, dtype)
+        for index, layer in enumerate(mine.keys):
+            plain.keys[index], plain.values[index] = read8(layer.cache, pages=layer.pages, dtype=dtype)
+        width = 7
+        tokens = torch.randint(0, QWEN3["vocab_size"], (3, width), generator=g).to(device)
+        parents = torch.tensor([-1, 0, 0, 1, 1, 3, 2], device=device).expand(3, width)
+        masks, depths = tree_masks(parents)
+        out = [text.verify(tokens, held, cache, aq.DraftCache.allocate(QWEN3, 3, width, device, dtype), masks, depths, cos, sin)
+               for cache in (mine, plain)]
+        assert torch.equal(*out)
+
+
 def drained(decoder, prompts, tokens):
     admitted = decoder.admit(prompts, tokens)
     results = {}
