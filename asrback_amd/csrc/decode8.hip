@@ -585,7 +585,7 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
       // Scales that the powers of two would put out of range (a value's above 128, a key's
       // above some 2^95 over the largest query): the tile's bytes are converted.
       const float biased = scale * (lane < 32 ? biased_unit : 0x1p120f);
-      const bool convert = !S::kBiased || __any(!(biased <= 0x1p127f));
+      const bool convert = !S::kBiased || __any(!(fabsf(biased) <= 0x1p127f));
       sm_scale[wave][lane] = convert ? (lane < 32 ? key_unit(scale) : scale * (S::kBiased ? 0x1p-13f : 1.f)) : biased;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
       __builtin_amdgcn_wave_barrier();

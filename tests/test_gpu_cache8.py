@@ -366,6 +366,32 @@ def test_tiny_queries_beside_large_values(dtype):
         check(out, queries.cpu(), [t.cpu() for t in cache.tensors], lengths, queries_off=0.0 if dtype == BF16 else 2.0**-21)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_scales_below_zero(dtype):
+    """Another quantizer's scales may be negative, and large: of values, of keys that queries
+    are small for."""
+    from asrback_amd.cache8 import Cache8, decode8, read8
+
+    g = torch.Generator().manual_seed(29)
+    batch, heads, kv, d, length = 2, 4, 2, 128, 300
+    _, (k, v, ks, vs) = random_cache(batch, length, kv, d, g)
+    lengths = [length, 77]
+    signs = [torch.randint(0, 2, ks.shape, generator=g) * 2.0 - 1 for _ in "kv"]
+    for s in signs:
+        s[..., :160] = -1  # whole tiles
+    for power, values in ((0, 1.0), (0, 2.0**16), (90, 2.0**5), (-60, 2.0**-40)):
+        tensors = k, v, signs[0] * ks * 2.0**power, signs[1] * vs * values
+        q = (torch.randn(batch, heads, d, generator=g) * 2.0 ** (-power - 2)).to(dtype)
+        say("negative", dtype, power, values)
+        cache = Cache8(*(t.cuda() for t in tensors))
+        # (The bound takes magnitudes: of scales with a sign, those of the numbers they scale.)
+        flat = [k * signs[0].transpose(1, 2)[..., None].to(torch.int8), v * signs[1].transpose(1, 2)[..., None].to(torch.int8),
+                tensors[2].abs(), tensors[3].abs()]
+        check(decode8(q.cuda(), cache, lengths=spread(lengths)), q, flat, lengths)
+        for out, t, s in zip(read8(cache, dtype=dtype), (k, v), tensors[2:]):
+            assert torch.equal(out.cpu(), (t.float() * s.transpose(1, 2)[..., None]).to(dtype))
+
+
 def test_long_cache_past_32_bits():
     """Positions whose offsets pass 2^31 and 2^32 bytes."""
     from asrback_amd.cache8 import Cache8, decode8, read8, write8
