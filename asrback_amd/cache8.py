@@ -374,7 +374,8 @@ def _decode(what: str, q: Tensor, cache: Cache8, lengths: Tensor | None, scale: 
     fields = _cache_fields(cache, pages, batch, index)
     if not given:
         out = q.new_empty(shape)
-    code, span = _DTYPES[q.dtype], window or 0
+    # (A cache has at most 2^30 positions.)
+    code, span = _DTYPES[q.dtype], min(window or 0, 1 << 30)
     step = (*fields, q.data_ptr(), out.data_ptr(), *q.stride()[:2], *out.stride()[:2],
             0 if lengths is None else lengths.data_ptr(), lengths is not None and lengths.dtype is torch.int64, heads_q, span,
             code, head_dim**-0.5 if scale is None else scale)

@@ -366,6 +366,18 @@ def test_tiny_queries_beside_large_values(dtype):
         check(out, queries.cpu(), [t.cpu() for t in cache.tensors], lengths, queries_off=0.0 if dtype == BF16 else 2.0**-21)
 
 
+def test_windows_past_32_bits():
+    from asrback_amd.cache8 import decode8
+
+    g = torch.Generator().manual_seed(31)
+    cache, _ = random_cache(2, 5000, 2, 64, g)
+    q, lengths = torch.randn(2, 4, 64, generator=g).to("cuda", BF16), spread([5000, 321])
+    say("windows")
+    whole = decode8(q, cache, lengths=lengths)
+    for window in (5000, 1 << 30, (1 << 31) - 1, 1 << 32, 1 << 80):
+        assert torch.equal(decode8(q, cache, lengths=lengths, window=window), whole)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_scales_below_zero(dtype):
     """Another quantizer's scales may be negative, and large: of values, of keys that queries
