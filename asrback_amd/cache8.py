@@ -43,9 +43,9 @@ class Cache8:
     length)`` with a unit last stride.  With a :class:`~asrback_amd.attention.PageTable`
     at a call they are pools, ``(num_pages, page_size, heads_kv, head_dim)`` and
     ``(num_pages, heads_kv, page_size)``.  Tensors that hold an element more than once, as
-    expanded ones do, or share memory can be read but not written.  As a view of them would, it keeps the memory
-    and the layout that they have when it is made: a tensor that is resized or set to
-    another memory afterwards does not change it."""
+    expanded ones do, or share memory can be read but not written.  As a view of them
+    would, it keeps the memory and the layout that they have when it is made: a tensor
+    that is resized or set to another memory afterwards does not change it."""
 
     keys: Tensor
     values: Tensor

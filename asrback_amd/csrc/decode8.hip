@@ -481,9 +481,10 @@ __global__ __launch_bounds__(64 * W, (Decode8Shape<T, HD>::kPerSimd)) void decod
     lds_barrier();
     read_queries(reinterpret_cast<const T*>(rows), HD);
   }
-  // What a key's scale is multiplied by where bytes are biased, and what the queries are
-  // (2^up): where bytes are converted, that is taken off together with the scales, since by
-  // itself it has powers of two that float32 has not.
+  // bf16 queries are multiplied by 2^up below, and the keys' scales take that off again:
+  // where bytes are biased they are multiplied by biased_unit, c 2^(133 - up), and where
+  // they are converted key_unit puts c 2^-up to them, which alone may be less than float32
+  // holds.
   float biased_unit = 0.f;
   int up = 0;
   auto key_unit = [&](float key_scale) {

@@ -12,8 +12,9 @@
 // registers, more by tiles through LDS, of which several sizes (launch_typed says which
 // and why).  One row of 2048 to 2048 outputs takes 4.5 us, of which the launch and
 // two round trips to memory are most; 4099 rows of 2048 to 2 x 6144, gated, 109 to 113 us
-// from card to card: 206 G operations at 1.83 to 1.89 P/s.  There the matrix cores are busy for 60% of the time, at a
-// clock that their power holds near 1.7 GHz (a single workgroup runs at 2.3).
+// from card to card: 206 G operations at 1.83 to 1.89 P/s.  There the matrix cores are busy
+// for 60% of the time, at a clock that their power holds near 1.7 GHz (a single workgroup
+// runs at 2.3).
 #include "kernels.hpp"
 #include "layers.hpp"
 #include "ring_common.hpp"
