@@ -231,10 +231,10 @@ def test_caches_that_hold_elements_twice():
             with pytest.raises(RuntimeError, match="GPU only"):
                 call()
     # Keys that are the values, too, or reach into them; parts of the same pages are apart.
-    flat, pool = torch.zeros(2 * 1536 + 64, dtype=torch.int8), torch.zeros(2, 2, 8, 3, 64, dtype=torch.int8)
+    flat, pool = torch.zeros(whole[0].numel() + 64, dtype=torch.int8), torch.zeros(2, 2, 8, 3, 64, dtype=torch.int8)
     scales = torch.zeros(2, 2, 3, 8)
     for tensors, taken in (((whole[0], whole[0], *whole[2:]), False), ((*whole[:2], whole[2], whole[2]), False),
-                           ((flat[:3072].view(2, 8, 3, 64), flat[64:].view(2, 8, 3, 64), *whole[2:]), False),
+                           ((flat[:-64].view(2, 8, 3, 64), flat[64:].view(2, 8, 3, 64), *whole[2:]), False),
                            ((pool[:, 0], pool[:, 1], scales[:, 0], scales[:, 1]), True)):
         with pytest.raises(RuntimeError if taken else ValueError, match="GPU only" if taken else "more than once"):
             write8(Cache8(*tensors), k, k, None, positions)
